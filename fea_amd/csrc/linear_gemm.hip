@@ -1,0 +1,219 @@
+// Tiled product of the many-class loss heads with its three epilogues: log-sum-exp partials, softmax gradient, store.
+//
+//   z[m][n] = (sum_k a[m][k] b[n][k] + bias[n]) / T
+//   LIN_LSE:   per row and column tile (max, sum exp(z - max)); no z leaves the registers
+//   LIN_DZ:    dz = g_m exp(z - lse_m), rounded once to the storage type (it is the operand of the next two products on the
+//              matrix pipe; the sums there are fp32), stored row-major and transposed so that both products find their
+//              reduction axis contiguous
+//   LIN_STORE: out = z, or fp32 slabs of a split reduction (joined by the caller in split order: no atomics)
+//
+// 128 x 128 tile, 4 waves of 64 x 64 (2 x 2 accumulators of 32 x 32), reduction in 128-byte steps of every row (64 bf16 / 32 fp32),
+// two LDS stages filled through registers so that rows, columns and reduction of any length are cut by a guard on the load.
+// The operands of the MFMA are swapped (classes as its rows), so a lane holds one label row and 32 of its classes: the softmax
+// sums are in-lane sums and one exchange between wave halves.
+#include "linear_loss.h"
+
+static constexpr int LG_T = 128, LG_STAGE = 2 * LG_T * 128;
+
+template <typename T> __device__ __forceinline__ void lg_store4(T* p, const float (&v)[4], int n) {
+    if (n >= 4 && (((uintptr_t)p) & (4 * sizeof(T) - 1)) == 0) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        else { const bf16x4 x = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}; *reinterpret_cast<bf16x4*>(p) = x; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (i < n) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+template <typename T, int EPI>
+__global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
+    constexpr int EPC = Elem<T>::EPC, CK = Elem<T>::CK;
+    __shared__ __attribute__((aligned(128))) char smem[2 * LG_STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave & 1, wn = wave >> 1, l32 = lane & 31, hf = lane >> 5;
+    // consecutive tiles of an XCD share the class tile and walk the label rows: the larger operand is read once
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int tm = id % g.ntm, rest = id / g.ntm, tn = rest % g.ntn, sp = rest / g.ntn;
+    const int m0 = tm * LG_T, n0 = tn * LG_T;
+    const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, k1 = EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K;
+
+    // staging: thread -> rows r + 32 i, 16-byte chunk c of the 128-byte row, XOR-swizzled by the row
+    const int r = tid >> 3, c = tid & 7;
+    const T* const ap = (const T*)g.a;
+    const T* const bp = (const T*)g.b;
+    u32x4 ra[4], rb[4];
+    auto fetch = [&](int k) {
+        const int kk = k + c * EPC;
+        const bool kin = kk < k1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int m = m0 + r + 32 * i, n = n0 + r + 32 * i;
+            ra[i] = kin && m < g.M ? *reinterpret_cast<const u32x4*>(ap + m * g.lda + kk) : u32x4{0, 0, 0, 0};
+            rb[i] = kin && n < g.N ? *reinterpret_cast<const u32x4*>(bp + n * g.ldb + kk) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto put = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int off = (r + 32 * i) * 128 + ((c ^ (r & 7)) << 4);
+            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + off) = ra[i];
+            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + LG_T * 128 + off) = rb[i];
+        }
+    };
+    f32x16 acc[2][2];                 // [label tile][class tile]
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    if (k0 < k1) fetch(k0);
+    int st = 0;
+    for (int k = k0; k < k1; k += CK, st ^= 1) {
+        put(st);
+        __syncthreads();              // one barrier per step: the other stage was last read in front of the previous one
+        if (k + CK < k1) fetch(k + CK);
+        const char* sa = smem + st * LG_STAGE + (wm * 64 + l32) * 128;
+        const char* sb = smem + st * LG_STAGE + LG_T * 128 + (wn * 64 + l32) * 128;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int off = ((2 * s + hf) ^ (l32 & 7)) << 4;
+            const u32x4 a0 = *reinterpret_cast<const u32x4*>(sa + off), a1 = *reinterpret_cast<const u32x4*>(sa + 32 * 128 + off);
+            const u32x4 b0 = *reinterpret_cast<const u32x4*>(sb + off), b1 = *reinterpret_cast<const u32x4*>(sb + 32 * 128 + off);
+            mma16(acc[0][0], b0, a0, (const T*)nullptr); mma16(acc[0][1], b1, a0, (const T*)nullptr);
+            mma16(acc[1][0], b0, a1, (const T*)nullptr); mma16(acc[1][1], b1, a1, (const T*)nullptr);
+        }
+    }
+    __syncthreads();
+
+    // lane: label row mrow(i), register e of class tile j: class ncol(j, e)
+    auto mrow = [&](int i) { return m0 + wm * 64 + i * 32 + l32; };
+    auto ncol = [&](int j, int e) { return n0 + wn * 64 + j * 32 + 8 * (e >> 2) + 4 * hf + (e & 3); };
+
+    if constexpr (EPI == LIN_STORE) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int m = mrow(i);
+            if (m >= g.M) continue;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int n = ncol(j, e);
+                    if (n >= g.N) continue;
+                    const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                    if (g.slab) lg_store4(g.slab + ((long long)sp * g.M + m) * g.N + n, v, g.N - n);
+                    else        lg_store4((T*)g.out + m * g.ldo + n, v, g.N - n);
+                }
+        }
+        return;
+    }
+
+    // z in place; classes behind the last are -inf
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int n = ncol(j, e);
+            const float b = g.bias && n < g.N ? g.bias[n] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[i][j][e] = n < g.N ? (acc[i][j][e] + b) * g.inv_t : -INFINITY;
+        }
+
+    if constexpr (EPI == LIN_LSE) {
+        float2* const red = reinterpret_cast<float2*>(smem);       // [wn][128 rows]
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float base = mx == -INFINITY ? 0.f : mx;         // every class masked by a -inf bias: the sum is 0, not NaN
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum += __expf(acc[i][j][e] - base);
+            sum += __shfl_xor(sum, 32);
+            if (hf == 0) red[wn * LG_T + wm * 64 + i * 32 + l32] = make_float2(mx, sum);
+        }
+        __syncthreads();
+        if (tid < LG_T && m0 + tid < g.M) {
+            const float2 p = red[tid], q = red[LG_T + tid];
+            const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
+            g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, p.y * __expf(p.x - base) + q.y * __expf(q.x - base));
+        }
+    }
+
+    if constexpr (EPI == LIN_DZ) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int m = mrow(i);
+            const float2 st2 = m < g.M ? g.stat[m] : make_float2(0.f, 0.f);
+            const bool dead = st2.y == 0.f;                        // the row does not count: 0 whatever its hidden state holds
+            const float lse = st2.x, sc = dead ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, st2.y, m);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float q = __expf(acc[i][j][e] - lse) * sc;
+                    acc[i][j][e] = dead || ncol(j, e) >= g.N ? 0.f : q;
+                }
+        }
+        if (g.colsum) {
+            float* const red = reinterpret_cast<float*>(smem);     // [wm][128 classes]
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float s = acc[0][j][e] + acc[1][j][e];
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) s += __shfl_xor(s, d);
+                    if (l32 == 0) red[wm * LG_T + ncol(j, e) - n0] = s;
+                }
+            __syncthreads();
+            if (tid < LG_T && n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LG_T + tid];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int m = mrow(i);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int n = ncol(j, e);
+                    const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                    if (m < g.M && n < g.Npad) lg_store4((T*)g.dz + m * g.lddz + n, v, g.Npad - n);
+                    if (g.dzt && m < g.Mpad)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) if (n + x < g.N) ((T*)g.dzt)[(n + x) * g.lddzt + m] = from_f32<T>(v[x]);
+                }
+        }
+    }
+}
+
+int fea_lin_tile_m(int, int) { return LG_T; }
+int fea_lin_tile_n(int, int) { return LG_T; }
+
+template <typename T> static void lin_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE>), dim3(grid), dim3(256), 0, s, g);
+    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ>), dim3(grid), dim3(256), 0, s, g);
+    else                    hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE>), dim3(grid), dim3(256), 0, s, g);
+}
+
+int fea_lin_gemm(int epi, int dtype, LinGemm g, hipStream_t s) {
+    const int epc = dtype == FEA_BF16 ? 8 : 4;
+    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && g.lda >= g.K && g.ldb >= g.K
+              && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0, FEA_E_BADARG, "lin_gemm: operands %d x %d x %d not aligned", g.M, g.N, g.K);
+    g.ntm = (g.M + LG_T - 1) / LG_T; g.ntn = (g.N + LG_T - 1) / LG_T;
+    if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
+    const long long grid = (long long)g.ntm * g.ntn * g.splits;
+    FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
+    if (dtype == FEA_BF16) lin_launch<__bf16>(epi, g, (unsigned)grid, s);
+    else                   lin_launch<float>(epi, g, (unsigned)grid, s);
+    FEA_LAUNCH_CHECK();
+    return FEA_OK;
+}

@@ -1,0 +1,44 @@
+// Shared between the files of the many-class loss heads (linear_loss.hip: entry points, statistics, layouts;
+// linear_gemm.hip: the tiled product and its epilogues).
+#pragma once
+#include "common.h"
+
+// C = A . B^T with the reduction axis contiguous in both operands.  A row = a label row, B row = a class (LIN_LSE, LIN_DZ);
+// LIN_STORE is a plain product.  Row starts are 16-byte aligned, K is a multiple of 16 bytes of elements.
+enum { LIN_LSE = 0, LIN_DZ = 1, LIN_STORE = 2 };
+
+struct LinGemm {
+    const void *a, *b;
+    long long lda, ldb;
+    int M, N, K;                      // rows of A, rows of B, reduction
+    // LIN_LSE, LIN_DZ: z = (a . b + bias) * inv_t
+    const float* bias;                // [N], nullable
+    float inv_t;
+    float2* part;                     // LIN_LSE: [M][ntn] (max, sum of exp(z - max)) of one column tile
+    const float2* stat;               // LIN_DZ: [M] (log sum exp, gate)
+    const float* gout; int gstride;   // LIN_DZ: upstream gradient, one value (stride 0) or one per row
+    const int* count;                 // LIN_DZ: rows that count (mean), nullable
+    float t;                          // LIN_DZ: temperature
+    void *dz, *dzt;                   // LIN_DZ: [M][lddz], [N][lddzt]; dzt nullable
+    long long lddz, lddzt;
+    int Npad, Mpad;                   // LIN_DZ: columns / rows written, zero behind N / M
+    float* colsum;                    // LIN_DZ: [tiles of A rows][N], nullable: sums of g * softmax over the tile's rows
+    long long ldcol;
+    // LIN_STORE: split over K into `splits` parts of kper: direct store to out (splits == 1, slab == NULL) or fp32 slabs
+    void* out; long long ldo;
+    float* slab;                      // [splits][M][N]
+    int splits, kper;
+    int ntm, ntn;
+};
+
+// gradient scale of a row: d loss / d (row loss) times the temperature; 0 for a row that does not count
+__device__ __forceinline__ float lin_row_scale(const float* gout, int gstride, const int* count, float t, float gate, long long row) {
+    float g = gout[row * gstride] * t;
+    if (count) { const int c = *count; g /= (float)(c > 0 ? c : 1); }
+    return gate != 0.f ? g : 0.f;
+}
+
+// linear_gemm.hip
+int fea_lin_gemm(int epi, int dtype, LinGemm g, hipStream_t s);
+int fea_lin_tile_m(int dtype, int M);       // rows of A / B per tile of the product (heights of `colsum`, `part`)
+int fea_lin_tile_n(int dtype, int M);

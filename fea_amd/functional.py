@@ -1,5 +1,6 @@
 """Segmentation loss, mask binarisation and IoU on the HIP kernels
-(build-defined, the reference has none)."""
+(build-defined, the reference has none), and the loss heads over many classes:
+`linear_cross_entropy`, `linear_distillation`."""
 from __future__ import annotations
 
 import torch
@@ -98,3 +99,150 @@ def threshold_mask(logits: torch.Tensor) -> torch.Tensor:
 def iou_from_counts(inter: torch.Tensor, union: torch.Tensor):
     iou = torch.where(union > 0, inter.double() / union.clamp(min=1).double(), torch.ones_like(inter, dtype=torch.float64))
     return iou, iou.mean()
+
+
+# ---- loss heads over many classes ---------------------------------------------------------------------------------------
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., D] -> [rows, D] as the kernels read it: contiguous rows, 16-byte aligned where D allows it."""
+    t = t.detach()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    epc = 16 // t.element_size()
+    d = t.shape[1]
+    if (t.stride(1) != 1 and d > 1) or t.stride(0) < d or (d % epc == 0 and (t.data_ptr() % 16 or t.stride(0) % epc)):
+        t = t.contiguous()
+        if d % epc == 0 and t.data_ptr() % 16:         # contiguous already, but a view at an odd offset
+            t = t.clone()
+    return t
+
+
+def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads):
+    """One forward call.  grads: 0, or what the backward will want (1 hidden, 2 weight, 4 bias).  Returns (loss, saved)."""
+    dev = hidden.device
+    h, w = _aligned_rows(hidden), _aligned_rows(weight)
+    (rows, d), v = h.shape, w.shape[0]
+    k = 1 if tlog is None else index.shape[-1]
+    ix = index.detach().to(torch.int64).contiguous()
+    b = None if bias is None else bias.detach().contiguous()
+    dt = L.dt_code(h.dtype)
+    f32 = {"dtype": torch.float32, "device": dev}
+    stat = torch.empty((rows, 2), **f32) if grads else None
+    dsel = torch.empty((rows, k), **f32) if grads else None
+    psel = torch.empty((rows, k), **f32) if grads & 4 else None
+    rowloss = torch.empty(rows, **f32) if reduction == "none" else None
+    loss = torch.empty((), **f32) if reduction != "none" else None
+    count = torch.empty((), dtype=torch.int32, device=dev) if reduction != "none" else None
+    n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    tail = (stat, dsel, psel, rowloss, loss, count, int(reduction == "mean"), ws, n, rows, d, v, dt, L.stream_ptr())
+    if tlog is None:
+        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, *tail)
+    else:
+        tl = tlog.detach().contiguous()
+        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, *tail)
+    return (loss if rowloss is None else rowloss.view(index.shape if tlog is None else index.shape[:-1])), (h, w, b, ix, stat, dsel, psel, count)
+
+
+class _LinearLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
+        grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want)
+        loss, saved = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
+        h, w, b, ix, stat, dsel, psel, count = saved
+        # the operands themselves are saved, so that autograd sees a change in place between forward and backward
+        ctx.save_for_backward(hidden, weight, bias, ix, stat, dsel, psel, count if reduction == "mean" else None)
+        ctx.how = (temperature, reduction, dsel.shape[1], grads)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        hidden, weight, bias, ix, stat, dsel, psel, count = ctx.saved_tensors
+        temperature, reduction, k, grads = ctx.how
+        with torch.cuda.device(hidden.device):
+            h, w = _aligned_rows(hidden), _aligned_rows(weight)
+            b = None if bias is None else bias.detach().contiguous()
+            (rows, d), v = h.shape, w.shape[0]
+            dt = L.dt_code(h.dtype)
+            dh = torch.empty(hidden.shape, dtype=h.dtype, device=h.device) if grads & 1 else None
+            dw = torch.empty(weight.shape, dtype=w.dtype, device=w.device) if grads & 2 else None
+            db = torch.empty(v, dtype=torch.float32, device=h.device) if grads & 4 else None
+            go = gout.detach().float().contiguous()
+            n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, grads)
+            ws = torch.empty(n, dtype=torch.uint8, device=h.device)
+            L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, count, go, int(reduction == "none"),
+                   temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr())
+        return dh, dw, db, None, None, None, None, None
+
+
+def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"{who}: reduction {reduction!r} (use 'mean', 'sum' or 'none')")
+    if not isinstance(hidden, torch.Tensor) or not isinstance(weight, torch.Tensor) or not isinstance(index, torch.Tensor):
+        raise ValueError(f"{who}: hidden, weight and the labels are tensors")
+    if hidden.dtype != weight.dtype or hidden.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{who}: hidden and weight are both float32 or both bfloat16 (got {hidden.dtype}, {weight.dtype})")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"{who}: hidden [..., D] and weight [classes, D] do not fit (got {tuple(hidden.shape)}, {tuple(weight.shape)})")
+    if index.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise ValueError(f"{who}: labels are integers (got {index.dtype})")
+    lead = index.shape if tlog is None else index.shape[:-1]
+    if lead != hidden.shape[:-1]:
+        raise ValueError(f"{who}: one label row for each hidden row (got {tuple(index.shape)} for hidden {tuple(hidden.shape)})")
+    if bias is not None:
+        if bias.dtype not in (torch.float32, weight.dtype) or bias.shape != weight.shape[:1]:
+            raise ValueError(f"{who}: bias is [classes] in float32 or the weight's type (got {tuple(bias.shape)}, {bias.dtype})")
+        bias = bias.float()
+    for t in (hidden, weight, bias, index, tlog):
+        if t is not None and not t.is_cuda:
+            raise L.FeaError(f"{who} runs on a ROCm device only")
+        if t is not None and t.device != hidden.device:
+            raise ValueError(f"{who}: operands on {hidden.device} and {t.device}")
+    rows = index.numel() if tlog is None else index.numel() // index.shape[-1]
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, weight, bias))
+    if rows == 0:
+        # nothing counts: the loss is 0 and so is every gradient
+        zero = (hidden.sum() + weight[:0].sum() + (0 if bias is None else bias[:0].sum())).float() if train else hidden.new_zeros((), dtype=torch.float32)
+        return zero if reduction != "none" else zero.expand(lead)
+    with torch.cuda.device(hidden.device):
+        if not train:
+            return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, 0)[0]
+        return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor = None,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of `hidden @ weight.T + bias` against one label per row, without keeping the logits.
+
+    hidden [..., D] and weight [classes, D]: both float32 or both bfloat16 (sums, softmax and loss in 32 bits); target [...]
+    integers; bias [classes], float32 or the weight's type.  Rows whose target is `ignore_index` do not count: loss 0 and
+    gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
+    reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
+    Differentiable once, in hidden, weight and bias; the backward recomputes the logits in pieces of the classes.
+    An NHWC feature map and a 1x1 convolution's weight viewed [classes, channels] are taken as they are."""
+    return _linear_loss("linear_cross_entropy", hidden, weight, bias, target, None, int(ignore_index), 1.0, reduction)
+
+
+def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                        bias: torch.Tensor = None, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """Distillation of `hidden @ weight.T + bias` from a teacher's top logits, without keeping the student's logits.
+
+    teacher_logits [..., K] (float32 or bfloat16) and teacher_index [..., K] (integers): the teacher's K (1..256) largest logits of
+    a row and their classes; a negative index is no entry.  With p = softmax(teacher_logits / T) over a row's entries and
+    q = softmax of all the student's logits / T, the loss of a row is T^2 sum_k p_k (log p_k - log q_{index_k}).  Rows without
+    an entry (or with -inf logits alone) do not count.  A class named twice in a row has the sum of both shares; an index
+    beyond the classes, a NaN or +inf teacher logit make the loss and the gradients NaN.  The teacher has no gradient.
+    hidden, weight, bias, reduction and the result as in `linear_cross_entropy`."""
+    who = "linear_distillation"
+    if not isinstance(teacher_logits, torch.Tensor) or not isinstance(teacher_index, torch.Tensor):
+        raise ValueError(f"{who}: teacher_logits and teacher_index are tensors")
+    if teacher_logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{who}: teacher_logits are float32 or bfloat16 (got {teacher_logits.dtype})")
+    if teacher_logits.dim() < 1 or teacher_logits.shape != teacher_index.shape or not 1 <= teacher_logits.shape[-1] <= 256:
+        raise ValueError(f"{who}: teacher_logits and teacher_index are [..., K] with K from 1 to 256 (got {tuple(teacher_logits.shape)}, "
+                         f"{tuple(teacher_index.shape)})")
+    temperature = float(temperature)
+    if not 1e-3 <= temperature <= 1e3:
+        raise ValueError(f"{who}: temperature {temperature} (0.001 to 1000)")
+    return _linear_loss(who, hidden, weight, bias, teacher_index, teacher_logits, 0, temperature, reduction)

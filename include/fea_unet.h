@@ -345,6 +345,37 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
                         const double* sumsq, double max_norm, double lr, double beta1, double beta2, double eps,
                         double weight_decay, int step, void* stream);
 
+/* ---- loss heads over many classes (not in the reference: its head has 6 sigmoid classes, models.py:23) ----------------
+ * A projection z = (h . w^T + bias) / T of hidden rows h[rows][ldh] onto V classes w[V][ldw] (D features, fp32 or bf16, both of
+ * `dtype`; bias[V] fp32, nullable) and a loss of its softmax, without keeping z.
+ *   fea_linear_ce_fwd (T = 1): loss_n = lse_n - z_{n,target[n]}; rows with target = ignore_index do not count.
+ *   fea_linear_kd_fwd: the teacher's K entries of a row are (teacher_index, teacher_logits); index < 0 = no entry;
+ *     p = softmax(teacher_logits / T) over the row's entries; loss_n = T^2 sum_k p_k (log p_k - z_{n,index_k} + lse_n).
+ *     The same class may be named twice (its shares add up).  Rows without an entry above -inf do not count.
+ * A row that does not count has loss 0 and gradients 0 whatever its hidden state holds.  A target outside [0, V), an index >= V, a
+ * teacher logit that is NaN or +inf: the row's loss and the gradients it reaches are NaN (nothing is read out of range).
+ * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
+ * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce), and psel[rows][K]
+ * if the bias gradient is wanted (all nullable).
+ *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1): recomputes the logits in pieces of the
+ *     classes and writes dh[rows][D], dw[V][D] (contiguous, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
+ *     value (gout_stride 0) or one per row (1); count: divide it by count[0] (mean) or NULL.
+ * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are copied into the workspace.
+ * ws: fea_linear_loss_ws_bytes(..., grads) bytes, 256-byte aligned; grads = 0 for the forwards, 1 dh + 2 dw + 4 db for the backward
+ * (0 bytes = sizes that are refused).  Results are the same from run to run. */
+size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);
+int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
+                      long long ignore_index, float* stat, float* dsel, float* psel, float* loss_rows, float* loss, int* count, int mean,
+                      void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
+int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const void* teacher_logits,
+                      int teacher_dtype, const long long* teacher_index, int K, float temperature, float* stat, float* dsel, float* psel,
+                      float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                      int dtype, void* stream);
+int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* index, int K,
+                        const float* stat, const float* dsel, const float* psel, const int* count, const float* gout, int gout_stride,
+                        float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                        int dtype, void* stream);
+
 /* ---- input pipeline ------------------------------------------------
  * The reference's per-image transform, custom_dataset.py:23-28 (applied at :69-71):
  * Resize((S,S)) on a PIL image -> ToTensor() -> Normalize(mean, std).  The resize is

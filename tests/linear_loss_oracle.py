@@ -1,0 +1,92 @@
+"""The loss heads over many classes in 64 bits, with the bounds that their kernels' arithmetic gives.
+
+u = torch.finfo(dtype).eps / 2 (a rounding to the storage type), e = 2^-24 (a rounding in 32 bits), with B = max_v sum_d |h_d w_d| + |b_v|:
+  a logit is off by dz <= (D + 4) e B / T (D products and sums, bias, scale), an exponential by 3 e more and e |z - lse| for its argument;
+  log-sum-exp by the largest of these and the sum's (16 + V / 64) e;  so a loss by 2 of them, a softmax value q by the same relative to q.
+  dz = g (q - p) is rounded once to the storage type; dh and dw add the products' fp32 sums and one rounding to the storage type."""
+import torch
+
+E = 2.0 ** -24
+
+
+def case(rows, dim, classes, dtype, seed=0, top=0, ignored=0.0, short=0.0, bias=False):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(rows, dim, generator=g).to(dtype)
+    w = (torch.randn(classes, dim, generator=g) * (1.5 / dim ** 0.5)).to(dtype)
+    b = torch.randn(classes, generator=g) * 0.3 if bias else None
+    gone = torch.rand(rows, generator=g) < ignored
+    if not top:
+        t = torch.randint(0, classes, (rows,), generator=g)
+        return h, w, b, t.masked_fill(gone, -100)
+    i = torch.randint(0, classes, (rows, top), generator=g)          # the same class twice in a row happens
+    i[torch.rand(rows, top, generator=g) < short] = -1
+    i[gone] = -1
+    return h, w, b, i, (torch.randn(rows, top, generator=g) * 2 + 5).to(dtype)
+
+
+def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, reduction="mean", gout=None):
+    """{"loss", "hidden", "weight", "bias"}: values and bounds, as (value, bound) pairs in 64 bits.  gout: upstream gradient of the losses
+    (rows) for "none", else of the result."""
+    dtype, t = h.dtype, temperature
+    u = torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else E
+    hd, wd = h.double().reshape(-1, h.shape[-1]), w.double()
+    rows, dim = hd.shape
+    v = wd.shape[0]
+    bd = torch.zeros(v, dtype=torch.float64) if b is None else b.double()
+    z = (hd @ wd.T + bd) / t
+    lse = torch.logsumexp(z, 1)
+    q = torch.exp(z - lse[:, None])
+    p = torch.zeros_like(z)
+    if tlog is None:
+        ix = index.reshape(-1)
+        on = ix != ignore_index
+        p[on, ix[on]] = 1.0
+        loss = torch.where(on, lse - z.gather(1, torch.where(on, ix, 0)[:, None])[:, 0], 0.0)
+        scale = 1.0
+        spread = torch.zeros(rows, dtype=torch.float64)
+    else:
+        ix, a = index.reshape(rows, -1), tlog.double().reshape(rows, -1) / t
+        a = a.masked_fill(ix < 0, -torch.inf)
+        on = (a > -torch.inf).any(1)
+        pk = torch.softmax(torch.where(on[:, None], a, 0.0), 1) * on[:, None]
+        p.scatter_add_(1, ix.clamp(min=0), pk)
+        zk = z.gather(1, ix.clamp(min=0))
+        loss = t * t * torch.where(pk > 0, pk * (torch.log(pk.clamp(min=1e-300)) - zk + lse[:, None]), 0.0).sum(1)
+        scale = t * t
+        spread = (pk * (torch.log(pk.clamp(min=1e-300)).abs() + zk.abs() + lse.abs()[:, None])).nan_to_num(0.0, 0.0, 0.0).sum(1)
+    n = max(1, int(on.sum()))
+    big = (hd.abs() @ wd.abs().T + torch.where(bd > -1e30, bd, 0.0).abs()).amax(1)
+    dz_log = ((dim + 4) * E * big / t + (16 + v / 64) * E + 3 * E + E * (z - lse[:, None]).masked_fill(z < -1e30, 0).abs().amax(1)).masked_fill(~on, 0.0)
+    loss_off = scale * (2 * dz_log + E * lse.abs().masked_fill(~on, 0.0) + (8 + (0 if tlog is None else index.shape[-1])) * E * (spread + 1))
+    loss = torch.where(on, loss, 0.0)
+    if reduction == "none":
+        g = torch.ones(rows, dtype=torch.float64) if gout is None else gout.double().reshape(-1)
+        out = {"loss": (loss, loss_off + E * loss.abs())}
+    else:
+        div = n if reduction == "mean" else 1
+        g = torch.full((rows,), (1.0 if gout is None else float(gout)) / div, dtype=torch.float64)
+        out = {"loss": (loss.sum() / div, loss_off.sum() / div + 2 * E * loss.abs().sum() / div)}
+    g = g * t * on
+    q, p = q * on[:, None], p * on[:, None]
+    q = q.nan_to_num(0.0) if not on.all() else q
+    hd = torch.where(on[:, None], hd, 0.0)
+    dz = g[:, None] * (q - p)
+    off = g.abs()[:, None] * (q * 2 * dz_log[:, None] + (8 + (0 if tlog is None else index.shape[-1])) * E * (p + q)) + u * dz.abs() + 2 * E * dz.abs()
+    dh, dw = dz @ wd, dz.T @ hd
+    out["hidden"] = (dh, off @ wd.abs() + (v + 8) * E * (dz.abs() @ wd.abs()) + u * dh.abs() + 1e-37)
+    out["weight"] = (dw, off.T @ hd.abs() + (rows + 8) * E * (dz.abs().T @ hd.abs()) + u * dw.abs() + 1e-37)
+    offb = g.abs()[:, None] * (q * 2 * dz_log[:, None] + 8 * E * (p + q)) + 4 * E * g.abs()[:, None] * (q + p)
+    out["bias"] = (dz.sum(0), offb.sum(0) + 20 * E * (g.abs()[:, None] * (q + p)).sum(0) + 1e-37)
+    return out
+
+
+def check(name, got, want):
+    value, bound = want
+    got = got.detach().double().cpu().reshape(value.shape)
+    assert torch.equal(torch.isnan(got), torch.isnan(value)), f"{name}: NaN in other places"
+    far = (got - value).abs() - bound
+    far = far[torch.isfinite(value)]
+    same = got[~torch.isfinite(value) & ~torch.isnan(value)] == value[~torch.isfinite(value) & ~torch.isnan(value)]
+    assert bool(same.all()), f"{name}: other infinities"
+    assert far.numel() == 0 or float(far.max()) <= 0, f"{name}: {float(far.max()):.3e} beyond its bound, worst ratio " \
+        f"{float(((got - value).abs() / bound)[torch.isfinite(value)].max()):.2f}"

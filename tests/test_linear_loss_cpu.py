@@ -1,0 +1,76 @@
+"""Refusals of the loss heads over many classes, and the oracle's own checks: no GPU is touched."""
+import pytest
+import torch
+
+from fea_amd import _lib as L
+from fea_amd import functional as F
+from tests import linear_loss_oracle as O
+
+H, W, T = torch.zeros(4, 8), torch.zeros(5, 8), torch.zeros(4, dtype=torch.int64)
+A, I = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("bad", [
+    {"reduction": "avg"}, {"hidden": H.half(), "weight": W.half()}, {"hidden": H.bfloat16()}, {"weight": W[:, :7]}, {"weight": W[0]},
+    {"weight": W[:0]}, {"hidden": H[:, :0], "weight": W[:, :0]}, {"target": T.float()}, {"target": T.bool()}, {"target": T[:3]},
+    {"target": T[:, None]}, {"bias": torch.zeros(4)}, {"bias": torch.zeros(5, dtype=torch.float64)}, {"hidden": None}, {"target": None}])
+def test_cross_entropy_refuses(bad):
+    kw = {"hidden": H, "weight": W, "target": T} | bad
+    with pytest.raises(ValueError, match="linear_cross_entropy"):
+        F.linear_cross_entropy(**kw)
+
+
+@pytest.mark.parametrize("bad", [
+    {"temperature": 0.0}, {"temperature": -1.0}, {"temperature": float("nan")}, {"temperature": float("inf")}, {"teacher_logits": A[:, :2]},
+    {"teacher_logits": A[:, :0], "teacher_index": I[:, :0]}, {"teacher_logits": A.double()}, {"teacher_index": A},
+    {"teacher_logits": A[:3], "teacher_index": I[:3]}, {"teacher_logits": torch.zeros(4, 257), "teacher_index": torch.zeros(4, 257, dtype=torch.int64)},
+    {"teacher_logits": None}, {"reduction": "batchmean"}])
+def test_distillation_refuses(bad):
+    kw = {"hidden": H, "weight": W, "teacher_logits": A, "teacher_index": I} | bad
+    with pytest.raises(ValueError, match="linear_distillation"):
+        F.linear_distillation(**kw)
+
+
+def test_no_cpu_path():
+    with pytest.raises(L.FeaError, match="ROCm device"):
+        F.linear_cross_entropy(H, W, T)
+    with pytest.raises(L.FeaError, match="ROCm device"):
+        F.linear_distillation(H, W, A, I)
+
+
+def test_workspace_sizes():
+    ws = L.load().fea_linear_loss_ws_bytes
+    assert ws(0, 8, 8, 1, 0, 0) == 0 and ws(8, 8, 8, 1, 5, 0) == 0 and ws(8, 8, 8, 0, 0, 7) == 0
+    for dt in (L.F32, L.BF16):
+        for rows, d, v, k in ((1, 8, 1, 1), (7, 5, 3, 2), (8192, 4096, 131072, 1), (1 << 24, 64, 6, 1), (1 << 20, 64, 100000, 4)):
+            assert 0 < ws(rows, d, v, k, dt, 0) < 6 << 30, (rows, d, v)
+            sizes = [ws(rows, d, v, k, dt, g) for g in (1, 2, 3, 7)]
+            assert sizes[0] <= sizes[2] <= sizes[3] and sizes[1] <= sizes[2], (rows, d, v)
+            assert sizes[3] < 24 << 30, (rows, d, v)
+
+
+@pytest.mark.parametrize("top", [0, 4])
+def test_oracle_against_autograd_in_64_bits(top):
+    c = O.case(20, 12, 30, torch.float32, seed=1, top=top, ignored=0.2, short=0.3, bias=True)
+    got = O.evaluate(*c, temperature=1.0 if not top else 2.0)
+    x = [t.double().requires_grad_(True) for t in c[:3]]
+    z = x[0] @ x[1].T + x[2]
+    if not top:
+        loss = torch.nn.functional.cross_entropy(z, c[3])
+    else:
+        there = c[3] >= 0
+        p = torch.softmax(torch.where(there, c[4].double() / 2.0, -1e30), 1) * there
+        logq = torch.log_softmax(z / 2.0, 1).gather(1, c[3].clamp(min=0))
+        loss = 4.0 * torch.where(there, torch.special.xlogy(p, p) - p * logq, 0.0).sum() / there.any(1).sum()
+    for k, g in zip(("hidden", "weight", "bias"), torch.autograd.grad(loss, x)):
+        assert torch.allclose(got[k][0], g, rtol=1e-9, atol=1e-12), k
+    assert torch.allclose(got["loss"][0], loss, rtol=1e-9)
+
+
+def test_check_finds_a_planted_error():
+    """The comparison the GPU tests rest on: a value beyond its bound, a NaN or an infinity in another place is found."""
+    value, bound = torch.tensor([1.0, 2.0], dtype=torch.float64), torch.tensor([1e-3, 1e-3], dtype=torch.float64)
+    O.check("x", torch.tensor([1.0005, 2.0]), (value, bound))
+    for bad in ([1.002, 2.0], [float("nan"), 2.0], [float("inf"), 2.0]):
+        with pytest.raises(AssertionError):
+            O.check("x", torch.tensor(bad), (value, bound))

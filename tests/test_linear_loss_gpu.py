@@ -1,0 +1,325 @@
+"""linear_cross_entropy and linear_distillation against their definition in 64 bits (tests/linear_loss_oracle.py)."""
+import pytest
+import torch
+
+from fea_amd import _lib as L
+from fea_amd import functional as F
+from tests import linear_loss_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float32, torch.bfloat16]
+SHAPES = [(1, 8, 1), (1, 1, 2), (1, 64, 600), (2, 5, 7), (3, 64, 6), (17, 33, 129), (64, 128, 128), (129, 72, 1000), (257, 200, 333),
+          (300, 96, 5003), (513, 640, 1537), (5000, 64, 6), (4097, 24, 33)]
+
+
+def _leaf(t):
+    return None if t is None else t.to(DEV).requires_grad_(True)
+
+
+def _run(h, w, b, index, tlog=None, gout=None, **how):
+    h, w, b = _leaf(h), _leaf(w), _leaf(b)
+    if tlog is None:
+        loss = F.linear_cross_entropy(h, w, index.to(DEV), bias=b, **how)
+    else:
+        loss = F.linear_distillation(h, w, tlog.to(DEV), index.to(DEV), bias=b, **how)
+    leaves = [t for t in (h, w, b) if t is not None]
+    grads = torch.autograd.grad(loss, leaves, None if gout is None else gout.to(DEV))
+    return dict(zip(["loss", "hidden", "weight", "bias"], [loss, *grads]))
+
+
+def _compare(got, want):
+    for k, v in got.items():
+        O.check(k, v, want[k])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_cross_entropy(shape, dtype):
+    h, w, b, t = O.case(*shape, dtype, seed=sum(shape), ignored=0.2, bias=shape[0] % 2 == 1)
+    _compare(_run(h, w, b, t), O.evaluate(h, w, b, t))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("top", [1, 5, 64])
+def test_distillation(shape, dtype, top):
+    h, w, b, i, a = O.case(*shape, dtype, seed=sum(shape) + top, top=top, ignored=0.2, short=0.3, bias=shape[0] % 2 == 1)
+    _compare(_run(h, w, b, i, a, temperature=2.0), O.evaluate(h, w, b, i, a, temperature=2.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("top", [0, 3])
+def test_reductions(dtype, reduction, top):
+    c = O.case(77, 40, 300, dtype, seed=5, top=top, ignored=0.2, bias=True)
+    gout = torch.randn(77, generator=torch.Generator().manual_seed(1)) if reduction == "none" else torch.tensor(-3.0)
+    kw = {"temperature": 0.5} if top else {}
+    _compare(_run(*c, gout=gout, reduction=reduction, **kw), O.evaluate(*c, gout=gout, reduction=reduction, **kw))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(300, 72, 900), (700, 40, 2000)])
+@pytest.mark.parametrize("top", [0, 4])
+def test_pieces(shape, dtype, top, monkeypatch):
+    """Many pieces of the rows (few classes) and of the classes (many): the sums over pieces, in 32 bits."""
+    monkeypatch.setenv("FEA_AMD_LINEAR_PIECE", str(1 << 16))
+    c = O.case(*shape, dtype, seed=9, top=top, ignored=0.1, short=0.2, bias=True)
+    _compare(_run(*c), O.evaluate(*c))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_counts(dtype):
+    h, w, b, t = O.case(9, 16, 50, dtype, bias=True)
+    got = _run(h, w, b, torch.full_like(t, -100))
+    assert all(float(v.detach().abs().max()) == 0.0 for v in got.values())
+    i = torch.full((9, 3), -1)
+    got = _run(h, w, b, i, torch.zeros(9, 3, dtype=dtype))
+    assert all(float(v.detach().abs().max()) == 0.0 for v in got.values())
+    got = _run(h, w, b, torch.zeros(9, 3, dtype=torch.int64), torch.full((9, 3), -torch.inf, dtype=dtype))
+    assert all(float(v.detach().abs().max()) == 0.0 for v in got.values())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_ignored_rows_may_hold_anything(dtype, top, bad):
+    """The hidden state of a row that does not count reaches neither the loss nor any gradient."""
+    c = list(O.case(70, 64, 200, dtype, seed=3, top=top, ignored=0.4, bias=True))
+    want = O.evaluate(*c)
+    gone = c[3] == -100 if not top else (c[3] < 0).all(1)
+    assert 5 < int(gone.sum()) < 65
+    c[0] = c[0].clone()
+    c[0][gone] = bad
+    _compare(_run(*c), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_classes(dtype):
+    """Classes masked by a bias of -inf or of the type's lowest value: softmax 0 and gradient 0 there."""
+    h, w, b, t = O.case(65, 48, 400, dtype, seed=4, bias=True)
+    b[100:228] = -torch.inf                                  # the whole of a column tile and parts of its neighbours
+    b[256:384] = torch.finfo(torch.float32).min
+    t = t % 100
+    got = _run(h, w, b, t)
+    _compare(got, O.evaluate(h, w, b, t))
+    assert float(got["weight"][100:228].abs().max()) == 0.0 and float(got["bias"][256:384].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_teacher_minus_infinity_is_no_share(dtype):
+    h, w, b, i, a = O.case(40, 32, 90, dtype, seed=6, top=6)
+    a[:, 2] = -torch.inf
+    a[7] = -torch.inf
+    _compare(_run(h, w, b, i, a), O.evaluate(h, w, b, i, a))
+
+
+def test_a_label_that_names_no_class_is_nan():
+    h, w, b, t = O.case(10, 32, 20, torch.float32, seed=7)
+    for bad in (20, 1 << 40, -5):
+        x = t.clone()
+        x[4] = bad
+        loss = F.linear_cross_entropy(h.to(DEV), w.to(DEV), x.to(DEV), reduction="none")
+        want = O.evaluate(h, w, b, t, reduction="none")["loss"][0]
+        assert torch.isnan(loss[4]) and torch.allclose(loss.cpu().double()[torch.arange(10) != 4], want[torch.arange(10) != 4], rtol=1e-5)
+    h, w, b, i, a = O.case(10, 32, 20, torch.float32, seed=7, top=3)
+    i[2, 1] = 20
+    a[5, 0] = torch.nan
+    a[6, 2] = torch.inf
+    got = _run(h, w, b, i, a, reduction="none", gout=torch.ones(10))
+    assert torch.isnan(got["loss"]).nonzero().flatten().tolist() == [2, 5, 6]
+    assert torch.isnan(got["hidden"]).all(1).nonzero().flatten().tolist() == [2, 5, 6]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layouts(dtype):
+    """Strided rows, odd storage offsets, leading dimensions, an expanded hidden state, other integer types, views of a 1x1
+    convolution's weight: the same values as contiguous ones."""
+    h, w, b, t = O.case(60, 64, 150, dtype, seed=8, ignored=0.1, bias=True)
+    want = _run(h, w, b, t)
+    wide = torch.zeros(60, 200, dtype=dtype)
+    wide[:, 3:67] = h
+    tall = torch.zeros(151 * 64 + 1, dtype=dtype)
+    tall[1:1 + 150 * 64] = w.reshape(-1)
+    for x in (_leaf(wide)[:, 3:67], _leaf(h.t().contiguous()).t(), _leaf(h).reshape(3, 4, 5, 64)):
+        y = _leaf(tall)[1:1 + 150 * 64].view(150, 64, 1, 1).view(150, 64)
+        for kind in (torch.int64, torch.int32, torch.int16):
+            loss = F.linear_cross_entropy(x, y, t.to(DEV).to(kind).reshape(x.shape[:-1]), bias=b.to(DEV))
+            gx, gy = torch.autograd.grad(loss, [x, y])
+            assert torch.equal(loss, want["loss"]) and torch.equal(gx.reshape(60, 64), want["hidden"]) and torch.equal(gy, want["weight"])
+    u8 = t.clamp(min=0)
+    loss = F.linear_cross_entropy(h.to(DEV), w.to(DEV), u8.to(torch.uint8).to(DEV), ignore_index=0, reduction="sum")
+    O.check("loss", loss, O.evaluate(h, w, None, u8, ignore_index=0, reduction="sum")["loss"])
+    one = _leaf(h[:1])
+    loss = F.linear_cross_entropy(one.expand(60, 64), w.to(DEV), t.to(DEV), reduction="sum")
+    ref = O.evaluate(h[:1].expand(60, 64), w, None, t, reduction="sum")
+    O.check("loss", loss, ref["loss"])
+    g = torch.autograd.grad(loss, one)[0].double().cpu()
+    tol = ref["hidden"][1].sum(0) + 60 * torch.finfo(dtype).eps / 2 * ref["hidden"][0].abs().sum(0)
+    assert bool(((g - ref["hidden"][0].sum(0)).abs() <= tol).all())
+    bare = F.linear_cross_entropy(h[0].to(DEV), w.to(DEV), t[0].to(DEV))
+    assert bare.shape == () and torch.equal(bare, F.linear_cross_entropy(h[:1].to(DEV), w.to(DEV), t[:1].to(DEV)))
+
+
+def test_only_the_gradients_that_are_wanted():
+    c = O.case(50, 64, 200, torch.bfloat16, seed=2, bias=True)
+    want = _run(*c)
+    for names in (["hidden"], ["weight"], ["bias"], ["weight", "bias"]):
+        x = {k: v.to(DEV).requires_grad_(k in names) for k, v in zip(("hidden", "weight", "bias"), c)}
+        loss = F.linear_cross_entropy(x["hidden"], x["weight"], c[3].to(DEV), bias=x["bias"])
+        for k, g in zip(names, torch.autograd.grad(loss, [x[k] for k in names])):
+            assert torch.equal(g, want[k]), (names, k)
+    with torch.no_grad():
+        loss = F.linear_cross_entropy(x["hidden"], x["weight"], c[3].to(DEV), bias=x["bias"])
+    assert not loss.requires_grad and torch.equal(loss, want["loss"])
+
+
+def test_bf16_bias_and_empty_batch():
+    h, w, b, t = O.case(20, 32, 64, torch.bfloat16, seed=2, bias=True)
+    b = b.bfloat16()
+    x = _leaf(b)
+    loss = F.linear_cross_entropy(h.to(DEV), w.to(DEV), t.to(DEV), bias=x)
+    g = torch.autograd.grad(loss, x)[0]
+    ref = O.evaluate(h, w, b, t)
+    assert g.dtype == torch.bfloat16
+    O.check("bias", g, (ref["bias"][0], ref["bias"][1] + 2.0 ** -8 * ref["bias"][0].abs()))
+    e, w = _leaf(h[:0]), _leaf(w)
+    for loss in (F.linear_cross_entropy(e, w, t[:0].to(DEV)), F.linear_distillation(e, w, h[:0, :4].to(DEV), t[:0, None].expand(0, 4).to(DEV))):
+        gh, gw = torch.autograd.grad(loss, [e, w])
+        assert float(loss) == 0.0 and gh.shape == (0, 32) and float(gw.abs().max()) == 0.0
+    assert F.linear_cross_entropy(e, w, t[:0].to(DEV), reduction="none").shape == (0,)
+
+
+@pytest.mark.parametrize("top", [0, 2])
+def test_gradient_against_differences(top):
+    """Central differences of the fp32 loss along a direction.  The step's cubic term is below (0.02)^2 of the slope; the two losses
+    are off by 1e-6 each, over 2 x 0.02."""
+    c = O.case(30, 24, 70, torch.float32, seed=11, top=top, ignored=0.1, bias=True)
+    kw = {"temperature": 1.5} if top else {}
+    got = _run(*c, **kw)
+    g = torch.Generator().manual_seed(3)
+    for k, name in enumerate(["hidden", "weight", "bias"]):
+        d = torch.randn(c[k].shape, generator=g)
+        d /= d.norm()
+        step = 0.02
+        pair = []
+        for sign in (1, -1):
+            x = list(c)
+            x[k] = x[k] + sign * step * d
+            pair.append(float(_run(*x, **kw)["loss"]))
+        slope = float((got[name].cpu() * d).sum())
+        curve = float(O.evaluate(*c, **kw)[name][0].norm())
+        assert abs((pair[0] - pair[1]) / (2 * step) - slope) <= 2e-6 / (2 * step) + 4e-4 * max(curve, 1.0), name
+
+
+def test_same_result_every_time_and_on_another_stream():
+    c = O.case(700, 64, 1200, torch.bfloat16, seed=12, top=4, bias=True)
+    want = _run(*c)
+    s = torch.cuda.Stream()
+    for _ in range(3):
+        got = _run(*c)
+        with torch.cuda.stream(s):
+            other = _run(*c)
+        torch.cuda.synchronize()
+        for k in want:
+            assert torch.equal(got[k], want[k]) and torch.equal(other[k], want[k]), k
+
+
+@pytest.mark.parametrize("top", [0, 3])
+def test_captured_and_replayed(top):
+    """Forward and backward in one captured graph, replayed with other inputs, the program's own work in between; a second graph
+    of the same operator keeps its own workspaces."""
+    cases = [O.case(130, 64, 500, torch.bfloat16, seed=s, top=top, ignored=0.1, bias=True) for s in (1, 2, 3)]
+    graphs = []
+    for n in range(2):
+        x = [t.to(DEV) for t in cases[0]]
+        for t in x[:3]:
+            t.requires_grad_(True)
+
+        def step():
+            loss = F.linear_distillation(x[0], x[1], x[4], x[3], bias=x[2]) if top else F.linear_cross_entropy(x[0], x[1], x[3], bias=x[2])
+            return [loss.detach(), *torch.autograd.grad(loss, x[:3])]
+
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, x, out))
+    for c in cases + cases[:1]:
+        want = _run(*c)
+        for g, x, out in graphs:
+            with torch.no_grad():
+                for dst, src in zip(x, c):
+                    dst.copy_(src.to(DEV))
+        for g, x, out in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for g, x, out in graphs:
+            for k, v in zip(("loss", "hidden", "weight", "bias"), out):
+                assert torch.equal(v, want[k]), k
+
+
+def test_together_in_a_training_loop():
+    """Labels and a teacher together on one head, as a distillation step uses them: both losses, one backward, an optimizer step;
+    against the same step from the definition's gradients."""
+    h, w, b, t = O.case(200, 64, 300, torch.float32, seed=21, ignored=0.2, bias=True)
+    i, a = O.case(200, 64, 300, torch.float32, seed=22, top=8, short=0.2)[3:]
+    head = torch.nn.Linear(64, 300).to(DEV)
+    with torch.no_grad():
+        head.weight.copy_(w)
+        head.bias.copy_(b)
+    opt = torch.optim.SGD(head.parameters(), lr=0.5)
+    x = h.to(DEV).requires_grad_(True)
+    loss = 0.3 * F.linear_cross_entropy(x, head.weight, t.to(DEV), bias=head.bias) \
+        + 0.7 * F.linear_distillation(x, head.weight, a.to(DEV), i.to(DEV), bias=head.bias, temperature=2.0)
+    loss.backward()
+    opt.step()
+    p, q = O.evaluate(h, w, b, t), O.evaluate(h, w, b, i, a, temperature=2.0)
+
+    def both(k):
+        return 0.3 * p[k][0] + 0.7 * q[k][0], 0.3 * p[k][1] + 0.7 * q[k][1] + 4 * O.E * (p[k][0].abs() + q[k][0].abs())
+    O.check("loss", loss, both("loss"))
+    O.check("hidden", x.grad, both("hidden"))
+    for name, now, start in (("weight", head.weight, w), ("bias", head.bias, b)):
+        value, bound = both(name)
+        O.check(name, now, (start.double() - 0.5 * value, 0.5 * bound + 2 * O.E * (start.double().abs() + value.abs())))
+
+
+def test_double_backward_is_refused():
+    h, w, b, t = O.case(5, 16, 9, torch.float32)
+    x = _leaf(h)
+    g = torch.autograd.grad(F.linear_cross_entropy(x, w.to(DEV), t.to(DEV)), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_change_in_place_between_forward_and_backward_is_refused():
+    h, w, b, t = O.case(5, 16, 9, torch.float32)
+    x, y = _leaf(h), _leaf(w)
+    loss = F.linear_cross_entropy(x, y, t.to(DEV))
+    with torch.no_grad():
+        y.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+
+
+def test_workspace_and_operands_are_checked():
+    """The C entry points refuse what they cannot serve, before any launch."""
+    h, w, _, t = O.case(16, 32, 40, torch.float32)
+    h, w, t = h.to(DEV), w.to(DEV), t.to(DEV)
+    n = L.load().fea_linear_loss_ws_bytes(16, 32, 40, 1, L.F32, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    out = torch.empty(16, device=DEV)
+
+    def fwd(h=h, ldh=32, ws=ws, n=n, rows=16, d=32, v=40, dt=L.F32):
+        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, None, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
+    fwd()
+    for bad in ({"n": n - 1}, {"ws": None}, {"ldh": 31}, {"ldh": 33}, {"h": None}, {"dt": 7}, {"rows": 0}, {"v": 0}, {"d": 0}, {"h": h.data_ptr() + 4},
+                {"ws": ws.data_ptr() + 16}, {"d": 1 << 17, "ldh": 1 << 17}):
+        with pytest.raises(L.FeaError):
+            fwd(**bad)
+    torch.cuda.synchronize()
