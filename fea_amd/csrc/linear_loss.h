@@ -22,11 +22,12 @@ struct LinGemm {
     void *dz, *dzt;                   // LIN_DZ: [M][lddz], [N][lddzt]; dzt nullable
     long long lddz, lddzt;
     int Npad, Mpad;                   // LIN_DZ: columns / rows written, zero behind N / M
-    float* colsum;                    // LIN_DZ: [tiles of A rows][N], nullable: sums of g * softmax over the tile's rows
+    float* colsum;                    // LIN_DZ: [tiles of A rows][N], nullable: sums of row scale * softmax over the tile's rows
     long long ldcol;
     // LIN_STORE: split over K into `splits` parts of kper: direct store to out (splits == 1, slab == NULL) or fp32 slabs
     void* out; long long ldo;
     float* slab;                      // [splits][M][N]
+    int scale;                        // 0: none, 1: times the row scale of A's row, 2: times the common scale (gout, count, t above)
     int splits, kper;
     int ntm, ntn;
 };
@@ -37,6 +38,30 @@ __device__ __forceinline__ float lin_row_scale(const float* gout, int gstride, c
     if (count) { const int c = *count; g /= (float)(c > 0 ? c : 1); }
     return gate != 0.f ? g : 0.f;
 }
+
+// Few classes, few features, many rows (linear_few.hip)
+struct LinFew {
+    const void *h, *w;
+    long long ldh, ldw;
+    const float* bias;
+    const long long* index;               // [rows][K]
+    const void* tlog; int tdt;            // forward: NULL = cross entropy
+    long long ignore;
+    float t, inv_t;
+    float2* stat;                         // forward: written (nullable); backward: read
+    float* psel;                          // [rows][K] teacher shares: forward writes (nullable), backward reads (NULL: cross entropy)
+    float* loss_rows;
+    double* bsum; int* bcnt;              // [fea_lin_few_blocks]
+    const float* gout; int gstride;
+    const int* count;
+    void* dh;
+    float *slab, *dbslab; long long slab_ld;   // [blocks][32 * (32 or 64)], [blocks][32]
+    long long rows; int D, V, K;
+};
+bool fea_lin_few(long long rows, int D, int V);
+int fea_lin_few_blocks(long long rows);
+int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s);
+int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 
 // linear_gemm.hip
 int fea_lin_gemm(int epi, int dtype, LinGemm g, hipStream_t s);

@@ -28,17 +28,21 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(const T* __restrict__ in,
 }
 
 // out[c][r] = in[r][c] (r < R), zero for R <= r < Rpad; rows whose gate is 0 count as zeros: what an ignored row holds (an
-// infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must not reach the weight.
+// infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must not reach the weight.  gout (nullable): rows
+// times their own upstream gradient.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_transpose_kernel(const T* __restrict__ in, long long ld, T* __restrict__ out, long long ldo,
-                                                            long long R, long long Rpad, int C, const float2* __restrict__ stat) {
+                                                            long long R, long long Rpad, int C, const float2* __restrict__ stat,
+                                                            const float* __restrict__ gout, float t) {
     __shared__ T tile[64][64 + 8 / sizeof(T)];
     const long long r0 = (long long)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
 #pragma unroll 4
     for (int i = y; i < 64; i += 4) {
         const long long r = r0 + i;
-        tile[i][x] = r < R && c0 + x < C && (!stat || stat[r].y != 0.f) ? in[r * ld + c0 + x] : from_f32<T>(0.f);
+        T v = r < R && c0 + x < C && (!stat || stat[r].y != 0.f) ? in[r * ld + c0 + x] : from_f32<T>(0.f);
+        if (gout && r < R && stat[r].y != 0.f) v = from_f32<T>(to_f32(v) * lin_row_scale(gout, 1, nullptr, t, 1.f, r));
+        tile[i][x] = v;
     }
     __syncthreads();
 #pragma unroll 4
@@ -48,36 +52,37 @@ __global__ __launch_bounds__(256) void lin_transpose_kernel(const T* __restrict_
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
 
-// zsel[n][k] = h_n . w_{index[n][k]} + b: one wave per entry.  Absent entries (index < 0 or >= V) are not read.
+// zsel[n][k] = h_n . w_{index[n][k]} + b: L lanes (a power of two that covers the row in 16-byte loads, 64 at most) per entry.
+// Absent entries (index < 0 or >= V) are not read.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_select_kernel(const T* __restrict__ h, long long ldh, const T* __restrict__ w, long long ldw,
                                                          const float* __restrict__ bias, const long long* __restrict__ index, int K,
-                                                         float* __restrict__ zsel, long long entries, int D, int V, long long e0) {
+                                                         float* __restrict__ zsel, long long entries, int D, int V, int L) {
     constexpr int EPC = Elem<T>::EPC;
-    const long long e = e0 + (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (e >= entries) return;
-    const long long i = index[e];
-    float s = 0.f;
-    if (i >= 0 && i < V) {
-        const T* a = h + e / K * ldh;
-        const T* b = w + i * ldw;
-        const bool vec = ((ldh | ldw | D) % EPC == 0) && (((uintptr_t)h | (uintptr_t)w) % 16 == 0);
-        if (vec) {
-            for (int d = lane * EPC; d < D; d += 64 * EPC) {
-                T x[EPC], y[EPC];
-                *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(a + d);
-                *reinterpret_cast<u32x4*>(y) = *reinterpret_cast<const u32x4*>(b + d);
+    const int lane = threadIdx.x & (L - 1), per = 256 / L;
+    const bool vec = ((ldh | ldw | D) % EPC == 0) && (((uintptr_t)h | (uintptr_t)w) % 16 == 0);
+    for (long long b0 = (long long)blockIdx.x * per; b0 < entries; b0 += (long long)gridDim.x * per) {
+        const long long e = b0 + threadIdx.x / L;
+        const long long i = e < entries ? index[e] : -1;
+        const bool there = i >= 0 && i < V;
+        float s = 0.f;
+        if (there) {
+            const T* a = h + e / K * ldh;
+            const T* b = w + i * ldw;
+            if (vec) {
+                for (int d = lane * EPC; d < D; d += L * EPC) {
+                    T x[EPC], y[EPC];
+                    *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(a + d);
+                    *reinterpret_cast<u32x4*>(y) = *reinterpret_cast<const u32x4*>(b + d);
 #pragma unroll
-                for (int q = 0; q < EPC; ++q) s += to_f32(x[q]) * to_f32(y[q]);
-            }
-        } else
-            for (int d = lane; d < D; d += 64) s += to_f32(a[d]) * to_f32(b[d]);
-#pragma unroll
-        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-        if (bias) s += bias[i];
+                    for (int q = 0; q < EPC; ++q) s += to_f32(x[q]) * to_f32(y[q]);
+                }
+            } else
+                for (int d = lane; d < D; d += L) s += to_f32(a[d]) * to_f32(b[d]);
+        }
+        for (int d = L >> 1; d; d >>= 1) s += __shfl_xor(s, d);
+        if (lane == 0 && e < entries) zsel[e] = there && bias ? s + bias[i] : s;
     }
-    if (lane == 0) zsel[e] = s;
 }
 
 struct LinJoin {
@@ -124,11 +129,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
                 if (t < 0 || t >= j.V) { lse = NAN; loss = NAN; }                 // a label that names no class: loud, and not read
                 else { loss = lse - j.zsel[row]; if (loss < 0.f) loss = 0.f; }    // (the two sums are rounded apart: -1e-7 is 0)
                 if (gl == 0 && j.dsel) j.dsel[row] = expm1f(-loss);
-                if (gl == 0 && j.psel) j.psel[row] = 1.f;
-            } else if (in && gl == 0) {
-                if (j.dsel) j.dsel[row] = 0.f;
-                if (j.psel) j.psel[row] = 0.f;
-            }
+            } else if (in && gl == 0 && j.dsel) j.dsel[row] = 0.f;
         } else {
             // teacher: softmax over its entries (those with a class and a logit above -inf)
             float tm = -INFINITY;
@@ -156,14 +157,11 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
                         const float lp = lin_tlog(j, e0 + k) * j.inv_t - tm - lt, p = expf(lp);
                         const float zq = j.zsel[e0 + k] * j.inv_t - lse;
                         if (p > 0.f) loss += p * (lp - zq);
-                        if (j.dsel || j.psel) {
-                            // the same class twice in a row: each entry holds the sum over both, psel keeps it at the first
-                            float all = 0.f;
-                            bool first = true;
-                            for (int q = 0; q < j.K; ++q)
-                                if (j.index[e0 + q] == i) { all += expf(lin_tlog(j, e0 + q) * j.inv_t - tm - lt); first &= q >= k; }
+                        ps = p;
+                        if (j.dsel) {
+                            float all = 0.f;              // the same class twice in a row: each entry holds the sum over both
+                            for (int q = 0; q < j.K; ++q) if (j.index[e0 + q] == i) all += expf(lin_tlog(j, e0 + q) * j.inv_t - tm - lt);
                             ds = expf(zq) - all;
-                            ps = first ? all : 0.f;
                         }
                     }
                 }
@@ -213,19 +211,17 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 
-// dz at the selected classes of the piece [v0, v0 + N): g * (softmax - teacher), from the forward's fp32 values.  Entries that
-// name the same class hold the same value.
+// dz at the selected classes of the piece [v0, v0 + N): softmax - teacher, from the forward's fp32 values.  Entries that name the
+// same class hold the same value.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_scatter_kernel(const long long* __restrict__ index, const float* __restrict__ dsel, int K,
-                                                          const float2* __restrict__ stat, const float* gout, int gstride, const int* count, float t,
-                                                          T* dz, long long lddz, T* dzt, long long lddzt, long long v0, int N, long long entries) {
+                                                          const float2* __restrict__ stat, T* dz, long long lddz, T* dzt, long long lddzt, long long v0, int N, long long entries) {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= entries) return;
     const long long m = e / K, i = index[e] - v0;
     if (i < 0 || i >= N) return;
-    const float gate = stat[m].y;
-    if (gate == 0.f) return;
-    const T v = from_f32<T>(dsel[e] * lin_row_scale(gout, gstride, count, t, gate, m));
+    if (stat[m].y == 0.f) return;
+    const T v = from_f32<T>(dsel[e]);
     dz[m * lddz + i] = v;
     if (dzt) dzt[i * lddzt + m] = v;
 }
@@ -241,25 +237,28 @@ __global__ __launch_bounds__(256) void lin_reduce_kernel(const float* __restrict
     }
 }
 
-// db[v] (+)= sum over row tiles of colsum[tile][v] - sum of g * teacher over the entries that name v.  One workgroup owns 256
-// classes; its waves walk the entries in order and the lane that owns a class adds its hits: the order is fixed.
+// Partial bias gradient of one chunk of LIN_DB_TILES row tiles: sum over its tiles of colsum[tile][v] - sum of g * teacher share over
+// its rows' entries that name v (psel NULL: share 1).  One workgroup owns 256 classes of one chunk; its waves walk the entries in
+// order and the lane that owns a class adds its hits: the order is fixed.
+static constexpr int LIN_DB_TILES = 16;
 __global__ __launch_bounds__(256) void lin_dbias_kernel(const float* __restrict__ colsum, int tiles, long long ldcol, const long long* __restrict__ index,
                                                         const float* __restrict__ psel, int K, const float2* __restrict__ stat, const float* gout,
                                                         int gstride, const int* count, float t, long long v0, int N, long long entries,
-                                                        float* db, int accumulate) {
+                                                        long long chunk, double* out) {
     __shared__ double part[4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = blockIdx.x * 256;
+    const long long ea = blockIdx.y * chunk, eb = ea + chunk < entries ? ea + chunk : entries;
     double acc[4] = {0.0, 0.0, 0.0, 0.0};             // classes b0 + lane + 64 q
-    for (long long e0 = wave * 64; e0 < entries; e0 += 256) {
+    for (long long e0 = ea + wave * 64; e0 < eb; e0 += 256) {
         const long long e = e0 + lane;
-        long long i = e < entries ? index[e] - v0 - b0 : -1;
+        const long long i = e < eb ? index[e] - v0 - b0 : -1;
         float val = 0.f;
         bool hit = i >= 0 && i < 256 && b0 + i < N;
         if (hit) {
             const long long m = e / K;
             const float gate = stat[m].y;
             hit = gate != 0.f;
-            if (hit) val = psel[e] * lin_row_scale(gout, gstride, count, t, gate, m);
+            if (hit) val = (psel ? psel[e] : 1.f) * lin_row_scale(gout, gstride, count, t, gate, m);
         }
         unsigned long long mask = __ballot(hit);
         while (mask) {
@@ -279,9 +278,20 @@ __global__ __launch_bounds__(256) void lin_dbias_kernel(const float* __restrict_
     const int v = b0 + threadIdx.x;
     if (v < N) {
         double s = -(part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]);
-        for (int i = 0; i < tiles; ++i) s += (double)colsum[i * ldcol + v];
-        db[v] = (float)(s + (accumulate ? (double)db[v] : 0.0));
+        const int t1 = min(tiles, ((int)blockIdx.y + 1) * LIN_DB_TILES);
+        for (int i = blockIdx.y * LIN_DB_TILES; i < t1; ++i) s += (double)colsum[i * ldcol + v];
+        out[(long long)blockIdx.y * N + v] = s;
     }
+}
+
+// db[v] (+)= sum over the chunks, in order
+__global__ __launch_bounds__(256) void lin_dbias_join_kernel(const double* __restrict__ part, int chunks, int N, float* db, int accumulate) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= N) return;
+    double s = accumulate ? (double)db[v] : 0.0;
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) s += part[(long long)c * N + v];
+    db[v] = (float)s;
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -355,6 +365,12 @@ static LinBwd lin_bwd_plan(const LinDims& d) {
 struct LinFwdWs { void *hp, *wp; float2* part; float* zsel; double* bsum; int* bcnt; };
 static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFwdWs& w) {
     LinCarve c{base};
+    if (fea_lin_few(d.rows, d.D, d.V)) {
+        w = LinFwdWs{};
+        w.bsum = c.take<double>(fea_lin_few_blocks(d.rows));
+        w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows));
+        return c.at;
+    }
     w.part = c.take<float2>(p.rc * p.ntn);
     w.zsel = c.take<float>(d.rows * d.K);
     w.bsum = c.take<double>(p.blocks);
@@ -364,11 +380,17 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
     return c.at;
 }
 
-struct LinBwdWs { void *hp, *wp, *ht, *wt, *dz, *dzt; float *slab, *acch, *accw, *colsum; };
+struct LinBwdWs { void *hp, *wp, *ht, *wt, *dz, *dzt; float *slab, *acch, *accw, *colsum; double* dbpart; };
 static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* base, LinBwdWs& w) {
     LinCarve c{base};
     const long long vp = up(p.vc, d.epc), rp = up(p.rc, d.epc);
     w = LinBwdWs{};
+    if (fea_lin_few(d.rows, d.D, d.V)) {
+        if (want & 2) w.slab = c.take<float>(fea_lin_few_blocks(d.rows) * 32ll * 64);
+        if (want & 4) w.colsum = c.take<float>(fea_lin_few_blocks(d.rows) * 32ll);
+        w.dz = c.take<char>(256);
+        return c.at;
+    }
     if (d.packed()) { w.hp = c.take<char>(p.rc * d.Dp * d.es); w.wp = c.take<char>((long long)p.vc * d.Dp * d.es); }
     w.dz = c.take<char>(p.rc * vp * d.es);
     if (want & 2) { w.dzt = c.take<char>(p.vc * rp * d.es); w.ht = c.take<char>(d.D * rp * d.es); }
@@ -379,7 +401,7 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     w.slab = c.take<float>(slab);
     if ((want & 1) && p.nvc > 1) w.acch = c.take<float>(p.rc * d.D);
     if ((want & 2) && p.nrc > 1) w.accw = c.take<float>((long long)d.V * d.D);
-    if (want & 4) w.colsum = c.take<float>(p.tiles_c * up(p.vc, 64));
+    if (want & 4) { w.colsum = c.take<float>(p.tiles_c * up(p.vc, 64)); w.dbpart = c.take<double>((p.tiles_c + LIN_DB_TILES - 1) / LIN_DB_TILES * p.vc); }
     return c.at;
 }
 
@@ -400,10 +422,10 @@ static int lin_pack(const LinDims& d, const void* in, long long ld, void* out, l
     return FEA_OK;
 }
 
-static int lin_transpose(const LinDims& d, const void* in, long long ld, void* out, long long ldo, long long R, long long Rpad, const float2* stat, hipStream_t s) {
+static int lin_transpose(const LinDims& d, const void* in, long long ld, void* out, long long ldo, long long R, long long Rpad, const float2* stat, const float* gout, float t, hipStream_t s) {
     const dim3 grid((unsigned)((Rpad + 63) / 64), (unsigned)((d.D + 63) / 64));
-    if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_transpose_kernel<__bf16>, grid, dim3(256), 0, s, (const __bf16*)in, ld, (__bf16*)out, ldo, R, Rpad, d.D, stat);
-    else                     hipLaunchKernelGGL(lin_transpose_kernel<float>, grid, dim3(256), 0, s, (const float*)in, ld, (float*)out, ldo, R, Rpad, d.D, stat);
+    if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_transpose_kernel<__bf16>, grid, dim3(256), 0, s, (const __bf16*)in, ld, (__bf16*)out, ldo, R, Rpad, d.D, stat, gout, t);
+    else                     hipLaunchKernelGGL(lin_transpose_kernel<float>, grid, dim3(256), 0, s, (const float*)in, ld, (float*)out, ldo, R, Rpad, d.D, stat, gout, t);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
@@ -443,17 +465,27 @@ static int lin_forward(const char* who, const LinDims& d, const void* h, long lo
     FEA_CHECK(!loss == !count, FEA_E_BADARG, "%s: loss and count go together", who);
     FEA_CHECK(loss || j.loss_rows, FEA_E_BADARG, "%s: nothing to write", who);
 
-    const long long entries = d.rows * d.K;
-    {
-        const long long blocks = (entries + 3) / 4;
-        FEA_CHECK(blocks <= (1ll << 23) * 64, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld selected entries", who, entries);
-        for (long long b0 = 0; b0 < blocks; b0 += 1 << 22) {
-            const unsigned grid = (unsigned)(blocks - b0 < (1 << 22) ? blocks - b0 : 1 << 22);
-            const long long e0 = b0 * 4;
-            if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, e0);
-            else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, e0);
+    if (fea_lin_few(d.rows, d.D, d.V)) {
+        LinFew f{};
+        f.h = h; f.w = w; f.ldh = ldh; f.ldw = ldw; f.bias = bias; f.index = j.index; f.tlog = j.tlog; f.tdt = j.tdt; f.ignore = j.ignore;
+        f.t = j.t; f.inv_t = j.inv_t; f.stat = j.stat; f.psel = j.psel; f.loss_rows = j.loss_rows;
+        f.bsum = loss ? b.bsum : nullptr; f.bcnt = b.bcnt; f.rows = d.rows; f.D = d.D; f.V = d.V; f.K = d.K;
+        LIN_TRY(fea_lin_few_fwd(f, d.dtype, s));
+        if (loss) {
+            hipLaunchKernelGGL(lin_total_kernel, dim3(1), dim3(1024), 0, s, (const double*)b.bsum, (const int*)b.bcnt, (long long)fea_lin_few_blocks(d.rows), mean, loss, count);
             FEA_LAUNCH_CHECK();
         }
+        return FEA_OK;
+    }
+    const long long entries = d.rows * d.K;
+    {
+        int lanes = 1;
+        while (lanes < 64 && lanes * d.epc < d.D) lanes *= 2;
+        const long long blocks = (entries * lanes + 255) / 256;
+        const unsigned grid = (unsigned)(blocks < 1 << 16 ? blocks : 1 << 16);
+        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes);
+        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes);
+        FEA_LAUNCH_CHECK();
     }
     const void* wm = w;
     long long ldwm = ldw;
@@ -490,12 +522,12 @@ static int lin_forward(const char* who, const LinDims& d, const void* h, long lo
 }
 
 extern "C" int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
-                                 long long ignore_index, float* stat, float* dsel, float* psel, float* loss_rows, float* loss, int* count, int mean,
+                                 long long ignore_index, float* stat, float* dsel, float* loss_rows, float* loss, int* count, int mean,
                                  void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream) {
     FEA_CHECK(target, FEA_E_BADARG, "fea_linear_ce_fwd: null target");
     LinJoin j{};
     j.index = target; j.ignore = ignore_index; j.t = j.inv_t = 1.f;
-    j.stat = (float2*)stat; j.dsel = dsel; j.psel = psel; j.loss_rows = loss_rows;
+    j.stat = (float2*)stat; j.dsel = dsel; j.loss_rows = loss_rows;
     return lin_forward("fea_linear_ce_fwd", lin_dims(rows, D, V, 1, dtype), h, ldh, w, ldw, bias, j, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
 }
 
@@ -523,7 +555,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     FEA_CHECK(index && stat && dsel && gout, FEA_E_BADARG, "%s: null operand", who);
     FEA_CHECK(gout_stride == 0 || gout_stride == 1, FEA_E_BADARG, "%s: gout_stride %d", who, gout_stride);
     FEA_CHECK(dh || dw || db, FEA_E_BADARG, "%s: no gradient asked for", who);
-    FEA_CHECK(!db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
+    FEA_CHECK(K == 1 || !db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
     FEA_CHECK(temperature > 0.f && isfinite(temperature) && isfinite(1.f / temperature), FEA_E_BADARG, "%s: temperature %g", who, (double)temperature);
     const int want = (dh ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0);
     const LinBwd p = lin_bwd_plan(d);
@@ -531,6 +563,13 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     const size_t need = lin_bwd_carve(d, p, want, (char*)ws, b);
     FEA_CHECK(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, FEA_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, need, ws_bytes);
 
+    if (fea_lin_few(rows, D, V)) {
+        LinFew f{};
+        f.h = h; f.w = w; f.ldh = ldh; f.ldw = ldw; f.bias = bias; f.index = index; f.t = temperature; f.inv_t = 1.f / temperature;
+        f.stat = (float2*)stat; f.psel = (float*)psel; f.gout = gout; f.gstride = gout_stride; f.count = count;
+        f.dh = dh; f.slab = b.slab; f.dbslab = b.colsum; f.rows = rows; f.D = D; f.V = V; f.K = K;
+        return fea_lin_few_bwd(f, dtype, dw, db, s);
+    }
     const int ck = dtype == FEA_BF16 ? 64 : 32;
     for (int ir = 0; ir < p.nrc; ++ir) {
         const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc, np = up(n, d.epc);
@@ -540,7 +579,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
         const void* hm = hr;
         long long ldhm = ldh;
         if (d.packed()) { LIN_TRY(lin_pack(d, hr, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
-        if (dw) LIN_TRY(lin_transpose(d, hr, ldh, b.ht, np, n, np, st, s));
+        if (dw) LIN_TRY(lin_transpose(d, hr, ldh, b.ht, np, n, np, st, gout_stride ? go : nullptr, temperature, s));
         for (int iv = 0; iv < p.nvc; ++iv) {
             const long long v0 = (long long)iv * p.vc;
             const int nv = (int)(V - v0 < p.vc ? V - v0 : p.vc), nvp = (int)up(nv, d.epc);
@@ -558,18 +597,21 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
             const unsigned sg = (unsigned)((entries + 255) / 256);
-            if (dtype == FEA_BF16) hipLaunchKernelGGL(lin_scatter_kernel<__bf16>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, go, gout_stride, count, temperature, (__bf16*)b.dz, (long long)nvp, (__bf16*)g.dzt, np, v0, nv, entries);
-            else                   hipLaunchKernelGGL(lin_scatter_kernel<float>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, go, gout_stride, count, temperature, (float*)b.dz, (long long)nvp, (float*)g.dzt, np, v0, nv, entries);
+            if (dtype == FEA_BF16) hipLaunchKernelGGL(lin_scatter_kernel<__bf16>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, (long long)nvp, (__bf16*)g.dzt, np, v0, nv, entries);
+            else                   hipLaunchKernelGGL(lin_scatter_kernel<float>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, (long long)nvp, (float*)g.dzt, np, v0, nv, entries);
             FEA_LAUNCH_CHECK();
             if (db) {
-                const int tiles = (int)((n + fea_lin_tile_m(dtype, 0) - 1) / fea_lin_tile_m(dtype, 0));
-                hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel + r0 * K, K, st, go, gout_stride, count, temperature, v0, nv, entries, db + v0, ir > 0 ? 1 : 0);
+                const int tm = fea_lin_tile_m(dtype, 0), tiles = (int)((n + tm - 1) / tm), chunks = (tiles + LIN_DB_TILES - 1) / LIN_DB_TILES;
+                hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(256), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, (long long)LIN_DB_TILES * tm * K, b.dbpart);
+                FEA_LAUNCH_CHECK();
+                hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);
                 FEA_LAUNCH_CHECK();
             }
             if (dh) {
-                LIN_TRY(lin_transpose(d, wr, ldw, b.wt, nvp, nv, nvp, nullptr, s));
+                LIN_TRY(lin_transpose(d, wr, ldw, b.wt, nvp, nv, nvp, nullptr, nullptr, 1.f, s));
                 LinGemm m{};
                 m.a = b.dz; m.lda = nvp; m.b = b.wt; m.ldb = nvp; m.M = (int)n; m.N = D; m.K = nvp;
+                m.scale = 1; m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
                 void* out = (char*)dh + r0 * D * d.es;
                 const bool direct = p.sh == 1 && p.nvc == 1;
                 m.splits = p.sh; m.kper = (int)up((nvp + p.sh - 1) / p.sh, ck);
@@ -580,6 +622,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             if (dw) {
                 LinGemm m{};
                 m.a = b.dzt; m.lda = np; m.b = b.ht; m.ldb = np; m.M = nv; m.N = D; m.K = (int)np;
+                m.scale = gout_stride ? 0 : 2; m.gout = go; m.count = count; m.t = temperature;
                 void* out = (char*)dw + v0 * D * d.es;
                 float* acc = b.accw ? b.accw + v0 * D : nullptr;
                 const bool direct = p.sw == 1 && p.nrc == 1;

@@ -129,18 +129,18 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     f32 = {"dtype": torch.float32, "device": dev}
     stat = torch.empty((rows, 2), **f32) if grads else None
     dsel = torch.empty((rows, k), **f32) if grads else None
-    psel = torch.empty((rows, k), **f32) if grads & 4 else None
+    psel = torch.empty((rows, k), **f32) if grads and tlog is not None else None
     rowloss = torch.empty(rows, **f32) if reduction == "none" else None
     loss = torch.empty((), **f32) if reduction != "none" else None
     count = torch.empty((), dtype=torch.int32, device=dev) if reduction != "none" else None
     n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    tail = (stat, dsel, psel, rowloss, loss, count, int(reduction == "mean"), ws, n, rows, d, v, dt, L.stream_ptr())
+    tail = (rowloss, loss, count, int(reduction == "mean"), ws, n, rows, d, v, dt, L.stream_ptr())
     if tlog is None:
-        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, *tail)
+        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, *tail)
     else:
         tl = tlog.detach().contiguous()
-        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, *tail)
+        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, *tail)
     return (loss if rowloss is None else rowloss.view(index.shape if tlog is None else index.shape[:-1])), (h, w, b, ix, stat, dsel, psel, count)
 
 

@@ -355,9 +355,9 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * A row that does not count has loss 0 and gradients 0 whatever its hidden state holds.  A target outside [0, V), an index >= V, a
  * teacher logit that is NaN or +inf: the row's loss and the gradients it reaches are NaN (nothing is read out of range).
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
- * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce), and psel[rows][K]
- * if the bias gradient is wanted (all nullable).
- *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1): recomputes the logits in pieces of the
+ * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
+ * psel[rows][K] (all nullable).
+ *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): recomputes the logits in pieces of the
  *     classes and writes dh[rows][D], dw[V][D] (contiguous, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
  *     value (gout_stride 0) or one per row (1); count: divide it by count[0] (mean) or NULL.
  * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are copied into the workspace.
@@ -365,7 +365,7 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * (0 bytes = sizes that are refused).  Results are the same from run to run. */
 size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);
 int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
-                      long long ignore_index, float* stat, float* dsel, float* psel, float* loss_rows, float* loss, int* count, int mean,
+                      long long ignore_index, float* stat, float* dsel, float* loss_rows, float* loss, int* count, int mean,
                       void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
 int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const void* teacher_logits,
                       int teacher_dtype, const long long* teacher_index, int K, float temperature, float* stat, float* dsel, float* psel,

@@ -3,7 +3,10 @@
 u = torch.finfo(dtype).eps / 2 (a rounding to the storage type), e = 2^-24 (a rounding in 32 bits), with B = max_v sum_d |h_d w_d| + |b_v|:
   a logit is off by dz <= (D + 4) e B / T (D products and sums, bias, scale), an exponential by 3 e more and e |z - lse| for its argument;
   log-sum-exp by the largest of these and the sum's (16 + V / 64) e;  so a loss by 2 of them, a softmax value q by the same relative to q.
-  dz = g (q - p) is rounded once to the storage type; dh and dw add the products' fp32 sums and one rounding to the storage type."""
+  dz = g (q - p) is rounded once to the storage type; dh and dw add the products' fp32 sums and one rounding to the storage type.
+  Where every row has its own upstream gradient, dw's product takes rnd(q - p) and rnd(g h), two operands rounded once each:
+  |rnd(x) rnd(y) - x y| <= (2 u + u^2) |x y|, so its terms |dz| |h| are off by u (1 + u) more than with one upstream gradient
+  (which meets the fp32 sum). """
 import torch
 
 E = 2.0 ** -24
@@ -74,7 +77,8 @@ def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, redu
     off = g.abs()[:, None] * (q * 2 * dz_log[:, None] + (8 + (0 if tlog is None else index.shape[-1])) * E * (p + q)) + u * dz.abs() + 2 * E * dz.abs()
     dh, dw = dz @ wd, dz.T @ hd
     out["hidden"] = (dh, off @ wd.abs() + (v + 8) * E * (dz.abs() @ wd.abs()) + u * dh.abs() + 1e-37)
-    out["weight"] = (dw, off.T @ hd.abs() + (rows + 8) * E * (dz.abs().T @ hd.abs()) + u * dw.abs() + 1e-37)
+    own = u * (1 + u) if reduction == "none" else 0.0
+    out["weight"] = (dw, off.T @ hd.abs() + own * (dz.abs().T @ hd.abs()) + (rows + 8) * E * (dz.abs().T @ hd.abs()) + u * dw.abs() + 1e-37)
     offb = g.abs()[:, None] * (q * 2 * dz_log[:, None] + 8 * E * (p + q)) + 4 * E * g.abs()[:, None] * (q + p)
     out["bias"] = (dz.sum(0), offb.sum(0) + 20 * E * (g.abs()[:, None] * (q + p)).sum(0) + 1e-37)
     return out

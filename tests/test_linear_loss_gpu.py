@@ -9,8 +9,8 @@ from tests import linear_loss_oracle as O
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 TYPES = [torch.float32, torch.bfloat16]
-SHAPES = [(1, 8, 1), (1, 1, 2), (1, 64, 600), (2, 5, 7), (3, 64, 6), (17, 33, 129), (64, 128, 128), (129, 72, 1000), (257, 200, 333),
-          (300, 96, 5003), (513, 640, 1537), (5000, 64, 6), (4097, 24, 33)]
+SHAPES = [(1, 8, 1), (1, 1, 2), (1, 64, 600), (2, 5, 7), (3, 64, 6), (17, 33, 129), (64, 128, 128), (129, 72, 1000), (5000, 72, 40), (257, 200, 333),
+          (300, 96, 5003), (513, 640, 1537), (5000, 64, 6), (4097, 24, 33), (4096, 64, 32), (4100, 33, 13), (6001, 16, 2), (4111, 40, 24), (5003, 7, 1)]
 
 
 def _leaf(t):
@@ -51,9 +51,10 @@ def test_distillation(shape, dtype, top):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", ["sum", "none"])
 @pytest.mark.parametrize("top", [0, 3])
-def test_reductions(dtype, reduction, top):
-    c = O.case(77, 40, 300, dtype, seed=5, top=top, ignored=0.2, bias=True)
-    gout = torch.randn(77, generator=torch.Generator().manual_seed(1)) if reduction == "none" else torch.tensor(-3.0)
+@pytest.mark.parametrize("shape", [(77, 40, 300), (4500, 24, 11)])
+def test_reductions(shape, dtype, reduction, top):
+    c = O.case(*shape, dtype, seed=5, top=top, ignored=0.2, bias=True)
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(1)) if reduction == "none" else torch.tensor(-3.0)
     kw = {"temperature": 0.5} if top else {}
     _compare(_run(*c, gout=gout, reduction=reduction, **kw), O.evaluate(*c, gout=gout, reduction=reduction, **kw))
 
@@ -69,26 +70,28 @@ def test_pieces(shape, dtype, top, monkeypatch):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_nothing_counts(dtype):
-    h, w, b, t = O.case(9, 16, 50, dtype, bias=True)
+@pytest.mark.parametrize("rows", [9, 4100])
+def test_nothing_counts(dtype, rows):
+    h, w, b, t = O.case(rows, 16, 20, dtype, bias=True)
     got = _run(h, w, b, torch.full_like(t, -100))
     assert all(float(v.detach().abs().max()) == 0.0 for v in got.values())
-    i = torch.full((9, 3), -1)
-    got = _run(h, w, b, i, torch.zeros(9, 3, dtype=dtype))
+    i = torch.full((rows, 3), -1)
+    got = _run(h, w, b, i, torch.zeros(rows, 3, dtype=dtype))
     assert all(float(v.detach().abs().max()) == 0.0 for v in got.values())
-    got = _run(h, w, b, torch.zeros(9, 3, dtype=torch.int64), torch.full((9, 3), -torch.inf, dtype=dtype))
+    got = _run(h, w, b, torch.zeros(rows, 3, dtype=torch.int64), torch.full((rows, 3), -torch.inf, dtype=dtype))
     assert all(float(v.detach().abs().max()) == 0.0 for v in got.values())
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("top", [0, 3])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_ignored_rows_may_hold_anything(dtype, top, bad):
+@pytest.mark.parametrize("shape", [(70, 64, 200), (4200, 64, 7)])
+def test_ignored_rows_may_hold_anything(shape, dtype, top, bad):
     """The hidden state of a row that does not count reaches neither the loss nor any gradient."""
-    c = list(O.case(70, 64, 200, dtype, seed=3, top=top, ignored=0.4, bias=True))
+    c = list(O.case(*shape, dtype, seed=3, top=top, ignored=0.4, bias=True))
     want = O.evaluate(*c)
     gone = c[3] == -100 if not top else (c[3] < 0).all(1)
-    assert 5 < int(gone.sum()) < 65
+    assert 5 < int(gone.sum()) < shape[0] - 5
     c[0] = c[0].clone()
     c[0][gone] = bad
     _compare(_run(*c), want)
@@ -104,6 +107,12 @@ def test_masked_classes(dtype):
     got = _run(h, w, b, t)
     _compare(got, O.evaluate(h, w, b, t))
     assert float(got["weight"][100:228].abs().max()) == 0.0 and float(got["bias"][256:384].abs().max()) == 0.0
+    h, w, b, t = O.case(4100, 48, 9, dtype, seed=4, bias=True)
+    b[3], b[8] = -torch.inf, torch.finfo(torch.float32).min
+    t = t % 3
+    got = _run(h, w, b, t)
+    _compare(got, O.evaluate(h, w, b, t))
+    assert float(got["weight"][3].abs().max()) == 0.0 and float(got["bias"][8]) == 0.0
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -114,19 +123,21 @@ def test_teacher_minus_infinity_is_no_share(dtype):
     _compare(_run(h, w, b, i, a), O.evaluate(h, w, b, i, a))
 
 
-def test_a_label_that_names_no_class_is_nan():
-    h, w, b, t = O.case(10, 32, 20, torch.float32, seed=7)
+@pytest.mark.parametrize("rows", [10, 4100])
+def test_a_label_that_names_no_class_is_nan(rows):
+    h, w, b, t = O.case(rows, 32, 20, torch.float32, seed=7)
     for bad in (20, 1 << 40, -5):
         x = t.clone()
         x[4] = bad
         loss = F.linear_cross_entropy(h.to(DEV), w.to(DEV), x.to(DEV), reduction="none")
         want = O.evaluate(h, w, b, t, reduction="none")["loss"][0]
-        assert torch.isnan(loss[4]) and torch.allclose(loss.cpu().double()[torch.arange(10) != 4], want[torch.arange(10) != 4], rtol=1e-5)
-    h, w, b, i, a = O.case(10, 32, 20, torch.float32, seed=7, top=3)
+        rest = torch.arange(rows) != 4
+        assert torch.isnan(loss[4]) and torch.allclose(loss.cpu().double()[rest], want[rest], rtol=1e-5)
+    h, w, b, i, a = O.case(rows, 32, 20, torch.float32, seed=7, top=3)
     i[2, 1] = 20
     a[5, 0] = torch.nan
     a[6, 2] = torch.inf
-    got = _run(h, w, b, i, a, reduction="none", gout=torch.ones(10))
+    got = _run(h, w, b, i, a, reduction="none", gout=torch.ones(rows))
     assert torch.isnan(got["loss"]).nonzero().flatten().tolist() == [2, 5, 6]
     assert torch.isnan(got["hidden"]).all(1).nonzero().flatten().tolist() == [2, 5, 6]
 
@@ -186,7 +197,7 @@ def test_bf16_bias_and_empty_batch():
     e, w = _leaf(h[:0]), _leaf(w)
     for loss in (F.linear_cross_entropy(e, w, t[:0].to(DEV)), F.linear_distillation(e, w, h[:0, :4].to(DEV), t[:0, None].expand(0, 4).to(DEV))):
         gh, gw = torch.autograd.grad(loss, [e, w])
-        assert float(loss) == 0.0 and gh.shape == (0, 32) and float(gw.abs().max()) == 0.0
+        assert float(loss.detach()) == 0.0 and gh.shape == (0, 32) and float(gw.abs().max()) == 0.0
     assert F.linear_cross_entropy(e, w, t[:0].to(DEV), reduction="none").shape == (0,)
 
 
@@ -316,7 +327,7 @@ def test_workspace_and_operands_are_checked():
     out = torch.empty(16, device=DEV)
 
     def fwd(h=h, ldh=32, ws=ws, n=n, rows=16, d=32, v=40, dt=L.F32):
-        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, None, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
+        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
     fwd()
     for bad in ({"n": n - 1}, {"ws": None}, {"ldh": 31}, {"ldh": 33}, {"h": None}, {"dt": 7}, {"rows": 0}, {"v": 0}, {"d": 0}, {"h": h.data_ptr() + 4},
                 {"ws": ws.data_ptr() + 16}, {"d": 1 << 17, "ldh": 1 << 17}):
