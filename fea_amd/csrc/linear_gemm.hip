@@ -200,8 +200,25 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     }
 }
 
-int fea_lin_tile_m(int, int) { return LG_T; }
-int fea_lin_tile_n(int, int) { return LG_T; }
+// Tile and split of a product: the one whose modelled time is least, from the rates that the two kernels reach on full chips.  Both
+// take whole rounds of the chip (256 workgroups of the large tile, 512 of the small one); the parts of a split reduction are written
+// and read once more, at least 512 (bf16) or 256 (fp32) channels each.
+LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split) {
+    LinTile best{128, 1};
+    double least = 1e30;
+    for (int tile = 128; tile <= (dtype == FEA_BF16 ? 256 : 128); tile += 128) {
+        const double slots = tile == 256 ? 256 : 512;
+        const double rate = dtype == FEA_F32 ? 100e12 : tile == 256 ? 1300e12 : 700e12;
+        const long long tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
+        for (int sp = 1; sp <= (split ? 32 : 1); ++sp) {
+            if (sp > 1 && K / sp < (dtype == FEA_F32 ? 256 : 512)) break;
+            const double rounds = (double)((tiles * sp + (long long)slots - 1) / (long long)slots);
+            const double t = rounds * (2.0 * tile * tile * ((double)K / sp + 128) / (rate / slots)) + (sp > 1 ? 2.0 * sp * M * N * 4 / 4e12 + 3e-6 : 0.0);
+            if (t < least * 0.999) { least = t; best = LinTile{tile, sp}; }
+        }
+    }
+    return best;
+}
 
 template <typename T> static void lin_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
     if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE>), dim3(grid), dim3(256), 0, s, g);
@@ -209,16 +226,18 @@ template <typename T> static void lin_launch(int epi, const LinGemm& g, unsigned
     else                    hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE>), dim3(grid), dim3(256), 0, s, g);
 }
 
-int fea_lin_gemm(int epi, int dtype, LinGemm g, hipStream_t s) {
+int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     const int epc = dtype == FEA_BF16 ? 8 : 4;
     FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && g.lda >= g.K && g.ldb >= g.K
               && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0, FEA_E_BADARG, "lin_gemm: operands %d x %d x %d not aligned", g.M, g.N, g.K);
-    g.ntm = (g.M + LG_T - 1) / LG_T; g.ntn = (g.N + LG_T - 1) / LG_T;
+    FEA_CHECK(tile == 128 || (dtype == FEA_BF16 && g.lda < (1 << 21) && g.ldb < (1 << 21)), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
+    g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
     const long long grid = (long long)g.ntm * g.ntn * g.splits;
     FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
-    if (dtype == FEA_BF16) lin_launch<__bf16>(epi, g, (unsigned)grid, s);
-    else                   lin_launch<float>(epi, g, (unsigned)grid, s);
+    if (tile == 256)            fea_lin_gemm256(epi, g, (unsigned)grid, s);
+    else if (dtype == FEA_BF16) lin_launch<__bf16>(epi, g, (unsigned)grid, s);
+    else                        lin_launch<float>(epi, g, (unsigned)grid, s);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }

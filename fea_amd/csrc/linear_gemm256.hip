@@ -1,0 +1,271 @@
+// The product of the many-class loss heads for large bf16 operands: 256 x 256 tiles, with the epilogues of linear_gemm.hip.
+//
+// A tile of T x T takes T T / (2 T) = T / 2 multiply-adds per operand element it reads: at 256 a CU at full matrix rate asks for
+// 32 B per cycle from L2 (128: 64 B, twice what L2 gives) and for 64 KB of LDS reads per 32-channel step of 1,024 cycles.  Four waves of
+// 128 x 128 read each operand twice (8 fragments of each per step and wave: half the LDS rate); eight waves of 128 x 64 would read
+// 96 KB, with the fill the whole LDS rate.  So: one workgroup of 4 waves per CU, one wave per SIMD, 8 x 8 accumulators of
+// v_mfma_f32_16x16x32_bf16 in the 256 accumulation registers, the rest in the other 256.
+//
+// Reduction in chunks of 64 channels (whole 128-byte lines), two LDS stages.  In the first half of chunk c every fourth MFMA is
+// followed by one fragment read (second half of c), one LDS write of chunk c + 1 from the registers and one load of chunk c + 2 into
+// the registers just freed; one barrier; in the second half the fragments of chunk c + 1 are read.  Loads are buffer loads with
+// every bound in the lane's offset, so rows, classes and channels behind the end arrive as zeros without a branch.
+#include "linear_loss.h"
+
+static constexpr int LB_T = 256, LB_OP = LB_T * 128, LB_STAGE = 2 * LB_OP;
+
+// XOR of a 128-byte row's 16-byte chunk index: conflict-free ds_read_b128 of 16 rows x 4 chunks
+__device__ __forceinline__ int lb_swz(int row) { return ((row >> 1) & 3) << 1; }
+
+__device__ __forceinline__ uint32_t lb_pack(float a, float b) {
+    typedef __attribute__((ext_vector_type(2))) float f2;
+    typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, b2));
+}
+
+template <int EPI>
+__global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
+    __shared__ __attribute__((aligned(128))) char smem[2 * LB_STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave & 1, wn = wave >> 1, r16 = lane & 15, q16 = lane >> 4;
+    // tiles in groups of 8 row tiles, walked along the classes: the 32 tiles that an XCD has in flight are 8 x 4
+    constexpr int GM = 8;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int per = g.ntm * g.ntn, sp = id / per, it = id - sp * per;
+    const int grp = it / (GM * g.ntn), gm = min(GM, g.ntm - grp * GM), in = it - grp * GM * g.ntn;
+    const int tm = grp * GM + in % gm, tn = in / gm;
+    const int m0 = tm * LB_T, n0 = tn * LB_T;
+    const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, K = max((EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K) - k0, 0);
+    const int nc = (K + 63) >> 6;
+
+    const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.a + m0 * g.lda + k0), 0,
+        K ? (int)(((min(LB_T, g.M - m0) - 1) * g.lda + K) * 2) : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.b + n0 * g.ldb + k0), 0,
+        K ? (int)(((min(LB_T, g.N - n0) - 1) * g.ldb + K) * 2) : 0, 0x00020000);
+
+    // staging: thread -> rows r + 32 i of either operand, 16-byte chunk c
+    const int r = tid >> 3, c = tid & 7;
+    const unsigned va = (unsigned)(r * (int)g.lda * 2 + c * 16), vb = (unsigned)(r * (int)g.ldb * 2 + c * 16);
+    const unsigned sa = 64 * (unsigned)g.lda, sb = 64 * (unsigned)g.ldb;
+    const int wofs = r * 128 + ((c ^ lb_swz(r)) << 4);
+    u32x4 st[16];
+    auto gload = [&](int ch, int i) {
+        const bool kin = ch * 64 + c * 8 < K;
+        if (i < 8) st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ch * 128 + i * sa : 0x7fffff00u, 0, 0));
+        else       st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + ch * 128 + (i - 8) * sb : 0x7fffff00u, 0, 0));
+    };
+    auto lput = [&](int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i >> 3) * LB_OP + wofs + (i & 7) * 32 * 128) = st[i]; };
+
+    const int fofs0 = r16 * 128 + ((q16 ^ lb_swz(r16)) << 4), fofs1 = fofs0 ^ 64;
+    const int fa = wm * 128 * 128, fb = LB_OP + wn * 128 * 128;
+    u32x4 A[2][8], B[2][8];
+    auto frd = [&](int stage, int ks, int i) {
+        const char* p = smem + stage * LB_STAGE + (ks ? fofs1 : fofs0) + (i & 7) * 16 * 128;
+        if (i < 8) A[ks][i] = *reinterpret_cast<const u32x4*>(p + fa);
+        else       B[ks][i - 8] = *reinterpret_cast<const u32x4*>(p + fb);
+    };
+    f32x4 acc[8][8];                  // [label tile][class tile]: lane = label r16 of the tile, registers = classes 4 q16 .. + 3
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto mma = [&](int ks) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
+    };
+
+#pragma unroll
+    for (int i = 0; i < 16; ++i) gload(0, i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lput(0, i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) gload(1, i);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) frd(0, 0, i);
+
+    for (int ch = 0; ch < nc; ++ch) {
+        const int s = ch & 1;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { frd(s, 1, i); lput(s ^ 1, i); gload(ch + 2, i); }
+        mma(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {        // 2 MFMA, LDS read, MFMA, LDS write, MFMA, load
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // chunk c + 1 is in LDS and nobody reads this stage's first half or the other stage any more
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) frd(s ^ 1, 0, i);
+        mma(1);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    }
+    __syncthreads();
+
+    auto mrow = [&](int i) { return m0 + wm * 128 + i * 16 + r16; };
+    auto ncol = [&](int j) { return n0 + wn * 128 + j * 16 + 4 * q16; };
+    // two class tiles 2 p, 2 p + 1 of one label: after the exchange between neighbouring 16-lane rows a lane holds 8 consecutive
+    // classes, starting at
+    const int pcol = n0 + wn * 128 + (q16 & 1) * 16 + (q16 >> 1) * 8;
+    auto pair = [&](const f32x4& x, const f32x4& y) {
+        const auto r0 = __builtin_amdgcn_permlane16_swap(lb_pack(x[0], x[1]), lb_pack(y[0], y[1]), false, false);
+        const auto r1 = __builtin_amdgcn_permlane16_swap(lb_pack(x[2], x[3]), lb_pack(y[2], y[3]), false, false);
+        return u32x4{r0[0], r1[0], r0[1], r1[1]};
+    };
+
+    if constexpr (EPI == LIN_STORE) {
+        const float common = g.scale == 2 ? lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0) : 1.f;
+        const bool wide = g.slab ? g.N % 4 == 0 : g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int m = mrow(i);
+            const float sc = g.scale == 1 ? (m < g.M ? lin_row_scale(g.gout, g.gstride, g.count, g.t, g.stat[m].y, m) : 0.f) : common;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[i][j] *= sc;
+            if (g.slab) {
+                float* const o = g.slab + ((long long)sp * g.M + m) * g.N;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int n = ncol(j);
+                    if (wide) { if (m < g.M && n < g.N) *reinterpret_cast<f32x4*>(o + n) = acc[i][j]; }
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) if (m < g.M && n + e < g.N) o[n + e] = acc[i][j][e];
+                }
+            } else {
+                __bf16* const o = (__bf16*)g.out + m * g.ldo;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    if (wide) {
+                        const u32x4 v = pair(acc[i][2 * p], acc[i][2 * p + 1]);
+                        if (m < g.M && pcol + 32 * p < g.N) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
+                    } else
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int n = ncol(2 * p + (e >> 2)) + (e & 3);
+                            if (m < g.M && n < g.N) o[n] = (__bf16)acc[i][2 * p + (e >> 2)][e & 3];
+                        }
+                }
+            }
+        }
+    } else {
+        // z in place; classes behind the last are -inf
+        const bool edge = n0 + LB_T > g.N;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = ncol(j) + e;
+                const float b = g.bias && n < g.N ? g.bias[n] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i][j][e] = edge && n >= g.N ? -INFINITY : (acc[i][j][e] + b) * g.inv_t;
+            }
+    }
+
+    if constexpr (EPI == LIN_LSE) {
+        float2* const red = reinterpret_cast<float2*>(smem);       // [wn][256 labels]
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx = fmaxf(fmaxf(mx, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float base = mx == -INFINITY ? 0.f : mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += __expf(acc[i][j][e] - base);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (q16 == 0) red[wn * LB_T + wm * 128 + i * 16 + r16] = make_float2(mx, sum);
+        }
+        __syncthreads();
+        if (m0 + tid < g.M) {
+            const float2 p = red[tid], q = red[LB_T + tid];
+            const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
+            g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, p.y * __expf(p.x - base) + q.y * __expf(q.x - base));
+        }
+    }
+
+    if constexpr (EPI == LIN_DZ) {
+        float sc[8];
+        const bool odd = lane & 1;
+        const int tcol = 2 * (lane & 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int m = mrow(i);
+            const float2 s2 = m < g.M ? g.stat[m] : make_float2(0.f, 0.f);
+            const bool dead = s2.y == 0.f;
+            sc[i] = dead || !g.colsum ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, s2.y, m);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float q = __expf(acc[i][j][e] - s2.x);
+                    acc[i][j][e] = dead || (n0 + LB_T > g.N && ncol(j) + e >= g.N) ? 0.f : q;
+                }
+            __bf16* const o = (__bf16*)g.dz + m * g.lddz;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const u32x4 v = pair(acc[i][2 * p], acc[i][2 * p + 1]);
+                if (m < g.M && pcol + 32 * p < g.Npad) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
+            }
+            if (g.dzt) {
+                // neighbouring lanes hold neighbouring labels: they trade halves, so that each has 2 labels of 2 classes
+                const int me = m & ~1;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t d0 = lb_pack(acc[i][j][0], acc[i][j][1]), d1 = lb_pack(acc[i][j][2], acc[i][j][3]);
+                    const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? d0 : d1), 0xb1, 0xf, 0xf, false);
+                    const uint32_t lo = odd ? t : d0, hi = odd ? d1 : t;          // label me, me + 1 of classes ncol + tcol, + 1
+                    const uint32_t c0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u), c1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                    const int n = ncol(j) + tcol;
+                    if (me < g.Mpad) {
+                        if (n < g.N) *reinterpret_cast<uint32_t*>((__bf16*)g.dzt + n * g.lddzt + me) = c0;
+                        if (n + 1 < g.N) *reinterpret_cast<uint32_t*>((__bf16*)g.dzt + (n + 1) * g.lddzt + me) = c1;
+                    }
+                }
+            }
+        }
+        if (g.colsum) {
+            float* const red = reinterpret_cast<float*>(smem);     // [wm][256 classes]
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s += acc[i][j][e] * sc[i];
+#pragma unroll
+                    for (int d = 8; d; d >>= 1) s += __shfl_xor(s, d);
+                    if (r16 == 0) red[wm * LB_T + ncol(j) + e - n0] = s;
+                }
+            __syncthreads();
+            if (n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LB_T + tid];
+        }
+    }
+}
+
+void fea_lin_gemm256(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE>), dim3(grid), dim3(256), 0, s, g);
+    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ>), dim3(grid), dim3(256), 0, s, g);
+    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE>), dim3(grid), dim3(256), 0, s, g);
+}

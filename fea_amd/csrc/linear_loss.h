@@ -63,7 +63,9 @@ int fea_lin_few_blocks(long long rows);
 int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s);
 int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 
-// linear_gemm.hip
-int fea_lin_gemm(int epi, int dtype, LinGemm g, hipStream_t s);
-int fea_lin_tile_m(int dtype, int M);       // rows of A / B per tile of the product (heights of `colsum`, `part`)
-int fea_lin_tile_n(int dtype, int M);
+// linear_gemm.hip: which tile a product takes (256: linear_gemm256.hip, 128: linear_gemm.hip) and into how many parts its reduction is split
+struct LinTile { int tile, splits; };
+LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split);
+int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s);
+// linear_gemm256.hip
+void fea_lin_gemm256(int epi, const LinGemm& g, unsigned grid, hipStream_t s);

@@ -308,22 +308,25 @@ struct LinDims {
     long long rows; int D, V, K, dtype, es, epc;
     int Dp;                       // D rounded up to 16 bytes: operands with another D are copied with zeros behind it
     bool packed() const { return Dp != D; }
+    bool wide;                    // row strides of 2^21 elements or more (a slice of something very wide): the 128 tile, which has 64-bit offsets
 };
 
 static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
-    LinDims d{rows, D, V, K, dtype, dtype == FEA_BF16 ? 2 : 4, dtype == FEA_BF16 ? 8 : 4, 0};
+    LinDims d{rows, D, V, K, dtype, dtype == FEA_BF16 ? 2 : 4, dtype == FEA_BF16 ? 8 : 4, 0, false};
     d.Dp = (int)up(D, d.epc);
     return d;
 }
 
 // Forward: rows in chunks that bound the partial table to 128 MB.
-struct LinFwd { long long rc; int ntn, G; long long blocks; };
+struct LinFwd { long long rc; int tile, ntn, G; long long blocks; };
 static LinFwd lin_fwd_plan(const LinDims& d) {
     LinFwd p;
-    p.ntn = (d.V + fea_lin_tile_n(d.dtype, 0) - 1) / fea_lin_tile_n(d.dtype, 0);
-    const long long cap = (1ll << 24) / p.ntn;
-    p.rc = cap < 128 ? 128 : cap / 128 * 128;
+    const long long cap = (1ll << 24) / ((d.V + 127) / 128);
+    p.rc = cap < 256 ? 256 : cap / 256 * 256;
     if (p.rc > d.rows) p.rc = d.rows;
+    p.tile = fea_lin_tile(d.dtype, p.rc, d.V, d.Dp, false).tile;
+    if (d.wide) p.tile = 128;
+    p.ntn = (d.V + p.tile - 1) / p.tile;
     p.G = 1;
     while (p.G < 64 && (p.G < p.ntn || p.G < d.K)) p.G *= 2;
     p.blocks = (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
@@ -337,28 +340,20 @@ static long long lin_piece() {
     const long long v = e ? atoll(e) : 0;
     return v >= 1 << 14 && v < 1 << 28 ? v : 1ll << 28;
 }
-struct LinBwd { long long rc; int vc, nrc, nvc, sh, sw; long long tiles_c; };
-static int lin_splits(long long tiles, long long K, int ck) {
-    // a product with fewer tiles than the chip has workgroup slots is split over its reduction axis, at least 16 steps a part
-    const long long want = 512 / (tiles > 0 ? tiles : 1), most = K / (16 * ck);
-    long long s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-}
+struct LinBwd { long long rc; int vc, nrc, nvc, tz; LinTile th, tw; };
 static LinBwd lin_bwd_plan(const LinDims& d) {
     LinBwd p;
     const long long piece = lin_piece();
     p.rc = d.rows < 32768 ? d.rows : 32768;
-    if (d.V <= 1024) { const long long most = piece / up(d.V > d.D ? d.V : d.D, 128); p.rc = d.rows < most ? d.rows : most < 128 ? 128 : most / 128 * 128; }
-    long long vc = piece / (p.rc > 0 ? up(p.rc, 128) : 1) / 128 * 128;
-    if (vc < 128) vc = 128;
+    if (d.V <= 1024) { const long long most = piece / up(d.V > d.D ? d.V : d.D, 256); p.rc = d.rows < most ? d.rows : most < 256 ? 256 : most / 256 * 256; }
+    long long vc = piece / (p.rc > 0 ? up(p.rc, 256) : 1) / 256 * 256;
+    if (vc < 256) vc = 256;
     p.vc = (int)(vc < d.V ? vc : d.V);
     p.nrc = p.rc ? (int)((d.rows + p.rc - 1) / p.rc) : 0;
     p.nvc = (d.V + p.vc - 1) / p.vc;
-    const int ck = d.dtype == FEA_BF16 ? 64 : 32, t = fea_lin_tile_m(d.dtype, 0);
-    auto tl = [&](long long a) { return (a + t - 1) / t; };
-    p.sh = lin_splits(tl(p.rc) * tl(d.D), p.vc, ck);
-    p.sw = lin_splits(tl(p.vc) * tl(d.D), p.rc, ck);
-    p.tiles_c = tl(p.rc);
+    p.tz = d.wide ? 128 : fea_lin_tile(d.dtype, p.rc, p.vc, d.Dp, false).tile;
+    p.th = fea_lin_tile(d.dtype, p.rc, d.D, p.vc, true);
+    p.tw = fea_lin_tile(d.dtype, p.vc, d.D, p.rc, true);
     return p;
 }
 
@@ -371,7 +366,7 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
         w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows));
         return c.at;
     }
-    w.part = c.take<float2>(p.rc * p.ntn);
+    w.part = c.take<float2>(p.rc * ((d.V + 127) / 128));           // (sized for the smaller tile: row strides may ask for it)
     w.zsel = c.take<float>(d.rows * d.K);
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
@@ -396,12 +391,12 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     if (want & 2) { w.dzt = c.take<char>(p.vc * rp * d.es); w.ht = c.take<char>(d.D * rp * d.es); }
     if (want & 1) w.wt = c.take<char>(d.D * vp * d.es);
     long long slab = 0;
-    if ((want & 1) && (p.sh > 1 || p.nvc > 1)) slab = p.sh * p.rc * d.D;
-    if ((want & 2) && (p.sw > 1 || p.nrc > 1) && slab < (long long)p.sw * p.vc * d.D) slab = (long long)p.sw * p.vc * d.D;
+    if ((want & 1) && (p.th.splits > 1 || p.nvc > 1)) slab = p.th.splits * p.rc * d.D;
+    if ((want & 2) && (p.tw.splits > 1 || p.nrc > 1) && slab < (long long)p.tw.splits * p.vc * d.D) slab = (long long)p.tw.splits * p.vc * d.D;
     w.slab = c.take<float>(slab);
     if ((want & 1) && p.nvc > 1) w.acch = c.take<float>(p.rc * d.D);
     if ((want & 2) && p.nrc > 1) w.accw = c.take<float>((long long)d.V * d.D);
-    if (want & 4) { w.colsum = c.take<float>(p.tiles_c * up(p.vc, 64)); w.dbpart = c.take<double>((p.tiles_c + LIN_DB_TILES - 1) / LIN_DB_TILES * p.vc); }
+    if (want & 4) { const long long t = (p.rc + 127) / 128; w.colsum = c.take<float>(t * up(p.vc, 64)); w.dbpart = c.take<double>((t + LIN_DB_TILES - 1) / LIN_DB_TILES * p.vc); }
     return c.at;
 }
 
@@ -455,9 +450,10 @@ static int lin_check(const char* who, const LinDims& d, const void* h, long long
     return FEA_OK;
 }
 
-static int lin_forward(const char* who, const LinDims& d, const void* h, long long ldh, const void* w, long long ldw, const float* bias, LinJoin j,
+static int lin_forward(const char* who, LinDims d, const void* h, long long ldh, const void* w, long long ldw, const float* bias, LinJoin j,
                        float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
+    d.wide = !d.packed() && (ldh >= 1 << 21 || ldw >= 1 << 21);
     const LinFwd p = lin_fwd_plan(d);
     LinFwdWs b;
     const size_t need = lin_fwd_carve(d, p, (char*)ws, b);
@@ -499,7 +495,7 @@ static int lin_forward(const char* who, const LinDims& d, const void* h, long lo
         LinGemm g{};
         g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = d.V; g.K = d.Dp;
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
-        LIN_TRY(fea_lin_gemm(LIN_LSE, d.dtype, g, s));
+        LIN_TRY(fea_lin_gemm(LIN_LSE, d.dtype, p.tile, g, s));
         LinJoin q = j;
         q.part = b.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
         q.zsel = b.zsel + r * d.K; q.index = j.index + r * d.K;
@@ -549,9 +545,10 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                                    float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
                                    int dtype, void* stream) {
     const char* who = "fea_linear_loss_bwd";
-    const LinDims d = lin_dims(rows, D, V, K, dtype);
+    LinDims d = lin_dims(rows, D, V, K, dtype);
     hipStream_t s = (hipStream_t)stream;
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
+    d.wide = !d.packed() && (ldh >= 1 << 21 || ldw >= 1 << 21);
     FEA_CHECK(index && stat && dsel && gout, FEA_E_BADARG, "%s: null operand", who);
     FEA_CHECK(gout_stride == 0 || gout_stride == 1, FEA_E_BADARG, "%s: gout_stride %d", who, gout_stride);
     FEA_CHECK(dh || dw || db, FEA_E_BADARG, "%s: no gradient asked for", who);
@@ -570,7 +567,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
         f.dh = dh; f.slab = b.slab; f.dbslab = b.colsum; f.rows = rows; f.D = D; f.V = V; f.K = K;
         return fea_lin_few_bwd(f, dtype, dw, db, s);
     }
-    const int ck = dtype == FEA_BF16 ? 64 : 32;
+    const int ck = 64;
     for (int ir = 0; ir < p.nrc; ++ir) {
         const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc, np = up(n, d.epc);
         const char* hr = (const char*)h + r0 * ldh * d.es;
@@ -593,7 +590,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             g.count = count; g.t = temperature;
             g.dz = b.dz; g.lddz = nvp; g.Npad = nvp; g.dzt = dw ? b.dzt : nullptr; g.lddzt = np; g.Mpad = (int)np;
             g.colsum = db ? b.colsum : nullptr; g.ldcol = up(p.vc, 64);
-            LIN_TRY(fea_lin_gemm(LIN_DZ, dtype, g, s));
+            LIN_TRY(fea_lin_gemm(LIN_DZ, dtype, p.tz, g, s));
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
             const unsigned sg = (unsigned)((entries + 255) / 256);
@@ -601,7 +598,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             else                   hipLaunchKernelGGL(lin_scatter_kernel<float>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, (long long)nvp, (float*)g.dzt, np, v0, nv, entries);
             FEA_LAUNCH_CHECK();
             if (db) {
-                const int tm = fea_lin_tile_m(dtype, 0), tiles = (int)((n + tm - 1) / tm), chunks = (tiles + LIN_DB_TILES - 1) / LIN_DB_TILES;
+                const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (tiles + LIN_DB_TILES - 1) / LIN_DB_TILES;
                 hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(256), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, (long long)LIN_DB_TILES * tm * K, b.dbpart);
                 FEA_LAUNCH_CHECK();
                 hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);
@@ -613,11 +610,11 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 m.a = b.dz; m.lda = nvp; m.b = b.wt; m.ldb = nvp; m.M = (int)n; m.N = D; m.K = nvp;
                 m.scale = 1; m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
                 void* out = (char*)dh + r0 * D * d.es;
-                const bool direct = p.sh == 1 && p.nvc == 1;
-                m.splits = p.sh; m.kper = (int)up((nvp + p.sh - 1) / p.sh, ck);
+                const bool direct = p.th.splits == 1 && p.nvc == 1;
+                m.splits = p.th.splits; m.kper = (int)up((nvp + m.splits - 1) / m.splits, ck);
                 if (direct) { m.out = out; m.ldo = D; } else m.slab = b.slab;
-                LIN_TRY(fea_lin_gemm(LIN_STORE, dtype, m, s));
-                if (!direct) LIN_TRY(lin_reduce(d, b.slab, p.sh, n * D, iv > 0 ? b.acch : nullptr, iv + 1 < p.nvc ? b.acch : nullptr, iv + 1 < p.nvc ? nullptr : out, s));
+                LIN_TRY(fea_lin_gemm(LIN_STORE, dtype, p.th.tile, m, s));
+                if (!direct) LIN_TRY(lin_reduce(d, b.slab, m.splits, n * D, iv > 0 ? b.acch : nullptr, iv + 1 < p.nvc ? b.acch : nullptr, iv + 1 < p.nvc ? nullptr : out, s));
             }
             if (dw) {
                 LinGemm m{};
@@ -625,11 +622,11 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 m.scale = gout_stride ? 0 : 2; m.gout = go; m.count = count; m.t = temperature;
                 void* out = (char*)dw + v0 * D * d.es;
                 float* acc = b.accw ? b.accw + v0 * D : nullptr;
-                const bool direct = p.sw == 1 && p.nrc == 1;
-                m.splits = p.sw; m.kper = (int)up((np + p.sw - 1) / p.sw, ck);
+                const bool direct = p.tw.splits == 1 && p.nrc == 1;
+                m.splits = p.tw.splits; m.kper = (int)up((np + m.splits - 1) / m.splits, ck);
                 if (direct) { m.out = out; m.ldo = D; } else m.slab = b.slab;
-                LIN_TRY(fea_lin_gemm(LIN_STORE, dtype, m, s));
-                if (!direct) LIN_TRY(lin_reduce(d, b.slab, p.sw, (long long)nv * D, ir > 0 ? acc : nullptr, ir + 1 < p.nrc ? acc : nullptr, ir + 1 < p.nrc ? nullptr : out, s));
+                LIN_TRY(fea_lin_gemm(LIN_STORE, dtype, p.tw.tile, m, s));
+                if (!direct) LIN_TRY(lin_reduce(d, b.slab, m.splits, (long long)nv * D, ir > 0 ? acc : nullptr, ir + 1 < p.nrc ? acc : nullptr, ir + 1 < p.nrc ? nullptr : out, s));
             }
         }
     }

@@ -69,6 +69,14 @@ def test_pieces(shape, dtype, top, monkeypatch):
     _compare(_run(*c), O.evaluate(*c))
 
 
+@pytest.mark.parametrize("shape", [(4096, 64, 4096), (4000, 200, 4100), (2049, 1096, 2310), (4097, 72, 8185), (300, 520, 40000)])
+@pytest.mark.parametrize("top", [0, 5])
+def test_large_tiles(shape, top):
+    """bf16 sizes that take the 256 x 256 tile in some or all of their products, with ragged ends in every direction."""
+    c = O.case(*shape, torch.bfloat16, seed=3, top=top, ignored=0.1, short=0.2, bias=shape[0] % 2 == 0)
+    _compare(_run(*c, reduction="sum"), O.evaluate(*c, reduction="sum"))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [9, 4100])
 def test_nothing_counts(dtype, rows):
@@ -217,7 +225,7 @@ def test_gradient_against_differences(top):
         for sign in (1, -1):
             x = list(c)
             x[k] = x[k] + sign * step * d
-            pair.append(float(_run(*x, **kw)["loss"]))
+            pair.append(float(_run(*x, **kw)["loss"].detach()))
         slope = float((got[name].cpu() * d).sum())
         curve = float(O.evaluate(*c, **kw)[name][0].norm())
         assert abs((pair[0] - pair[1]) / (2 * step) - slope) <= 2e-6 / (2 * step) + 4e-4 * max(curve, 1.0), name
