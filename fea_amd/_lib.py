@@ -148,8 +148,9 @@ def ptr(t):
     return t.data_ptr()
 
 
-def stream_ptr():
-    return torch.cuda.current_stream().cuda_stream
+def stream_ptr(device=None):
+    """The current stream of the current device, or of a device index."""
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def call(name: str, *args):

@@ -17,16 +17,7 @@
 struct LinI { static __device__ __forceinline__ int cls(int i, int hf) { return 8 * (i >> 2) + 4 * hf + (i & 3); } };
 
 template <typename T, bool ALN>
-__device__ __forceinline__ u32x4 few_load(const T* row, int d, int D) {
-    constexpr int EPC = Elem<T>::EPC;
-    if constexpr (ALN) return d < D ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0, 0, 0, 0};
-    else {
-        T x[EPC];
-#pragma unroll
-        for (int e = 0; e < EPC; ++e) x[e] = d + e < D ? row[d + e] : from_f32<T>(0.f);
-        return *reinterpret_cast<const u32x4*>(x);
-    }
-}
+__device__ __forceinline__ u32x4 few_load(const T* row, int d, int D) { return lin_load16<T, ALN>(row + d, D - d); }
 // registers EPC s .. EPC s + EPC - 1 of a result as one operand step
 template <typename T> __device__ __forceinline__ u32x4 few_pack(const float* v) {
     if constexpr (sizeof(T) == 4) { const f32x4 x = {v[0], v[1], v[2], v[3]}; return __builtin_bit_cast(u32x4, x); }

@@ -26,7 +26,7 @@ template <typename T> __device__ __forceinline__ void lg_store4(T* p, const floa
     }
 }
 
-template <typename T, int EPI>
+template <typename T, int EPI, bool ALN>
 __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     constexpr int EPC = Elem<T>::EPC, CK = Elem<T>::CK;
     __shared__ __attribute__((aligned(128))) char smem[2 * LG_STAGE];
@@ -45,12 +45,11 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     u32x4 ra[4], rb[4];
     auto fetch = [&](int k) {
         const int kk = k + c * EPC;
-        const bool kin = kk < k1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int m = m0 + r + 32 * i, n = n0 + r + 32 * i;
-            ra[i] = kin && m < g.M ? *reinterpret_cast<const u32x4*>(ap + m * g.lda + kk) : u32x4{0, 0, 0, 0};
-            rb[i] = kin && n < g.N ? *reinterpret_cast<const u32x4*>(bp + n * g.ldb + kk) : u32x4{0, 0, 0, 0};
+            ra[i] = m < g.M ? lin_load16<T, ALN>(ap + m * g.lda + kk, k1 - kk) : u32x4{0, 0, 0, 0};
+            rb[i] = n < g.N ? lin_load16<T, ALN>(bp + n * g.ldb + kk, k1 - kk) : u32x4{0, 0, 0, 0};
         }
     };
     auto put = [&](int st) {
@@ -220,24 +219,29 @@ LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool spli
     return best;
 }
 
-template <typename T> static void lin_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE>), dim3(grid), dim3(256), 0, s, g);
-    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ>), dim3(grid), dim3(256), 0, s, g);
-    else                    hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE>), dim3(grid), dim3(256), 0, s, g);
+template <typename T> static void lin_launch(int epi, bool aln, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (epi == LIN_LSE) {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, true>), dim3(grid), dim3(256), 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, false>), dim3(grid), dim3(256), 0, s, g);
+    } else if (epi == LIN_DZ) {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, true>), dim3(grid), dim3(256), 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, false>), dim3(grid), dim3(256), 0, s, g);
+    } else       hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE, true>), dim3(grid), dim3(256), 0, s, g);
 }
 
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     const int epc = dtype == FEA_BF16 ? 8 : 4;
-    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && g.lda >= g.K && g.ldb >= g.K
-              && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0, FEA_E_BADARG, "lin_gemm: operands %d x %d x %d not aligned", g.M, g.N, g.K);
+    const bool aln = g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0;
+    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.lda >= g.K && g.ldb >= g.K && (aln || (tile == 128 && epi != LIN_STORE)), FEA_E_BADARG,
+              "lin_gemm: operands of %d x %d x %d, tile %d", g.M, g.N, g.K, tile);
     FEA_CHECK(tile == 128 || (dtype == FEA_BF16 && g.lda < (1 << 21) && g.ldb < (1 << 21)), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
     g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
     const long long grid = (long long)g.ntm * g.ntn * g.splits;
     FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
     if (tile == 256)            fea_lin_gemm256(epi, g, (unsigned)grid, s);
-    else if (dtype == FEA_BF16) lin_launch<__bf16>(epi, g, (unsigned)grid, s);
-    else                        lin_launch<float>(epi, g, (unsigned)grid, s);
+    else if (dtype == FEA_BF16) lin_launch<__bf16>(epi, aln, g, (unsigned)grid, s);
+    else                        lin_launch<float>(epi, aln, g, (unsigned)grid, s);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }

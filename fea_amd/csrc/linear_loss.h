@@ -39,6 +39,21 @@ __device__ __forceinline__ float lin_row_scale(const float* gout, int gstride, c
     return gate != 0.f ? g : 0.f;
 }
 
+// 16 bytes of a row of which `left` elements remain (any sign), zeros behind them.  ALN: rows are 16-byte aligned and `left` is a multiple of
+// 16 bytes.  Else the load is unaligned (one instruction all the same) or, at the end of the row, element by element.
+template <typename T, bool ALN> __device__ __forceinline__ u32x4 lin_load16(const T* p, int left) {
+    constexpr int EPC = Elem<T>::EPC;
+    if constexpr (ALN) return left > 0 ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
+    else {
+        T x[EPC];
+        if (left >= EPC) __builtin_memcpy(x, p, 16);
+        else
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) x[e] = e < left ? p[e] : from_f32<T>(0.f);
+        return *reinterpret_cast<const u32x4*>(x);
+    }
+}
+
 // Few classes, few features, many rows (linear_few.hip)
 struct LinFew {
     const void *h, *w;
@@ -67,5 +82,7 @@ int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 struct LinTile { int tile, splits; };
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split);
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s);
+// linear_rows.hip: LIN_LSE of up to 64 label rows; g.part [M][classes / 64]
+int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s);
 // linear_gemm256.hip
 void fea_lin_gemm256(int epi, const LinGemm& g, unsigned grid, hipStream_t s);

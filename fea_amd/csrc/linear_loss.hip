@@ -52,42 +52,45 @@ __global__ __launch_bounds__(256) void lin_transpose_kernel(const T* __restrict_
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
 
+// a . b over D elements by L lanes (a power of two), the sum in each of them
+template <typename T, bool VEC>
+__device__ __forceinline__ float lin_dot(const T* a, const T* b, int D, int lane, int L) {
+    constexpr int EPC = Elem<T>::EPC;
+    float s = 0.f;
+    if constexpr (VEC) {
+        for (int d = lane * EPC; d < D; d += L * EPC) {
+            T x[EPC], y[EPC];
+            *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(a + d);
+            *reinterpret_cast<u32x4*>(y) = *reinterpret_cast<const u32x4*>(b + d);
+#pragma unroll
+            for (int q = 0; q < EPC; ++q) s += to_f32(x[q]) * to_f32(y[q]);
+        }
+    } else
+        for (int d = lane; d < D; d += L) s += to_f32(a[d]) * to_f32(b[d]);
+    for (int d = L >> 1; d; d >>= 1) s += __shfl_xor(s, d);
+    return s;
+}
+
 // zsel[n][k] = h_n . w_{index[n][k]} + b: L lanes (a power of two that covers the row in 16-byte loads, 64 at most) per entry.
 // Absent entries (index < 0 or >= V) are not read.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_select_kernel(const T* __restrict__ h, long long ldh, const T* __restrict__ w, long long ldw,
                                                          const float* __restrict__ bias, const long long* __restrict__ index, int K,
-                                                         float* __restrict__ zsel, long long entries, int D, int V, int L) {
-    constexpr int EPC = Elem<T>::EPC;
+                                                         float* __restrict__ zsel, long long entries, int D, int V, int L, int vec) {
     const int lane = threadIdx.x & (L - 1), per = 256 / L;
-    const bool vec = ((ldh | ldw | D) % EPC == 0) && (((uintptr_t)h | (uintptr_t)w) % 16 == 0);
     for (long long b0 = (long long)blockIdx.x * per; b0 < entries; b0 += (long long)gridDim.x * per) {
         const long long e = b0 + threadIdx.x / L;
         const long long i = e < entries ? index[e] : -1;
-        const bool there = i >= 0 && i < V;
-        float s = 0.f;
-        if (there) {
-            const T* a = h + e / K * ldh;
-            const T* b = w + i * ldw;
-            if (vec) {
-                for (int d = lane * EPC; d < D; d += L * EPC) {
-                    T x[EPC], y[EPC];
-                    *reinterpret_cast<u32x4*>(x) = *reinterpret_cast<const u32x4*>(a + d);
-                    *reinterpret_cast<u32x4*>(y) = *reinterpret_cast<const u32x4*>(b + d);
-#pragma unroll
-                    for (int q = 0; q < EPC; ++q) s += to_f32(x[q]) * to_f32(y[q]);
-                }
-            } else
-                for (int d = lane; d < D; d += L) s += to_f32(a[d]) * to_f32(b[d]);
-        }
-        for (int d = L >> 1; d; d >>= 1) s += __shfl_xor(s, d);
-        if (lane == 0 && e < entries) zsel[e] = there && bias ? s + bias[i] : s;
+        if (i < 0 || i >= V) continue;                       // (the L lanes of an entry go together)
+        const T* a = h + e / K * ldh;
+        const float s = vec ? lin_dot<T, true>(a, w + i * ldw, D, lane, L) : lin_dot<T, false>(a, w + i * ldw, D, lane, L);
+        if (lane == 0) zsel[e] = bias ? s + bias[i] : s;
     }
 }
 
 struct LinJoin {
     const float2* part; int ntn;          // [rows][ntn]
-    const float* zsel;                    // [rows][K]
+    float* zsel;                          // [rows][K]
     const long long* index;               // [rows][K]
     const void* tlog; int tdt;            // NULL: cross entropy (K = 1)
     long long ignore;
@@ -104,10 +107,7 @@ __device__ __forceinline__ float lin_tlog(const LinJoin& j, long long e) {
 }
 
 // G lanes join the column tiles of a row and turn its selected logits into the loss and the gradient at the selected classes.
-__global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
-    const int G = j.G, gl = threadIdx.x % G;
-    const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const bool in = row < j.rows;
+__device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, long long row, bool in) {
     float loss = 0.f;
     bool counts = false;
     {
@@ -188,6 +188,27 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
         }
         if (threadIdx.x == 0) { j.bsum[blockIdx.x] = ls[0]; j.bcnt[blockIdx.x] = lc[0]; }
     }
+}
+
+__global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
+    const long long row = (long long)blockIdx.x * (256 / j.G) + threadIdx.x / j.G;
+    lin_join_body(j, j.G, threadIdx.x % j.G, row, row < j.rows);
+}
+
+// The same for few rows, one workgroup per row, the selected logits and the join in one launch: all waves take entries, then the
+// first one joins.
+template <typename T>
+__global__ __launch_bounds__(256) void lin_join_rows_kernel(const LinJoin j, const T* h, long long ldh, const T* w, long long ldw, const float* bias, int D, int vec) {
+    const long long row = blockIdx.x;
+    for (int k = threadIdx.x >> 6; k < j.K; k += 4) {
+        const long long i = j.index[row * j.K + k];
+        if (i < 0 || i >= j.V) continue;
+        const float s = vec ? lin_dot<T, true>(h + row * ldh, w + i * ldw, D, threadIdx.x & 63, 64) : lin_dot<T, false>(h + row * ldh, w + i * ldw, D, threadIdx.x & 63, 64);
+        if ((threadIdx.x & 63) == 0) j.zsel[row * j.K + k] = bias ? s + bias[i] : s;
+    }
+    __threadfence_block();
+    __syncthreads();
+    lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64);
 }
 
 // loss[0] = sum, or sum / rows that count (0 where none does); count[0] = rows that count
@@ -324,12 +345,11 @@ static LinFwd lin_fwd_plan(const LinDims& d) {
     const long long cap = (1ll << 24) / ((d.V + 127) / 128);
     p.rc = cap < 256 ? 256 : cap / 256 * 256;
     if (p.rc > d.rows) p.rc = d.rows;
-    p.tile = fea_lin_tile(d.dtype, p.rc, d.V, d.Dp, false).tile;
-    if (d.wide) p.tile = 128;
+    p.tile = d.rows <= 64 ? 64 : d.wide ? 128 : fea_lin_tile(d.dtype, p.rc, d.V, d.Dp, false).tile;
     p.ntn = (d.V + p.tile - 1) / p.tile;
     p.G = 1;
     while (p.G < 64 && (p.G < p.ntn || p.G < d.K)) p.G *= 2;
-    p.blocks = (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
+    p.blocks = p.tile == 64 ? d.rows : (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
     return p;
 }
 
@@ -366,12 +386,12 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
         w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows));
         return c.at;
     }
-    w.part = c.take<float2>(p.rc * ((d.V + 127) / 128));           // (sized for the smaller tile: row strides may ask for it)
+    w.part = c.take<float2>(p.rc * ((d.V + (p.tile == 64 ? 63 : 127)) / (p.tile == 64 ? 64 : 128)));           // (sized for the smaller tile: row strides may ask for it)
     w.zsel = c.take<float>(d.rows * d.K);
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
-    w.hp = d.packed() ? c.take<char>(p.rc * d.Dp * d.es) : nullptr;
-    w.wp = d.packed() ? c.take<char>((long long)d.V * d.Dp * d.es) : nullptr;
+    w.hp = w.wp = nullptr;
+    if (d.packed() && p.tile == 256) { w.hp = c.take<char>(p.rc * d.Dp * d.es); w.wp = c.take<char>((long long)d.V * d.Dp * d.es); }
     return c.at;
 }
 
@@ -386,7 +406,7 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
         w.dz = c.take<char>(256);
         return c.at;
     }
-    if (d.packed()) { w.hp = c.take<char>(p.rc * d.Dp * d.es); w.wp = c.take<char>((long long)p.vc * d.Dp * d.es); }
+    if (d.packed() && p.tz == 256) { w.hp = c.take<char>(p.rc * d.Dp * d.es); w.wp = c.take<char>((long long)p.vc * d.Dp * d.es); }
     w.dz = c.take<char>(p.rc * vp * d.es);
     if (want & 2) { w.dzt = c.take<char>(p.vc * rp * d.es); w.ht = c.take<char>(d.D * rp * d.es); }
     if (want & 1) w.wt = c.take<char>(d.D * vp * d.es);
@@ -474,28 +494,31 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         return FEA_OK;
     }
     const long long entries = d.rows * d.K;
-    {
+    if (p.tile != 64) {
         int lanes = 1;
         while (lanes < 64 && lanes * d.epc < d.D) lanes *= 2;
         const long long blocks = (entries * lanes + 255) / 256;
         const unsigned grid = (unsigned)(blocks < 1 << 16 ? blocks : 1 << 16);
-        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes);
-        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes);
+        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.packed() ? 0 : 1);
+        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.packed() ? 0 : 1);
         FEA_LAUNCH_CHECK();
     }
     const void* wm = w;
     long long ldwm = ldw;
-    if (d.packed()) { LIN_TRY(lin_pack(d, w, ldw, b.wp, d.V, s)); wm = b.wp; ldwm = d.Dp; }
+    const bool pack = d.packed() && p.tile == 256;       // (the other kernels take rows of any alignment)
+    const int Kg = pack ? d.Dp : d.D;
+    if (pack) { LIN_TRY(lin_pack(d, w, ldw, b.wp, d.V, s)); wm = b.wp; ldwm = d.Dp; }
     long long blk = 0;
     for (long long r = 0; r < d.rows; r += p.rc) {
         const long long n = d.rows - r < p.rc ? d.rows - r : p.rc;
         const void* hm = (const char*)h + r * ldh * d.es;
         long long ldhm = ldh;
-        if (d.packed()) { LIN_TRY(lin_pack(d, hm, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
+        if (pack) { LIN_TRY(lin_pack(d, hm, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
         LinGemm g{};
-        g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = d.V; g.K = d.Dp;
+        g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = d.V; g.K = Kg;
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
-        LIN_TRY(fea_lin_gemm(LIN_LSE, d.dtype, p.tile, g, s));
+        if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.packed(), g, s));
+        else LIN_TRY(fea_lin_gemm(LIN_LSE, d.dtype, p.tile, g, s));
         LinJoin q = j;
         q.part = b.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
         q.zsel = b.zsel + r * d.K; q.index = j.index + r * d.K;
@@ -505,8 +528,10 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         if (q.psel) q.psel += r * d.K;
         if (q.loss_rows) q.loss_rows += r;
         q.bsum = loss ? b.bsum + blk : nullptr; q.bcnt = b.bcnt + blk;
-        const long long grid = (n + 256 / p.G - 1) / (256 / p.G);
-        hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
+        const long long grid = p.tile == 64 ? n : (n + 256 / p.G - 1) / (256 / p.G);
+        if (p.tile != 64)               hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
+        else if (d.dtype == FEA_BF16)   hipLaunchKernelGGL(lin_join_rows_kernel<__bf16>, dim3((unsigned)grid), dim3(256), 0, s, q, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, d.D, d.packed() ? 0 : 1);
+        else                            hipLaunchKernelGGL(lin_join_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, q, (const float*)h, ldh, (const float*)w, ldw, bias, d.D, d.packed() ? 0 : 1);
         FEA_LAUNCH_CHECK();
         blk += grid;
     }
@@ -568,6 +593,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
         return fea_lin_few_bwd(f, dtype, dw, db, s);
     }
     const int ck = 64;
+    const bool pack = d.packed() && p.tz == 256;
     for (int ir = 0; ir < p.nrc; ++ir) {
         const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc, np = up(n, d.epc);
         const char* hr = (const char*)h + r0 * ldh * d.es;
@@ -575,7 +601,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
         const float* go = gout + r0 * gout_stride;
         const void* hm = hr;
         long long ldhm = ldh;
-        if (d.packed()) { LIN_TRY(lin_pack(d, hr, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
+        if (pack) { LIN_TRY(lin_pack(d, hr, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
         if (dw) LIN_TRY(lin_transpose(d, hr, ldh, b.ht, np, n, np, st, gout_stride ? go : nullptr, temperature, s));
         for (int iv = 0; iv < p.nvc; ++iv) {
             const long long v0 = (long long)iv * p.vc;
@@ -583,9 +609,9 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             const char* wr = (const char*)w + v0 * ldw * d.es;
             const void* wm = wr;
             long long ldwm = ldw;
-            if (d.packed()) { LIN_TRY(lin_pack(d, wr, ldw, b.wp, nv, s)); wm = b.wp; ldwm = d.Dp; }
+            if (pack) { LIN_TRY(lin_pack(d, wr, ldw, b.wp, nv, s)); wm = b.wp; ldwm = d.Dp; }
             LinGemm g{};
-            g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = nv; g.K = d.Dp;
+            g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = nv; g.K = pack ? d.Dp : D;
             g.bias = bias ? bias + v0 : nullptr; g.inv_t = 1.f / temperature; g.stat = st; g.gout = go; g.gstride = gout_stride;
             g.count = count; g.t = temperature;
             g.dz = b.dz; g.lddz = nvp; g.Npad = nvp; g.dzt = dw ? b.dzt : nullptr; g.lddzt = np; g.Mpad = (int)np;

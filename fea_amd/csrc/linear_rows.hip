@@ -1,0 +1,126 @@
+// Log-sum-exp of the logits of a few label rows (up to 64) over many classes: the weight is read once, straight into the matrix
+// operands, and everything else has to keep out of its way.
+//
+// One wave owns 16 classes over the whole reduction (v_mfma 16x16: 16 classes x 16 labels per product, NR of them); a workgroup of 4
+// waves 64 classes.  The weight goes from memory to registers (a wave's 16 rows x 512 bytes in flight while the 512 bytes before
+// are multiplied); the labels' hidden states, which all waves share, through LDS in the same chunks.
+// Bound by the weight's bytes: see the figures at fea_lin_rows.
+#include "linear_loss.h"
+
+__device__ __forceinline__ void mma16x16(f32x4& acc, const u32x4& a, const u32x4& b, const __bf16*) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16x16(f32x4& acc, const u32x4& a, const u32x4& b, const float*) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y.y, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y.z, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, acc, 0, 0, 0);
+}
+
+static constexpr int LR_CB = 512, LR_LD = LR_CB + 16;     // bytes of a chunk of a row; its distance in LDS (16 rows in 16 bank groups)
+
+template <typename T, int NR, bool ALN>
+__global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
+    constexpr int EPC = Elem<T>::EPC, CE = LR_CB / (int)sizeof(T), NS = LR_CB / 64;     // elements, products of a chunk
+    __shared__ __attribute__((aligned(16))) char hs[2][16 * NR * LR_LD];
+    __shared__ float2 red[4][16 * NR];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q16 = lane >> 4;
+    const int n0 = blockIdx.x * 64 + wave * 16;
+    const T* const w = (const T*)g.b + (long long)min(n0 + r16, g.N - 1) * g.ldb;
+    const T* const h = (const T*)g.a;
+    u32x4 wv[2][NS];
+    auto wload = [&](int buf, int k0) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int k = k0 + (4 * s + q16) * EPC;
+            wv[buf][s] = lin_load16<T, ALN>(w + k, g.K - k);
+        }
+    };
+    constexpr int HP = NR * 16 * (LR_CB / 16) / 256;          // 16-byte pieces of the labels' chunk per thread
+    u32x4 hv[HP];
+    auto hload = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < HP; ++i) {
+            const int p = tid + 256 * i, row = p >> 5, k = k0 + (p & 31) * EPC;
+            hv[i] = row < g.M ? lin_load16<T, ALN>(h + row * g.lda + k, g.K - k) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto hput = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < HP; ++i) {
+            const int p = tid + 256 * i;
+            *reinterpret_cast<u32x4*>(hs[buf] + (p >> 5) * LR_LD + (p & 31) * 16) = hv[i];
+        }
+    };
+    f32x4 acc[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto mul = [&](int buf) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+                mma16x16(acc[i], wv[buf][s], *reinterpret_cast<const u32x4*>(hs[buf] + (16 * i + r16) * LR_LD + (4 * s + q16) * 16), (const T*)nullptr);
+    };
+    hload(0);
+    wload(0, 0);
+    // two chunks per round, so that the buffers' indexes are constants
+    for (int k0 = 0; k0 < g.K; k0 += 2 * CE) {
+        hput(0);
+        hload(k0 + CE);
+        wload(1, k0 + CE);
+        __syncthreads();              // (also: every wave is done with the other buffer)
+        mul(0);
+        hput(1);
+        hload(k0 + 2 * CE);
+        wload(0, k0 + 2 * CE);
+        __syncthreads();
+        mul(1);
+    }
+    // lane: label 16 i + r16, classes n0 + 4 q16 .. + 3
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = g.bias && n0 + 4 * q16 + e < g.N ? g.bias[n0 + 4 * q16 + e] : 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        float z[4], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { z[e] = n0 + 4 * q16 + e < g.N ? (acc[i][e] + bias[e]) * g.inv_t : -INFINITY; mx = fmaxf(mx, z[e]); }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += __expf(z[e] - base);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (q16 == 0) red[wave][16 * i + r16] = make_float2(mx, sum);
+    }
+    __syncthreads();
+    if (tid < 16 * NR && tid < g.M) {
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, red[k][tid].x);
+        const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += red[k][tid].y * __expf(red[k][tid].x - base);
+        g.part[(long long)tid * g.ntn + blockIdx.x] = make_float2(mx, sum);
+    }
+}
+
+template <typename T, bool ALN> static void rows_launch(const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (g.M <= 16)      hipLaunchKernelGGL((lin_rows_kernel<T, 1, ALN>), dim3(grid), dim3(256), 0, s, g);
+    else if (g.M <= 32) hipLaunchKernelGGL((lin_rows_kernel<T, 2, ALN>), dim3(grid), dim3(256), 0, s, g);
+    else                hipLaunchKernelGGL((lin_rows_kernel<T, 4, ALN>), dim3(grid), dim3(256), 0, s, g);
+}
+
+// LIN_LSE of at most 64 label rows, operands of any alignment; part has one column per 64 classes
+int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s) {
+    FEA_CHECK(g.M > 0 && g.M <= 64 && g.N > 0 && g.K > 0, FEA_E_BADARG, "lin_rows: %d x %d x %d", g.M, g.N, g.K);
+    g.ntn = (g.N + 63) / 64;
+    const unsigned grid = (unsigned)g.ntn;
+    if (dtype == FEA_BF16) { if (aligned) rows_launch<__bf16, true>(g, grid, s); else rows_launch<__bf16, false>(g, grid, s); }
+    else                   { if (aligned) rows_launch<float, true>(g, grid, s); else rows_launch<float, false>(g, grid, s); }
+    FEA_LAUNCH_CHECK();
+    return FEA_OK;
+}

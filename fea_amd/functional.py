@@ -123,33 +123,40 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     h, w = _aligned_rows(hidden), _aligned_rows(weight)
     (rows, d), v = h.shape, w.shape[0]
     k = 1 if tlog is None else index.shape[-1]
-    ix = index.detach().to(torch.int64).contiguous()
+    ix = index.detach()
+    if ix.dtype != torch.int64:
+        ix = ix.to(torch.int64)
+    ix = ix.contiguous()
     b = None if bias is None else bias.detach().contiguous()
     dt = L.dt_code(h.dtype)
-    f32 = {"dtype": torch.float32, "device": dev}
-    stat = torch.empty((rows, 2), **f32) if grads else None
-    dsel = torch.empty((rows, k), **f32) if grads else None
-    psel = torch.empty((rows, k), **f32) if grads and tlog is not None else None
-    rowloss = torch.empty(rows, **f32) if reduction == "none" else None
-    loss = torch.empty((), **f32) if reduction != "none" else None
-    count = torch.empty((), dtype=torch.int32, device=dev) if reduction != "none" else None
+    stat = dsel = psel = count = None
+    if grads:
+        stat = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+        dsel = torch.empty((rows, k), dtype=torch.float32, device=dev)
+        psel = torch.empty((rows, k), dtype=torch.float32, device=dev) if tlog is not None else None
+    if reduction == "none":
+        loss = torch.empty(index.shape if tlog is None else index.shape[:-1], dtype=torch.float32, device=dev)
+        outs = (loss, None, None, 0)
+    else:
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        count = torch.empty((), dtype=torch.int32, device=dev)
+        outs = (None, loss, count, int(reduction == "mean"))
     n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    tail = (rowloss, loss, count, int(reduction == "mean"), ws, n, rows, d, v, dt, L.stream_ptr())
     if tlog is None:
-        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, *tail)
+        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, *outs, ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
     else:
         tl = tlog.detach().contiguous()
-        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, *tail)
-    return (loss if rowloss is None else rowloss.view(index.shape if tlog is None else index.shape[:-1])), (h, w, b, ix, stat, dsel, psel, count)
+        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, *outs,
+               ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
+    return loss, (ix, stat, dsel, psel, count)
 
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
         grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want)
-        loss, saved = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
-        h, w, b, ix, stat, dsel, psel, count = saved
+        loss, (ix, stat, dsel, psel, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
         # the operands themselves are saved, so that autograd sees a change in place between forward and backward
         ctx.save_for_backward(hidden, weight, bias, ix, stat, dsel, psel, count if reduction == "mean" else None)
         ctx.how = (temperature, reduction, dsel.shape[1], grads)
@@ -160,20 +167,23 @@ class _LinearLoss(torch.autograd.Function):
     def backward(ctx, gout):
         hidden, weight, bias, ix, stat, dsel, psel, count = ctx.saved_tensors
         temperature, reduction, k, grads = ctx.how
-        with torch.cuda.device(hidden.device):
-            h, w = _aligned_rows(hidden), _aligned_rows(weight)
-            b = None if bias is None else bias.detach().contiguous()
-            (rows, d), v = h.shape, w.shape[0]
-            dt = L.dt_code(h.dtype)
-            dh = torch.empty(hidden.shape, dtype=h.dtype, device=h.device) if grads & 1 else None
-            dw = torch.empty(weight.shape, dtype=w.dtype, device=w.device) if grads & 2 else None
-            db = torch.empty(v, dtype=torch.float32, device=h.device) if grads & 4 else None
-            go = gout.detach().float().contiguous()
-            n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, grads)
-            ws = torch.empty(n, dtype=torch.uint8, device=h.device)
-            L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, count, go, int(reduction == "none"),
-                   temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr())
+        # (the autograd engine runs this on the forward's device and stream)
+        h, w = _aligned_rows(hidden), _aligned_rows(weight)
+        b = None if bias is None else bias.detach().contiguous()
+        (rows, d), v = h.shape, w.shape[0]
+        dt = L.dt_code(h.dtype)
+        dh = torch.empty(hidden.shape, dtype=h.dtype, device=h.device) if grads & 1 else None
+        dw = torch.empty(weight.shape, dtype=w.dtype, device=w.device) if grads & 2 else None
+        db = torch.empty(v, dtype=torch.float32, device=h.device) if grads & 4 else None
+        go = gout.detach().contiguous()
+        n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, grads)
+        ws = torch.empty(n, dtype=torch.uint8, device=h.device)
+        L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, count, go, int(reduction == "none"),
+               temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr(h.device.index))
         return dh, dw, db, None, None, None, None, None
+
+
+_LABELS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
@@ -185,7 +195,7 @@ def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperatu
         raise ValueError(f"{who}: hidden and weight are both float32 or both bfloat16 (got {hidden.dtype}, {weight.dtype})")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"{who}: hidden [..., D] and weight [classes, D] do not fit (got {tuple(hidden.shape)}, {tuple(weight.shape)})")
-    if index.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+    if index.dtype not in _LABELS:
         raise ValueError(f"{who}: labels are integers (got {index.dtype})")
     lead = index.shape if tlog is None else index.shape[:-1]
     if lead != hidden.shape[:-1]:
@@ -194,21 +204,23 @@ def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperatu
         if bias.dtype not in (torch.float32, weight.dtype) or bias.shape != weight.shape[:1]:
             raise ValueError(f"{who}: bias is [classes] in float32 or the weight's type (got {tuple(bias.shape)}, {bias.dtype})")
         bias = bias.float()
+    dev = hidden.device
     for t in (hidden, weight, bias, index, tlog):
-        if t is not None and not t.is_cuda:
-            raise L.FeaError(f"{who} runs on a ROCm device only")
-        if t is not None and t.device != hidden.device:
-            raise ValueError(f"{who}: operands on {hidden.device} and {t.device}")
-    rows = index.numel() if tlog is None else index.numel() // index.shape[-1]
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (hidden, weight, bias))
-    if rows == 0:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{who}: operands on {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise L.FeaError(f"{who} runs on a ROCm device only")
+    train = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    if lead.numel() == 0:
         # nothing counts: the loss is 0 and so is every gradient
         zero = (hidden.sum() + weight[:0].sum() + (0 if bias is None else bias[:0].sum())).float() if train else hidden.new_zeros((), dtype=torch.float32)
         return zero if reduction != "none" else zero.expand(lead)
-    with torch.cuda.device(hidden.device):
-        if not train:
-            return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, 0)[0]
-        return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
+    if not train:
+        return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, 0)[0]
+    return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor = None,

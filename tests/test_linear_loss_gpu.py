@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 TYPES = [torch.float32, torch.bfloat16]
 SHAPES = [(1, 8, 1), (1, 1, 2), (1, 64, 600), (2, 5, 7), (3, 64, 6), (17, 33, 129), (64, 128, 128), (129, 72, 1000), (5000, 72, 40), (257, 200, 333),
-          (300, 96, 5003), (513, 640, 1537), (5000, 64, 6), (4097, 24, 33), (4096, 64, 32), (4100, 33, 13), (6001, 16, 2), (4111, 40, 24), (5003, 7, 1)]
+          (300, 96, 5003), (513, 640, 1537), (5000, 64, 6), (4097, 24, 33), (4096, 64, 32), (4100, 33, 13), (6001, 16, 2), (4111, 40, 24), (5003, 7, 1), (33, 515, 1000),
+          (48, 1024, 777), (16, 300, 2049)]
 
 
 def _leaf(t):
