@@ -26,7 +26,7 @@ template <typename T> __device__ __forceinline__ void lg_store4(T* p, const floa
     }
 }
 
-template <typename T, int EPI, bool ALN>
+template <typename T, int EPI, bool ALN, bool PL>
 __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     constexpr int EPC = Elem<T>::EPC, CK = Elem<T>::CK;
     __shared__ __attribute__((aligned(128))) char smem[2 * LG_STAGE];
@@ -43,13 +43,20 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     const T* const ap = (const T*)g.a;
     const T* const bp = (const T*)g.b;
     u32x4 ra[4], rb[4];
+    int pair = PL ? k0 / g.Kp : 0, pk = PL ? k0 - pair * g.Kp : 0;
     auto fetch = [&](int k) {
-        const int kk = k + c * EPC;
+        const int left = k1 - k - c * EPC;
+        int ka = k + c * EPC, kb = ka;
+        if constexpr (PL) {
+            ka = lin_plane_a(pair) * g.Kp + pk + c * EPC; kb = lin_plane_b(pair) * g.Kp + pk + c * EPC;
+            pk += CK;
+            if (pk >= g.Kp) { pk = 0; ++pair; }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int m = m0 + r + 32 * i, n = n0 + r + 32 * i;
-            ra[i] = m < g.M ? lin_load16<T, ALN>(ap + m * g.lda + kk, k1 - kk) : u32x4{0, 0, 0, 0};
-            rb[i] = n < g.N ? lin_load16<T, ALN>(bp + n * g.ldb + kk, k1 - kk) : u32x4{0, 0, 0, 0};
+            ra[i] = m < g.M ? lin_load16<T, ALN>(ap + m * g.lda + ka, left) : u32x4{0, 0, 0, 0};
+            rb[i] = n < g.N ? lin_load16<T, ALN>(bp + n * g.ldb + kb, left) : u32x4{0, 0, 0, 0};
         }
     };
     auto put = [&](int st) {
@@ -182,30 +189,36 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             if (tid < LG_T && n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LG_T + tid];
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int m = mrow(i);
+        for (int pl = 0; pl < (PL ? 3 : 1); ++pl) {
+            T* const dz = (T*)g.dz + (PL ? (long long)pl * g.Npad : 0);
+            T* const dzt = (T*)g.dzt + (PL ? (long long)pl * g.Mpad : 0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int i = 0; i < 2; ++i) {
+                const int m = mrow(i);
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const int n = ncol(j, e);
-                    const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                    if (m < g.M && n < g.Npad) lg_store4((T*)g.dz + m * g.lddz + n, v, g.Npad - n);
-                    if (g.dzt && m < g.Mpad)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) if (n + x < g.N) ((T*)g.dzt)[(n + x) * g.lddzt + m] = from_f32<T>(v[x]);
-                }
+                    for (int e = 0; e < 16; e += 4) {
+                        const int n = ncol(j, e);
+                        const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                        if (m < g.M && n < g.Npad) lg_store4(dz + m * g.lddz + n, v, g.Npad - n);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (g.dzt && m < g.Mpad && n + x < g.N) dzt[(n + x) * g.lddzt + m] = from_f32<T>(v[x]);
+                            if constexpr (PL) acc[i][j][e + x] -= to_f32(from_f32<T>(v[x]));
+                        }
+                    }
+            }
         }
     }
 }
 
-// Tile and split of a product: the one whose modelled time is least, from the rates that the two kernels reach on full chips.  Both
-// take whole rounds of the chip (256 workgroups of the large tile, 512 of the small one); the parts of a split reduction are written
-// and read once more, at least 512 (bf16) or 256 (fp32) channels each.
+// Tile and split of a product: the one whose modelled time is least, from the rates that the kernels reach on full chips (fp32 100, bf16 700
+// and 1,300 TFLOP/s).  Both take whole rounds of the chip (256 workgroups of the large tile, 512 of the small one); the parts of a split
+// reduction are written and read once more, at least 512 (bf16) or 256 (fp32) channels each.  dtype FEA_PL: K is six times the planes'.
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split) {
-    LinTile best{128, 1};
-    double least = 1e30;
-    for (int tile = 128; tile <= (dtype == FEA_BF16 ? 256 : 128); tile += 128) {
+    LinTile best{128, 1, 1e30};
+    for (int tile = 128; tile <= (dtype == FEA_F32 ? 128 : 256); tile += 128) {
         const double slots = tile == 256 ? 256 : 512;
         const double rate = dtype == FEA_F32 ? 100e12 : tile == 256 ? 1300e12 : 700e12;
         const long long tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
@@ -213,7 +226,7 @@ LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool spli
             if (sp > 1 && K / sp < (dtype == FEA_F32 ? 256 : 512)) break;
             const double rounds = (double)((tiles * sp + (long long)slots - 1) / (long long)slots);
             const double t = rounds * (2.0 * tile * tile * ((double)K / sp + 128) / (rate / slots)) + (sp > 1 ? 2.0 * sp * M * N * 4 / 4e12 + 3e-6 : 0.0);
-            if (t < least * 0.999) { least = t; best = LinTile{tile, sp}; }
+            if (t < best.time * 0.999) best = LinTile{tile, sp, t};
         }
     }
     return best;
@@ -221,25 +234,33 @@ LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool spli
 
 template <typename T> static void lin_launch(int epi, bool aln, const LinGemm& g, unsigned grid, hipStream_t s) {
     if (epi == LIN_LSE) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, true>), dim3(grid), dim3(256), 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, false>), dim3(grid), dim3(256), 0, s, g);
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, true, false>), dim3(grid), dim3(256), 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, false, false>), dim3(grid), dim3(256), 0, s, g);
     } else if (epi == LIN_DZ) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, true>), dim3(grid), dim3(256), 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, false>), dim3(grid), dim3(256), 0, s, g);
-    } else       hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE, true>), dim3(grid), dim3(256), 0, s, g);
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, true, false>), dim3(grid), dim3(256), 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, false, false>), dim3(grid), dim3(256), 0, s, g);
+    } else       hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE, true, false>), dim3(grid), dim3(256), 0, s, g);
+}
+static void lin_launch_planes(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm_kernel<__bf16, LIN_LSE, true, true>), dim3(grid), dim3(256), 0, s, g);
+    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm_kernel<__bf16, LIN_DZ, true, true>), dim3(grid), dim3(256), 0, s, g);
+    else                    hipLaunchKernelGGL((lin_gemm_kernel<__bf16, LIN_STORE, true, true>), dim3(grid), dim3(256), 0, s, g);
 }
 
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
-    const int epc = dtype == FEA_BF16 ? 8 : 4;
+    const int epc = dtype == FEA_F32 ? 4 : 8;
     const bool aln = g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0;
-    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.lda >= g.K && g.ldb >= g.K && (aln || (tile == 128 && epi != LIN_STORE)), FEA_E_BADARG,
+    const long long row = dtype == FEA_PL ? 3ll * g.Kp : g.K;
+    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.lda >= row && g.ldb >= row && (aln || (tile == 128 && epi != LIN_STORE && dtype != FEA_PL)), FEA_E_BADARG,
               "lin_gemm: operands of %d x %d x %d, tile %d", g.M, g.N, g.K, tile);
-    FEA_CHECK(tile == 128 || (dtype == FEA_BF16 && g.lda < (1 << 21) && g.ldb < (1 << 21)), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
+    FEA_CHECK(dtype != FEA_PL || (g.Kp > 0 && g.Kp % 64 == 0 && g.K == 6 * g.Kp && (epi != LIN_STORE || g.slab)), FEA_E_BADARG, "lin_gemm: planes of %d, K %d", g.Kp, g.K);
+    FEA_CHECK(tile == 128 || (dtype != FEA_F32 && g.lda < (1 << 21) && g.ldb < (1 << 21)), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
     g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
     const long long grid = (long long)g.ntm * g.ntn * g.splits;
     FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
-    if (tile == 256)            fea_lin_gemm256(epi, g, (unsigned)grid, s);
+    if (tile == 256)            fea_lin_gemm256(epi, dtype == FEA_PL, g, (unsigned)grid, s);
+    else if (dtype == FEA_PL)   lin_launch_planes(epi, g, (unsigned)grid, s);
     else if (dtype == FEA_BF16) lin_launch<__bf16>(epi, aln, g, (unsigned)grid, s);
     else                        lin_launch<float>(epi, aln, g, (unsigned)grid, s);
     FEA_LAUNCH_CHECK();

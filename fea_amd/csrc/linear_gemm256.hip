@@ -23,7 +23,7 @@ __device__ __forceinline__ uint32_t lb_pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, b2));
 }
 
-template <int EPI>
+template <int EPI, bool PL>
 __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
     __shared__ __attribute__((aligned(128))) char smem[2 * LB_STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -38,10 +38,11 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
     const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, K = max((EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K) - k0, 0);
     const int nc = (K + 63) >> 6;
 
-    const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.a + m0 * g.lda + k0), 0,
-        K ? (int)(((min(LB_T, g.M - m0) - 1) * g.lda + K) * 2) : 0, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.b + n0 * g.ldb + k0), 0,
-        K ? (int)(((min(LB_T, g.N - n0) - 1) * g.ldb + K) * 2) : 0, 0x00020000);
+    const int kb = PL ? 0 : k0, kl = PL ? 3 * g.Kp : K;      // first channel and length of a row, as the buffers see it
+    const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.a + m0 * g.lda + kb), 0,
+        K ? (int)(((min(LB_T, g.M - m0) - 1) * g.lda + kl) * 2) : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.b + n0 * g.ldb + kb), 0,
+        K ? (int)(((min(LB_T, g.N - n0) - 1) * g.ldb + kl) * 2) : 0, 0x00020000);
 
     // staging: thread -> rows r + 32 i of either operand, 16-byte chunk c
     const int r = tid >> 3, c = tid & 7;
@@ -49,10 +50,20 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
     const unsigned sa = 64 * (unsigned)g.lda, sb = 64 * (unsigned)g.ldb;
     const int wofs = r * 128 + ((c ^ lb_swz(r)) << 4);
     u32x4 st[16];
-    auto gload = [&](int ch, int i) {
-        const bool kin = ch * 64 + c * 8 < K;
-        if (i < 8) st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ch * 128 + i * sa : 0x7fffff00u, 0, 0));
-        else       st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + ch * 128 + (i - 8) * sb : 0x7fffff00u, 0, 0));
+    int pair = PL ? k0 / g.Kp : 0, pk = PL ? k0 - pair * g.Kp : 0;       // FEA_PL: the pair of planes and the channel that are loaded next
+    unsigned ka = 0, kc = 0;
+    bool kin = false;
+    auto advance = [&](int ch) {      // byte offsets of chunk ch in a row of either operand
+        kin = ch * 64 + c * 8 < K;
+        if constexpr (PL) {
+            ka = 2u * (unsigned)(lin_plane_a(pair) * g.Kp + pk); kc = 2u * (unsigned)(lin_plane_b(pair) * g.Kp + pk);
+            pk += 64;
+            if (pk >= g.Kp) { pk = 0; ++pair; }
+        } else ka = kc = ch * 128;
+    };
+    auto gload = [&](int i) {
+        if (i < 8) st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ka + i * sa : 0x7fffff00u, 0, 0));
+        else       st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + kc + (i - 8) * sb : 0x7fffff00u, 0, 0));
     };
     auto lput = [&](int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i >> 3) * LB_OP + wofs + (i & 7) * 32 * 128) = st[i]; };
 
@@ -77,21 +88,24 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
     };
 
+    advance(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) gload(0, i);
+    for (int i = 0; i < 16; ++i) gload(i);
 #pragma unroll
     for (int i = 0; i < 16; ++i) lput(0, i);
+    advance(1);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) gload(1, i);
+    for (int i = 0; i < 16; ++i) gload(i);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 16; ++i) frd(0, 0, i);
 
     for (int ch = 0; ch < nc; ++ch) {
         const int s = ch & 1;
+        advance(ch + 2);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { frd(s, 1, i); lput(s ^ 1, i); gload(ch + 2, i); }
+        for (int i = 0; i < 16; ++i) { frd(s, 1, i); lput(s ^ 1, i); gload(i); }
         mma(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {        // 2 MFMA, LDS read, MFMA, LDS write, MFMA, load
@@ -123,7 +137,7 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
     // two class tiles 2 p, 2 p + 1 of one label: after the exchange between neighbouring 16-lane rows a lane holds 8 consecutive
     // classes, starting at
     const int pcol = n0 + wn * 128 + (q16 & 1) * 16 + (q16 >> 1) * 8;
-    auto pair = [&](const f32x4& x, const f32x4& y) {
+    auto pairs = [&](const f32x4& x, const f32x4& y) {
         const auto r0 = __builtin_amdgcn_permlane16_swap(lb_pack(x[0], x[1]), lb_pack(y[0], y[1]), false, false);
         const auto r1 = __builtin_amdgcn_permlane16_swap(lb_pack(x[2], x[3]), lb_pack(y[2], y[3]), false, false);
         return u32x4{r0[0], r1[0], r0[1], r1[1]};
@@ -153,7 +167,7 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     if (wide) {
-                        const u32x4 v = pair(acc[i][2 * p], acc[i][2 * p + 1]);
+                        const u32x4 v = pairs(acc[i][2 * p], acc[i][2 * p + 1]);
                         if (m < g.M && pcol + 32 * p < g.N) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
                     } else
 #pragma unroll
@@ -207,8 +221,6 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
 
     if constexpr (EPI == LIN_DZ) {
         float sc[8];
-        const bool odd = lane & 1;
-        const int tcol = 2 * (lane & 1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int m = mrow(i);
@@ -222,28 +234,6 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
                     const float q = __expf(acc[i][j][e] - s2.x);
                     acc[i][j][e] = dead || (n0 + LB_T > g.N && ncol(j) + e >= g.N) ? 0.f : q;
                 }
-            __bf16* const o = (__bf16*)g.dz + m * g.lddz;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const u32x4 v = pair(acc[i][2 * p], acc[i][2 * p + 1]);
-                if (m < g.M && pcol + 32 * p < g.Npad) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
-            }
-            if (g.dzt) {
-                // neighbouring lanes hold neighbouring labels: they trade halves, so that each has 2 labels of 2 classes
-                const int me = m & ~1;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t d0 = lb_pack(acc[i][j][0], acc[i][j][1]), d1 = lb_pack(acc[i][j][2], acc[i][j][3]);
-                    const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? d0 : d1), 0xb1, 0xf, 0xf, false);
-                    const uint32_t lo = odd ? t : d0, hi = odd ? d1 : t;          // label me, me + 1 of classes ncol + tcol, + 1
-                    const uint32_t c0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u), c1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                    const int n = ncol(j) + tcol;
-                    if (me < g.Mpad) {
-                        if (n < g.N) *reinterpret_cast<uint32_t*>((__bf16*)g.dzt + n * g.lddzt + me) = c0;
-                        if (n + 1 < g.N) *reinterpret_cast<uint32_t*>((__bf16*)g.dzt + (n + 1) * g.lddzt + me) = c1;
-                    }
-                }
-            }
         }
         if (g.colsum) {
             float* const red = reinterpret_cast<float*>(smem);     // [wm][256 classes]
@@ -261,11 +251,52 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
             __syncthreads();
             if (n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LB_T + tid];
         }
+        const bool odd = lane & 1;
+        const int tcol = 2 * (lane & 1);
+#pragma unroll
+        for (int pl = 0; pl < (PL ? 3 : 1); ++pl) {
+            __bf16* const dz = (__bf16*)g.dz + (PL ? (long long)pl * g.Npad : 0);
+            __bf16* const dzt = (__bf16*)g.dzt + (PL ? (long long)pl * g.Mpad : 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int m = mrow(i);
+                __bf16* const o = dz + m * g.lddz;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const u32x4 v = pairs(acc[i][2 * p], acc[i][2 * p + 1]);
+                    if (m < g.M && pcol + 32 * p < g.Npad) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
+                }
+                if (g.dzt) {
+                    // neighbouring lanes hold neighbouring labels: they trade halves, so that each has 2 labels of 2 classes
+                    const int me = m & ~1;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t d0 = lb_pack(acc[i][j][0], acc[i][j][1]), d1 = lb_pack(acc[i][j][2], acc[i][j][3]);
+                        const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? d0 : d1), 0xb1, 0xf, 0xf, false);
+                        const uint32_t lo = odd ? t : d0, hi = odd ? d1 : t;          // label me, me + 1 of classes ncol + tcol, + 1
+                        const uint32_t c0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u), c1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                        const int n = ncol(j) + tcol;
+                        if (me < g.Mpad) {
+                            if (n < g.N) *reinterpret_cast<uint32_t*>(dzt + n * g.lddzt + me) = c0;
+                            if (n + 1 < g.N) *reinterpret_cast<uint32_t*>(dzt + (n + 1) * g.lddzt + me) = c1;
+                        }
+                    }
+                }
+                if constexpr (PL)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] -= (float)(__bf16)acc[i][j][e];
+            }
+        }
     }
 }
 
-void fea_lin_gemm256(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE>), dim3(grid), dim3(256), 0, s, g);
-    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ>), dim3(grid), dim3(256), 0, s, g);
-    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE>), dim3(grid), dim3(256), 0, s, g);
+template <bool PL> static void lb_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE, PL>), dim3(grid), dim3(256), 0, s, g);
+    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ, PL>), dim3(grid), dim3(256), 0, s, g);
+    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE, PL>), dim3(grid), dim3(256), 0, s, g);
+}
+void fea_lin_gemm256(int epi, bool planes, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (planes) lb_launch<true>(epi, g, grid, s); else lb_launch<false>(epi, g, grid, s);
 }

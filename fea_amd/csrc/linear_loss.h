@@ -7,7 +7,16 @@
 // LIN_STORE is a plain product.  Row starts are 16-byte aligned, K is a multiple of 16 bytes of elements.
 enum { LIN_LSE = 0, LIN_DZ = 1, LIN_STORE = 2 };
 
+// fp32 operands of large products as three bf16 planes: x = x0 + x1 + x2, each the rounding of what the ones before leave, so the sum holds
+// all 24 bits.  A row is [plane 0 | plane 1 | plane 2] of Kp (a multiple of 64) elements, zero behind the end.  A product runs over the six
+// pairs of planes whose weight is above 2^-24 (x1 y1, x2 y0, x0 y2, x1 y0, x0 y1, x0 y0, the small ones first, all into one fp32 sum): the
+// bf16 matrix rate is 16 times the fp32 one, so six products still gain 2.7.  FEA_PL is the form's dtype code inside these files.
+#define FEA_PL 2
+__device__ __forceinline__ int lin_plane_a(int pair) { return (0x001021 >> (4 * pair)) & 15; }
+__device__ __forceinline__ int lin_plane_b(int pair) { return (0x010201 >> (4 * pair)) & 15; }
+
 struct LinGemm {
+    int Kp;                           // FEA_PL: elements of a plane; K = 6 Kp
     const void *a, *b;
     long long lda, ldb;
     int M, N, K;                      // rows of A, rows of B, reduction
@@ -79,10 +88,10 @@ int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s);
 int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 
 // linear_gemm.hip: which tile a product takes (256: linear_gemm256.hip, 128: linear_gemm.hip) and into how many parts its reduction is split
-struct LinTile { int tile, splits; };
+struct LinTile { int tile, splits; double time; };
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split);
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s);
 // linear_rows.hip: LIN_LSE of up to 64 label rows; g.part [M][classes / 64]
 int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s);
 // linear_gemm256.hip
-void fea_lin_gemm256(int epi, const LinGemm& g, unsigned grid, hipStream_t s);
+void fea_lin_gemm256(int epi, bool planes, const LinGemm& g, unsigned grid, hipStream_t s);

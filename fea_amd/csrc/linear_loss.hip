@@ -27,27 +27,100 @@ __global__ __launch_bounds__(256) void lin_pack_kernel(const T* __restrict__ in,
     }
 }
 
-// out[c][r] = in[r][c] (r < R), zero for R <= r < Rpad; rows whose gate is 0 count as zeros: what an ignored row holds (an
-// infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must not reach the weight.  gout (nullable): rows
-// times their own upstream gradient.
-template <typename T>
-__global__ __launch_bounds__(256) void lin_transpose_kernel(const T* __restrict__ in, long long ld, T* __restrict__ out, long long ldo,
-                                                            long long R, long long Rpad, int C, const float2* __restrict__ stat,
-                                                            const float* __restrict__ gout, float t) {
-    __shared__ T tile[64][64 + 8 / sizeof(T)];
+// x as three bf16 planes (linear_loss.h): what each leaves goes to the next
+__device__ __forceinline__ void lin_split3(float v, __bf16& x0, __bf16& x1, __bf16& x2) {
+    x0 = (__bf16)v; v -= (float)x0;
+    x1 = (__bf16)v; v -= (float)x1;
+    x2 = (__bf16)v;
+}
+
+// out[r][plane][c] = planes of in[r][c], zero for C <= c < Kp: 8 elements per thread
+__global__ __launch_bounds__(256) void lin_planes_kernel(const float* __restrict__ in, long long ld, __bf16* __restrict__ out, int Kp, int C, long long total8) {
+    const int per = Kp / 8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total8; i += (long long)gridDim.x * 256) {
+        const long long r = i / per;
+        const int c = (int)(i - r * per) * 8;
+        const float* p = in + r * ld + c;
+        __bf16 x[3][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lin_split3(c + e < C ? p[e] : 0.f, x[0][e], x[1][e], x[2][e]);
+        __bf16* o = out + r * 3 * Kp + c;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(o + (long long)q * Kp) = *reinterpret_cast<const u32x4*>(x[q]);
+    }
+}
+
+// out[c][r] = in[r][c] (r < R), zero for R <= r < Rpad (a multiple of 64); rows whose gate is 0 count as zeros: what an ignored row
+// holds (an infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must not reach the weight.  gout
+// (nullable): rows times their own upstream gradient.  64 x 64 tiles.
+struct LinTrans { long long ld, ldo, R, Rpad; int C; const float2* stat; const float* gout; float t; };
+
+__device__ __forceinline__ float lin_trans_factor(const LinTrans& a, long long r) { return a.gout ? lin_row_scale(a.gout, 1, nullptr, a.t, 1.f, r) : 1.f; }
+
+// fp32 (out fp32, or three bf16 planes per row of out: PL)
+template <bool PL>
+__global__ __launch_bounds__(256) void lin_transpose32_kernel(const float* __restrict__ in, void* __restrict__ out, const LinTrans a) {
+    __shared__ float tile[64][65];
     const long long r0 = (long long)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
 #pragma unroll 4
     for (int i = y; i < 64; i += 4) {
         const long long r = r0 + i;
-        T v = r < R && c0 + x < C && (!stat || stat[r].y != 0.f) ? in[r * ld + c0 + x] : from_f32<T>(0.f);
-        if (gout && r < R && stat[r].y != 0.f) v = from_f32<T>(to_f32(v) * lin_row_scale(gout, 1, nullptr, t, 1.f, r));
-        tile[i][x] = v;
+        const bool on = r < a.R && (!a.stat || a.stat[r].y != 0.f);
+        tile[i][x] = on && c0 + x < a.C ? in[r * a.ld + c0 + x] * lin_trans_factor(a, r) : 0.f;
     }
     __syncthreads();
+    if constexpr (!PL) {
 #pragma unroll 4
-    for (int i = y; i < 64; i += 4)
-        if (c0 + i < C && r0 + x < Rpad) out[(long long)(c0 + i) * ldo + r0 + x] = tile[x][i];
+        for (int i = y; i < 64; i += 4)
+            if (c0 + i < a.C) ((float*)out)[(c0 + i) * a.ldo + r0 + x] = tile[x][i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = (threadIdx.x >> 3) + 32 * i, q = (threadIdx.x & 7) * 8;
+            if (c0 + c >= a.C) continue;
+            __bf16 v[3][8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) lin_split3(tile[q + e][c], v[0][e], v[1][e], v[2][e]);
+            __bf16* o = (__bf16*)out + (c0 + c) * a.ldo + r0 + q;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(o + p * a.Rpad) = *reinterpret_cast<const u32x4*>(v[p]);
+        }
+    }
+}
+
+// bf16: 16-byte loads and stores; a thread turns 2 rows x 8 columns into 8 dwords (two rows of a column each) on the way into LDS
+template <bool ALN>
+__global__ __launch_bounds__(256) void lin_transpose16_kernel(const __bf16* __restrict__ in, __bf16* __restrict__ out, const LinTrans a) {
+    __shared__ __attribute__((aligned(16))) uint32_t tile[64][36];        // [column][row pair]
+    const long long r0 = (long long)blockIdx.x * 64;
+    const int c0 = blockIdx.y * 64, hi = threadIdx.x >> 3, lo = threadIdx.x & 7;
+    u32x4 v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const long long r = r0 + 2 * hi + i;
+        const bool on = r < a.R && (!a.stat || a.stat[r].y != 0.f);
+        v[i] = on ? lin_load16<__bf16, ALN>(in + r * a.ld + c0 + 8 * lo, a.C - c0 - 8 * lo) : u32x4{0, 0, 0, 0};
+        if (a.gout && on) {
+            const float f = lin_trans_factor(a, r);
+            __bf16 x[8];
+            *reinterpret_cast<u32x4*>(x) = v[i];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (__bf16)((float)x[e] * f);
+            v[i] = *reinterpret_cast<const u32x4*>(x);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        tile[8 * lo + 2 * j][hi] = __builtin_amdgcn_perm(v[1][j], v[0][j], 0x05040100u);
+        tile[8 * lo + 2 * j + 1][hi] = __builtin_amdgcn_perm(v[1][j], v[0][j], 0x07060302u);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = hi + 32 * i;
+        if (c0 + c < a.C) *reinterpret_cast<u32x4*>(out + (c0 + c) * a.ldo + r0 + 8 * lo) = *reinterpret_cast<const u32x4*>(&tile[c][4 * lo]);
+    }
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
@@ -107,20 +180,10 @@ __device__ __forceinline__ float lin_tlog(const LinJoin& j, long long e) {
 }
 
 // G lanes join the column tiles of a row and turn its selected logits into the loss and the gradient at the selected classes.
-__device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, long long row, bool in) {
+__device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, long long row, bool in, float lse) {
     float loss = 0.f;
     bool counts = false;
     {
-        float mx = -INFINITY, sum = 0.f;
-        if (in) {
-            for (int i = gl; i < j.ntn; i += G) mx = fmaxf(mx, j.part[row * j.ntn + i].x);
-        }
-        for (int d = G >> 1; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-        const float base = mx == -INFINITY ? 0.f : mx;
-        if (in)
-            for (int i = gl; i < j.ntn; i += G) { const float2 p = j.part[row * j.ntn + i]; sum += p.y * expf(p.x - base); }
-        for (int d = G >> 1; d; d >>= 1) sum += __shfl_xor(sum, d);
-        float lse = logf(sum) + base;
         const long long e0 = row * j.K;
         if (!j.tlog) {
             const long long t = in ? j.index[row] : j.ignore;
@@ -190,25 +253,47 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
     }
 }
 
+// (max, sum) of two parts
+__device__ __forceinline__ float2 lin_merge(float2 a, float2 b) {
+    const float mx = fmaxf(a.x, b.x), base = mx == -INFINITY ? 0.f : mx;
+    return make_float2(mx, a.y * expf(a.x - base) + b.y * expf(b.x - base));
+}
+__device__ __forceinline__ float2 lin_merge_lanes(float2 a, int G) {
+    for (int d = G >> 1; d; d >>= 1) a = lin_merge(a, make_float2(__shfl_xor(a.x, d), __shfl_xor(a.y, d)));
+    return a;
+}
+__device__ __forceinline__ float lin_lse_of(float2 a) { return logf(a.y) + (a.x == -INFINITY ? 0.f : a.x); }
+
 __global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
     const long long row = (long long)blockIdx.x * (256 / j.G) + threadIdx.x / j.G;
-    lin_join_body(j, j.G, threadIdx.x % j.G, row, row < j.rows);
+    const int gl = threadIdx.x % j.G;
+    float2 a = make_float2(-INFINITY, 0.f);
+    if (row < j.rows)
+#pragma unroll 4
+        for (int i = gl; i < j.ntn; i += j.G) a = lin_merge(a, j.part[row * j.ntn + i]);
+    lin_join_body(j, j.G, gl, row, row < j.rows, lin_lse_of(lin_merge_lanes(a, j.G)));
 }
 
-// The same for few rows, one workgroup per row, the selected logits and the join in one launch: all waves take entries, then the
-// first one joins.
+// The same for few rows, one workgroup per row, the selected logits and the join in one launch: all waves take entries and tiles,
+// then the first one joins.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_join_rows_kernel(const LinJoin j, const T* h, long long ldh, const T* w, long long ldw, const float* bias, int D, int vec) {
+    __shared__ float2 red[4];
     const long long row = blockIdx.x;
+    float2 a = make_float2(-INFINITY, 0.f);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < j.ntn; i += 256) a = lin_merge(a, j.part[row * j.ntn + i]);
     for (int k = threadIdx.x >> 6; k < j.K; k += 4) {
         const long long i = j.index[row * j.K + k];
         if (i < 0 || i >= j.V) continue;
         const float s = vec ? lin_dot<T, true>(h + row * ldh, w + i * ldw, D, threadIdx.x & 63, 64) : lin_dot<T, false>(h + row * ldh, w + i * ldw, D, threadIdx.x & 63, 64);
         if ((threadIdx.x & 63) == 0) j.zsel[row * j.K + k] = bias ? s + bias[i] : s;
     }
+    a = lin_merge_lanes(a, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __threadfence_block();
     __syncthreads();
-    lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64);
+    lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64, lin_lse_of(lin_merge(lin_merge(red[0], red[1]), lin_merge(red[2], red[3]))));
 }
 
 // loss[0] = sum, or sum / rows that count (0 where none does); count[0] = rows that count
@@ -234,17 +319,27 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 
 // dz at the selected classes of the piece [v0, v0 + N): softmax - teacher, from the forward's fp32 values.  Entries that name the
 // same class hold the same value.
-template <typename T>
+template <typename T, bool PL>
 __global__ __launch_bounds__(256) void lin_scatter_kernel(const long long* __restrict__ index, const float* __restrict__ dsel, int K,
-                                                          const float2* __restrict__ stat, T* dz, long long lddz, T* dzt, long long lddzt, long long v0, int N, long long entries) {
+                                                          const float2* __restrict__ stat, T* dz, long long lddz, T* dzt, long long lddzt, long long v0, int N, long long entries,
+                                                          int Npad, long long Mpad) {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= entries) return;
     const long long m = e / K, i = index[e] - v0;
     if (i < 0 || i >= N) return;
     if (stat[m].y == 0.f) return;
-    const T v = from_f32<T>(dsel[e]);
-    dz[m * lddz + i] = v;
-    if (dzt) dzt[i * lddzt + m] = v;
+    if constexpr (PL) {
+        T x[3];
+        lin_split3(dsel[e], x[0], x[1], x[2]);
+        for (int p = 0; p < 3; ++p) {
+            dz[m * lddz + (long long)p * Npad + i] = x[p];
+            if (dzt) dzt[i * lddzt + p * Mpad + m] = x[p];
+        }
+    } else {
+        const T v = from_f32<T>(dsel[e]);
+        dz[m * lddz + i] = v;
+        if (dzt) dzt[i * lddzt + m] = v;
+    }
 }
 
 // out = acc + slabs in split order; acc (nullable) is the fp32 sum of earlier pieces, accout where later ones follow
@@ -327,28 +422,45 @@ struct LinCarve {
 
 struct LinDims {
     long long rows; int D, V, K, dtype, es, epc;
-    int Dp;                       // D rounded up to 16 bytes: operands with another D are copied with zeros behind it
-    bool packed() const { return Dp != D; }
+    bool odd() const { return D % epc != 0; }      // rows that are no multiple of 16 bytes
     bool wide;                    // row strides of 2^21 elements or more (a slice of something very wide): the 128 tile, which has 64-bit offsets
 };
 
 static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
-    LinDims d{rows, D, V, K, dtype, dtype == FEA_BF16 ? 2 : 4, dtype == FEA_BF16 ? 8 : 4, 0, false};
-    d.Dp = (int)up(D, d.epc);
+    LinDims d{rows, D, V, K, dtype, dtype == FEA_BF16 ? 2 : 4, dtype == FEA_BF16 ? 8 : 4, false};
     return d;
 }
 
+// The form that a call's products take: the operands as they are, or fp32 as three bf16 planes where the copies pay.
+struct LinForm {
+    int dt, es, mul, pad;         // dtype of the products, bytes of an element, elements of a row per channel, what a row is rounded up to
+    long long row(long long k) const { return up(k, pad) * mul; }          // elements of a row of k channels
+    int K(long long k) const { return (int)(dt == FEA_PL ? 6 * up(k, 64) : up(k, pad)); }
+};
+static LinForm lin_form(int dtype, bool planes) {
+    if (planes) return LinForm{FEA_PL, 2, 3, 64};
+    return dtype == FEA_BF16 ? LinForm{FEA_BF16, 2, 1, 64} : LinForm{FEA_F32, 4, 1, 64};
+}
+
 // Forward: rows in chunks that bound the partial table to 128 MB.
-struct LinFwd { long long rc; int tile, ntn, G; long long blocks; };
+struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; };
 static LinFwd lin_fwd_plan(const LinDims& d) {
     LinFwd p;
     const long long cap = (1ll << 24) / ((d.V + 127) / 128);
     p.rc = cap < 256 ? 256 : cap / 256 * 256;
     if (p.rc > d.rows) p.rc = d.rows;
-    p.tile = d.rows <= 64 ? 64 : d.wide ? 128 : fea_lin_tile(d.dtype, p.rc, d.V, d.Dp, false).tile;
+    LinTile t = fea_lin_tile(d.dtype, p.rc, d.V, d.D, false);
+    p.planes = false;
+    if (d.dtype == FEA_F32) {     // 10 bytes per element for the copies, against a third of the matrix time
+        const LinTile q = fea_lin_tile(FEA_PL, p.rc, d.V, 6 * up(d.D, 64), false);
+        if (q.time + ((double)p.rc + d.V) * d.D * 10 / 4e12 + 6e-6 < t.time) { t = q; p.planes = true; }
+    }
+    p.tile = t.tile;
+    if (d.wide && !p.planes) p.tile = 128;
+    if (d.rows <= 64) { p.tile = 64; p.planes = false; }
     p.ntn = (d.V + p.tile - 1) / p.tile;
     p.G = 1;
-    while (p.G < 64 && (p.G < p.ntn || p.G < d.K)) p.G *= 2;
+    while (p.G < 64 && (p.G < (d.V + 127) / 128 || p.G < d.K)) p.G *= 2;
     p.blocks = p.tile == 64 ? d.rows : (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
     return p;
 }
@@ -360,8 +472,8 @@ static long long lin_piece() {
     const long long v = e ? atoll(e) : 0;
     return v >= 1 << 14 && v < 1 << 28 ? v : 1ll << 28;
 }
-struct LinBwd { long long rc; int vc, nrc, nvc, tz; LinTile th, tw; };
-static LinBwd lin_bwd_plan(const LinDims& d) {
+struct LinBwd { long long rc; int vc, nrc, nvc, tz; bool planes; LinTile th, tw; };
+static LinBwd lin_bwd_plan(const LinDims& d, int want) {
     LinBwd p;
     const long long piece = lin_piece();
     p.rc = d.rows < 32768 ? d.rows : 32768;
@@ -371,9 +483,21 @@ static LinBwd lin_bwd_plan(const LinDims& d) {
     p.vc = (int)(vc < d.V ? vc : d.V);
     p.nrc = p.rc ? (int)((d.rows + p.rc - 1) / p.rc) : 0;
     p.nvc = (d.V + p.vc - 1) / p.vc;
-    p.tz = d.wide ? 128 : fea_lin_tile(d.dtype, p.rc, p.vc, d.Dp, false).tile;
-    p.th = fea_lin_tile(d.dtype, p.rc, d.D, p.vc, true);
-    p.tw = fea_lin_tile(d.dtype, p.vc, d.D, p.rc, true);
+    LinTile tz;
+    auto tiles = [&](int dt, int mul, LinTile& z, LinTile& h, LinTile& w) {
+        z = fea_lin_tile(dt, p.rc, p.vc, mul * up(d.D, 64), false);
+        h = fea_lin_tile(dt, p.rc, d.D, mul * up(p.vc, 64), true);
+        w = fea_lin_tile(dt, p.vc, d.D, mul * up(p.rc, 64), true);
+        return z.time + (want & 1 ? h.time : 0.0) + (want & 2 ? w.time : 0.0);
+    };
+    const double t = tiles(d.dtype, 1, tz, p.th, p.tw);
+    p.planes = false;
+    if (d.dtype == FEA_F32 && 3 * up(p.rc > p.vc ? p.rc : p.vc, 64) < 1 << 21) {     // (the strides that the large tile takes)
+        LinTile z, h, w;
+        const double q = tiles(FEA_PL, 6, z, h, w);
+        if (q + (((double)p.rc + p.vc) * d.D * 12 + 4.0 * p.rc * p.vc) / 4e12 + 6e-6 < t) { tz = z; p.th = h; p.tw = w; p.planes = true; }
+    }
+    p.tz = d.wide && !p.planes ? 128 : tz.tile;
     return p;
 }
 
@@ -386,19 +510,23 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
         w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows));
         return c.at;
     }
-    w.part = c.take<float2>(p.rc * ((d.V + (p.tile == 64 ? 63 : 127)) / (p.tile == 64 ? 64 : 128)));           // (sized for the smaller tile: row strides may ask for it)
+    const int t = p.tile == 64 ? 64 : 128;               // (not 256: wide row strides, which a size query does not know, ask for 128)
+    w.part = c.take<float2>(p.rc * ((d.V + t - 1) / t));
     w.zsel = c.take<float>(d.rows * d.K);
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
     w.hp = w.wp = nullptr;
-    if (d.packed() && p.tile == 256) { w.hp = c.take<char>(p.rc * d.Dp * d.es); w.wp = c.take<char>((long long)d.V * d.Dp * d.es); }
+    if (p.planes || (d.odd() && p.tile == 256)) {
+        const LinForm f = lin_form(d.dtype, p.planes);
+        w.hp = c.take<char>(p.rc * f.row(d.D) * f.es);
+        w.wp = c.take<char>(d.V * f.row(d.D) * f.es);
+    }
     return c.at;
 }
 
 struct LinBwdWs { void *hp, *wp, *ht, *wt, *dz, *dzt; float *slab, *acch, *accw, *colsum; double* dbpart; };
 static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* base, LinBwdWs& w) {
     LinCarve c{base};
-    const long long vp = up(p.vc, d.epc), rp = up(p.rc, d.epc);
     w = LinBwdWs{};
     if (fea_lin_few(d.rows, d.D, d.V)) {
         if (want & 2) w.slab = c.take<float>(fea_lin_few_blocks(d.rows) * 32ll * 64);
@@ -406,10 +534,11 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
         w.dz = c.take<char>(256);
         return c.at;
     }
-    if (d.packed() && p.tz == 256) { w.hp = c.take<char>(p.rc * d.Dp * d.es); w.wp = c.take<char>((long long)p.vc * d.Dp * d.es); }
-    w.dz = c.take<char>(p.rc * vp * d.es);
-    if (want & 2) { w.dzt = c.take<char>(p.vc * rp * d.es); w.ht = c.take<char>(d.D * rp * d.es); }
-    if (want & 1) w.wt = c.take<char>(d.D * vp * d.es);
+    const LinForm f = lin_form(d.dtype, p.planes);
+    if (p.planes || (d.odd() && p.tz == 256)) { w.hp = c.take<char>(p.rc * f.row(d.D) * f.es); w.wp = c.take<char>(p.vc * f.row(d.D) * f.es); }
+    w.dz = c.take<char>(p.rc * f.row(p.vc) * f.es);
+    if (want & 2) { w.dzt = c.take<char>(p.vc * f.row(p.rc) * f.es); w.ht = c.take<char>(d.D * f.row(p.rc) * f.es); }
+    if (want & 1) w.wt = c.take<char>(d.D * f.row(p.vc) * f.es);
     long long slab = 0;
     if ((want & 1) && (p.th.splits > 1 || p.nvc > 1)) slab = p.th.splits * p.rc * d.D;
     if ((want & 2) && (p.tw.splits > 1 || p.nrc > 1) && slab < (long long)p.tw.splits * p.vc * d.D) slab = (long long)p.tw.splits * p.vc * d.D;
@@ -425,22 +554,29 @@ extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, 
     const LinDims d = lin_dims(rows, D, V, K, dtype);
     if (!grads) { LinFwdWs w; return lin_fwd_carve(d, lin_fwd_plan(d), nullptr, w); }
     LinBwdWs w;
-    return lin_bwd_carve(d, lin_bwd_plan(d), grads, nullptr, w);
+    return lin_bwd_carve(d, lin_bwd_plan(d, grads), grads, nullptr, w);
 }
 
-static int lin_pack(const LinDims& d, const void* in, long long ld, void* out, long long R, hipStream_t s) {
-    const long long n = R * d.Dp;
-    const unsigned grid = (unsigned)(n / 1024 < 1 ? 1 : n / 1024 > 16384 ? 16384 : n / 1024);
-    if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_pack_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)in, ld, (__bf16*)out, d.Dp, d.D, n);
-    else                     hipLaunchKernelGGL(lin_pack_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)in, ld, (float*)out, d.Dp, d.D, n);
+// rows of D elements as the products take them: planes, or copies with zeros behind the end
+static int lin_pack(const LinDims& d, const LinForm& f, const void* in, long long ld, void* out, long long R, hipStream_t s) {
+    const int Cp = (int)up(d.D, f.pad);
+    const long long n = f.dt == FEA_PL ? R * Cp / 8 : R * Cp, b = (n + 1023) / 1024;
+    const unsigned grid = (unsigned)(b > 16384 ? 16384 : b);
+    if (f.dt == FEA_PL)        hipLaunchKernelGGL(lin_planes_kernel, dim3(grid), dim3(256), 0, s, (const float*)in, ld, (__bf16*)out, Cp, d.D, n);
+    else if (f.dt == FEA_BF16) hipLaunchKernelGGL(lin_pack_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)in, ld, (__bf16*)out, Cp, d.D, n);
+    else                       hipLaunchKernelGGL(lin_pack_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)in, ld, (float*)out, Cp, d.D, n);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
 
-static int lin_transpose(const LinDims& d, const void* in, long long ld, void* out, long long ldo, long long R, long long Rpad, const float2* stat, const float* gout, float t, hipStream_t s) {
-    const dim3 grid((unsigned)((Rpad + 63) / 64), (unsigned)((d.D + 63) / 64));
-    if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_transpose_kernel<__bf16>, grid, dim3(256), 0, s, (const __bf16*)in, ld, (__bf16*)out, ldo, R, Rpad, d.D, stat, gout, t);
-    else                     hipLaunchKernelGGL(lin_transpose_kernel<float>, grid, dim3(256), 0, s, (const float*)in, ld, (float*)out, ldo, R, Rpad, d.D, stat, gout, t);
+static int lin_transpose(const LinDims& d, const LinForm& f, const void* in, long long ld, void* out, long long R, const float2* stat, const float* gout, float t, hipStream_t s) {
+    const long long Rp = up(R, f.pad);
+    const LinTrans a{ld, f.row(R), R, Rp, d.D, stat, gout, t};
+    const dim3 grid((unsigned)(Rp / 64), (unsigned)((d.D + 63) / 64));
+    if (f.dt == FEA_PL)       hipLaunchKernelGGL(lin_transpose32_kernel<true>, grid, dim3(256), 0, s, (const float*)in, out, a);
+    else if (f.dt == FEA_F32) hipLaunchKernelGGL(lin_transpose32_kernel<false>, grid, dim3(256), 0, s, (const float*)in, out, a);
+    else if (d.odd())         hipLaunchKernelGGL(lin_transpose16_kernel<false>, grid, dim3(256), 0, s, (const __bf16*)in, (__bf16*)out, a);
+    else                      hipLaunchKernelGGL(lin_transpose16_kernel<true>, grid, dim3(256), 0, s, (const __bf16*)in, (__bf16*)out, a);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
@@ -464,7 +600,7 @@ static int lin_check(const char* who, const LinDims& d, const void* h, long long
     FEA_CHECK(h && w, FEA_E_BADARG, "%s: null operand", who);
     FEA_CHECK(ldh >= d.D && ldw >= d.D, FEA_E_BADARG, "%s: row stride below the %d features (hidden %lld, weight %lld)", who, d.D, ldh, ldw);
     FEA_CHECK(((uintptr_t)h | (uintptr_t)w) % d.es == 0 && (uintptr_t)bias % 4 == 0, FEA_E_BADARG, "%s: misaligned operand", who);
-    if (!d.packed())
+    if (!d.odd())
         FEA_CHECK(((uintptr_t)h | (uintptr_t)w) % 16 == 0 && ldh % d.epc == 0 && ldw % d.epc == 0, FEA_E_BADARG,
                   "%s: hidden and weight need 16-byte aligned rows when the features are a multiple of %d", who, d.epc);
     return FEA_OK;
@@ -473,7 +609,7 @@ static int lin_check(const char* who, const LinDims& d, const void* h, long long
 static int lin_forward(const char* who, LinDims d, const void* h, long long ldh, const void* w, long long ldw, const float* bias, LinJoin j,
                        float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
-    d.wide = !d.packed() && (ldh >= 1 << 21 || ldw >= 1 << 21);
+    d.wide = !d.odd() && (ldh >= 1 << 21 || ldw >= 1 << 21);
     const LinFwd p = lin_fwd_plan(d);
     LinFwdWs b;
     const size_t need = lin_fwd_carve(d, p, (char*)ws, b);
@@ -499,26 +635,24 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         while (lanes < 64 && lanes * d.epc < d.D) lanes *= 2;
         const long long blocks = (entries * lanes + 255) / 256;
         const unsigned grid = (unsigned)(blocks < 1 << 16 ? blocks : 1 << 16);
-        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.packed() ? 0 : 1);
-        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.packed() ? 0 : 1);
+        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.odd() ? 0 : 1);
+        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.odd() ? 0 : 1);
         FEA_LAUNCH_CHECK();
     }
-    const void* wm = w;
-    long long ldwm = ldw;
-    const bool pack = d.packed() && p.tile == 256;       // (the other kernels take rows of any alignment)
-    const int Kg = pack ? d.Dp : d.D;
-    if (pack) { LIN_TRY(lin_pack(d, w, ldw, b.wp, d.V, s)); wm = b.wp; ldwm = d.Dp; }
+    const LinForm f = lin_form(d.dtype, p.planes);
+    const bool pack = p.planes || (d.odd() && p.tile == 256);       // (the other kernels take rows of any alignment)
+    if (pack) LIN_TRY(lin_pack(d, f, w, ldw, b.wp, d.V, s));
     long long blk = 0;
     for (long long r = 0; r < d.rows; r += p.rc) {
         const long long n = d.rows - r < p.rc ? d.rows - r : p.rc;
-        const void* hm = (const char*)h + r * ldh * d.es;
-        long long ldhm = ldh;
-        if (pack) { LIN_TRY(lin_pack(d, hm, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
+        const void* hr = (const char*)h + r * ldh * d.es;
+        if (pack) LIN_TRY(lin_pack(d, f, hr, ldh, b.hp, n, s));
         LinGemm g{};
-        g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = d.V; g.K = Kg;
+        g.a = pack ? b.hp : hr; g.lda = pack ? f.row(d.D) : ldh; g.b = pack ? b.wp : w; g.ldb = pack ? f.row(d.D) : ldw;
+        g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
-        if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.packed(), g, s));
-        else LIN_TRY(fea_lin_gemm(LIN_LSE, d.dtype, p.tile, g, s));
+        if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
+        else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;
         q.part = b.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
         q.zsel = b.zsel + r * d.K; q.index = j.index + r * d.K;
@@ -530,8 +664,8 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         q.bsum = loss ? b.bsum + blk : nullptr; q.bcnt = b.bcnt + blk;
         const long long grid = p.tile == 64 ? n : (n + 256 / p.G - 1) / (256 / p.G);
         if (p.tile != 64)               hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
-        else if (d.dtype == FEA_BF16)   hipLaunchKernelGGL(lin_join_rows_kernel<__bf16>, dim3((unsigned)grid), dim3(256), 0, s, q, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, d.D, d.packed() ? 0 : 1);
-        else                            hipLaunchKernelGGL(lin_join_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, q, (const float*)h, ldh, (const float*)w, ldw, bias, d.D, d.packed() ? 0 : 1);
+        else if (d.dtype == FEA_BF16)   hipLaunchKernelGGL(lin_join_rows_kernel<__bf16>, dim3((unsigned)grid), dim3(256), 0, s, q, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, d.D, d.odd() ? 0 : 1);
+        else                            hipLaunchKernelGGL(lin_join_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, q, (const float*)h, ldh, (const float*)w, ldw, bias, d.D, d.odd() ? 0 : 1);
         FEA_LAUNCH_CHECK();
         blk += grid;
     }
@@ -573,14 +707,15 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     LinDims d = lin_dims(rows, D, V, K, dtype);
     hipStream_t s = (hipStream_t)stream;
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
-    d.wide = !d.packed() && (ldh >= 1 << 21 || ldw >= 1 << 21);
+    d.wide = !d.odd() && (ldh >= 1 << 21 || ldw >= 1 << 21);
     FEA_CHECK(index && stat && dsel && gout, FEA_E_BADARG, "%s: null operand", who);
     FEA_CHECK(gout_stride == 0 || gout_stride == 1, FEA_E_BADARG, "%s: gout_stride %d", who, gout_stride);
     FEA_CHECK(dh || dw || db, FEA_E_BADARG, "%s: no gradient asked for", who);
+    FEA_CHECK(((uintptr_t)dh | (uintptr_t)dw) % 16 == 0 && (uintptr_t)db % 4 == 0, FEA_E_BADARG, "%s: misaligned gradient", who);
     FEA_CHECK(K == 1 || !db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
     FEA_CHECK(temperature > 0.f && isfinite(temperature) && isfinite(1.f / temperature), FEA_E_BADARG, "%s: temperature %g", who, (double)temperature);
     const int want = (dh ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0);
-    const LinBwd p = lin_bwd_plan(d);
+    const LinBwd p = lin_bwd_plan(d, want);
     LinBwdWs b;
     const size_t need = lin_bwd_carve(d, p, want, (char*)ws, b);
     FEA_CHECK(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, FEA_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, need, ws_bytes);
@@ -592,36 +727,34 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
         f.dh = dh; f.slab = b.slab; f.dbslab = b.colsum; f.rows = rows; f.D = D; f.V = V; f.K = K;
         return fea_lin_few_bwd(f, dtype, dw, db, s);
     }
-    const int ck = 64;
-    const bool pack = d.packed() && p.tz == 256;
+    const LinForm f = lin_form(dtype, p.planes);
+    const bool pack = p.planes || (d.odd() && p.tz == 256);
     for (int ir = 0; ir < p.nrc; ++ir) {
-        const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc, np = up(n, d.epc);
+        const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc;
         const char* hr = (const char*)h + r0 * ldh * d.es;
         const float2* st = (const float2*)stat + r0;
         const float* go = gout + r0 * gout_stride;
-        const void* hm = hr;
-        long long ldhm = ldh;
-        if (pack) { LIN_TRY(lin_pack(d, hr, ldh, b.hp, n, s)); hm = b.hp; ldhm = d.Dp; }
-        if (dw) LIN_TRY(lin_transpose(d, hr, ldh, b.ht, np, n, np, st, gout_stride ? go : nullptr, temperature, s));
+        if (pack) LIN_TRY(lin_pack(d, f, hr, ldh, b.hp, n, s));
+        if (dw) LIN_TRY(lin_transpose(d, f, hr, ldh, b.ht, n, st, gout_stride ? go : nullptr, temperature, s));
         for (int iv = 0; iv < p.nvc; ++iv) {
             const long long v0 = (long long)iv * p.vc;
-            const int nv = (int)(V - v0 < p.vc ? V - v0 : p.vc), nvp = (int)up(nv, d.epc);
+            const int nv = (int)(V - v0 < p.vc ? V - v0 : p.vc);
             const char* wr = (const char*)w + v0 * ldw * d.es;
-            const void* wm = wr;
-            long long ldwm = ldw;
-            if (pack) { LIN_TRY(lin_pack(d, wr, ldw, b.wp, nv, s)); wm = b.wp; ldwm = d.Dp; }
+            if (pack) LIN_TRY(lin_pack(d, f, wr, ldw, b.wp, nv, s));
             LinGemm g{};
-            g.a = hm; g.lda = ldhm; g.b = wm; g.ldb = ldwm; g.M = (int)n; g.N = nv; g.K = pack ? d.Dp : D;
+            g.a = pack ? b.hp : (const void*)hr; g.lda = pack ? f.row(D) : ldh; g.b = pack ? b.wp : (const void*)wr; g.ldb = pack ? f.row(D) : ldw;
+            g.M = (int)n; g.N = nv; g.K = pack ? f.K(D) : D; g.Kp = (int)up(D, 64);
             g.bias = bias ? bias + v0 : nullptr; g.inv_t = 1.f / temperature; g.stat = st; g.gout = go; g.gstride = gout_stride;
             g.count = count; g.t = temperature;
-            g.dz = b.dz; g.lddz = nvp; g.Npad = nvp; g.dzt = dw ? b.dzt : nullptr; g.lddzt = np; g.Mpad = (int)np;
+            g.dz = b.dz; g.lddz = f.row(nv); g.Npad = (int)up(nv, f.pad); g.dzt = dw ? b.dzt : nullptr; g.lddzt = f.row(n); g.Mpad = (int)up(n, f.pad);
             g.colsum = db ? b.colsum : nullptr; g.ldcol = up(p.vc, 64);
-            LIN_TRY(fea_lin_gemm(LIN_DZ, dtype, p.tz, g, s));
+            LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
             const unsigned sg = (unsigned)((entries + 255) / 256);
-            if (dtype == FEA_BF16) hipLaunchKernelGGL(lin_scatter_kernel<__bf16>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, (long long)nvp, (__bf16*)g.dzt, np, v0, nv, entries);
-            else                   hipLaunchKernelGGL(lin_scatter_kernel<float>, dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, (long long)nvp, (float*)g.dzt, np, v0, nv, entries);
+            if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, (__bf16*)g.dzt, g.lddzt, v0, nv, entries, g.Npad, (long long)g.Mpad);
+            else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, (__bf16*)g.dzt, g.lddzt, v0, nv, entries, 0, 0ll);
+            else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, (float*)g.dzt, g.lddzt, v0, nv, entries, 0, 0ll);
             FEA_LAUNCH_CHECK();
             if (db) {
                 const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (tiles + LIN_DB_TILES - 1) / LIN_DB_TILES;
@@ -630,29 +763,27 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);
                 FEA_LAUNCH_CHECK();
             }
+            // out (contiguous rows of D) = A . B^T over k channels: straight to out, or through fp32 slabs where the reduction is split
+            // or pieces before this one (acc) or behind it add to the sum
+            auto product = [&](const LinGemm& from, const void* A, const void* B, long long M, long long k, const LinTile& t, void* out, float* acc, bool first, bool last) {
+                LinGemm m = from;
+                m.a = A; m.b = B; m.lda = m.ldb = f.row(k); m.M = (int)M; m.N = D; m.K = f.K(k); m.Kp = (int)up(k, 64);
+                m.splits = t.splits; m.kper = (int)up((m.K + t.splits - 1) / t.splits, 64);
+                const bool direct = t.splits == 1 && first && last;
+                if (direct && f.dt != FEA_PL) { m.out = out; m.ldo = D; } else m.slab = direct ? (float*)out : b.slab;
+                LIN_TRY(fea_lin_gemm(LIN_STORE, f.dt, t.tile, m, s));
+                return direct ? FEA_OK : lin_reduce(d, b.slab, t.splits, M * D, first ? nullptr : acc, last ? nullptr : acc, last ? out : nullptr, s);
+            };
+            LinGemm m{};
+            m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
             if (dh) {
-                LIN_TRY(lin_transpose(d, wr, ldw, b.wt, nvp, nv, nvp, nullptr, nullptr, 1.f, s));
-                LinGemm m{};
-                m.a = b.dz; m.lda = nvp; m.b = b.wt; m.ldb = nvp; m.M = (int)n; m.N = D; m.K = nvp;
-                m.scale = 1; m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
-                void* out = (char*)dh + r0 * D * d.es;
-                const bool direct = p.th.splits == 1 && p.nvc == 1;
-                m.splits = p.th.splits; m.kper = (int)up((nvp + m.splits - 1) / m.splits, ck);
-                if (direct) { m.out = out; m.ldo = D; } else m.slab = b.slab;
-                LIN_TRY(fea_lin_gemm(LIN_STORE, dtype, p.th.tile, m, s));
-                if (!direct) LIN_TRY(lin_reduce(d, b.slab, m.splits, n * D, iv > 0 ? b.acch : nullptr, iv + 1 < p.nvc ? b.acch : nullptr, iv + 1 < p.nvc ? nullptr : out, s));
+                LIN_TRY(lin_transpose(d, f, wr, ldw, b.wt, nv, nullptr, nullptr, 1.f, s));
+                m.scale = 1;
+                LIN_TRY(product(m, b.dz, b.wt, n, nv, p.th, (char*)dh + r0 * D * d.es, b.acch, iv == 0, iv + 1 == p.nvc));
             }
             if (dw) {
-                LinGemm m{};
-                m.a = b.dzt; m.lda = np; m.b = b.ht; m.ldb = np; m.M = nv; m.N = D; m.K = (int)np;
-                m.scale = gout_stride ? 0 : 2; m.gout = go; m.count = count; m.t = temperature;
-                void* out = (char*)dw + v0 * D * d.es;
-                float* acc = b.accw ? b.accw + v0 * D : nullptr;
-                const bool direct = p.tw.splits == 1 && p.nrc == 1;
-                m.splits = p.tw.splits; m.kper = (int)up((np + m.splits - 1) / m.splits, ck);
-                if (direct) { m.out = out; m.ldo = D; } else m.slab = b.slab;
-                LIN_TRY(fea_lin_gemm(LIN_STORE, dtype, p.tw.tile, m, s));
-                if (!direct) LIN_TRY(lin_reduce(d, b.slab, m.splits, (long long)nv * D, ir > 0 ? acc : nullptr, ir + 1 < p.nrc ? acc : nullptr, ir + 1 < p.nrc ? nullptr : out, s));
+                m.scale = gout_stride ? 0 : 2;
+                LIN_TRY(product(m, b.dzt, b.ht, nv, n, p.tw, (char*)dw + v0 * D * d.es, b.accw ? b.accw + v0 * D : nullptr, ir == 0, ir + 1 == p.nrc));
             }
         }
     }

@@ -18,10 +18,11 @@ __device__ __forceinline__ void mma16x16(f32x4& acc, const u32x4& a, const u32x4
     acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, acc, 0, 0, 0);
 }
 
-static constexpr int LR_CB = 512, LR_LD = LR_CB + 16;     // bytes of a chunk of a row; its distance in LDS (16 rows in 16 bank groups)
-
 template <typename T, int NR, bool ALN>
 __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
+    // bytes of a chunk of a row (with 64 labels half of it, so that four workgroups fit a CU: 1.5 rounds of two took 10 % longer than one of
+    // four); a row's distance in LDS puts 16 rows in 16 bank groups
+    constexpr int LR_CB = NR == 4 ? 256 : 512, LR_LD = LR_CB + 16, PR = LR_CB / 16;
     constexpr int EPC = Elem<T>::EPC, CE = LR_CB / (int)sizeof(T), NS = LR_CB / 64;     // elements, products of a chunk
     __shared__ __attribute__((aligned(16))) char hs[2][16 * NR * LR_LD];
     __shared__ float2 red[4][16 * NR];
@@ -37,12 +38,12 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
             wv[buf][s] = lin_load16<T, ALN>(w + k, g.K - k);
         }
     };
-    constexpr int HP = NR * 16 * (LR_CB / 16) / 256;          // 16-byte pieces of the labels' chunk per thread
+    constexpr int HP = NR * 16 * PR / 256;          // 16-byte pieces of the labels' chunk per thread
     u32x4 hv[HP];
     auto hload = [&](int k0) {
 #pragma unroll
         for (int i = 0; i < HP; ++i) {
-            const int p = tid + 256 * i, row = p >> 5, k = k0 + (p & 31) * EPC;
+            const int p = tid + 256 * i, row = p / PR, k = k0 + (p % PR) * EPC;
             hv[i] = row < g.M ? lin_load16<T, ALN>(h + row * g.lda + k, g.K - k) : u32x4{0, 0, 0, 0};
         }
     };
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
 #pragma unroll
         for (int i = 0; i < HP; ++i) {
             const int p = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(hs[buf] + (p >> 5) * LR_LD + (p & 31) * 16) = hv[i];
+            *reinterpret_cast<u32x4*>(hs[buf] + (p / PR) * LR_LD + (p % PR) * 16) = hv[i];
         }
     };
     f32x4 acc[NR];

@@ -358,9 +358,10 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
  * psel[rows][K] (all nullable).
  *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): recomputes the logits in pieces of the
- *     classes and writes dh[rows][D], dw[V][D] (contiguous, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
+ *     classes and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
  *     value (gout_stride 0) or one per row (1); count: divide it by count[0] (mean) or NULL.
- * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are copied into the workspace.
+ * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are taken at any alignment.
+ * fp32: products of a certain size run as six products of bf16 planes (24 bits in three), the others on the fp32 matrix rate.
  * ws: fea_linear_loss_ws_bytes(..., grads) bytes, 256-byte aligned; grads = 0 for the forwards, 1 dh + 2 dw + 4 db for the backward
  * (0 bytes = sizes that are refused).  Results are the same from run to run. */
 size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);

@@ -70,11 +70,13 @@ def test_pieces(shape, dtype, top, monkeypatch):
     _compare(_run(*c), O.evaluate(*c))
 
 
-@pytest.mark.parametrize("shape", [(4096, 64, 4096), (4000, 200, 4100), (2049, 1096, 2310), (4097, 72, 8185), (300, 520, 40000)])
+@pytest.mark.parametrize("shape", [(4096, 64, 4096), (4000, 200, 4100), (2049, 1096, 2310), (4097, 72, 8185), (300, 520, 40000), (1300, 643, 2011)])
 @pytest.mark.parametrize("top", [0, 5])
-def test_large_tiles(shape, top):
-    """bf16 sizes that take the 256 x 256 tile in some or all of their products, with ragged ends in every direction."""
-    c = O.case(*shape, torch.bfloat16, seed=3, top=top, ignored=0.1, short=0.2, bias=shape[0] % 2 == 0)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_tiles(shape, top, dtype):
+    """Sizes that take the 256 x 256 tile (fp32: as planes of bf16) in some or all of their products, with ragged ends in every
+    direction."""
+    c = O.case(*shape, dtype, seed=3, top=top, ignored=0.1, short=0.2, bias=shape[0] % 2 == 0)
     _compare(_run(*c, reduction="sum"), O.evaluate(*c, reduction="sum"))
 
 
