@@ -9,7 +9,7 @@
 //   LIN_STORE: out = scale * (a . b), or fp32 slabs of a split reduction (joined by the caller in split order: no atomics)
 //
 // 128 x 128 tile, 4 waves of 64 x 64 (2 x 2 accumulators of 32 x 32), reduction in 128-byte steps of every row (64 bf16 / 32 fp32),
-// two LDS stages filled through registers so that rows, columns and reduction of any length are cut by a guard on the load.
+// two LDS stages filled through registers, two steps ahead, so that rows, columns and reduction of any length are cut by a guard on the load.
 // The operands of the MFMA are swapped (classes as its rows), so a lane holds one label row and 32 of its classes: the softmax
 // sums are in-lane sums and one exchange between wave halves.
 #include "linear_loss.h"
@@ -42,9 +42,9 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     const int r = tid >> 3, c = tid & 7;
     const T* const ap = (const T*)g.a;
     const T* const bp = (const T*)g.b;
-    u32x4 ra[4], rb[4];
+    u32x4 ra[2][4], rb[2][4];          // two steps on the way: the first is needed a whole step after it was asked for
     int pair = PL ? k0 / g.Kp : 0, pk = PL ? k0 - pair * g.Kp : 0;
-    auto fetch = [&](int k) {
+    auto fetch = [&](int u, int k) {
         const int left = k1 - k - c * EPC;
         int ka = k + c * EPC, kb = ka;
         if constexpr (PL) {
@@ -55,16 +55,16 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int m = m0 + r + 32 * i, n = n0 + r + 32 * i;
-            ra[i] = m < g.M ? lin_load16<T, ALN>(ap + m * g.lda + ka, left) : u32x4{0, 0, 0, 0};
-            rb[i] = n < g.N ? lin_load16<T, ALN>(bp + n * g.ldb + kb, left) : u32x4{0, 0, 0, 0};
+            ra[u][i] = m < g.M ? lin_load16<T, ALN>(ap + m * g.lda + ka, left) : u32x4{0, 0, 0, 0};
+            rb[u][i] = n < g.N ? lin_load16<T, ALN>(bp + n * g.ldb + kb, left) : u32x4{0, 0, 0, 0};
         }
     };
     auto put = [&](int st) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int off = (r + 32 * i) * 128 + ((c ^ (r & 7)) << 4);
-            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + off) = ra[i];
-            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + LG_T * 128 + off) = rb[i];
+            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + off) = ra[st][i];
+            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + LG_T * 128 + off) = rb[st][i];
         }
     };
     f32x16 acc[2][2];                 // [label tile][class tile]
@@ -75,12 +75,12 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-    if (k0 < k1) fetch(k0);
-    int st = 0;
-    for (int k = k0; k < k1; k += CK, st ^= 1) {
+    if (k0 < k1) fetch(0, k0);
+    if (k0 + CK < k1) fetch(1, k0 + CK);
+    auto step = [&](int st, int k) {   // stage and register set of the same parity
         put(st);
         __syncthreads();              // one barrier per step: the other stage was last read in front of the previous one
-        if (k + CK < k1) fetch(k + CK);
+        if (k + 2 * CK < k1) fetch(st, k + 2 * CK);
         const char* sa = smem + st * LG_STAGE + (wm * 64 + l32) * 128;
         const char* sb = smem + st * LG_STAGE + LG_T * 128 + (wn * 64 + l32) * 128;
 #pragma unroll
@@ -91,6 +91,10 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             mma16(acc[0][0], b0, a0, (const T*)nullptr); mma16(acc[0][1], b1, a0, (const T*)nullptr);
             mma16(acc[1][0], b0, a1, (const T*)nullptr); mma16(acc[1][1], b1, a1, (const T*)nullptr);
         }
+    };
+    for (int k = k0; k < k1; k += 2 * CK) {
+        step(0, k);
+        if (k + CK < k1) step(1, k + CK);
     }
     __syncthreads();
 
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
                     const int n = ncol(j, e);
                     if (n >= g.N) continue;
                     const float v[4] = {acc[i][j][e] * sc, acc[i][j][e + 1] * sc, acc[i][j][e + 2] * sc, acc[i][j][e + 3] * sc};
-                    if (g.slab) lg_store4(g.slab + ((long long)sp * g.M + m) * g.N + n, v, g.N - n);
+                    if (g.slab) lg_store4(g.slab + ((long long)sp * g.M + m) * g.ldo + n, v, (int)g.ldo - n);
                     else        lg_store4((T*)g.out + m * g.ldo + n, v, g.N - n);
                 }
         }
@@ -241,12 +245,6 @@ template <typename T> static void lin_launch(int epi, bool aln, const LinGemm& g
         else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, false, false>), dim3(grid), dim3(256), 0, s, g);
     } else       hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE, true, false>), dim3(grid), dim3(256), 0, s, g);
 }
-static void lin_launch_planes(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm_kernel<__bf16, LIN_LSE, true, true>), dim3(grid), dim3(256), 0, s, g);
-    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm_kernel<__bf16, LIN_DZ, true, true>), dim3(grid), dim3(256), 0, s, g);
-    else                    hipLaunchKernelGGL((lin_gemm_kernel<__bf16, LIN_STORE, true, true>), dim3(grid), dim3(256), 0, s, g);
-}
-
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     const int epc = dtype == FEA_F32 ? 4 : 8;
     const bool aln = g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0;
@@ -254,13 +252,13 @@ int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.lda >= row && g.ldb >= row && (aln || (tile == 128 && epi != LIN_STORE && dtype != FEA_PL)), FEA_E_BADARG,
               "lin_gemm: operands of %d x %d x %d, tile %d", g.M, g.N, g.K, tile);
     FEA_CHECK(dtype != FEA_PL || (g.Kp > 0 && g.Kp % 64 == 0 && g.K == 6 * g.Kp && (epi != LIN_STORE || g.slab)), FEA_E_BADARG, "lin_gemm: planes of %d, K %d", g.Kp, g.K);
-    FEA_CHECK(tile == 128 || (dtype != FEA_F32 && g.lda < (1 << 21) && g.ldb < (1 << 21)), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
+    const bool fast = dtype != FEA_F32 && aln && g.lda < (1 << 21) && g.ldb < (1 << 21);
+    FEA_CHECK(fast || (tile == 128 && dtype != FEA_PL), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
     g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
     const long long grid = (long long)g.ntm * g.ntn * g.splits;
     FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
-    if (tile == 256)            fea_lin_gemm256(epi, dtype == FEA_PL, g, (unsigned)grid, s);
-    else if (dtype == FEA_PL)   lin_launch_planes(epi, g, (unsigned)grid, s);
+    if (fast)                   fea_lin_gemm256(epi, tile, dtype == FEA_PL, g, (unsigned)grid, s);
     else if (dtype == FEA_BF16) lin_launch<__bf16>(epi, aln, g, (unsigned)grid, s);
     else                        lin_launch<float>(epi, aln, g, (unsigned)grid, s);
     FEA_LAUNCH_CHECK();

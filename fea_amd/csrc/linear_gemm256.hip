@@ -12,7 +12,10 @@
 // every bound in the lane's offset, so rows, classes and channels behind the end arrive as zeros without a branch.
 #include "linear_loss.h"
 
-static constexpr int LB_T = 256, LB_OP = LB_T * 128, LB_STAGE = 2 * LB_OP;
+#ifndef LB_ROT
+#define LB_ROT 1
+#endif
+
 
 // XOR of a 128-byte row's 16-byte chunk index: conflict-free ds_read_b128 of 16 rows x 4 chunks
 __device__ __forceinline__ int lb_swz(int row) { return ((row >> 1) & 3) << 1; }
@@ -23,13 +26,15 @@ __device__ __forceinline__ uint32_t lb_pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, b2));
 }
 
-template <int EPI, bool PL>
-__global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
+// NT: 16-row tiles of a wave in either direction (8: 256 x 256 per workgroup, one per CU; 4: 128 x 128, two per CU)
+template <int EPI, bool PL, int NT>
+__global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const LinGemm g) {
+    constexpr int LB_T = 32 * NT, LB_W = 16 * NT, LB_OP = LB_T * 128, LB_STAGE = 2 * LB_OP, NL = 2 * NT;
     __shared__ __attribute__((aligned(128))) char smem[2 * LB_STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave & 1, wn = wave >> 1, r16 = lane & 15, q16 = lane >> 4;
     // tiles in groups of 8 row tiles, walked along the classes: the 32 tiles that an XCD has in flight are 8 x 4
-    constexpr int GM = 8;
+    constexpr int GM = NT;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int per = g.ntm * g.ntn, sp = id / per, it = id - sp * per;
     const int grp = it / (GM * g.ntn), gm = min(GM, g.ntm - grp * GM), in = it - grp * GM * g.ntn;
@@ -44,76 +49,86 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
     const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.b + n0 * g.ldb + kb), 0,
         K ? (int)(((min(LB_T, g.N - n0) - 1) * g.ldb + kl) * 2) : 0, 0x00020000);
 
-    // staging: thread -> rows r + 32 i of either operand, 16-byte chunk c
+    // staging: thread -> LDS rows r + 32 i of either operand, 16-byte chunk c.  What lies in an LDS row is chosen for the epilogue: the
+    // lane that ends up with column r16 of the products holds NT consecutive labels (over its tiles i), and with tiles 2 p, 2 p + 1 of
+    // the classes 8 consecutive ones: 16-byte stores of either order of dz without an exchange between lanes.
     const int r = tid >> 3, c = tid & 7;
-    const unsigned va = (unsigned)(r * (int)g.lda * 2 + c * 16), vb = (unsigned)(r * (int)g.ldb * 2 + c * 16);
-    const unsigned sa = 64 * (unsigned)g.lda, sb = 64 * (unsigned)g.ldb;
+    const int ra = (r & 15) * NT + (r >> 4), rb = ((r >> 4) & 1) * 4 + ((r >> 2) & 3) * 8 + (r & 3);
+    const unsigned va = (unsigned)(ra * (int)g.lda * 2 + c * 16), vb = (unsigned)(rb * (int)g.ldb * 2 + c * 16);
+    const unsigned ua = 2 * (unsigned)g.lda, sb = 64 * (unsigned)g.ldb;      // bytes of a label's row, of 32 classes' rows
     const int wofs = r * 128 + ((c ^ lb_swz(r)) << 4);
-    u32x4 st[16];
-    int pair = PL ? k0 / g.Kp : 0, pk = PL ? k0 - pair * g.Kp : 0;       // FEA_PL: the pair of planes and the channel that are loaded next
+    u32x4 st[NL];
+    // the XCDs start their reduction an eighth apart (it ends where it began): in step, every workgroup of the chip would ask for the
+    // same columns of its rows at a time.  Within an XCD all are in step: they share operands in its L2.
+    int at = LB_ROT ? (int)(blockIdx.x & 7) * nc >> 3 : 0;
+    int pair = PL ? (k0 + at * 64) / g.Kp : 0, pk = PL ? k0 + at * 64 - pair * g.Kp : 0;       // FEA_PL: the pair of planes and the channel that are loaded next
     unsigned ka = 0, kc = 0;
     bool kin = false;
-    auto advance = [&](int ch) {      // byte offsets of chunk ch in a row of either operand
-        kin = ch * 64 + c * 8 < K;
-        if constexpr (PL) {
-            ka = 2u * (unsigned)(lin_plane_a(pair) * g.Kp + pk); kc = 2u * (unsigned)(lin_plane_b(pair) * g.Kp + pk);
+    auto advance = [&](int ch) {      // byte offsets of the chunk that is loaded ch-th in a row of either operand
+        kin = ch < nc && at * 64 + c * 8 < K;
+        if constexpr (PL) { ka = 2u * (unsigned)(lin_plane_a(pair) * g.Kp + pk); kc = 2u * (unsigned)(lin_plane_b(pair) * g.Kp + pk); }
+        else ka = kc = at * 128;
+        if (++at == nc) {
+            at = 0;
+            if constexpr (PL) { pair = k0 / g.Kp; pk = k0 - pair * g.Kp; }
+        } else if constexpr (PL) {
             pk += 64;
             if (pk >= g.Kp) { pk = 0; ++pair; }
-        } else ka = kc = ch * 128;
+        }
     };
     auto gload = [&](int i) {
-        if (i < 8) st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ka + i * sa : 0x7fffff00u, 0, 0));
-        else       st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + kc + (i - 8) * sb : 0x7fffff00u, 0, 0));
+        if (i < NT) st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ka + (i / (NT / 2) * LB_W + 2 * (i % (NT / 2))) * ua : 0x7fffff00u, 0, 0));
+        else        st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + kc + (i - NT) * sb : 0x7fffff00u, 0, 0));
     };
-    auto lput = [&](int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i >> 3) * LB_OP + wofs + (i & 7) * 32 * 128) = st[i]; };
+    auto lput = [&](int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i / NT) * LB_OP + wofs + (i % NT) * 32 * 128) = st[i]; };
 
     const int fofs0 = r16 * 128 + ((q16 ^ lb_swz(r16)) << 4), fofs1 = fofs0 ^ 64;
-    const int fa = wm * 128 * 128, fb = LB_OP + wn * 128 * 128;
-    u32x4 A[2][8], B[2][8];
+    const int fa = wm * LB_W * 128, fb = LB_OP + wn * LB_W * 128;
+    u32x4 A[2][NT], B[2][NT];
     auto frd = [&](int stage, int ks, int i) {
-        const char* p = smem + stage * LB_STAGE + (ks ? fofs1 : fofs0) + (i & 7) * 16 * 128;
-        if (i < 8) A[ks][i] = *reinterpret_cast<const u32x4*>(p + fa);
-        else       B[ks][i - 8] = *reinterpret_cast<const u32x4*>(p + fb);
+        const char* p = smem + stage * LB_STAGE + (ks ? fofs1 : fofs0) + (i % NT) * 16 * 128;
+        if (i < NT) A[ks][i] = *reinterpret_cast<const u32x4*>(p + fa);
+        else        B[ks][i - NT] = *reinterpret_cast<const u32x4*>(p + fb);
     };
-    f32x4 acc[8][8];                  // [label tile][class tile]: lane = label r16 of the tile, registers = classes 4 q16 .. + 3
+    f32x4 acc[NT][NT];                // [label tile][class tile]
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto mma = [&](int ks) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < NT; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
     };
 
     advance(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) gload(i);
+    for (int i = 0; i < NL; ++i) gload(i);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) lput(0, i);
+    for (int i = 0; i < NL; ++i) lput(0, i);
     advance(1);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) gload(i);
+    for (int i = 0; i < NL; ++i) gload(i);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) frd(0, 0, i);
+    for (int i = 0; i < NL; ++i) frd(0, 0, i);
 
     for (int ch = 0; ch < nc; ++ch) {
         const int s = ch & 1;
         advance(ch + 2);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { frd(s, 1, i); lput(s ^ 1, i); gload(i); }
+        for (int i = 0; i < NL; ++i) { frd(s, 1, i); lput(s ^ 1, i); gload(i); }
         mma(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {        // 2 MFMA, LDS read, MFMA, LDS write, MFMA, load
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        for (int i = 0; i < NL; ++i) {        // 2 MFMA, LDS read, MFMA, LDS write, MFMA, load
+            if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); else if (i & 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (NT == 8 || 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -122,40 +137,34 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) frd(s ^ 1, 0, i);
+        for (int i = 0; i < NL; ++i) frd(s ^ 1, 0, i);
         mma(1);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        for (int i = 0; i < NL; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NT / 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
     }
     __syncthreads();
 
-    auto mrow = [&](int i) { return m0 + wm * 128 + i * 16 + r16; };
-    auto ncol = [&](int j) { return n0 + wn * 128 + j * 16 + 4 * q16; };
-    // two class tiles 2 p, 2 p + 1 of one label: after the exchange between neighbouring 16-lane rows a lane holds 8 consecutive
-    // classes, starting at
-    const int pcol = n0 + wn * 128 + (q16 & 1) * 16 + (q16 >> 1) * 8;
-    auto pairs = [&](const f32x4& x, const f32x4& y) {
-        const auto r0 = __builtin_amdgcn_permlane16_swap(lb_pack(x[0], x[1]), lb_pack(y[0], y[1]), false, false);
-        const auto r1 = __builtin_amdgcn_permlane16_swap(lb_pack(x[2], x[3]), lb_pack(y[2], y[3]), false, false);
-        return u32x4{r0[0], r1[0], r0[1], r1[1]};
-    };
+    auto mrow = [&](int i) { return m0 + wm * LB_W + r16 * NT + i; };                                    // label of tile i
+    auto ncol = [&](int j) { return n0 + wn * LB_W + (j >> 1) * 32 + q16 * 8 + (j & 1) * 4; };           // first of 4 classes of tile j
+    const int pcol = n0 + wn * LB_W + q16 * 8;                                                           // first of 8 classes of tiles 0, 1
+    auto pairs = [&](const f32x4& x, const f32x4& y) { return u32x4{lb_pack(x[0], x[1]), lb_pack(x[2], x[3]), lb_pack(y[0], y[1]), lb_pack(y[2], y[3])}; };
 
     if constexpr (EPI == LIN_STORE) {
         const float common = g.scale == 2 ? lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0) : 1.f;
-        const bool wide = g.slab ? g.N % 4 == 0 : g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0;
+        const bool wide = g.slab ? g.ldo % 4 == 0 : g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < NT; ++i) {
             const int m = mrow(i);
             const float sc = g.scale == 1 ? (m < g.M ? lin_row_scale(g.gout, g.gstride, g.count, g.t, g.stat[m].y, m) : 0.f) : common;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[i][j] *= sc;
+            for (int j = 0; j < NT; ++j) acc[i][j] *= sc;
             if (g.slab) {
-                float* const o = g.slab + ((long long)sp * g.M + m) * g.N;
+                float* const o = g.slab + ((long long)sp * g.M + m) * g.ldo;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < NT; ++j) {
                     const int n = ncol(j);
                     if (wide) { if (m < g.M && n < g.N) *reinterpret_cast<f32x4*>(o + n) = acc[i][j]; }
                     else
@@ -165,7 +174,7 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
             } else {
                 __bf16* const o = (__bf16*)g.out + m * g.ldo;
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
+                for (int p = 0; p < NT / 2; ++p) {
                     if (wide) {
                         const u32x4 v = pairs(acc[i][2 * p], acc[i][2 * p + 1]);
                         if (m < g.M && pcol + 32 * p < g.N) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
@@ -182,37 +191,37 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
         // z in place; classes behind the last are -inf
         const bool edge = n0 + LB_T > g.N;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int n = ncol(j) + e;
                 const float b = g.bias && n < g.N ? g.bias[n] : 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i][j][e] = edge && n >= g.N ? -INFINITY : (acc[i][j][e] + b) * g.inv_t;
+                for (int i = 0; i < NT; ++i) acc[i][j][e] = edge && n >= g.N ? -INFINITY : (acc[i][j][e] + b) * g.inv_t;
             }
     }
 
     if constexpr (EPI == LIN_LSE) {
         float2* const red = reinterpret_cast<float2*>(smem);       // [wn][256 labels]
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < NT; ++i) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mx = fmaxf(fmaxf(mx, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
+            for (int j = 0; j < NT; ++j) mx = fmaxf(fmaxf(mx, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float base = mx == -INFINITY ? 0.f : mx;
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum += __expf(acc[i][j][e] - base);
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (q16 == 0) red[wn * LB_T + wm * 128 + i * 16 + r16] = make_float2(mx, sum);
+            if (q16 == 0) red[wn * LB_T + wm * LB_W + r16 * NT + i] = make_float2(mx, sum);
         }
         __syncthreads();
-        if (m0 + tid < g.M) {
+        if (tid < LB_T && m0 + tid < g.M) {
             const float2 p = red[tid], q = red[LB_T + tid];
             const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
             g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, p.y * __expf(p.x - base) + q.y * __expf(q.x - base));
@@ -220,15 +229,15 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
     }
 
     if constexpr (EPI == LIN_DZ) {
-        float sc[8];
+        float sc[NT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < NT; ++i) {
             const int m = mrow(i);
             const float2 s2 = m < g.M ? g.stat[m] : make_float2(0.f, 0.f);
             const bool dead = s2.y == 0.f;
             sc[i] = dead || !g.colsum ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, s2.y, m);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float q = __expf(acc[i][j][e] - s2.x);
@@ -238,65 +247,61 @@ __global__ __launch_bounds__(256, 1) void lin_gemm256_kernel(const LinGemm g) {
         if (g.colsum) {
             float* const red = reinterpret_cast<float*>(smem);     // [wm][256 classes]
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     float s = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) s += acc[i][j][e] * sc[i];
+                    for (int i = 0; i < NT; ++i) s += acc[i][j][e] * sc[i];
 #pragma unroll
                     for (int d = 8; d; d >>= 1) s += __shfl_xor(s, d);
                     if (r16 == 0) red[wm * LB_T + ncol(j) + e - n0] = s;
                 }
             __syncthreads();
-            if (n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LB_T + tid];
+            if (tid < LB_T && n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LB_T + tid];
         }
-        const bool odd = lane & 1;
-        const int tcol = 2 * (lane & 1);
 #pragma unroll
         for (int pl = 0; pl < (PL ? 3 : 1); ++pl) {
             __bf16* const dz = (__bf16*)g.dz + (PL ? (long long)pl * g.Npad : 0);
             __bf16* const dzt = (__bf16*)g.dzt + (PL ? (long long)pl * g.Mpad : 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < NT; ++i) {
                 const int m = mrow(i);
                 __bf16* const o = dz + m * g.lddz;
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
+                for (int p = 0; p < NT / 2; ++p) {
                     const u32x4 v = pairs(acc[i][2 * p], acc[i][2 * p + 1]);
                     if (m < g.M && pcol + 32 * p < g.Npad) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
                 }
-                if (g.dzt) {
-                    // neighbouring lanes hold neighbouring labels: they trade halves, so that each has 2 labels of 2 classes
-                    const int me = m & ~1;
+            }
+            if (g.dzt && mrow(0) < g.Mpad)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t d0 = lb_pack(acc[i][j][0], acc[i][j][1]), d1 = lb_pack(acc[i][j][2], acc[i][j][3]);
-                        const uint32_t t = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? d0 : d1), 0xb1, 0xf, 0xf, false);
-                        const uint32_t lo = odd ? t : d0, hi = odd ? d1 : t;          // label me, me + 1 of classes ncol + tcol, + 1
-                        const uint32_t c0 = __builtin_amdgcn_perm(hi, lo, 0x05040100u), c1 = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                        const int n = ncol(j) + tcol;
-                        if (me < g.Mpad) {
-                            if (n < g.N) *reinterpret_cast<uint32_t*>(dzt + n * g.lddzt + me) = c0;
-                            if (n + 1 < g.N) *reinterpret_cast<uint32_t*>(dzt + (n + 1) * g.lddzt + me) = c1;
-                        }
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int n = ncol(j) + e;
+                        if (n >= g.N) continue;
+                        __bf16* const o = dzt + n * g.lddzt + mrow(0);
+                        if constexpr (NT == 8) *reinterpret_cast<u32x4*>(o) = u32x4{lb_pack(acc[0][j][e], acc[1][j][e]), lb_pack(acc[2][j][e], acc[3][j][e]), lb_pack(acc[NT - 4][j][e], acc[NT - 3][j][e]), lb_pack(acc[NT - 2][j][e], acc[NT - 1][j][e])};
+                        else                   *reinterpret_cast<u32x2*>(o) = u32x2{lb_pack(acc[0][j][e], acc[1][j][e]), lb_pack(acc[2][j][e], acc[3][j][e])};
                     }
-                }
-                if constexpr (PL)
+            if constexpr (PL)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) acc[i][j][e] -= (float)(__bf16)acc[i][j][e];
-            }
         }
     }
 }
 
-template <bool PL> static void lb_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE, PL>), dim3(grid), dim3(256), 0, s, g);
-    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ, PL>), dim3(grid), dim3(256), 0, s, g);
-    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE, PL>), dim3(grid), dim3(256), 0, s, g);
+template <bool PL, int NT> static void lb_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE, PL, NT>), dim3(grid), dim3(256), 0, s, g);
+    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ, PL, NT>), dim3(grid), dim3(256), 0, s, g);
+    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE, PL, NT>), dim3(grid), dim3(256), 0, s, g);
 }
-void fea_lin_gemm256(int epi, bool planes, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (planes) lb_launch<true>(epi, g, grid, s); else lb_launch<false>(epi, g, grid, s);
+void fea_lin_gemm256(int epi, int tile, bool planes, const LinGemm& g, unsigned grid, hipStream_t s) {
+    if (tile == 256) { if (planes) lb_launch<true, 8>(epi, g, grid, s); else lb_launch<false, 8>(epi, g, grid, s); }
+    else             { if (planes) lb_launch<true, 4>(epi, g, grid, s); else lb_launch<false, 4>(epi, g, grid, s); }
 }

@@ -35,7 +35,7 @@ struct LinGemm {
     long long ldcol;
     // LIN_STORE: split over K into `splits` parts of kper: direct store to out (splits == 1, slab == NULL) or fp32 slabs
     void* out; long long ldo;
-    float* slab;                      // [splits][M][N]
+    float* slab;                      // [splits][M][ldo], ldo a multiple of 4 (columns behind N hold nothing)
     int scale;                        // 0: none, 1: times the row scale of A's row, 2: times the common scale (gout, count, t above)
     int splits, kper;
     int ntm, ntn;
@@ -94,4 +94,4 @@ int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s);
 // linear_rows.hip: LIN_LSE of up to 64 label rows; g.part [M][classes / 64]
 int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s);
 // linear_gemm256.hip
-void fea_lin_gemm256(int epi, bool planes, const LinGemm& g, unsigned grid, hipStream_t s);
+void fea_lin_gemm256(int epi, int tile, bool planes, const LinGemm& g, unsigned grid, hipStream_t s);

@@ -17,16 +17,6 @@
 
 // ---- layouts ------------------------------------------------------------------------------------------------------------
 
-// out[r][c] = in[r][c], zero for C <= c < Cpad: rows of a length that is no multiple of 16 bytes
-template <typename T>
-__global__ __launch_bounds__(256) void lin_pack_kernel(const T* __restrict__ in, long long ld, T* __restrict__ out, int Cpad, int C, long long total) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / Cpad;
-        const int c = (int)(i - r * Cpad);
-        out[i] = c < C ? in[r * ld + c] : from_f32<T>(0.f);
-    }
-}
-
 // x as three bf16 planes (linear_loss.h): what each leaves goes to the next
 __device__ __forceinline__ void lin_split3(float v, __bf16& x0, __bf16& x1, __bf16& x2) {
     x0 = (__bf16)v; v -= (float)x0;
@@ -34,75 +24,98 @@ __device__ __forceinline__ void lin_split3(float v, __bf16& x0, __bf16& x1, __bf
     x2 = (__bf16)v;
 }
 
-// out[r][plane][c] = planes of in[r][c], zero for C <= c < Kp: 8 elements per thread
-__global__ __launch_bounds__(256) void lin_planes_kernel(const float* __restrict__ in, long long ld, __bf16* __restrict__ out, int Kp, int C, long long total8) {
-    const int per = Kp / 8;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total8; i += (long long)gridDim.x * 256) {
-        const long long r = i / per;
-        const int c = (int)(i - r * per) * 8;
-        const float* p = in + r * ld + c;
-        __bf16 x[3][8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) lin_split3(c + e < C ? p[e] : 0.f, x[0][e], x[1][e], x[2][e]);
-        __bf16* o = out + r * 3 * Kp + c;
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(o + (long long)q * Kp) = *reinterpret_cast<const u32x4*>(x[q]);
-    }
+// Copies of an operand in [R][ld]: `rows` [R][ldr] (zero for C <= c < Cpad) and `cols` [C][ldc] (zero for R <= r < Rpad), either nullable; Cpad and
+// Rpad are multiples of 64.  With planes (fp32 in, bf16 out) a row holds three of Cpad / Rpad elements.  In `cols`, rows whose gate is 0
+// count as zeros: what an ignored row holds (an infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must
+// not reach the weight; and with gout every row is multiplied by its own upstream gradient.  Two operands per launch, 64 x 64 tiles.
+struct LinCopy { const void* in; void *rows, *cols; long long ld, ldr, ldc, R, Rpad; int C, Cpad; const float2* stat; const float* gout; float t; long long tiles; };
+struct LinCopies { LinCopy a, b; };
+
+__device__ __forceinline__ bool lin_copy_tile(const LinCopies& both, LinCopy& j, long long& r0, int& c0) {
+    const bool second = blockIdx.x >= both.a.tiles;
+    j = second ? both.b : both.a;
+    const long long tile = blockIdx.x - (second ? both.a.tiles : 0);
+    const int nc = j.Cpad / 64;
+    r0 = tile / nc * 64;
+    c0 = (int)(tile % nc) * 64;
+    return j.in != nullptr;
 }
+__device__ __forceinline__ bool lin_copy_gate(const LinCopy& j, long long r) { return r < j.R && (!j.stat || j.stat[r].y != 0.f); }
+__device__ __forceinline__ float lin_copy_factor(const LinCopy& j, long long r) { return j.gout ? lin_row_scale(j.gout, 1, nullptr, j.t, 1.f, r) : 1.f; }
 
-// out[c][r] = in[r][c] (r < R), zero for R <= r < Rpad (a multiple of 64); rows whose gate is 0 count as zeros: what an ignored row
-// holds (an infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must not reach the weight.  gout
-// (nullable): rows times their own upstream gradient.  64 x 64 tiles.
-struct LinTrans { long long ld, ldo, R, Rpad; int C; const float2* stat; const float* gout; float t; };
-
-__device__ __forceinline__ float lin_trans_factor(const LinTrans& a, long long r) { return a.gout ? lin_row_scale(a.gout, 1, nullptr, a.t, 1.f, r) : 1.f; }
-
-// fp32 (out fp32, or three bf16 planes per row of out: PL)
+// fp32 (out fp32, or three bf16 planes: PL)
 template <bool PL>
-__global__ __launch_bounds__(256) void lin_transpose32_kernel(const float* __restrict__ in, void* __restrict__ out, const LinTrans a) {
+__global__ __launch_bounds__(256) void lin_copy32_kernel(const LinCopies both) {
     __shared__ float tile[64][65];
-    const long long r0 = (long long)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    LinCopy j;
+    long long r0;
+    int c0;
+    if (!lin_copy_tile(both, j, r0, c0)) return;
+    const float* const in = (const float*)j.in;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6, hi = threadIdx.x >> 3, lo = (threadIdx.x & 7) * 8;
 #pragma unroll 4
-    for (int i = y; i < 64; i += 4) {
-        const long long r = r0 + i;
-        const bool on = r < a.R && (!a.stat || a.stat[r].y != 0.f);
-        tile[i][x] = on && c0 + x < a.C ? in[r * a.ld + c0 + x] * lin_trans_factor(a, r) : 0.f;
-    }
+    for (int i = y; i < 64; i += 4) tile[i][x] = r0 + i < j.R && c0 + x < j.C ? in[(r0 + i) * j.ld + c0 + x] : 0.f;
     __syncthreads();
-    if constexpr (!PL) {
-#pragma unroll 4
-        for (int i = y; i < 64; i += 4)
-            if (c0 + i < a.C) ((float*)out)[(c0 + i) * a.ldo + r0 + x] = tile[x][i];
-    } else {
+    if (j.rows)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int c = (threadIdx.x >> 3) + 32 * i, q = (threadIdx.x & 7) * 8;
-            if (c0 + c >= a.C) continue;
-            __bf16 v[3][8];
+            const int r = hi + 32 * i;
+            if (r0 + r >= j.R) continue;
+            if constexpr (PL) {
+                __bf16 v[3][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) lin_split3(tile[q + e][c], v[0][e], v[1][e], v[2][e]);
-            __bf16* o = (__bf16*)out + (c0 + c) * a.ldo + r0 + q;
+                for (int e = 0; e < 8; ++e) lin_split3(tile[r][lo + e], v[0][e], v[1][e], v[2][e]);
+                __bf16* const o = (__bf16*)j.rows + (r0 + r) * j.ldr + c0 + lo;
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(o + p * a.Rpad) = *reinterpret_cast<const u32x4*>(v[p]);
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(o + (long long)p * j.Cpad) = *reinterpret_cast<const u32x4*>(v[p]);
+            } else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ((float*)j.rows)[(r0 + r) * j.ldr + c0 + lo + e] = tile[r][lo + e];
+        }
+    if (j.cols) {
+        if (j.stat) {
+            __syncthreads();
+#pragma unroll 4
+            for (int i = y; i < 64; i += 4) tile[i][x] = lin_copy_gate(j, r0 + i) ? tile[i][x] * lin_copy_factor(j, r0 + i) : 0.f;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int c = hi + 32 * i;
+            if (c0 + c >= j.C) continue;
+            if constexpr (PL) {
+                __bf16 v[3][8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) lin_split3(tile[lo + e][c], v[0][e], v[1][e], v[2][e]);
+                __bf16* const o = (__bf16*)j.cols + (c0 + c) * j.ldc + r0 + lo;
+#pragma unroll
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(o + p * j.Rpad) = *reinterpret_cast<const u32x4*>(v[p]);
+            } else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ((float*)j.cols)[(c0 + c) * j.ldc + r0 + lo + e] = tile[lo + e][c];
         }
     }
 }
 
 // bf16: 16-byte loads and stores; a thread turns 2 rows x 8 columns into 8 dwords (two rows of a column each) on the way into LDS
 template <bool ALN>
-__global__ __launch_bounds__(256) void lin_transpose16_kernel(const __bf16* __restrict__ in, __bf16* __restrict__ out, const LinTrans a) {
+__global__ __launch_bounds__(256) void lin_copy16_kernel(const LinCopies both) {
     __shared__ __attribute__((aligned(16))) uint32_t tile[64][36];        // [column][row pair]
-    const long long r0 = (long long)blockIdx.x * 64;
-    const int c0 = blockIdx.y * 64, hi = threadIdx.x >> 3, lo = threadIdx.x & 7;
+    LinCopy j;
+    long long r0;
+    int c0;
+    if (!lin_copy_tile(both, j, r0, c0)) return;
+    const __bf16* const in = (const __bf16*)j.in;
+    const int hi = threadIdx.x >> 3, lo = threadIdx.x & 7;
     u32x4 v[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const long long r = r0 + 2 * hi + i;
-        const bool on = r < a.R && (!a.stat || a.stat[r].y != 0.f);
-        v[i] = on ? lin_load16<__bf16, ALN>(in + r * a.ld + c0 + 8 * lo, a.C - c0 - 8 * lo) : u32x4{0, 0, 0, 0};
-        if (a.gout && on) {
-            const float f = lin_trans_factor(a, r);
+        v[i] = r < j.R ? lin_load16<__bf16, ALN>(in + r * j.ld + c0 + 8 * lo, j.C - c0 - 8 * lo) : u32x4{0, 0, 0, 0};
+        if (j.rows && r < j.R) *reinterpret_cast<u32x4*>((__bf16*)j.rows + r * j.ldr + c0 + 8 * lo) = v[i];
+        if (!lin_copy_gate(j, r)) v[i] = u32x4{0, 0, 0, 0};
+        else if (j.gout) {
+            const float f = lin_copy_factor(j, r);
             __bf16 x[8];
             *reinterpret_cast<u32x4*>(x) = v[i];
 #pragma unroll
@@ -110,16 +123,17 @@ __global__ __launch_bounds__(256) void lin_transpose16_kernel(const __bf16* __re
             v[i] = *reinterpret_cast<const u32x4*>(x);
         }
     }
+    if (!j.cols) return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        tile[8 * lo + 2 * j][hi] = __builtin_amdgcn_perm(v[1][j], v[0][j], 0x05040100u);
-        tile[8 * lo + 2 * j + 1][hi] = __builtin_amdgcn_perm(v[1][j], v[0][j], 0x07060302u);
+    for (int q = 0; q < 4; ++q) {
+        tile[8 * lo + 2 * q][hi] = __builtin_amdgcn_perm(v[1][q], v[0][q], 0x05040100u);
+        tile[8 * lo + 2 * q + 1][hi] = __builtin_amdgcn_perm(v[1][q], v[0][q], 0x07060302u);
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int c = hi + 32 * i;
-        if (c0 + c < a.C) *reinterpret_cast<u32x4*>(out + (c0 + c) * a.ldo + r0 + 8 * lo) = *reinterpret_cast<const u32x4*>(&tile[c][4 * lo]);
+        if (c0 + c < j.C) *reinterpret_cast<u32x4*>((__bf16*)j.cols + (c0 + c) * j.ldc + r0 + 8 * lo) = *reinterpret_cast<const u32x4*>(&tile[c][4 * lo]);
     }
 }
 
@@ -342,49 +356,65 @@ __global__ __launch_bounds__(256) void lin_scatter_kernel(const long long* __res
     }
 }
 
-// out = acc + slabs in split order; acc (nullable) is the fp32 sum of earlier pieces, accout where later ones follow
+// out = acc + slabs in split order, rows of N in slabs with rows of ld = N rounded up to 4; acc (nullable, rows of ld) is the fp32 sum of
+// earlier pieces, accout where later ones follow.  4 columns per thread.
 template <typename T>
-__global__ __launch_bounds__(256) void lin_reduce_kernel(const float* __restrict__ slab, int splits, long long n, const float* acc, float* accout, T* out) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        float s = acc ? acc[i] : 0.f;
-        for (int p = 0; p < splits; ++p) s += slab[p * n + i];
-        if (accout) accout[i] = s;
-        if (out) out[i] = from_f32<T>(s);
+__global__ __launch_bounds__(256) void lin_reduce_kernel(const float* __restrict__ slab, int splits, long long M, int N, int ld, const float* acc, float* accout, T* out) {
+    const long long n = M * ld, i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    f32x4 s = acc ? *reinterpret_cast<const f32x4*>(acc + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int p = 0; p < splits; ++p) s += *reinterpret_cast<const f32x4*>(slab + p * n + i);
+    if (accout) *reinterpret_cast<f32x4*>(accout + i) = s;
+    if (out) {
+        const long long m = i / ld;
+        const int c = (int)(i - m * ld);
+        T* const o = out + m * N + c;
+        if (N == ld) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(o) = s;
+            else { const bf16x4 v = {(__bf16)s[0], (__bf16)s[1], (__bf16)s[2], (__bf16)s[3]}; *reinterpret_cast<bf16x4*>(o) = v; }
+        } else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (c + e < N) o[e] = from_f32<T>(s[e]);
     }
 }
 
-// Partial bias gradient of one chunk of LIN_DB_TILES row tiles: sum over its tiles of colsum[tile][v] - sum of g * teacher share over
+// Partial bias gradient of one chunk of LIN_DB_ROWS rows: sum over its row tiles of colsum[tile][v] - sum of g * teacher share over
 // its rows' entries that name v (psel NULL: share 1).  One workgroup owns 256 classes of one chunk; its waves walk the entries in
 // order and the lane that owns a class adds its hits: the order is fixed.
-static constexpr int LIN_DB_TILES = 16;
+static constexpr int LIN_DB_ROWS = 512;
 __global__ __launch_bounds__(256) void lin_dbias_kernel(const float* __restrict__ colsum, int tiles, long long ldcol, const long long* __restrict__ index,
                                                         const float* __restrict__ psel, int K, const float2* __restrict__ stat, const float* gout,
                                                         int gstride, const int* count, float t, long long v0, int N, long long entries,
-                                                        long long chunk, double* out) {
+                                                        int per, long long chunk, double* out) {
     __shared__ double part[4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = blockIdx.x * 256;
     const long long ea = blockIdx.y * chunk, eb = ea + chunk < entries ? ea + chunk : entries;
     double acc[4] = {0.0, 0.0, 0.0, 0.0};             // classes b0 + lane + 64 q
-    for (long long e0 = ea + wave * 64; e0 < eb; e0 += 256) {
-        const long long e = e0 + lane;
-        const long long i = e < eb ? index[e] - v0 - b0 : -1;
-        float val = 0.f;
-        bool hit = i >= 0 && i < 256 && b0 + i < N;
-        if (hit) {
-            const long long m = e / K;
-            const float gate = stat[m].y;
-            hit = gate != 0.f;
-            if (hit) val = (psel ? psel[e] : 1.f) * lin_row_scale(gout, gstride, count, t, gate, m);
-        }
-        unsigned long long mask = __ballot(hit);
-        while (mask) {
-            const int l = __builtin_ctzll(mask);
-            mask &= mask - 1;
-            const int c = __shfl((int)i, l);
-            const float v = __shfl(val, l);
-            if ((c & 63) == lane) {
+    for (long long e0 = ea + wave * 256; e0 < eb; e0 += 1024) {
+        int i[4];
+        float val[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) if (c >> 6 == q) acc[q] += (double)v;
+        for (int u = 0; u < 4; ++u) {                 // (four entries of a lane at a time: their loads are in flight together)
+            const long long e = e0 + 64 * u + lane;
+            const long long x = e < eb ? index[e] - v0 - b0 : -1;
+            const bool hit = x >= 0 && x < 256 && b0 + x < N;
+            const long long m = hit ? e / K : 0;
+            val[u] = hit ? (psel ? psel[e] : 1.f) * lin_row_scale(gout, gstride, count, t, stat[m].y, m) : 0.f;
+            i[u] = hit ? (int)x : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            unsigned long long mask = __ballot(i[u] >= 0 && val[u] != 0.f);
+            while (mask) {
+                const int l = __builtin_ctzll(mask);
+                mask &= mask - 1;
+                const int c = __shfl(i[u], l);
+                const float v = __shfl(val[u], l);
+                if ((c & 63) == lane) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) if (c >> 6 == q) acc[q] += (double)v;
+                }
             }
         }
     }
@@ -394,8 +424,8 @@ __global__ __launch_bounds__(256) void lin_dbias_kernel(const float* __restrict_
     const int v = b0 + threadIdx.x;
     if (v < N) {
         double s = -(part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]);
-        const int t1 = min(tiles, ((int)blockIdx.y + 1) * LIN_DB_TILES);
-        for (int i = blockIdx.y * LIN_DB_TILES; i < t1; ++i) s += (double)colsum[i * ldcol + v];
+        const int t1 = min(tiles, ((int)blockIdx.y + 1) * per);
+        for (int i = blockIdx.y * per; i < t1; ++i) s += (double)colsum[i * ldcol + v];
         out[(long long)blockIdx.y * N + v] = s;
     }
 }
@@ -423,6 +453,7 @@ struct LinCarve {
 struct LinDims {
     long long rows; int D, V, K, dtype, es, epc;
     bool odd() const { return D % epc != 0; }      // rows that are no multiple of 16 bytes
+    bool straight() const { return !odd(); }       // gradients go straight to their rows (others through slabs, which have wide stores)
     bool wide;                    // row strides of 2^21 elements or more (a slice of something very wide): the 128 tile, which has 64-bit offsets
 };
 
@@ -516,7 +547,7 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
     w.hp = w.wp = nullptr;
-    if (p.planes || (d.odd() && p.tile == 256)) {
+    if (p.planes || (d.dtype == FEA_BF16 && d.odd() && p.tile != 64)) {
         const LinForm f = lin_form(d.dtype, p.planes);
         w.hp = c.take<char>(p.rc * f.row(d.D) * f.es);
         w.wp = c.take<char>(d.V * f.row(d.D) * f.es);
@@ -535,17 +566,18 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
         return c.at;
     }
     const LinForm f = lin_form(d.dtype, p.planes);
-    if (p.planes || (d.odd() && p.tz == 256)) { w.hp = c.take<char>(p.rc * f.row(d.D) * f.es); w.wp = c.take<char>(p.vc * f.row(d.D) * f.es); }
+    if (p.planes || (d.dtype == FEA_BF16 && d.odd())) { w.hp = c.take<char>(p.rc * f.row(d.D) * f.es); w.wp = c.take<char>(p.vc * f.row(d.D) * f.es); }
     w.dz = c.take<char>(p.rc * f.row(p.vc) * f.es);
     if (want & 2) { w.dzt = c.take<char>(p.vc * f.row(p.rc) * f.es); w.ht = c.take<char>(d.D * f.row(p.rc) * f.es); }
     if (want & 1) w.wt = c.take<char>(d.D * f.row(p.vc) * f.es);
     long long slab = 0;
-    if ((want & 1) && (p.th.splits > 1 || p.nvc > 1)) slab = p.th.splits * p.rc * d.D;
-    if ((want & 2) && (p.tw.splits > 1 || p.nrc > 1) && slab < (long long)p.tw.splits * p.vc * d.D) slab = (long long)p.tw.splits * p.vc * d.D;
+    const long long ld = up(d.D, 4);
+    if ((want & 1) && !(p.th.splits == 1 && p.nvc == 1 && d.straight())) slab = p.th.splits * p.rc * ld;
+    if ((want & 2) && !(p.tw.splits == 1 && p.nrc == 1 && d.straight()) && slab < (long long)p.tw.splits * p.vc * ld) slab = (long long)p.tw.splits * p.vc * ld;
     w.slab = c.take<float>(slab);
-    if ((want & 1) && p.nvc > 1) w.acch = c.take<float>(p.rc * d.D);
-    if ((want & 2) && p.nrc > 1) w.accw = c.take<float>((long long)d.V * d.D);
-    if (want & 4) { const long long t = (p.rc + 127) / 128; w.colsum = c.take<float>(t * up(p.vc, 64)); w.dbpart = c.take<double>((t + LIN_DB_TILES - 1) / LIN_DB_TILES * p.vc); }
+    if ((want & 1) && p.nvc > 1) w.acch = c.take<float>(p.rc * ld);
+    if ((want & 2) && p.nrc > 1) w.accw = c.take<float>(d.V * ld);
+    if (want & 4) { const long long t = (p.rc + 127) / 128; w.colsum = c.take<float>(t * up(p.vc, 64)); w.dbpart = c.take<double>((p.rc + LIN_DB_ROWS - 1) / LIN_DB_ROWS * p.vc); }
     return c.at;
 }
 
@@ -557,34 +589,33 @@ extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, 
     return lin_bwd_carve(d, lin_bwd_plan(d, grads), grads, nullptr, w);
 }
 
-// rows of D elements as the products take them: planes, or copies with zeros behind the end
-static int lin_pack(const LinDims& d, const LinForm& f, const void* in, long long ld, void* out, long long R, hipStream_t s) {
-    const int Cp = (int)up(d.D, f.pad);
-    const long long n = f.dt == FEA_PL ? R * Cp / 8 : R * Cp, b = (n + 1023) / 1024;
-    const unsigned grid = (unsigned)(b > 16384 ? 16384 : b);
-    if (f.dt == FEA_PL)        hipLaunchKernelGGL(lin_planes_kernel, dim3(grid), dim3(256), 0, s, (const float*)in, ld, (__bf16*)out, Cp, d.D, n);
-    else if (f.dt == FEA_BF16) hipLaunchKernelGGL(lin_pack_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)in, ld, (__bf16*)out, Cp, d.D, n);
-    else                       hipLaunchKernelGGL(lin_pack_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)in, ld, (float*)out, Cp, d.D, n);
+// an operand of R rows and where its copies go
+static LinCopy lin_copy_of(const LinDims& d, const LinForm& f, const void* in, long long ld, long long R, void* rows, void* cols) {
+    LinCopy j{};
+    j.in = rows || cols ? in : nullptr; j.rows = rows; j.cols = cols; j.ld = ld; j.R = R; j.Rpad = up(R, 64); j.C = d.D; j.Cpad = (int)up(d.D, 64);
+    j.ldr = f.row(d.D); j.ldc = f.row(R);
+    j.tiles = j.in ? j.Rpad / 64 * (j.Cpad / 64) : 0;
+    return j;
+}
+static int lin_copy(const LinDims& d, const LinForm& f, const LinCopy& a, const LinCopy& b, hipStream_t s) {
+    const LinCopies both{a, b};
+    const long long n = a.tiles + b.tiles;
+    if (!n) return FEA_OK;
+    FEA_CHECK(n < 1 << 24, FEA_E_UNSUPPORTED_SHAPE, "lin_copy: %lld tiles", n);
+    const dim3 grid((unsigned)n);
+    if (f.dt == FEA_PL)       hipLaunchKernelGGL(lin_copy32_kernel<true>, grid, dim3(256), 0, s, both);
+    else if (f.dt == FEA_F32) hipLaunchKernelGGL(lin_copy32_kernel<false>, grid, dim3(256), 0, s, both);
+    else if (d.odd())         hipLaunchKernelGGL(lin_copy16_kernel<false>, grid, dim3(256), 0, s, both);
+    else                      hipLaunchKernelGGL(lin_copy16_kernel<true>, grid, dim3(256), 0, s, both);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
 
-static int lin_transpose(const LinDims& d, const LinForm& f, const void* in, long long ld, void* out, long long R, const float2* stat, const float* gout, float t, hipStream_t s) {
-    const long long Rp = up(R, f.pad);
-    const LinTrans a{ld, f.row(R), R, Rp, d.D, stat, gout, t};
-    const dim3 grid((unsigned)(Rp / 64), (unsigned)((d.D + 63) / 64));
-    if (f.dt == FEA_PL)       hipLaunchKernelGGL(lin_transpose32_kernel<true>, grid, dim3(256), 0, s, (const float*)in, out, a);
-    else if (f.dt == FEA_F32) hipLaunchKernelGGL(lin_transpose32_kernel<false>, grid, dim3(256), 0, s, (const float*)in, out, a);
-    else if (d.odd())         hipLaunchKernelGGL(lin_transpose16_kernel<false>, grid, dim3(256), 0, s, (const __bf16*)in, (__bf16*)out, a);
-    else                      hipLaunchKernelGGL(lin_transpose16_kernel<true>, grid, dim3(256), 0, s, (const __bf16*)in, (__bf16*)out, a);
-    FEA_LAUNCH_CHECK();
-    return FEA_OK;
-}
-
-static int lin_reduce(const LinDims& d, const float* slab, int splits, long long n, const float* acc, float* accout, void* out, hipStream_t s) {
-    const unsigned grid = (unsigned)(n / 1024 < 1 ? 1 : n / 1024 > 8192 ? 8192 : n / 1024);
-    if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_reduce_kernel<__bf16>, dim3(grid), dim3(256), 0, s, slab, splits, n, acc, accout, (__bf16*)out);
-    else                     hipLaunchKernelGGL(lin_reduce_kernel<float>, dim3(grid), dim3(256), 0, s, slab, splits, n, acc, accout, (float*)out);
+static int lin_reduce(const LinDims& d, const float* slab, int splits, long long M, const float* acc, float* accout, void* out, hipStream_t s) {
+    const int ld = (int)up(d.D, 4);
+    const dim3 grid((unsigned)((M * ld / 4 + 255) / 256));
+    if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_reduce_kernel<__bf16>, grid, dim3(256), 0, s, slab, splits, M, d.D, ld, acc, accout, (__bf16*)out);
+    else                     hipLaunchKernelGGL(lin_reduce_kernel<float>, grid, dim3(256), 0, s, slab, splits, M, d.D, ld, acc, accout, (float*)out);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
@@ -640,13 +671,12 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         FEA_LAUNCH_CHECK();
     }
     const LinForm f = lin_form(d.dtype, p.planes);
-    const bool pack = p.planes || (d.odd() && p.tile == 256);       // (the other kernels take rows of any alignment)
-    if (pack) LIN_TRY(lin_pack(d, f, w, ldw, b.wp, d.V, s));
+    const bool pack = p.planes || (d.dtype == FEA_BF16 && d.odd() && p.tile != 64);       // (the others take rows of any alignment)
     long long blk = 0;
     for (long long r = 0; r < d.rows; r += p.rc) {
         const long long n = d.rows - r < p.rc ? d.rows - r : p.rc;
         const void* hr = (const char*)h + r * ldh * d.es;
-        if (pack) LIN_TRY(lin_pack(d, f, hr, ldh, b.hp, n, s));
+        if (pack) LIN_TRY(lin_copy(d, f, lin_copy_of(d, f, hr, ldh, n, b.hp, nullptr), lin_copy_of(d, f, w, ldw, d.V, r ? nullptr : b.wp, nullptr), s));
         LinGemm g{};
         g.a = pack ? b.hp : hr; g.lda = pack ? f.row(d.D) : ldh; g.b = pack ? b.wp : w; g.ldb = pack ? f.row(d.D) : ldw;
         g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
@@ -728,19 +758,21 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
         return fea_lin_few_bwd(f, dtype, dw, db, s);
     }
     const LinForm f = lin_form(dtype, p.planes);
-    const bool pack = p.planes || (d.odd() && p.tz == 256);
+    const bool pack = p.planes || (dtype == FEA_BF16 && d.odd());
     for (int ir = 0; ir < p.nrc; ++ir) {
         const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc;
         const char* hr = (const char*)h + r0 * ldh * d.es;
         const float2* st = (const float2*)stat + r0;
         const float* go = gout + r0 * gout_stride;
-        if (pack) LIN_TRY(lin_pack(d, f, hr, ldh, b.hp, n, s));
-        if (dw) LIN_TRY(lin_transpose(d, f, hr, ldh, b.ht, n, st, gout_stride ? go : nullptr, temperature, s));
         for (int iv = 0; iv < p.nvc; ++iv) {
             const long long v0 = (long long)iv * p.vc;
             const int nv = (int)(V - v0 < p.vc ? V - v0 : p.vc);
             const char* wr = (const char*)w + v0 * ldw * d.es;
-            if (pack) LIN_TRY(lin_pack(d, f, wr, ldw, b.wp, nv, s));
+            // the operands' copies: hidden once for its rows, the weight's piece unless the only piece is there from the rows before
+            LinCopy jh = lin_copy_of(d, f, hr, ldh, n, pack && iv == 0 ? b.hp : nullptr, dw && iv == 0 ? b.ht : nullptr);
+            jh.stat = st; jh.gout = gout_stride ? go : nullptr; jh.t = temperature;
+            const bool fresh = ir == 0 || p.nvc > 1;
+            LIN_TRY(lin_copy(d, f, jh, lin_copy_of(d, f, wr, ldw, nv, pack && fresh ? b.wp : nullptr, dh && fresh ? b.wt : nullptr), s));
             LinGemm g{};
             g.a = pack ? b.hp : (const void*)hr; g.lda = pack ? f.row(D) : ldh; g.b = pack ? b.wp : (const void*)wr; g.ldb = pack ? f.row(D) : ldw;
             g.M = (int)n; g.N = nv; g.K = pack ? f.K(D) : D; g.Kp = (int)up(D, 64);
@@ -757,8 +789,8 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, (float*)g.dzt, g.lddzt, v0, nv, entries, 0, 0ll);
             FEA_LAUNCH_CHECK();
             if (db) {
-                const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (tiles + LIN_DB_TILES - 1) / LIN_DB_TILES;
-                hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(256), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, (long long)LIN_DB_TILES * tm * K, b.dbpart);
+                const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (int)((n + LIN_DB_ROWS - 1) / LIN_DB_ROWS);
+                hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(256), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, LIN_DB_ROWS / tm, (long long)LIN_DB_ROWS * K, b.dbpart);
                 FEA_LAUNCH_CHECK();
                 hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);
                 FEA_LAUNCH_CHECK();
@@ -769,21 +801,21 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 LinGemm m = from;
                 m.a = A; m.b = B; m.lda = m.ldb = f.row(k); m.M = (int)M; m.N = D; m.K = f.K(k); m.Kp = (int)up(k, 64);
                 m.splits = t.splits; m.kper = (int)up((m.K + t.splits - 1) / t.splits, 64);
-                const bool direct = t.splits == 1 && first && last;
-                if (direct && f.dt != FEA_PL) { m.out = out; m.ldo = D; } else m.slab = direct ? (float*)out : b.slab;
+                const bool direct = t.splits == 1 && first && last && d.straight();
+                m.ldo = up(D, 4);
+                if (direct && f.dt != FEA_PL) m.out = out; else m.slab = direct ? (float*)out : b.slab;
                 LIN_TRY(fea_lin_gemm(LIN_STORE, f.dt, t.tile, m, s));
-                return direct ? FEA_OK : lin_reduce(d, b.slab, t.splits, M * D, first ? nullptr : acc, last ? nullptr : acc, last ? out : nullptr, s);
+                return direct ? FEA_OK : lin_reduce(d, b.slab, t.splits, M, first ? nullptr : acc, last ? nullptr : acc, last ? out : nullptr, s);
             };
             LinGemm m{};
             m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
             if (dh) {
-                LIN_TRY(lin_transpose(d, f, wr, ldw, b.wt, nv, nullptr, nullptr, 1.f, s));
                 m.scale = 1;
                 LIN_TRY(product(m, b.dz, b.wt, n, nv, p.th, (char*)dh + r0 * D * d.es, b.acch, iv == 0, iv + 1 == p.nvc));
             }
             if (dw) {
                 m.scale = gout_stride ? 0 : 2;
-                LIN_TRY(product(m, b.dzt, b.ht, nv, n, p.tw, (char*)dw + v0 * D * d.es, b.accw ? b.accw + v0 * D : nullptr, ir == 0, ir + 1 == p.nrc));
+                LIN_TRY(product(m, b.dzt, b.ht, nv, n, p.tw, (char*)dw + v0 * D * d.es, b.accw ? b.accw + v0 * up(D, 4) : nullptr, ir == 0, ir + 1 == p.nrc));
             }
         }
     }

@@ -20,17 +20,17 @@ __device__ __forceinline__ void mma16x16(f32x4& acc, const u32x4& a, const u32x4
 
 template <typename T, int NR, bool ALN>
 __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
-    // bytes of a chunk of a row (with 64 labels half of it, so that four workgroups fit a CU: 1.5 rounds of two took 10 % longer than one of
-    // four); a row's distance in LDS puts 16 rows in 16 bank groups
-    constexpr int LR_CB = NR == 4 ? 256 : 512, LR_LD = LR_CB + 16, PR = LR_CB / 16;
-    constexpr int EPC = Elem<T>::EPC, CE = LR_CB / (int)sizeof(T), NS = LR_CB / 64;     // elements, products of a chunk
-    __shared__ __attribute__((aligned(16))) char hs[2][16 * NR * LR_LD];
+    // a chunk is 256 bytes of a row; three chunks of the weight are in flight while one is multiplied.  The distance of a row in LDS
+    // puts 16 rows in 16 bank groups
+    constexpr int CB = 256, LD = CB + 16, PR = CB / 16, RING = 4;
+    constexpr int EPC = Elem<T>::EPC, CE = CB / (int)sizeof(T), NS = CB / 64;     // elements, products of a chunk
+    __shared__ __attribute__((aligned(16))) char hs[2][16 * NR * LD];
     __shared__ float2 red[4][16 * NR];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q16 = lane >> 4;
     const int n0 = blockIdx.x * 64 + wave * 16;
     const T* const w = (const T*)g.b + (long long)min(n0 + r16, g.N - 1) * g.ldb;
     const T* const h = (const T*)g.a;
-    u32x4 wv[2][NS];
+    u32x4 wv[RING][NS];
     auto wload = [&](int buf, int k0) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -51,33 +51,34 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
 #pragma unroll
         for (int i = 0; i < HP; ++i) {
             const int p = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(hs[buf] + (p / PR) * LR_LD + (p % PR) * 16) = hv[i];
+            *reinterpret_cast<u32x4*>(hs[buf] + (p / PR) * LD + (p % PR) * 16) = hv[i];
         }
     };
     f32x4 acc[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto mul = [&](int buf) {
+    // The workgroups start their reduction at different chunks (it ends where it began): in step they would all ask for the same
+    // columns of rows that lie a power of two apart, that is for a few of the memory channels at a time.
+    const int rounds = (g.K + RING * CE - 1) / (RING * CE), nch = rounds * RING;
+    int at = (int)(blockIdx.x % (unsigned)nch);
+    auto chunk = [&](int ahead) { int c = at + ahead; return (c >= nch ? c - nch : c) * CE; };
+    hload(chunk(0));
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+    for (int i = 0; i < RING - 1; ++i) wload(i, chunk(i));
+    for (int r = 0; r < rounds; ++r) {
 #pragma unroll
-            for (int i = 0; i < NR; ++i)
-                mma16x16(acc[i], wv[buf][s], *reinterpret_cast<const u32x4*>(hs[buf] + (16 * i + r16) * LR_LD + (4 * s + q16) * 16), (const T*)nullptr);
-    };
-    hload(0);
-    wload(0, 0);
-    // two chunks per round, so that the buffers' indexes are constants
-    for (int k0 = 0; k0 < g.K; k0 += 2 * CE) {
-        hput(0);
-        hload(k0 + CE);
-        wload(1, k0 + CE);
-        __syncthreads();              // (also: every wave is done with the other buffer)
-        mul(0);
-        hput(1);
-        hload(k0 + 2 * CE);
-        wload(0, k0 + 2 * CE);
-        __syncthreads();
-        mul(1);
+        for (int c = 0; c < RING; ++c) {      // one round of the ring, so that the buffers' indexes are constants
+            hput(c & 1);
+            hload(chunk(1));
+            wload((c + RING - 1) % RING, chunk(RING - 1));
+            if (++at == nch) at = 0;
+            __syncthreads();                  // (also: every wave is done with the other buffer)
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+                    mma16x16(acc[i], wv[c][s], *reinterpret_cast<const u32x4*>(hs[c & 1] + (16 * i + r16) * LD + (4 * s + q16) * 16), (const T*)nullptr);
+        }
     }
     // lane: label 16 i + r16, classes n0 + 4 q16 .. + 3
     float bias[4];
