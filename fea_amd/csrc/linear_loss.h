@@ -39,6 +39,8 @@ struct LinGemm {
     int scale;                        // 0: none, 1: times the row scale of A's row, 2: times the common scale (gout, count, t above)
     int splits, kper;
     int ntm, ntn;
+    // fea_lin_rows: selected logits a . b + bias of the entries index[M][sel] (nullable)
+    float* zsel; const long long* index; int sel;
 };
 
 // gradient scale of a row: d loss / d (row loss) times the temperature; 0 for a row that does not count

@@ -288,24 +288,15 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinJoin j) {
     lin_join_body(j, j.G, gl, row, row < j.rows, lin_lse_of(lin_merge_lanes(a, j.G)));
 }
 
-// The same for few rows, one workgroup per row, the selected logits and the join in one launch: all waves take entries and tiles,
-// then the first one joins.
-template <typename T>
-__global__ __launch_bounds__(256) void lin_join_rows_kernel(const LinJoin j, const T* h, long long ldh, const T* w, long long ldw, const float* bias, int D, int vec) {
+// The same for few rows, one workgroup per row: all waves take tiles, then the first one joins.
+__global__ __launch_bounds__(256) void lin_join_rows_kernel(const LinJoin j) {
     __shared__ float2 red[4];
     const long long row = blockIdx.x;
     float2 a = make_float2(-INFINITY, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = threadIdx.x; i < j.ntn; i += 256) a = lin_merge(a, j.part[row * j.ntn + i]);
-    for (int k = threadIdx.x >> 6; k < j.K; k += 4) {
-        const long long i = j.index[row * j.K + k];
-        if (i < 0 || i >= j.V) continue;
-        const float s = vec ? lin_dot<T, true>(h + row * ldh, w + i * ldw, D, threadIdx.x & 63, 64) : lin_dot<T, false>(h + row * ldh, w + i * ldw, D, threadIdx.x & 63, 64);
-        if ((threadIdx.x & 63) == 0) j.zsel[row * j.K + k] = bias ? s + bias[i] : s;
-    }
     a = lin_merge_lanes(a, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __threadfence_block();
     __syncthreads();
     lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64, lin_lse_of(lin_merge(lin_merge(red[0], red[1]), lin_merge(red[2], red[3]))));
 }
@@ -661,7 +652,9 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         return FEA_OK;
     }
     const long long entries = d.rows * d.K;
-    if (p.tile != 64) {
+    // selected logits: in the few-rows kernel's epilogue, where every workgroup looks through all entries, or by gathered dot products
+    const bool inner = p.tile == 64 && entries <= 2048;
+    if (!inner) {
         int lanes = 1;
         while (lanes < 64 && lanes * d.epc < d.D) lanes *= 2;
         const long long blocks = (entries * lanes + 255) / 256;
@@ -681,6 +674,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         g.a = pack ? b.hp : hr; g.lda = pack ? f.row(d.D) : ldh; g.b = pack ? b.wp : w; g.ldb = pack ? f.row(d.D) : ldw;
         g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
+        if (inner) { g.zsel = b.zsel; g.index = j.index; g.sel = d.K; }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
         else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;
@@ -693,9 +687,8 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         if (q.loss_rows) q.loss_rows += r;
         q.bsum = loss ? b.bsum + blk : nullptr; q.bcnt = b.bcnt + blk;
         const long long grid = p.tile == 64 ? n : (n + 256 / p.G - 1) / (256 / p.G);
-        if (p.tile != 64)               hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
-        else if (d.dtype == FEA_BF16)   hipLaunchKernelGGL(lin_join_rows_kernel<__bf16>, dim3((unsigned)grid), dim3(256), 0, s, q, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, d.D, d.odd() ? 0 : 1);
-        else                            hipLaunchKernelGGL(lin_join_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, q, (const float*)h, ldh, (const float*)w, ldw, bias, d.D, d.odd() ? 0 : 1);
+        if (p.tile == 64) hipLaunchKernelGGL(lin_join_rows_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
+        else              hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
         FEA_LAUNCH_CHECK();
         blk += grid;
     }

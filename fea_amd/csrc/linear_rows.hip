@@ -19,15 +19,17 @@ __device__ __forceinline__ void mma16x16(f32x4& acc, const u32x4& a, const u32x4
 }
 
 template <typename T, int NR, bool ALN>
-__global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
-    // a chunk is 256 bytes of a row; three chunks of the weight are in flight while one is multiplied.  The distance of a row in LDS
-    // puts 16 rows in 16 bank groups
+__global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const LinGemm g) {
+    // a chunk is 256 bytes of a row; three chunks of the weight are in flight while one is multiplied.  The labels' chunk is asked for two
+    // steps before it goes to LDS: loads come back in order, so waiting for one that is a step old would be waiting for the weight's
+    // too.  The distance of a row in LDS puts 16 rows in 16 bank groups
+    constexpr int NT = 256, CLS = 64;
     constexpr int CB = 256, LD = CB + 16, PR = CB / 16, RING = 4;
     constexpr int EPC = Elem<T>::EPC, CE = CB / (int)sizeof(T), NS = CB / 64;     // elements, products of a chunk
     __shared__ __attribute__((aligned(16))) char hs[2][16 * NR * LD];
     __shared__ float2 red[4][16 * NR];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, q16 = lane >> 4;
-    const int n0 = blockIdx.x * 64 + wave * 16;
+    const int n0 = blockIdx.x * CLS + wave * 16;
     const T* const w = (const T*)g.b + (long long)min(n0 + r16, g.N - 1) * g.ldb;
     const T* const h = (const T*)g.a;
     u32x4 wv[RING][NS];
@@ -38,20 +40,20 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
             wv[buf][s] = lin_load16<T, ALN>(w + k, g.K - k);
         }
     };
-    constexpr int HP = NR * 16 * PR / 256;          // 16-byte pieces of the labels' chunk per thread
-    u32x4 hv[HP];
-    auto hload = [&](int k0) {
+    constexpr int HP = NR * 16 * PR / NT;           // 16-byte pieces of the labels' chunk per thread
+    u32x4 hv[2][HP];
+    auto hload = [&](int buf, int k0) {
 #pragma unroll
         for (int i = 0; i < HP; ++i) {
-            const int p = tid + 256 * i, row = p / PR, k = k0 + (p % PR) * EPC;
-            hv[i] = row < g.M ? lin_load16<T, ALN>(h + row * g.lda + k, g.K - k) : u32x4{0, 0, 0, 0};
+            const int p = tid + NT * i, row = p / PR, k = k0 + (p % PR) * EPC;
+            hv[buf][i] = row < g.M ? lin_load16<T, ALN>(h + row * g.lda + k, g.K - k) : u32x4{0, 0, 0, 0};
         }
     };
     auto hput = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < HP; ++i) {
-            const int p = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(hs[buf] + (p / PR) * LD + (p % PR) * 16) = hv[i];
+            const int p = tid + NT * i;
+            *reinterpret_cast<u32x4*>(hs[buf] + (p / PR) * LD + (p % PR) * 16) = hv[buf][i];
         }
     };
     f32x4 acc[NR];
@@ -60,19 +62,21 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
     // The workgroups start their reduction at different chunks (it ends where it began): in step they would all ask for the same
     // columns of rows that lie a power of two apart, that is for a few of the memory channels at a time.
     const int rounds = (g.K + RING * CE - 1) / (RING * CE), nch = rounds * RING;
-    int at = (int)(blockIdx.x % (unsigned)nch);
+    int at = (int)(3u * blockIdx.x % (unsigned)nch);
     auto chunk = [&](int ahead) { int c = at + ahead; return (c >= nch ? c - nch : c) * CE; };
-    hload(chunk(0));
-#pragma unroll
-    for (int i = 0; i < RING - 1; ++i) wload(i, chunk(i));
+    hload(0, chunk(0));
+    wload(0, chunk(0));
+    hload(1, chunk(1));
+    wload(1, chunk(1));
+    wload(2, chunk(2));
     for (int r = 0; r < rounds; ++r) {
 #pragma unroll
         for (int c = 0; c < RING; ++c) {      // one round of the ring, so that the buffers' indexes are constants
             hput(c & 1);
-            hload(chunk(1));
+            hload(c & 1, chunk(2));
             wload((c + RING - 1) % RING, chunk(RING - 1));
-            if (++at == nch) at = 0;
             __syncthreads();                  // (also: every wave is done with the other buffer)
+            if (++at == nch) at = 0;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
 #pragma unroll
@@ -80,6 +84,9 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
                     mma16x16(acc[i], wv[c][s], *reinterpret_cast<const u32x4*>(hs[c & 1] + (16 * i + r16) * LD + (4 * s + q16) * 16), (const T*)nullptr);
         }
     }
+    // the selected logits: every workgroup looks for its own classes among the entries
+    __syncthreads();
+    float (*const zt)[16 * NR + 1] = reinterpret_cast<float (*)[16 * NR + 1]>(&hs[0][0]);       // [classes][labels]
     // lane: label 16 i + r16, classes n0 + 4 q16 .. + 3
     float bias[4];
 #pragma unroll
@@ -88,7 +95,12 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
     for (int i = 0; i < NR; ++i) {
         float z[4], mx = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { z[e] = n0 + 4 * q16 + e < g.N ? (acc[i][e] + bias[e]) * g.inv_t : -INFINITY; mx = fmaxf(mx, z[e]); }
+        for (int e = 0; e < 4; ++e) {
+            const float raw = acc[i][e] + bias[e];
+            if (g.zsel) zt[wave * 16 + 4 * q16 + e][16 * i + r16] = raw;
+            z[e] = n0 + 4 * q16 + e < g.N ? raw * g.inv_t : -INFINITY;
+            mx = fmaxf(mx, z[e]);
+        }
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float base = mx == -INFINITY ? 0.f : mx;
@@ -99,6 +111,11 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
         if (q16 == 0) red[wave][16 * i + r16] = make_float2(mx, sum);
     }
     __syncthreads();
+    if (g.zsel)
+        for (int e = tid; e < g.M * g.sel; e += NT) {
+            const long long c = g.index[e] - (long long)blockIdx.x * CLS;
+            if (c >= 0 && c < CLS && (int)blockIdx.x * CLS + c < g.N) g.zsel[e] = zt[c][e / g.sel];
+        }
     if (tid < 16 * NR && tid < g.M) {
         float mx = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -113,10 +130,12 @@ __global__ __launch_bounds__(256) void lin_rows_kernel(const LinGemm g) {
 template <typename T, bool ALN> static void rows_launch(const LinGemm& g, unsigned grid, hipStream_t s) {
     if (g.M <= 16)      hipLaunchKernelGGL((lin_rows_kernel<T, 1, ALN>), dim3(grid), dim3(256), 0, s, g);
     else if (g.M <= 32) hipLaunchKernelGGL((lin_rows_kernel<T, 2, ALN>), dim3(grid), dim3(256), 0, s, g);
+    else if (g.M <= 48) hipLaunchKernelGGL((lin_rows_kernel<T, 3, ALN>), dim3(grid), dim3(256), 0, s, g);
     else                hipLaunchKernelGGL((lin_rows_kernel<T, 4, ALN>), dim3(grid), dim3(256), 0, s, g);
 }
 
-// LIN_LSE of at most 64 label rows, operands of any alignment; part has one column per 64 classes
+
+// LIN_LSE of at most 64 label rows, operands of any alignment
 int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s) {
     FEA_CHECK(g.M > 0 && g.M <= 64 && g.N > 0 && g.K > 0, FEA_E_BADARG, "lin_rows: %d x %d x %d", g.M, g.N, g.K);
     g.ntn = (g.N + 63) / 64;
