@@ -30,6 +30,30 @@ template <typename T> __device__ __forceinline__ float few_tlog(const void* p, i
     return dt == FEA_BF16 ? (float)((const __bf16*)p)[e] : ((const float*)p)[e];
 }
 
+// A row's teacher entries (forward: class and logit; backward: class and share): the first 4 are loaded together and kept, the
+// others are read as they are gone through.
+template <typename T> struct LinEntries {
+    static constexpr int KEEP = 4;
+    const LinFew& g;
+    long long e0;
+    long long i[KEEP];
+    float v[KEEP];
+    __device__ __forceinline__ float value(long long e) const { return g.tlog ? few_tlog<T>(g.tlog, g.tdt, e) : g.psel[e]; }
+    __device__ __forceinline__ LinEntries(const LinFew& g_, long long row) : g(g_), e0(row * g_.K) {
+        if (!g.tlog && (!g.psel || !g.gout)) return;      // cross entropy
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+            i[k] = k < g.K ? g.index[e0 + k] : -1;
+            v[k] = k < g.K ? value(e0 + k) : 0.f;
+        }
+    }
+    template <class F> __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) if (k < g.K) f(k, i[k], v[k]);
+        for (int k = KEEP; k < g.K; ++k) f(k, g.index[e0 + k], value(e0 + k));
+    }
+};
+
 // NB blocks of 32 features, NG groups of 8 classes (4 registers)
 template <typename T, int NB, int NG, bool ALN>
 __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
@@ -47,24 +71,28 @@ __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
 
     double total = 0.0;
     int counted = 0;
-    u32x4 nx[NK];
-    auto fetch = [&](long long tile) {
+    // two tiles on the way while one is worked on, their labels with them
+    u32x4 nx[2][NK];
+    long long nl[2];
+    auto fetch = [&](int u, long long tile) {
+        if (tile >= tiles) return;
         long long r = tile * 32 + l32;
         r = r < g.rows ? r : g.rows - 1;
         const T* p = (const T*)g.h + r * g.ldh;
 #pragma unroll
-        for (int k = 0; k < NK; ++k) nx[k] = few_load<T, ALN>(p, (2 * k + hf) * EPC, g.D);
+        for (int k = 0; k < NK; ++k) nx[u][k] = few_load<T, ALN>(p, (2 * k + hf) * EPC, g.D);
+        nl[u] = g.tlog ? 0 : g.index[r];
     };
-    if (wave < tiles) fetch(wave);
-    for (long long tile = wave; tile < tiles; tile += nwaves) {
+    auto body = [&](int u, long long tile) {
         u32x4 hx[NK];
 #pragma unroll
-        for (int k = 0; k < NK; ++k) hx[k] = nx[k];
+        for (int k = 0; k < NK; ++k) hx[k] = nx[u][k];
         const long long row = tile * 32 + l32;
         const bool in = row < g.rows;
         const long long rr = in ? row : g.rows - 1;
-        const long long label = g.tlog ? 0 : g.index[rr];
-        if (tile + nwaves < tiles) fetch(tile + nwaves);
+        const long long label = nl[u];
+        LinEntries<T> ent(g, rr);
+        fetch(u, tile + 2 * nwaves);
         f32x16 acc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -94,24 +122,21 @@ __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
             if (label < 0 || label >= g.V) { loss = NAN; lse = NAN; }
             if (!counts) loss = 0.f;
         } else {
-            const long long e0 = rr * g.K;
             float tm = -INFINITY, ts = 0.f;
             bool bad = false;
-            for (int k = 0; k < g.K; ++k) {
-                const long long i = g.index[e0 + k];
+            ent.each([&](int, long long i, float a) {
                 if (i >= g.V) bad = true;
-                if (i >= 0) { const float a = few_tlog<T>(g.tlog, g.tdt, e0 + k) * g.inv_t; bad |= !(a < INFINITY); tm = fmaxf(tm, a); }
-            }
+                if (i >= 0) { a *= g.inv_t; bad |= !(a < INFINITY); tm = fmaxf(tm, a); }
+            });
             counts = in && (bad || tm != -INFINITY);
             const float tb = tm == -INFINITY ? 0.f : tm;
-            for (int k = 0; k < g.K; ++k) if (g.index[e0 + k] >= 0) ts += expf(few_tlog<T>(g.tlog, g.tdt, e0 + k) * g.inv_t - tb);
+            ent.each([&](int, long long i, float a) { if (i >= 0) ts += expf(a * g.inv_t - tb); });
             const float lt = logf(ts);
             float pz = 0.f, pl = 0.f;                     // sum p z over the classes of this half; sum p (log p + lse)
-            for (int k = 0; k < g.K; ++k) {
-                const long long i = g.index[e0 + k];
+            ent.each([&](int k, long long i, float a) {
                 float p = 0.f;
                 if (i >= 0 && counts) {
-                    const float lp = few_tlog<T>(g.tlog, g.tdt, e0 + k) * g.inv_t - tb - lt;
+                    const float lp = a * g.inv_t - tb - lt;
                     p = bad ? NAN : expf(lp);
                     if (p > 0.f) {
                         pl += p * (lp + lse);
@@ -119,8 +144,8 @@ __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
                         for (int q = 0; q < NR; ++q) if (LinI::cls(q, hf) == i) pz += p * z[q];
                     }
                 }
-                if (g.psel && in && hf == 0) g.psel[e0 + k] = p;
-            }
+                if (g.psel && in && hf == 0) g.psel[rr * g.K + k] = p;
+            });
             pz += __shfl_xor(pz, 32);
             loss = (pl - pz) * g.t * g.t;
             if (bad) { loss = NAN; lse = NAN; }
@@ -132,6 +157,12 @@ __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
             total += (double)loss;
             counted += counts;
         }
+    };
+    fetch(0, wave);
+    fetch(1, wave + nwaves);
+    for (long long tile = wave; tile < tiles; tile += 2 * nwaves) {
+        body(0, tile);
+        if (tile + nwaves < tiles) body(1, tile + nwaves);
     }
     if (g.bsum) {
         __shared__ double ls[4];
@@ -188,30 +219,35 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dw[b][e] = 0.f;
 
-    u32x4 nx[NK];
-    auto fetch = [&](long long tile) {
+    u32x4 nx[2][NK];
+    float2 ns[2];
+    long long nl[2];
+    auto fetch = [&](int u, long long tile) {
+        if (tile >= tiles) return;
         long long r = tile * 32 + l32;
         r = r < g.rows ? r : g.rows - 1;
         const T* p = (const T*)g.h + r * g.ldh;
 #pragma unroll
-        for (int k = 0; k < NK; ++k) nx[k] = few_load<T, ALN>(p, (2 * k + hf) * EPC, g.D);
+        for (int k = 0; k < NK; ++k) nx[u][k] = few_load<T, ALN>(p, (2 * k + hf) * EPC, g.D);
+        ns[u] = g.stat[r];
+        nl[u] = g.psel ? -1 : g.index[r];
     };
-    if (wave < tiles) fetch(wave);
-    for (long long tile = wave; tile < tiles; tile += nwaves) {
+    auto body = [&](int u, long long tile) {
         u32x4 hx[NK];
         const long long row = tile * 32 + l32;
         const bool in = row < g.rows;
         const long long rr = in ? row : g.rows - 1;
-        const float2 st = g.stat[rr];
+        const float2 st = ns[u];
         const bool on = in && st.y != 0.f;
-        const long long label = g.psel ? -1 : g.index[rr];
+        const long long label = nl[u];
+        LinEntries<T> ent(g, rr);
         const float sc = lin_row_scale(g.gout, g.gstride, g.count, g.t, st.y, rr);
         // a row that does not count is read as zeros: its gradients are 0 whatever it holds
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hx[k][e] = on ? nx[k][e] : 0u;
-        if (tile + nwaves < tiles) fetch(tile + nwaves);
+            for (int e = 0; e < 4; ++e) hx[k][e] = on ? nx[u][k][e] : 0u;
+        fetch(u, tile + 2 * nwaves);
         f32x16 acc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -226,12 +262,10 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
             dz[i] = c == label ? q - 1.f : q;
         }
         if (g.psel)
-            for (int k = 0; k < g.K; ++k) {
-                const long long i = g.index[rr * g.K + k];
-                const float p = g.psel[rr * g.K + k];
+            ent.each([&](int, long long i, float p) {
 #pragma unroll
                 for (int q = 0; q < NR; ++q) if (LinI::cls(q, hf) == i) dz[q] -= p;
-            }
+            });
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             dz[i] = on && LinI::cls(i, hf) < g.V ? dz[i] : 0.f;
@@ -306,6 +340,12 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
                 for (int s = 0; s < RS; ++s) mma16(dw[b], za[s], few_pack<T>(v + EPC * s), (const T*)nullptr);
             }
         }
+    };
+    fetch(0, wave);
+    fetch(1, wave + nwaves);
+    for (long long tile = wave; tile < tiles; tile += 2 * nwaves) {
+        body(0, tile);
+        if (tile + nwaves < tiles) body(1, tile + nwaves);
     }
     // the four waves' sums, then one slab per workgroup: [32 classes][NB * 32 features], db behind it
     __shared__ float red[4][32 * 32];
@@ -333,25 +373,31 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
     }
 }
 
-// dw = scale * sum of the slabs, db = sum of the db slabs: 16 lanes share an element, then add in lane order
+// dw = scale * sum of the slabs, db = sum of the db slabs: one workgroup per 4 elements of a slab's row, 64 lanes take the slabs in turn and add up in
+// a fixed order
 template <typename T>
 __global__ __launch_bounds__(256) void lin_few_join_kernel(const LinFew g, int nslab, int ldd, T* dw, float* db) {
-    __shared__ double part[16][16];
-    const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
-    const long long i = (long long)blockIdx.x * 16 + x, nw = dw ? (long long)g.V * g.D : 0;
-    const bool isw = i < nw, isb = !isw && db && i < nw + g.V;
-    const float* p = nullptr;
-    long long step = 0;
-    if (isw) { p = g.slab + i / g.D * ldd + i % g.D; step = g.slab_ld; }
-    if (isb) { p = g.dbslab + (i - nw); step = 32; }
+    __shared__ double part[4][64];
+    const int x = threadIdx.x & 3, y = threadIdx.x >> 2;
+    const int per = dw ? (g.D + 3) / 4 : 0;                 // workgroups of a class's row of dw; those of db behind them
+    const int nw = g.V * per, c = blockIdx.x < nw ? blockIdx.x / per : -1, d = c < 0 ? (int)(blockIdx.x - nw) * 4 + x : (int)(blockIdx.x - c * per) * 4 + x;
+    const bool in = c < 0 ? d < g.V : d < g.D;
+    const float* p = c < 0 ? g.dbslab + d : g.slab + c * ldd + d;
+    const long long step = c < 0 ? 32 : g.slab_ld;
     double s = 0.0;
-    if (p) for (int k = y; k < nslab; k += 16) s += (double)p[k * step];
-    part[y][x] = s;
+    if (in)
+#pragma unroll 4
+        for (int k = y; k < nslab; k += 64) s += (double)p[k * step];
+    part[x][y] = s;
     __syncthreads();
-    if (y == 0 && p) {
-        for (int k = 1; k < 16; ++k) s += part[k][x];
-        if (isb) db[i - nw] = (float)s;
-        else dw[i] = from_f32<T>((float)s * (g.gstride ? 1.f : lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0)));
+    for (int w = 32; w; w >>= 1) {
+        if (y < w) part[x][y] += part[x][y + w];
+        __syncthreads();
+    }
+    if (y == 0 && in) {
+        s = part[x][0];
+        if (c < 0) db[d] = (float)s;
+        else dw[(long long)c * g.D + d] = from_f32<T>((float)s * (g.gstride ? 1.f : lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0)));
     }
 }
 
@@ -406,9 +452,9 @@ int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s) {
     if (dtype == FEA_BF16) few_launch<__bf16>(g, true, few_aligned(g, dtype), (unsigned)nslab, s);
     else                   few_launch<float>(g, true, few_aligned(g, dtype), (unsigned)nslab, s);
     FEA_LAUNCH_CHECK();
-    const long long n = (dw ? (long long)g.V * g.D : 0) + (db ? g.V : 0);
+    const int n = (dw ? g.V * ((g.D + 3) / 4) : 0) + (db ? (g.V + 3) / 4 : 0);
     if (n) {
-        const dim3 grid((unsigned)((n + 15) / 16));
+        const dim3 grid((unsigned)n);
         if (dtype == FEA_BF16) hipLaunchKernelGGL(lin_few_join_kernel<__bf16>, grid, dim3(256), 0, s, g, nslab, ldd, (__bf16*)dw, db);
         else                   hipLaunchKernelGGL(lin_few_join_kernel<float>, grid, dim3(256), 0, s, g, nslab, ldd, (float*)dw, db);
         FEA_LAUNCH_CHECK();
