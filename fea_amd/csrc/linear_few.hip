@@ -54,6 +54,62 @@ template <typename T> struct LinEntries {
     }
 };
 
+// A wave's 32 rows x NB blocks of 32 features on their way between memory, where a load or store takes whole rows (lanes along a row), and the
+// operand layout, where a lane is a row: through 32 rows of LDS that only this wave uses.  Lanes along a column directly would touch 32 lines
+// per load, a quarter of each.
+template <typename T, int NB, bool ALN> struct LinRows {
+    static constexpr int EPC = Elem<T>::EPC, CPR = NB * 32 / EPC, RPL = 64 / CPR, NK = 32 / RPL;     // 16-byte pieces of a row, rows of a load, loads
+    static constexpr int LD = CPR * 16 + 16;
+    char* lds;
+    int row, piece;                        // of this lane in load 0
+    __device__ __forceinline__ LinRows(char* p, int lane) : lds(p), row(lane / CPR), piece(lane % CPR) {}
+    __device__ __forceinline__ void load(u32x4 (&v)[NK], const T* h, long long ld, long long first, long long rows, int D) const {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            long long r = first + row + k * RPL;
+            r = r < rows ? r : rows - 1;
+            v[k] = few_load<T, ALN>(h + r * ld, piece * EPC, D);
+        }
+    }
+    static __device__ __forceinline__ void fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
+    // loaded pieces -> operand: piece 2 k + hf of row l32
+    __device__ __forceinline__ void turn(const u32x4 (&v)[NK], u32x4 (&x)[NK], int l32, int hf) const {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) *reinterpret_cast<u32x4*>(lds + (row + k * RPL) * LD + piece * 16) = v[k];
+        fence();
+#pragma unroll
+        for (int k = 0; k < NK; ++k) x[k] = *reinterpret_cast<const u32x4*>(lds + l32 * LD + (2 * k + hf) * 16);
+        fence();
+    }
+    // four consecutive features d .. d + 3 of row l32
+    __device__ __forceinline__ void put(const f32x16& o, int q, float sc, int l32, int d) const {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(lds + l32 * LD + d * 4) = f32x4{o[4 * q] * sc, o[4 * q + 1] * sc, o[4 * q + 2] * sc, o[4 * q + 3] * sc};
+        else *reinterpret_cast<bf16x4*>(lds + l32 * LD + d * 2) = bf16x4{(__bf16)(o[4 * q] * sc), (__bf16)(o[4 * q + 1] * sc), (__bf16)(o[4 * q + 2] * sc), (__bf16)(o[4 * q + 3] * sc)};
+    }
+    __device__ __forceinline__ void store(T* out, long long first, long long rows, int D) const {
+        fence();
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const long long r = first + row + k * RPL;
+            const int left = D - piece * EPC;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(lds + (row + k * RPL) * LD + piece * 16);
+            if (r >= rows || left <= 0) continue;
+            T* const o = out + r * D + piece * EPC;
+            if constexpr (ALN) *reinterpret_cast<u32x4*>(o) = v;
+            else {
+                if (left >= EPC) __builtin_memcpy(o, &v, 16);
+                else {
+                    T x[EPC];
+                    *reinterpret_cast<u32x4*>(x) = v;
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e) if (e < left) o[e] = x[e];
+                }
+            }
+        }
+        fence();
+    }
+};
+
 // NB blocks of 32 features, NG groups of 8 classes (4 registers)
 template <typename T, int NB, int NG, bool ALN>
 __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
@@ -71,22 +127,20 @@ __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
 
     double total = 0.0;
     int counted = 0;
+    __shared__ __attribute__((aligned(16))) char buf[4][32 * LinRows<T, NB, ALN>::LD];
+    const LinRows<T, NB, ALN> rows(buf[threadIdx.x >> 6], lane);
     // two tiles on the way while one is worked on, their labels with them
     u32x4 nx[2][NK];
     long long nl[2];
     auto fetch = [&](int u, long long tile) {
         if (tile >= tiles) return;
-        long long r = tile * 32 + l32;
-        r = r < g.rows ? r : g.rows - 1;
-        const T* p = (const T*)g.h + r * g.ldh;
-#pragma unroll
-        for (int k = 0; k < NK; ++k) nx[u][k] = few_load<T, ALN>(p, (2 * k + hf) * EPC, g.D);
+        rows.load(nx[u], (const T*)g.h, g.ldh, tile * 32, g.rows, g.D);
+        const long long r = tile * 32 + l32 < g.rows ? tile * 32 + l32 : g.rows - 1;
         nl[u] = g.tlog ? 0 : g.index[r];
     };
     auto body = [&](int u, long long tile) {
         u32x4 hx[NK];
-#pragma unroll
-        for (int k = 0; k < NK; ++k) hx[k] = nx[u][k];
+        rows.turn(nx[u], hx, l32, hf);
         const long long row = tile * 32 + l32;
         const bool in = row < g.rows;
         const long long rr = in ? row : g.rows - 1;
@@ -219,16 +273,15 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) dw[b][e] = 0.f;
 
+    __shared__ __attribute__((aligned(16))) char buf[4][32 * LinRows<T, NB, ALN>::LD];
+    const LinRows<T, NB, ALN> rows(buf[threadIdx.x >> 6], lane);
     u32x4 nx[2][NK];
     float2 ns[2];
     long long nl[2];
     auto fetch = [&](int u, long long tile) {
         if (tile >= tiles) return;
-        long long r = tile * 32 + l32;
-        r = r < g.rows ? r : g.rows - 1;
-        const T* p = (const T*)g.h + r * g.ldh;
-#pragma unroll
-        for (int k = 0; k < NK; ++k) nx[u][k] = few_load<T, ALN>(p, (2 * k + hf) * EPC, g.D);
+        rows.load(nx[u], (const T*)g.h, g.ldh, tile * 32, g.rows, g.D);
+        const long long r = tile * 32 + l32 < g.rows ? tile * 32 + l32 : g.rows - 1;
         ns[u] = g.stat[r];
         nl[u] = g.psel ? -1 : g.index[r];
     };
@@ -243,10 +296,11 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
         LinEntries<T> ent(g, rr);
         const float sc = lin_row_scale(g.gout, g.gstride, g.count, g.t, st.y, rr);
         // a row that does not count is read as zeros: its gradients are 0 whatever it holds
+        rows.turn(nx[u], hx, l32, hf);
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) hx[k][e] = on ? nx[u][k][e] : 0u;
+            for (int e = 0; e < 4; ++e) hx[k][e] = on ? hx[k][e] : 0u;
         fetch(u, tile + 2 * nwaves);
         f32x16 acc;
 #pragma unroll
@@ -282,28 +336,10 @@ __global__ __launch_bounds__(256) void lin_few_bwd_kernel(const LinFew g) {
                 for (int e = 0; e < 16; ++e) o[e] = 0.f;
 #pragma unroll
                 for (int s = 0; s < NS; ++s) mma16(o, wt[b][s], dzp[s], (const T*)nullptr);
-                T* const out = (T*)g.dh + rr * g.D + 32 * b;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] *= sc;
-                if constexpr (!ALN) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) if (in && 32 * b + LinI::cls(e, hf) < g.D) out[LinI::cls(e, hf)] = from_f32<T>(o[e]);
-                } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (in && 32 * b + 8 * q + 4 * hf < g.D) *reinterpret_cast<f32x4*>(out + 8 * q + 4 * hf) = f32x4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; q += 2) {      // the two wave halves trade quads: 8 consecutive features per lane
-                        const bf16x4 lo = {(__bf16)o[4 * q], (__bf16)o[4 * q + 1], (__bf16)o[4 * q + 2], (__bf16)o[4 * q + 3]};
-                        const bf16x4 hi = {(__bf16)o[4 * q + 4], (__bf16)o[4 * q + 5], (__bf16)o[4 * q + 6], (__bf16)o[4 * q + 7]};
-                        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-                        const auto r0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-                        const auto r1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
-                        if (in && 32 * b + 8 * (q + hf) < g.D) *reinterpret_cast<u32x4*>(out + 8 * (q + hf)) = u32x4{r0[0], r1[0], r0[1], r1[1]};
-                    }
-                }
+                for (int q = 0; q < 4; ++q) rows.put(o, q, sc, l32, 32 * b + 8 * q + 4 * hf);
             }
+            rows.store((T*)g.dh, tile * 32, g.rows, g.D);
         }
         if (g.slab) {
             if (rowg) {                                   // every row has its own factor: it goes to the row
@@ -407,10 +443,11 @@ __global__ __launch_bounds__(256) void lin_few_join_kernel(const LinFew g, int n
 // worth it; the rule does not change with the alignment.
 bool fea_lin_few(long long rows, int D, int V) { return V <= 32 && D <= 64 && rows >= 4096; }
 
-// workgroups: 4 per CU, fewer where they would get less than 4 tiles of 32 rows per wave
-int fea_lin_few_blocks(long long rows) {
-    const long long want = (rows + 511) / 512;
-    return (int)(want < 1024 ? want : 1024);
+// Workgroups, at least 4 tiles of 32 rows per wave.  Backward: two rounds of the two that a CU holds, since each leaves a slab.  Forward:
+// many, so that the last round, which does not fill the chip (a CU holds three), is short: 1,024 took 576 us for 16.8 M rows, 8,192 take 499 us.
+int fea_lin_few_blocks(long long rows, bool bwd) {
+    const long long want = (rows + 511) / 512, most = bwd ? 1024 : 8192;
+    return (int)(want < most ? want : most);
 }
 
 template <typename T, int NB, int NG> static void few_launch2(const LinFew& g, bool bwd, bool aln, unsigned grid, hipStream_t s) {
@@ -437,7 +474,7 @@ static bool few_aligned(const LinFew& g, int dtype) {
 }
 
 int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s) {
-    const unsigned grid = (unsigned)fea_lin_few_blocks(g.rows);
+    const unsigned grid = (unsigned)fea_lin_few_blocks(g.rows, false);
     if (dtype == FEA_BF16) few_launch<__bf16>(g, false, few_aligned(g, dtype), grid, s);
     else                   few_launch<float>(g, false, few_aligned(g, dtype), grid, s);
     FEA_LAUNCH_CHECK();
@@ -445,7 +482,7 @@ int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s) {
 }
 
 int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s) {
-    const int nslab = fea_lin_few_blocks(g.rows), ldd = g.D <= 32 ? 32 : 64;
+    const int nslab = fea_lin_few_blocks(g.rows, true), ldd = g.D <= 32 ? 32 : 64;
     g.slab_ld = 32 * ldd;
     if (!dw) g.slab = nullptr;
     if (!db) g.dbslab = nullptr;

@@ -85,7 +85,7 @@ struct LinFew {
     long long rows; int D, V, K;
 };
 bool fea_lin_few(long long rows, int D, int V);
-int fea_lin_few_blocks(long long rows);
+int fea_lin_few_blocks(long long rows, bool bwd);
 int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s);
 int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 

@@ -528,8 +528,8 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
     LinCarve c{base};
     if (fea_lin_few(d.rows, d.D, d.V)) {
         w = LinFwdWs{};
-        w.bsum = c.take<double>(fea_lin_few_blocks(d.rows));
-        w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows));
+        w.bsum = c.take<double>(fea_lin_few_blocks(d.rows, false));
+        w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows, false));
         return c.at;
     }
     const int t = p.tile == 64 ? 64 : 128;               // (not 256: wide row strides, which a size query does not know, ask for 128)
@@ -551,8 +551,8 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     LinCarve c{base};
     w = LinBwdWs{};
     if (fea_lin_few(d.rows, d.D, d.V)) {
-        if (want & 2) w.slab = c.take<float>(fea_lin_few_blocks(d.rows) * 32ll * 64);
-        if (want & 4) w.colsum = c.take<float>(fea_lin_few_blocks(d.rows) * 32ll);
+        if (want & 2) w.slab = c.take<float>(fea_lin_few_blocks(d.rows, true) * 32ll * 64);
+        if (want & 4) w.colsum = c.take<float>(fea_lin_few_blocks(d.rows, true) * 32ll);
         w.dz = c.take<char>(256);
         return c.at;
     }
@@ -646,7 +646,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         f.bsum = loss ? b.bsum : nullptr; f.bcnt = b.bcnt; f.rows = d.rows; f.D = d.D; f.V = d.V; f.K = d.K;
         LIN_TRY(fea_lin_few_fwd(f, d.dtype, s));
         if (loss) {
-            hipLaunchKernelGGL(lin_total_kernel, dim3(1), dim3(1024), 0, s, (const double*)b.bsum, (const int*)b.bcnt, (long long)fea_lin_few_blocks(d.rows), mean, loss, count);
+            hipLaunchKernelGGL(lin_total_kernel, dim3(1), dim3(1024), 0, s, (const double*)b.bsum, (const int*)b.bcnt, (long long)fea_lin_few_blocks(d.rows, false), mean, loss, count);
             FEA_LAUNCH_CHECK();
         }
         return FEA_OK;
