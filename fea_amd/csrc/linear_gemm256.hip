@@ -7,8 +7,8 @@
 // v_mfma_f32_16x16x32_bf16 in the 256 accumulation registers, the rest in the other 256.
 //
 // Reduction in chunks of 64 channels (whole 128-byte lines), two LDS stages.  In the first half of chunk c every fourth MFMA is
-// followed by one fragment read (second half of c), one LDS write of chunk c + 1 from the registers and one load of chunk c + 2 into
-// the registers just freed; one barrier; in the second half the fragments of chunk c + 1 are read.  Loads are buffer loads with
+// followed by one fragment read (second half of c), one LDS write of chunk c + 1 from the registers and one load of chunk c + 2 (c + 3 in
+// the 128 tile, which has registers for two chunks) into the registers just freed; one barrier; in the second half the fragments of chunk c + 1 are read.  Loads are buffer loads with
 // every bound in the lane's offset, so rows, classes and channels behind the end arrive as zeros without a branch.
 #include "linear_loss.h"
 
@@ -57,7 +57,8 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     const unsigned va = (unsigned)(ra * (int)g.lda * 2 + c * 16), vb = (unsigned)(rb * (int)g.ldb * 2 + c * 16);
     const unsigned ua = 2 * (unsigned)g.lda, sb = 64 * (unsigned)g.ldb;      // bytes of a label's row, of 32 classes' rows
     const int wofs = r * 128 + ((c ^ lb_swz(r)) << 4);
-    u32x4 st[NL];
+    constexpr int SETS = NT == 8 ? 1 : 2;      // chunks on the way in registers (two where there is room: a chunk is then shorter than a load)
+    u32x4 st[SETS][NL];
     // the XCDs start their reduction an eighth apart (it ends where it began): in step, every workgroup of the chip would ask for the
     // same columns of its rows at a time.  Within an XCD all are in step: they share operands in its L2.
     int at = LB_ROT ? (int)(blockIdx.x & 7) * nc >> 3 : 0;
@@ -76,11 +77,11 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             if (pk >= g.Kp) { pk = 0; ++pair; }
         }
     };
-    auto gload = [&](int i) {
-        if (i < NT) st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ka + (i / (NT / 2) * LB_W + 2 * (i % (NT / 2))) * ua : 0x7fffff00u, 0, 0));
-        else        st[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + kc + (i - NT) * sb : 0x7fffff00u, 0, 0));
+    auto gload = [&](int u, int i) {
+        if (i < NT) st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ka + (i / (NT / 2) * LB_W + 2 * (i % (NT / 2))) * ua : 0x7fffff00u, 0, 0));
+        else        st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + kc + (i - NT) * sb : 0x7fffff00u, 0, 0));
     };
-    auto lput = [&](int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i / NT) * LB_OP + wofs + (i % NT) * 32 * 128) = st[i]; };
+    auto lput = [&](int u, int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i / NT) * LB_OP + wofs + (i % NT) * 32 * 128) = st[u][i]; };
 
     const int fofs0 = r16 * 128 + ((q16 ^ lb_swz(r16)) << 4), fofs1 = fofs0 ^ 64;
     const int fa = wm * LB_W * 128, fb = LB_OP + wn * LB_W * 128;
@@ -105,34 +106,37 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
 
     advance(0);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) gload(i);
+    for (int i = 0; i < NL; ++i) gload(0, i);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) lput(0, i);
-    advance(1);
+    for (int i = 0; i < NL; ++i) lput(0, 0, i);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) gload(i);
+    for (int u = 0; u < SETS; ++u) {
+        advance(1 + u);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) gload((1 + u) % SETS, i);
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NL; ++i) frd(0, 0, i);
 
-    for (int ch = 0; ch < nc; ++ch) {
-        const int s = ch & 1;
-        advance(ch + 2);
+    // chunk ch of LDS stage s; chunk ch + 1 lies in register set u, where chunk ch + 1 + SETS follows it
+    auto step = [&](int ch, int s, int u) {
+        advance(ch + 1 + SETS);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) { frd(s, 1, i); lput(s ^ 1, i); gload(i); }
+        for (int i = 0; i < NL; ++i) { frd(s, 1, i); lput(u, s ^ 1, i); gload(u, i); }
         mma(0);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {        // 2 MFMA, LDS read, MFMA, LDS write, MFMA, load
+        for (int i = 0; i < NL; ++i) {        // 4 MFMA (2 where NT is 4), an LDS read, an LDS write, a load
             if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); else if (i & 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-            if (NT == 8 || 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        // chunk c + 1 is in LDS and nobody reads this stage's first half or the other stage any more
+        // chunk ch + 1 is in LDS and nobody reads this stage's first half or the other stage any more
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
@@ -143,6 +147,14 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         for (int i = 0; i < NL; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, NT / 2, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    };
+    if constexpr (SETS == 1) {
+        for (int ch = 0; ch < nc; ++ch) step(ch, ch & 1, 0);
+    } else {
+        for (int ch = 0; ch < nc; ch += 2) {
+            step(ch, 0, 1);
+            if (ch + 1 < nc) step(ch + 1, 1, 0);
         }
     }
     __syncthreads();

@@ -208,38 +208,52 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
                 if (gl == 0 && j.dsel) j.dsel[row] = expm1f(-loss);
             } else if (in && gl == 0 && j.dsel) j.dsel[row] = 0.f;
         } else {
-            // teacher: softmax over its entries (those with a class and a logit above -inf)
-            float tm = -INFINITY;
+            // teacher: softmax over its entries (those with a class and a logit above -inf); lane gl holds entries gl + G q
+            constexpr int Q = 4;                          // K <= 256, and K <= G where G < 64
+            long long ix[Q];
+            float tv[Q], tm = -INFINITY, ts = 0.f;
             bool bad = false;
-            if (in)
-                for (int k = gl; k < j.K; k += G) {
-                    const long long i = j.index[e0 + k];
-                    if (i >= j.V) bad = true;
-                    if (i >= 0) { const float a = lin_tlog(j, e0 + k) * j.inv_t; bad |= !(a < INFINITY); tm = fmaxf(tm, a); }
-                }
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const int k = gl + G * q;
+                const bool there = in && k < j.K;
+                ix[q] = there ? j.index[e0 + k] : -1;
+                tv[q] = there ? lin_tlog(j, e0 + k) * j.inv_t : -INFINITY;
+                if (ix[q] >= j.V) bad = true;
+                if (ix[q] >= 0) { bad |= !(tv[q] < INFINITY); tm = fmaxf(tm, tv[q]); }
+            }
             for (int d = G >> 1; d; d >>= 1) { tm = fmaxf(tm, __shfl_xor(tm, d)); bad |= __shfl_xor((int)bad, d) != 0; }
             counts = in && (tm != -INFINITY || bad);
-            float ts = 0.f;
-            if (counts && !bad)
-                for (int k = gl; k < j.K; k += G) if (j.index[e0 + k] >= 0) ts += expf(lin_tlog(j, e0 + k) * j.inv_t - tm);
+            const float tb = tm == -INFINITY ? 0.f : tm;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) if (ix[q] >= 0) ts += expf(tv[q] - tb);
             for (int d = G >> 1; d; d >>= 1) ts += __shfl_xor(ts, d);
             const float lt = logf(ts);
             if (bad) lse = NAN;
-            for (int k = gl; in && k < j.K; k += G) {
-                const long long i = j.index[e0 + k];
+            float p[Q], all[Q];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) { p[q] = counts && ix[q] >= 0 ? expf(tv[q] - tb - lt) : 0.f; all[q] = 0.f; }
+            if (j.dsel)                                   // the same class twice in a row: each entry holds the sum over both
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    for (int l = 0; l < G && l + G * q < j.K; ++l) {
+                        const int other = __shfl((int)ix[q], (threadIdx.x & 63 & ~(G - 1)) + l);
+                        const float share = __shfl(p[q], (threadIdx.x & 63 & ~(G - 1)) + l);
+#pragma unroll
+                        for (int o = 0; o < Q; ++o) all[o] += other == (int)ix[o] ? share : 0.f;
+                    }
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const int k = gl + G * q;
+                if (!in || k >= j.K) continue;
                 float ds = 0.f, ps = 0.f;
-                if (counts && i >= 0) {
+                if (counts && ix[q] >= 0) {
                     if (bad) { loss = ds = ps = NAN; }
                     else {
-                        const float lp = lin_tlog(j, e0 + k) * j.inv_t - tm - lt, p = expf(lp);
                         const float zq = j.zsel[e0 + k] * j.inv_t - lse;
-                        if (p > 0.f) loss += p * (lp - zq);
-                        ps = p;
-                        if (j.dsel) {
-                            float all = 0.f;              // the same class twice in a row: each entry holds the sum over both
-                            for (int q = 0; q < j.K; ++q) if (j.index[e0 + q] == i) all += expf(lin_tlog(j, e0 + q) * j.inv_t - tm - lt);
-                            ds = expf(zq) - all;
-                        }
+                        if (p[q] > 0.f) loss += p[q] * (tv[q] - tb - lt - zq);
+                        ds = expf(zq) - all[q];
+                        ps = p[q];
                     }
                 }
                 if (j.dsel) j.dsel[e0 + k] = ds;
@@ -373,16 +387,16 @@ __global__ __launch_bounds__(256) void lin_reduce_kernel(const float* __restrict
 // Partial bias gradient of one chunk of LIN_DB_ROWS rows: sum over its row tiles of colsum[tile][v] - sum of g * teacher share over
 // its rows' entries that name v (psel NULL: share 1).  One workgroup owns 256 classes of one chunk; its waves walk the entries in
 // order and the lane that owns a class adds its hits: the order is fixed.
-static constexpr int LIN_DB_ROWS = 512;
-__global__ __launch_bounds__(256) void lin_dbias_kernel(const float* __restrict__ colsum, int tiles, long long ldcol, const long long* __restrict__ index,
+static constexpr int LIN_DB_ROWS = 256, LIN_DB_WAVES = 16;
+__global__ __launch_bounds__(64 * LIN_DB_WAVES) void lin_dbias_kernel(const float* __restrict__ colsum, int tiles, long long ldcol, const long long* __restrict__ index,
                                                         const float* __restrict__ psel, int K, const float2* __restrict__ stat, const float* gout,
                                                         int gstride, const int* count, float t, long long v0, int N, long long entries,
                                                         int per, long long chunk, double* out) {
-    __shared__ double part[4][256];
+    __shared__ double part[LIN_DB_WAVES][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = blockIdx.x * 256;
     const long long ea = blockIdx.y * chunk, eb = ea + chunk < entries ? ea + chunk : entries;
     double acc[4] = {0.0, 0.0, 0.0, 0.0};             // classes b0 + lane + 64 q
-    for (long long e0 = ea + wave * 256; e0 < eb; e0 += 1024) {
+    for (long long e0 = ea + wave * 256; e0 < eb; e0 += 256 * LIN_DB_WAVES) {
         int i[4];
         float val[4];
 #pragma unroll
@@ -413,8 +427,10 @@ __global__ __launch_bounds__(256) void lin_dbias_kernel(const float* __restrict_
     for (int q = 0; q < 4; ++q) part[wave][lane + 64 * q] = acc[q];
     __syncthreads();
     const int v = b0 + threadIdx.x;
-    if (v < N) {
-        double s = -(part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]);
+    if (threadIdx.x < 256 && v < N) {
+        double s = 0.0;
+#pragma unroll
+        for (int w = 0; w < LIN_DB_WAVES; ++w) s -= part[w][threadIdx.x];
         const int t1 = min(tiles, ((int)blockIdx.y + 1) * per);
         for (int i = blockIdx.y * per; i < t1; ++i) s += (double)colsum[i * ldcol + v];
         out[(long long)blockIdx.y * N + v] = s;
@@ -783,7 +799,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             FEA_LAUNCH_CHECK();
             if (db) {
                 const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (int)((n + LIN_DB_ROWS - 1) / LIN_DB_ROWS);
-                hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(256), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, LIN_DB_ROWS / tm, (long long)LIN_DB_ROWS * K, b.dbpart);
+                hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(64 * LIN_DB_WAVES), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, LIN_DB_ROWS / tm, (long long)LIN_DB_ROWS * K, b.dbpart);
                 FEA_LAUNCH_CHECK();
                 hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);
                 FEA_LAUNCH_CHECK();
