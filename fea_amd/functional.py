@@ -233,7 +233,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
     Differentiable once, in hidden, weight and bias; the backward recomputes the logits in pieces of the classes.
     An NHWC feature map and a 1x1 convolution's weight viewed [classes, channels] are taken as they are."""
-    return _linear_loss("linear_cross_entropy", hidden, weight, bias, target, None, int(ignore_index), 1.0, reduction)
+    ignore_index = int(ignore_index)
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"linear_cross_entropy: ignore_index {ignore_index} is no 64-bit integer")
+    return _linear_loss("linear_cross_entropy", hidden, weight, bias, target, None, ignore_index, 1.0, reduction)
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,

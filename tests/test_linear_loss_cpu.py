@@ -13,7 +13,7 @@ A, I = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
 @pytest.mark.parametrize("bad", [
     {"reduction": "avg"}, {"hidden": H.half(), "weight": W.half()}, {"hidden": H.bfloat16()}, {"weight": W[:, :7]}, {"weight": W[0]},
     {"weight": W[:0]}, {"hidden": H[:, :0], "weight": W[:, :0]}, {"target": T.float()}, {"target": T.bool()}, {"target": T[:3]},
-    {"target": T[:, None]}, {"bias": torch.zeros(4)}, {"bias": torch.zeros(5, dtype=torch.float64)}, {"hidden": None}, {"target": None}])
+    {"target": T[:, None]}, {"bias": torch.zeros(4)}, {"bias": torch.zeros(5, dtype=torch.float64)}, {"hidden": None}, {"target": None}, {"ignore_index": 1 << 63}])
 def test_cross_entropy_refuses(bad):
     kw = {"hidden": H, "weight": W, "target": T} | bad
     with pytest.raises(ValueError, match="linear_cross_entropy"):

@@ -11,7 +11,7 @@ DEV = "cuda"
 TYPES = [torch.float32, torch.bfloat16]
 SHAPES = [(1, 8, 1), (1, 1, 2), (1, 64, 600), (2, 5, 7), (3, 64, 6), (17, 33, 129), (64, 128, 128), (129, 72, 1000), (5000, 72, 40), (257, 200, 333),
           (300, 96, 5003), (513, 640, 1537), (5000, 64, 6), (4097, 24, 33), (4096, 64, 32), (4100, 33, 13), (6001, 16, 2), (4111, 40, 24), (5003, 7, 1), (33, 515, 1000),
-          (48, 1024, 777), (16, 300, 2049)]
+          (48, 1024, 777), (16, 300, 2049), (150, 99, 700), (700, 51, 5000)]
 
 
 def _leaf(t):
@@ -47,6 +47,14 @@ def test_cross_entropy(shape, dtype):
 def test_distillation(shape, dtype, top):
     h, w, b, i, a = O.case(*shape, dtype, seed=sum(shape) + top, top=top, ignored=0.2, short=0.3, bias=shape[0] % 2 == 1)
     _compare(_run(h, w, b, i, a, temperature=2.0), O.evaluate(h, w, b, i, a, temperature=2.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(9, 40, 300), (40, 64, 300), (100, 64, 300), (4200, 16, 30)])
+def test_most_entries(shape, dtype):
+    """256 teacher entries per row, most classes named more than once."""
+    c = O.case(*shape, dtype, seed=31, top=256, ignored=0.1, short=0.2, bias=True)
+    _compare(_run(*c, temperature=3.0), O.evaluate(*c, temperature=3.0))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -181,6 +189,60 @@ def test_layouts(dtype):
     assert bool(((g - ref["hidden"][0].sum(0)).abs() <= tol).all())
     bare = F.linear_cross_entropy(h[0].to(DEV), w.to(DEV), t[0].to(DEV))
     assert bare.shape == () and torch.equal(bare, F.linear_cross_entropy(h[:1].to(DEV), w.to(DEV), t[:1].to(DEV)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_something_very_wide(dtype):
+    """Rows further apart than a buffer load's 32-bit offsets reach over a tile."""
+    h, w, b, t = O.case(70, 64, 300, dtype, seed=8, ignored=0.1, bias=True)
+    want = O.evaluate(h, w, b, t)
+    for n in range(2):
+        rows = [h, w]
+        wide = torch.zeros(rows[n].shape[0], (1 << 21) + 8, dtype=dtype, device=DEV)
+        wide[:, 8:72] = rows[n].to(DEV)
+        rows = [x.to(DEV) for x in rows]
+        rows[n] = wide[:, 8:72]
+        rows = [x.detach().requires_grad_(True) for x in rows]
+        loss = F.linear_cross_entropy(rows[0], rows[1], t.to(DEV), bias=b.to(DEV))
+        _compare(dict(zip(("loss", "hidden", "weight"), [loss, *torch.autograd.grad(loss, rows)])), want)
+
+
+def test_far_rows():
+    """More than 2^31 elements of hidden states: 8,300 copies of a batch, whose rows do not depend on each other."""
+    h, w, b, t = O.case(4096, 64, 6, torch.bfloat16, seed=40, ignored=0.1, bias=True)
+    base = _run(h, w, b, t, reduction="sum")
+    n = 8300
+    assert n * h.numel() > 1 << 31
+    far = _run(h.to(DEV).repeat(n, 1), w, b, t.to(DEV).repeat(n), reduction="sum")
+    assert torch.equal(far["hidden"].view(n, 4096, 64)[-1], base["hidden"]) and torch.equal(far["hidden"].view(n, 4096, 64)[n // 2], base["hidden"])
+    # sums of n equal parts: in 32 bits per workgroup, in 64 across, rounded once
+    for k, u in (("loss", 1e-5), ("weight", 2.0 ** -8 + 1e-5), ("bias", 1e-5)):
+        want = O.evaluate(h, w, b, t, reduction="sum")[k]
+        O.check(k, far[k] / n, (want[0], want[1] + u * want[0].abs() + 1e-5 * want[0].abs().max()))
+
+
+def test_far_classes():
+    """More than 2^31 elements of weight: 100 copies of 5,300 classes, labels among the last copy.  Each copy has a hundredth of the softmax."""
+    h, w, _, t = O.case(70, 4096, 5300, torch.bfloat16, seed=41)
+    n = 100
+    assert n * w.numel() > 1 << 31
+    base = O.evaluate(h, w, None, t, reduction="none")
+    x, y = _leaf(h), w.to(DEV).repeat(n, 1).requires_grad_(True)
+    loss = F.linear_cross_entropy(x, y, (t + (n - 1) * 5300).to(DEV), reduction="none")
+    gh, gw = torch.autograd.grad(loss.sum(), [x, y])
+    import math
+    O.check("loss", loss, (base["loss"][0] + math.log(n), base["loss"][1] + 4e-6))
+    # the copies' weights are equal, so dh is the base's; its sum runs over n times as many terms
+    O.check("hidden", gh, (base["hidden"][0], base["hidden"][1] * 1.5 + n * 5300 * O.E * base["hidden"][0].abs().mean()))
+    q = torch.softmax(h.double() @ w.double().T, 1)
+    free = q.T @ h.double() / n
+    bound = (q.T @ h.double().abs()) / n * 2.0 ** -6 + free.abs() * 2.0 ** -8
+    for k in (0, n // 2, n - 2):
+        O.check(f"copy {k}", gw[k * 5300:(k + 1) * 5300], (free, bound))
+    last = free.clone()
+    last.index_add_(0, t, -h.double())
+    hot = torch.zeros_like(bound).index_add_(0, t, h.double().abs())
+    O.check("the labels' copy", gw[(n - 1) * 5300:], (last, bound + 2.0 ** -6 * hot))
 
 
 def test_only_the_gradients_that_are_wanted():
