@@ -1,34 +1,33 @@
-// Tiled product of the many-class loss heads with its three epilogues: log-sum-exp partials, softmax gradient, store.
+// The fp32 products of the many-class loss heads on the exact fp32 matrix rate, any alignment, and the choice of a product's kernel.
 //
 //   z[m][n] = (sum_k a[m][k] b[n][k] + bias[n]) / T
 //   LIN_LSE:   per row and column tile (max, sum exp(z - max)); no z leaves the registers
-//   LIN_DZ:    q = exp(z - lse_m), rounded once to the storage type (it is the operand of the next two products on the
-//              matrix pipe; the sums there are fp32), stored row-major and transposed so that both products find their
-//              reduction axis contiguous.  The upstream gradient is not in it: a common factor rounds the labels' entries, all
-//              close to it, the same way in every row (bf16, 2,048 rows: 3.2e-3 off in dw and dh instead of 2.3e-3)
+//   LIN_DZ:    q = exp(z - lse_m), stored row-major; the label's entries are corrected behind it.  The upstream gradient is not in it: in the
+//              bf16 form a common factor would round the labels' entries, all close to it, the same way in every row (2,048 rows:
+//              3.2e-3 off in dw and dh instead of 1.8e-3)
 //   LIN_STORE: out = scale * (a . b), or fp32 slabs of a split reduction (joined by the caller in split order: no atomics)
 //
-// 128 x 128 tile, 4 waves of 64 x 64 (2 x 2 accumulators of 32 x 32), reduction in 128-byte steps of every row (64 bf16 / 32 fp32),
-// two LDS stages filled through registers, two steps ahead, so that rows, columns and reduction of any length are cut by a guard on the load.
-// The operands of the MFMA are swapped (classes as its rows), so a lane holds one label row and 32 of its classes: the softmax
-// sums are in-lane sums and one exchange between wave halves.
+// 128 x 128 tile, 4 waves of 64 x 64 (2 x 2 accumulators of 32 x 32), reduction in steps of 32 channels, two LDS stages filled through
+// registers, two steps ahead, so that rows, columns and reduction of any length are cut by a guard on the load.  The operands
+// of the MFMA are swapped (classes as its rows), so a lane holds one label row and 32 of its classes: the softmax sums are
+// in-lane sums and one exchange between wave halves.  An operand with its rows along the reduction keeps them in LDS, and a
+// fragment is four reads down a column.
+// Bound by the fp32 matrix rate: 1,531 x 643 x 10,007 takes 204 us (96 TFLOP/s), as planes (linear_gemm256.hip) 107 us; this kernel
+// serves what the planes' copies do not pay for.
 #include "linear_loss.h"
 
-static constexpr int LG_T = 128, LG_STAGE = 2 * LG_T * 128;
+static constexpr int LG_T = 128, LG_STAGE = 2 * LG_T * 128, LG_CK = 32;
 
-template <typename T> __device__ __forceinline__ void lg_store4(T* p, const float (&v)[4], int n) {
-    if (n >= 4 && (((uintptr_t)p) & (4 * sizeof(T) - 1)) == 0) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        else { const bf16x4 x = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}; *reinterpret_cast<bf16x4*>(p) = x; }
-    } else {
+__device__ __forceinline__ void lg_store4(float* p, const float (&v)[4], int n) {
+    if (n >= 4 && ((uintptr_t)p & 15) == 0) *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    else
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < n) p[i] = from_f32<T>(v[i]);
-    }
+        for (int i = 0; i < 4; ++i) if (i < n) p[i] = v[i];
 }
 
-template <typename T, int EPI, bool ALN, bool PL>
+template <int EPI, bool ALN, bool TA>
 __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
-    constexpr int EPC = Elem<T>::EPC, CK = Elem<T>::CK;
+    constexpr bool TB = EPI == LIN_STORE;
     __shared__ __attribute__((aligned(128))) char smem[2 * LG_STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave & 1, wn = wave >> 1, l32 = lane & 31, hf = lane >> 5;
@@ -38,34 +37,31 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     const int m0 = tm * LG_T, n0 = tn * LG_T;
     const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, k1 = EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K;
 
-    // staging: thread -> rows r + 32 i, 16-byte chunk c of the 128-byte row, XOR-swizzled by the row
-    const int r = tid >> 3, c = tid & 7;
-    const T* const ap = (const T*)g.a;
-    const T* const bp = (const T*)g.b;
+    // staging.  Rows along the tile: thread -> rows r + 32 i, 16-byte chunk c of 128 bytes, XOR-swizzled by the row.  Rows along the reduction:
+    // thread -> rows tr + 8 i of 32, 4 columns from 4 tc, columns XORed so that the two halves of a wave read different banks.
+    const int r = tid >> 3, c = tid & 7, tr = tid >> 5, tc = tid & 31;
+    const float *const ap = (const float*)g.a, *const bp = (const float*)g.b;
     u32x4 ra[2][4], rb[2][4];          // two steps on the way: the first is needed a whole step after it was asked for
-    int pair = PL ? k0 / g.Kp : 0, pk = PL ? k0 - pair * g.Kp : 0;
+    auto fetch1 = [&](const float* p, long long ld, int x0, int X, int k, int i, bool t) {
+        if (t) return k + tr + 8 * i < k1 ? lin_load16<float, ALN>(p + (k + tr + 8 * i) * ld + x0 + 4 * tc, X - x0 - 4 * tc) : u32x4{0, 0, 0, 0};
+        return x0 + r + 32 * i < X ? lin_load16<float, ALN>(p + (x0 + r + 32 * i) * ld + k + 4 * c, k1 - k - 4 * c) : u32x4{0, 0, 0, 0};
+    };
     auto fetch = [&](int u, int k) {
-        const int left = k1 - k - c * EPC;
-        int ka = k + c * EPC, kb = ka;
-        if constexpr (PL) {
-            ka = lin_plane_a(pair) * g.Kp + pk + c * EPC; kb = lin_plane_b(pair) * g.Kp + pk + c * EPC;
-            pk += CK;
-            if (pk >= g.Kp) { pk = 0; ++pair; }
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int m = m0 + r + 32 * i, n = n0 + r + 32 * i;
-            ra[u][i] = m < g.M ? lin_load16<T, ALN>(ap + m * g.lda + ka, left) : u32x4{0, 0, 0, 0};
-            rb[u][i] = n < g.N ? lin_load16<T, ALN>(bp + n * g.ldb + kb, left) : u32x4{0, 0, 0, 0};
+            ra[u][i] = fetch1(ap, g.lda, m0, g.M, k, i, TA);
+            rb[u][i] = fetch1(bp, g.ldb, n0, g.N, k, i, TB);
         }
     };
-    auto put = [&](int st) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int off = (r + 32 * i) * 128 + ((c ^ (r & 7)) << 4);
-            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + off) = ra[st][i];
-            *reinterpret_cast<u32x4*>(smem + st * LG_STAGE + LG_T * 128 + off) = rb[st][i];
-        }
+    auto put1 = [&](char* op, const u32x4& v, int i, bool t) {
+        const int row = t ? tr + 8 * i : r + 32 * i;
+        *reinterpret_cast<u32x4*>(op + (t ? row * 512 + ((tc ^ (((row >> 2) & 1) << 3)) << 4) : row * 128 + ((c ^ (row & 7)) << 4))) = v;
+    };
+    // fragment of 32 rows from x: lane l32 -> row, channels 8 s + 4 hf .. + 3
+    auto frag = [&](const char* op, int x, int s, bool t) {
+        if (!t) return *reinterpret_cast<const u32x4*>(op + (x + l32) * 128 + (((2 * s + hf) ^ (l32 & 7)) << 4));
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(op) + (8 * s + 4 * hf) * 128 + ((x + l32) ^ (hf << 5));
+        return u32x4{p[0], p[128], p[256], p[384]};
     };
     f32x16 acc[2][2];                 // [label tile][class tile]
 #pragma unroll
@@ -76,25 +72,26 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
     if (k0 < k1) fetch(0, k0);
-    if (k0 + CK < k1) fetch(1, k0 + CK);
+    if (k0 + LG_CK < k1) fetch(1, k0 + LG_CK);
+    const int live = g.M - m0 - __builtin_amdgcn_readfirstlane(wm) * 64;        // of few rows only the half or quarter that holds them is computed
     auto step = [&](int st, int k) {   // stage and register set of the same parity
-        put(st);
+        char* const sa = smem + st * LG_STAGE;
+        char* const sb = sa + LG_T * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { put1(sa, ra[st][i], i, TA); put1(sb, rb[st][i], i, TB); }
         __syncthreads();              // one barrier per step: the other stage was last read in front of the previous one
-        if (k + 2 * CK < k1) fetch(st, k + 2 * CK);
-        const char* sa = smem + st * LG_STAGE + (wm * 64 + l32) * 128;
-        const char* sb = smem + st * LG_STAGE + LG_T * 128 + (wn * 64 + l32) * 128;
+        if (k + 2 * LG_CK < k1) fetch(st, k + 2 * LG_CK);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const int off = ((2 * s + hf) ^ (l32 & 7)) << 4;
-            const u32x4 a0 = *reinterpret_cast<const u32x4*>(sa + off), a1 = *reinterpret_cast<const u32x4*>(sa + 32 * 128 + off);
-            const u32x4 b0 = *reinterpret_cast<const u32x4*>(sb + off), b1 = *reinterpret_cast<const u32x4*>(sb + 32 * 128 + off);
-            mma16(acc[0][0], b0, a0, (const T*)nullptr); mma16(acc[0][1], b1, a0, (const T*)nullptr);
-            mma16(acc[1][0], b0, a1, (const T*)nullptr); mma16(acc[1][1], b1, a1, (const T*)nullptr);
+            const u32x4 a0 = frag(sa, wm * 64, s, TA), a1 = frag(sa, wm * 64 + 32, s, TA);
+            const u32x4 b0 = frag(sb, wn * 64, s, TB), b1 = frag(sb, wn * 64 + 32, s, TB);
+            if (live > 0)  { mma16(acc[0][0], b0, a0, (const float*)nullptr); mma16(acc[0][1], b1, a0, (const float*)nullptr); }
+            if (live > 32) { mma16(acc[1][0], b0, a1, (const float*)nullptr); mma16(acc[1][1], b1, a1, (const float*)nullptr); }
         }
     };
-    for (int k = k0; k < k1; k += 2 * CK) {
+    for (int k = k0; k < k1; k += 2 * LG_CK) {
         step(0, k);
-        if (k + CK < k1) step(1, k + CK);
+        if (k + LG_CK < k1) step(1, k + LG_CK);
     }
     __syncthreads();
 
@@ -109,6 +106,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             if (m >= g.M) continue;
             const float sc = g.scale == 1 ? lin_row_scale(g.gout, g.gstride, g.count, g.t, g.stat[m].y, m)
                            : g.scale == 2 ? lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0) : 1.f;
+            float* const o = g.slab ? g.slab + ((long long)sp * g.M + m) * g.ldo : (float*)g.out + m * g.ldo;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -116,8 +114,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
                     const int n = ncol(j, e);
                     if (n >= g.N) continue;
                     const float v[4] = {acc[i][j][e] * sc, acc[i][j][e + 1] * sc, acc[i][j][e + 2] * sc, acc[i][j][e + 3] * sc};
-                    if (g.slab) lg_store4(g.slab + ((long long)sp * g.M + m) * g.ldo + n, v, (int)g.ldo - n);
-                    else        lg_store4((T*)g.out + m * g.ldo + n, v, g.N - n);
+                    lg_store4(o + n, v, (g.slab ? (int)g.ldo : g.N) - n);
                 }
         }
         return;
@@ -193,35 +190,28 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             if (tid < LG_T && n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LG_T + tid];
         }
 #pragma unroll
-        for (int pl = 0; pl < (PL ? 3 : 1); ++pl) {
-            T* const dz = (T*)g.dz + (PL ? (long long)pl * g.Npad : 0);
-            T* const dzt = (T*)g.dzt + (PL ? (long long)pl * g.Mpad : 0);
+        for (int i = 0; i < 2; ++i) {
+            const int m = mrow(i);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int m = mrow(i);
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const int n = ncol(j, e);
-                        const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                        if (m < g.M && n < g.Npad) lg_store4(dz + m * g.lddz + n, v, g.Npad - n);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            if (g.dzt && m < g.Mpad && n + x < g.N) dzt[(n + x) * g.lddzt + m] = from_f32<T>(v[x]);
-                            if constexpr (PL) acc[i][j][e + x] -= to_f32(from_f32<T>(v[x]));
-                        }
-                    }
-            }
+                for (int e = 0; e < 16; e += 4) {
+                    const int n = ncol(j, e);
+                    const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                    if (m < g.M && n < g.Npad) lg_store4((float*)g.dz + m * g.lddz + n, v, g.Npad - n);
+                }
         }
     }
 }
 
 // Tile and split of a product: the one whose modelled time is least, from the rates that the kernels reach on full chips (fp32 100, bf16 700
-// and 1,300 TFLOP/s).  Both take whole rounds of the chip (256 workgroups of the large tile, 512 of the small one); the parts of a split
-// reduction are written and read once more, at least 512 (bf16) or 256 (fp32) channels each.  dtype FEA_PL: K is six times the planes'.
+// and 1,300 TFLOP/s) and from the bytes of operands and result at 4 TB/s.  Both take whole rounds of the chip (256 workgroups of the large
+// tile, 512 of the small one); the parts of a split reduction are written and read once more, at least 512 (bf16) or 256 (fp32)
+// channels each.  dtype FEA_PL: K is six times the planes'.
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split) {
     LinTile best{128, 1, 1e30};
+    const double size = dtype == FEA_F32 ? 4 : dtype == FEA_BF16 ? 2 : 1;      // bytes per element of K: a plane pair's share is 6 of 6 K
+    const double bytes = ((double)M * K + (double)N * K) * size + (split ? (double)M * N * (dtype == FEA_BF16 ? 2 : 4) : 0.0);
     for (int tile = 128; tile <= (dtype == FEA_F32 ? 128 : 256); tile += 128) {
         const double slots = tile == 256 ? 256 : 512;
         const double rate = dtype == FEA_F32 ? 100e12 : tile == 256 ? 1300e12 : 700e12;
@@ -229,38 +219,43 @@ LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool spli
         for (int sp = 1; sp <= (split ? 32 : 1); ++sp) {
             if (sp > 1 && K / sp < (dtype == FEA_F32 ? 256 : 512)) break;
             const double rounds = (double)((tiles * sp + (long long)slots - 1) / (long long)slots);
-            const double t = rounds * (2.0 * tile * tile * ((double)K / sp + 128) / (rate / slots)) + (sp > 1 ? 2.0 * sp * M * N * 4 / 4e12 + 3e-6 : 0.0);
+            double t = rounds * (2.0 * tile * tile * ((double)K / sp + 128) / (rate / slots));
+            if (t < bytes / 4e12) t = bytes / 4e12;
+            t += sp > 1 ? 2.0 * sp * M * N * 4 / 4e12 + 3e-6 : 0.0;
             if (t < best.time * 0.999) best = LinTile{tile, sp, t};
         }
     }
     return best;
 }
 
-template <typename T> static void lin_launch(int epi, bool aln, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (epi == LIN_LSE) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, true, false>), dim3(grid), dim3(256), 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_LSE, false, false>), dim3(grid), dim3(256), 0, s, g);
-    } else if (epi == LIN_DZ) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, true, false>), dim3(grid), dim3(256), 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_DZ, false, false>), dim3(grid), dim3(256), 0, s, g);
-    } else       hipLaunchKernelGGL((lin_gemm_kernel<T, LIN_STORE, true, false>), dim3(grid), dim3(256), 0, s, g);
-}
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     const int epc = dtype == FEA_F32 ? 4 : 8;
-    const bool aln = g.K % epc == 0 && g.lda % epc == 0 && g.ldb % epc == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0;
-    const long long row = dtype == FEA_PL ? 3ll * g.Kp : g.K;
-    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.lda >= row && g.ldb >= row && (aln || (tile == 128 && epi != LIN_STORE && dtype != FEA_PL)), FEA_E_BADARG,
-              "lin_gemm: operands of %d x %d x %d, tile %d", g.M, g.N, g.K, tile);
-    FEA_CHECK(dtype != FEA_PL || (g.Kp > 0 && g.Kp % 64 == 0 && g.K == 6 * g.Kp && (epi != LIN_STORE || g.slab)), FEA_E_BADARG, "lin_gemm: planes of %d, K %d", g.Kp, g.K);
-    const bool fast = dtype != FEA_F32 && aln && g.lda < (1 << 21) && g.ldb < (1 << 21);
-    FEA_CHECK(fast || (tile == 128 && dtype != FEA_PL), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
+    const bool aln = g.lda % epc == 0 && g.ldb % epc == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 && (epi == LIN_STORE ? g.N % epc == 0 || dtype != FEA_F32 : g.K % epc == 0);
+    const long long k = dtype == FEA_PL ? 3ll * g.Kp : g.K;
+    FEA_CHECK(g.M > 0 && g.N > 0 && g.K > 0 && g.lda >= (epi == LIN_STORE && g.ta ? g.M : k) && g.ldb >= (epi == LIN_STORE ? g.N : k), FEA_E_BADARG,
+              "lin_gemm: operands of %d x %d x %d", g.M, g.N, g.K);
+    FEA_CHECK(dtype == FEA_F32 ? tile == 128 : aln && g.lda < (1 << 21) && g.ldb < (1 << 21), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
+    FEA_CHECK(dtype != FEA_PL || (g.Kp > 0 && g.Kp % 64 == 0 && g.K == 6 * g.Kp && g.Kr <= g.Kp && (epi != LIN_STORE || g.slab)), FEA_E_BADARG, "lin_gemm: planes of %d, K %d", g.Kp, g.K);
+    FEA_CHECK(epi != LIN_STORE || dtype == FEA_F32 || (g.Kr > 0 && g.Kr <= (dtype == FEA_PL ? g.Kp : g.K)), FEA_E_BADARG, "lin_gemm: reduction of %d of %d", g.Kr, g.K);
     g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
     const long long grid = (long long)g.ntm * g.ntn * g.splits;
     FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
-    if (fast)                   fea_lin_gemm256(epi, tile, dtype == FEA_PL, g, (unsigned)grid, s);
-    else if (dtype == FEA_BF16) lin_launch<__bf16>(epi, aln, g, (unsigned)grid, s);
-    else                        lin_launch<float>(epi, aln, g, (unsigned)grid, s);
+    const dim3 gr((unsigned)grid), bl(256);
+    if (dtype != FEA_F32) fea_lin_gemm256(epi, tile, dtype == FEA_PL, g, (unsigned)grid, s);
+    else if (epi == LIN_LSE) {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_LSE, true, false>), gr, bl, 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_LSE, false, false>), gr, bl, 0, s, g);
+    } else if (epi == LIN_DZ) {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_DZ, true, false>), gr, bl, 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_DZ, false, false>), gr, bl, 0, s, g);
+    } else if (g.ta) {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, true, true>), gr, bl, 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, false, true>), gr, bl, 0, s, g);
+    } else {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, true, false>), gr, bl, 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, false, false>), gr, bl, 0, s, g);
+    }
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }

@@ -12,9 +12,6 @@
 // every bound in the lane's offset, so rows, classes and channels behind the end arrive as zeros without a branch.
 #include "linear_loss.h"
 
-#ifndef LB_ROT
-#define LB_ROT 1
-#endif
 
 
 // XOR of a 128-byte row's 16-byte chunk index: conflict-free ds_read_b128 of 16 rows x 4 chunks
@@ -26,10 +23,15 @@ __device__ __forceinline__ uint32_t lb_pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, b2));
 }
 
-// NT: 16-row tiles of a wave in either direction (8: 256 x 256 per workgroup, one per CU; 4: 128 x 128, two per CU)
-template <int EPI, bool PL, int NT>
+// NT: 16-row tiles of a wave in either direction (8: 256 x 256 per workgroup, one per CU; 4: 128 x 128, two per CU).
+// TA, TB: the operand lies with its rows along the reduction ([k][m] / [k][n]: dz for dw, hidden and weight for dw and dh): its LDS tile is
+// 64 rows of the tile's width, and fragments come out of it by the transposing read (ds_read_b64_tr_b16), two for 8 channels.
+// No transposed copy of either weight, hidden or dz is ever made.
+template <int EPI, bool PL, int NT, bool TA, bool TB>
 __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const LinGemm g) {
-    constexpr int LB_T = 32 * NT, LB_W = 16 * NT, LB_OP = LB_T * 128, LB_STAGE = 2 * LB_OP, NL = 2 * NT;
+    constexpr int LB_T = 32 * NT, LB_W = 16 * NT, NL = 2 * NT;
+    constexpr int RB = 2 * LB_T + 32, TOP = 64 * RB + 8 * 128;                       // a row along the reduction, an operand of them
+    constexpr int LB_OP = TA ? TOP : LB_T * 128, LB_STAGE = LB_OP + (TB ? TOP : LB_T * 128);
     __shared__ __attribute__((aligned(128))) char smem[2 * LB_STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave & 1, wn = wave >> 1, r16 = lane & 15, q16 = lane >> 4;
@@ -43,32 +45,45 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, K = max((EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K) - k0, 0);
     const int nc = (K + 63) >> 6;
 
-    const int kb = PL ? 0 : k0, kl = PL ? 3 * g.Kp : K;      // first channel and length of a row, as the buffers see it
-    const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.a + m0 * g.lda + kb), 0,
-        K ? (int)(((min(LB_T, g.M - m0) - 1) * g.lda + kl) * 2) : 0, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc((void*)((const __bf16*)g.b + n0 * g.ldb + kb), 0,
-        K ? (int)(((min(LB_T, g.N - n0) - 1) * g.ldb + kl) * 2) : 0, 0x00020000);
+    auto rsrc = [&](const __bf16* p, long long ld, int rows, int cols) {       // rows x cols of a matrix; 0 rows: nothing is read
+        return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, rows > 0 ? (int)(((rows - 1) * ld + cols) * 2) : 0, 0x00020000);
+    };
+    const int kb = PL ? 0 : k0, kl = PL ? 3 * g.Kp : K;      // first channel and length of a row along the reduction
+    const __bf16 *const a = (const __bf16*)g.a, *const b = (const __bf16*)g.b;
+    __amdgpu_buffer_rsrc_t rsa = rsrc(a + m0 * g.lda + kb, g.lda, K ? min(LB_T, g.M - m0) : 0, kl);
+    __amdgpu_buffer_rsrc_t rsb = rsrc(b + n0 * g.ldb + kb, g.ldb, K ? min(LB_T, g.N - n0) : 0, kl);
 
-    // staging: thread -> LDS rows r + 32 i of either operand, 16-byte chunk c.  What lies in an LDS row is chosen for the epilogue: the
-    // lane that ends up with column r16 of the products holds NT consecutive labels (over its tiles i), and with tiles 2 p, 2 p + 1 of
-    // the classes 8 consecutive ones: 16-byte stores of either order of dz without an exchange between lanes.
+    // Staging, rows along the tile: thread -> LDS rows r + 32 i, 16-byte chunk c.  Which class lies in which LDS row is chosen for the
+    // epilogue: the lane that ends up with column r16 of the products holds, over tiles 2 p and 2 p + 1, 8 consecutive classes.
     const int r = tid >> 3, c = tid & 7;
-    const int ra = (r & 15) * NT + (r >> 4), rb = ((r >> 4) & 1) * 4 + ((r >> 2) & 3) * 8 + (r & 3);
-    const unsigned va = (unsigned)(ra * (int)g.lda * 2 + c * 16), vb = (unsigned)(rb * (int)g.ldb * 2 + c * 16);
-    const unsigned ua = 2 * (unsigned)g.lda, sb = 64 * (unsigned)g.ldb;      // bytes of a label's row, of 32 classes' rows
+    const int rb = ((r >> 4) & 1) * 4 + ((r >> 2) & 3) * 8 + (r & 3);
     const int wofs = r * 128 + ((c ^ lb_swz(r)) << 4);
+    // Rows along the reduction: thread -> rows tr + RPP i of the chunk's 64, 16-byte piece tc.  A row is 32 bytes longer than its data and every
+    // 8 rows have 128 more: the 8 rows x 32 bytes that half a wave takes in one transposing read lie in different banks, and
+    // tiles, steps and loads are constant offsets.
+    constexpr int CPR = LB_T / 8, RPP = 256 / CPR;
+    const int tr = tid / CPR, tc = tid % CPR;
+    const int tofs = tr * RB + (tr >> 3) * 128 + tc * 16;
+    const unsigned va = TA ? (unsigned)(tr * (int)g.lda * 2 + tc * 16) : (unsigned)(r * (int)g.lda * 2 + c * 16);
+    const unsigned vb = TB ? (unsigned)(tr * (int)g.ldb * 2 + tc * 16) : (unsigned)(rb * (int)g.ldb * 2 + c * 16);
+    const unsigned sa = 2 * (TA ? RPP : 32) * (unsigned)g.lda, sb = 2 * (TB ? RPP : 32) * (unsigned)g.ldb;      // bytes from load i to i + 1
     constexpr int SETS = NT == 8 ? 1 : 2;      // chunks on the way in registers (two where there is room: a chunk is then shorter than a load)
     u32x4 st[SETS][NL];
     // the XCDs start their reduction an eighth apart (it ends where it began): in step, every workgroup of the chip would ask for the
     // same columns of its rows at a time.  Within an XCD all are in step: they share operands in its L2.
-    int at = LB_ROT ? (int)(blockIdx.x & 7) * nc >> 3 : 0;
+    int at = (int)(blockIdx.x & 7) * nc >> 3;
     int pair = PL ? (k0 + at * 64) / g.Kp : 0, pk = PL ? k0 + at * 64 - pair * g.Kp : 0;       // FEA_PL: the pair of planes and the channel that are loaded next
     unsigned ka = 0, kc = 0;
     bool kin = false;
-    auto advance = [&](int ch) {      // byte offsets of the chunk that is loaded ch-th in a row of either operand
-        kin = ch < nc && at * 64 + c * 8 < K;
-        if constexpr (PL) { ka = 2u * (unsigned)(lin_plane_a(pair) * g.Kp + pk); kc = 2u * (unsigned)(lin_plane_b(pair) * g.Kp + pk); }
-        else ka = kc = at * 128;
+    const int ca = min(LB_T, (g.M - m0 + 7) & ~7), cb = min(LB_T, (g.N - n0 + 7) & ~7);        // (whole 16-byte pieces: rows are padded)
+    auto advance = [&](int ch) {      // where the chunk that is loaded ch-th lies in either operand
+        const bool live = ch < nc;
+        kin = live && at * 64 + c * 8 < K;
+        const int first = PL ? pk : k0 + at * 64, rows = live ? min(64, g.Kr - first) : 0;
+        if constexpr (TA) rsa = rsrc(a + first * g.lda + m0 + (PL ? lin_plane_a(pair) * g.Pa : 0), g.lda, rows, ca);
+        else ka = PL ? 2u * (unsigned)(lin_plane_a(pair) * g.Kp + pk) : at * 128;
+        if constexpr (TB) rsb = rsrc(b + first * g.ldb + n0 + (PL ? lin_plane_b(pair) * g.Pb : 0), g.ldb, rows, cb);
+        else kc = PL ? 2u * (unsigned)(lin_plane_b(pair) * g.Kp + pk) : at * 128;
         if (++at == nc) {
             at = 0;
             if constexpr (PL) { pair = k0 / g.Kp; pk = k0 - pair * g.Kp; }
@@ -78,30 +93,39 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         }
     };
     auto gload = [&](int u, int i) {
-        if (i < NT) st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, kin ? va + ka + (i / (NT / 2) * LB_W + 2 * (i % (NT / 2))) * ua : 0x7fffff00u, 0, 0));
-        else        st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, kin ? vb + kc + (i - NT) * sb : 0x7fffff00u, 0, 0));
+        if (i < NT) st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, TA || kin ? va + ka + i * sa : 0x7fffff00u, 0, 0));
+        else        st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, TB || kin ? vb + kc + (i - NT) * sb : 0x7fffff00u, 0, 0));
     };
-    auto lput = [&](int u, int stage, int i) { *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i / NT) * LB_OP + wofs + (i % NT) * 32 * 128) = st[u][i]; };
+    auto lput = [&](int u, int stage, int i) {
+        const int ofs = (i < NT ? TA : TB) ? tofs + (i % NT) * (RPP * RB + RPP / 8 * 128) : wofs + (i % NT) * 32 * 128;
+        *reinterpret_cast<u32x4*>(smem + stage * LB_STAGE + (i / NT) * LB_OP + ofs) = st[u][i];
+    };
 
+    // fragments: lane -> row r16 of tile i, channels 8 q16 .. + 7 of the 32 of step ks
     const int fofs0 = r16 * 128 + ((q16 ^ lb_swz(r16)) << 4), fofs1 = fofs0 ^ 64;
-    const int fa = wm * LB_W * 128, fb = LB_OP + wn * LB_W * 128;
+    const int fofst = (8 * q16 + (r16 >> 2)) * RB + q16 * 128 + (r16 & 3) * 8;       // 16 lanes: 4 rows of 16 columns
     u32x4 A[2][NT], B[2][NT];
+    auto frag = [&](const char* op, int w, int ks, int i, bool t) {
+        if (!t) return *reinterpret_cast<const u32x4*>(op + (ks ? fofs1 : fofs0) + (w * LB_W + i * 16) * 128);
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
+        const char* p = op + fofst + w * (2 * LB_W) + i * 32 + ks * (32 * RB + 4 * 128);
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p + 4 * RB)));
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
     auto frd = [&](int stage, int ks, int i) {
-        const char* p = smem + stage * LB_STAGE + (ks ? fofs1 : fofs0) + (i % NT) * 16 * 128;
-        if (i < NT) A[ks][i] = *reinterpret_cast<const u32x4*>(p + fa);
-        else        B[ks][i - NT] = *reinterpret_cast<const u32x4*>(p + fb);
+        if (i < NT) A[ks][i] = frag(smem + stage * LB_STAGE, wm, ks, i, TA);
+        else        B[ks][i - NT] = frag(smem + stage * LB_STAGE + LB_OP, wn, ks, i - NT, TB);
     };
     f32x4 acc[NT][NT];                // [label tile][class tile]
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto mma = [&](int ks) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
+    auto mma = [&](int ks, int i, int j) {
+        // (as inline asm where fragments come in halves: there the compiler moves accumulators between the register files in every step)
+        if constexpr (NT == 8 && (TA || TB)) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(B[ks][j]), "v"(A[ks][i]));
+        else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
     };
 
     advance(0);
@@ -113,44 +137,86 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     for (int u = 0; u < SETS; ++u) {
         advance(1 + u);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) gload((1 + u) % SETS, i);
+        for (int i = 0; i < NL; ++i) {        // (in the loop's order: its waits are counted for both ways in)
+            gload((1 + u) % SETS, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NL; ++i) frd(0, 0, i);
+    for (int i = 0; i < NL; ++i) {
+        const int f = i < NT ? i + NT : i - NT;
+        if (!(TA || TB) || f < 3 || f >= NT) frd(0, 0, f);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 
     // chunk ch of LDS stage s; chunk ch + 1 lies in register set u, where chunk ch + 1 + SETS follows it
     auto step = [&](int ch, int s, int u) {
+        auto landed = [&]() {         // chunk ch + 1 is in LDS and nobody reads this stage or the other one's old chunk any more
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
         advance(ch + 1 + SETS);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (TA || TB) {
+            // slots: half a row of MFMAs, then a fragment of the second half (in every second slot one of this half, three tiles ahead), an
+            // LDS write and a load
 #pragma unroll
-        for (int i = 0; i < NL; ++i) { frd(s, 1, i); lput(u, s ^ 1, i); gload(u, i); }
-        mma(0);
+            for (int q = 0; q < NL; ++q) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {        // 4 MFMA (2 where NT is 4), an LDS read, an LDS write, a load
-            if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); else if (i & 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // chunk ch + 1 is in LDS and nobody reads this stage's first half or the other stage any more
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < NT / 2; ++j) mma(0, q / 2, (q & 1) * (NT / 2) + j);
+                frd(s, 1, q < NT ? q + NT : q - NT);
+                if (q % 2 == 0 && q / 2 + 3 < NT) frd(s, 0, q / 2 + 3);
+                lput(u, s ^ 1, q);
+                gload(u, q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            landed();
 #pragma unroll
-        for (int i = 0; i < NL; ++i) frd(s ^ 1, 0, i);
-        mma(1);
+            for (int q = 0; q < NL; ++q) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, NT / 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                for (int j = 0; j < NT / 2; ++j) mma(1, q / 2, (q & 1) * (NT / 2) + j);
+                if (q < NT) frd(s ^ 1, 0, NT + q);
+                else if (q < NT + 3) frd(s ^ 1, 0, q - NT);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            // the same by group: 4 MFMA (2 where NT is 4), an LDS read, an LDS write, a load
+#pragma unroll
+            for (int q = 0; q < NL; ++q) { frd(s, 1, q); lput(u, s ^ 1, q); gload(u, q); }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma(0, i, j);
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+                if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); else if (q & 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            }
+            landed();
+#pragma unroll
+            for (int q = 0; q < NL; ++q) frd(s ^ 1, 0, q);
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma(1, i, j);
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NT / 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
         }
     };
     if constexpr (SETS == 1) {
         for (int ch = 0; ch < nc; ++ch) step(ch, ch & 1, 0);
+        // (the compiler does not know that inline asm has written the accumulators that are read from here on)
+        if constexpr (TA || TB) asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");
     } else {
         for (int ch = 0; ch < nc; ch += 2) {
             step(ch, 0, 1);
@@ -159,10 +225,18 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     }
     __syncthreads();
 
-    auto mrow = [&](int i) { return m0 + wm * LB_W + r16 * NT + i; };                                    // label of tile i
-    auto ncol = [&](int j) { return n0 + wn * LB_W + (j >> 1) * 32 + q16 * 8 + (j & 1) * 4; };           // first of 4 classes of tile j
-    const int pcol = n0 + wn * LB_W + q16 * 8;                                                           // first of 8 classes of tiles 0, 1
-    auto pairs = [&](const f32x4& x, const f32x4& y) { return u32x4{lb_pack(x[0], x[1]), lb_pack(x[2], x[3]), lb_pack(y[0], y[1]), lb_pack(y[2], y[3])}; };
+    auto mrow = [&](int i) { return m0 + wm * LB_W + i * 16 + r16; };                                    // label of tile i
+    // first of the 4 classes of tile j; first of the 8 that a lane has of tiles 0 and 1: as they lie, or after an exchange between
+    // neighbouring 16-lane rows
+    auto ncol = [&](int j) { return n0 + wn * LB_W + (TB ? j * 16 + 4 * q16 : (j >> 1) * 32 + q16 * 8 + (j & 1) * 4); };
+    const int pcol = n0 + wn * LB_W + (TB ? (q16 & 1) * 16 + (q16 >> 1) * 8 : q16 * 8);
+    auto pairs = [&](const f32x4& x, const f32x4& y) {
+        const u32x4 v = {lb_pack(x[0], x[1]), lb_pack(x[2], x[3]), lb_pack(y[0], y[1]), lb_pack(y[2], y[3])};
+        if constexpr (!TB) return v;
+        const auto r0 = __builtin_amdgcn_permlane16_swap(v[0], v[2], false, false);
+        const auto r1 = __builtin_amdgcn_permlane16_swap(v[1], v[3], false, false);
+        return u32x4{r0[0], r1[0], r0[1], r1[1]};
+    };
 
     if constexpr (EPI == LIN_STORE) {
         const float common = g.scale == 2 ? lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0) : 1.f;
@@ -230,7 +304,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                 for (int e = 0; e < 4; ++e) sum += __expf(acc[i][j][e] - base);
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (q16 == 0) red[wn * LB_T + wm * LB_W + r16 * NT + i] = make_float2(mx, sum);
+            if (q16 == 0) red[wn * LB_T + wm * LB_W + i * 16 + r16] = make_float2(mx, sum);
         }
         __syncthreads();
         if (tid < LB_T && m0 + tid < g.M) {
@@ -275,7 +349,6 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
 #pragma unroll
         for (int pl = 0; pl < (PL ? 3 : 1); ++pl) {
             __bf16* const dz = (__bf16*)g.dz + (PL ? (long long)pl * g.Npad : 0);
-            __bf16* const dzt = (__bf16*)g.dzt + (PL ? (long long)pl * g.Mpad : 0);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 const int m = mrow(i);
@@ -286,17 +359,6 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                     if (m < g.M && pcol + 32 * p < g.Npad) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
                 }
             }
-            if (g.dzt && mrow(0) < g.Mpad)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int n = ncol(j) + e;
-                        if (n >= g.N) continue;
-                        __bf16* const o = dzt + n * g.lddzt + mrow(0);
-                        if constexpr (NT == 8) *reinterpret_cast<u32x4*>(o) = u32x4{lb_pack(acc[0][j][e], acc[1][j][e]), lb_pack(acc[2][j][e], acc[3][j][e]), lb_pack(acc[NT - 4][j][e], acc[NT - 3][j][e]), lb_pack(acc[NT - 2][j][e], acc[NT - 1][j][e])};
-                        else                   *reinterpret_cast<u32x2*>(o) = u32x2{lb_pack(acc[0][j][e], acc[1][j][e]), lb_pack(acc[2][j][e], acc[3][j][e])};
-                    }
             if constexpr (PL)
 #pragma unroll
                 for (int i = 0; i < NT; ++i)
@@ -309,9 +371,10 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
 }
 
 template <bool PL, int NT> static void lb_launch(int epi, const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE, PL, NT>), dim3(grid), dim3(256), 0, s, g);
-    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ, PL, NT>), dim3(grid), dim3(256), 0, s, g);
-    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE, PL, NT>), dim3(grid), dim3(256), 0, s, g);
+    if (epi == LIN_LSE)     hipLaunchKernelGGL((lin_gemm256_kernel<LIN_LSE, PL, NT, false, false>), dim3(grid), dim3(256), 0, s, g);
+    else if (epi == LIN_DZ) hipLaunchKernelGGL((lin_gemm256_kernel<LIN_DZ, PL, NT, false, false>), dim3(grid), dim3(256), 0, s, g);
+    else if (g.ta)          hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE, PL, NT, true, true>), dim3(grid), dim3(256), 0, s, g);
+    else                    hipLaunchKernelGGL((lin_gemm256_kernel<LIN_STORE, PL, NT, false, true>), dim3(grid), dim3(256), 0, s, g);
 }
 void fea_lin_gemm256(int epi, int tile, bool planes, const LinGemm& g, unsigned grid, hipStream_t s) {
     if (tile == 256) { if (planes) lb_launch<true, 8>(epi, g, grid, s); else lb_launch<false, 8>(epi, g, grid, s); }

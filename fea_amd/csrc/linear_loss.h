@@ -3,40 +3,41 @@
 #pragma once
 #include "common.h"
 
-// C = A . B^T with the reduction axis contiguous in both operands.  A row = a label row, B row = a class (LIN_LSE, LIN_DZ);
-// LIN_STORE is a plain product.  Row starts are 16-byte aligned, K is a multiple of 16 bytes of elements.
+// LIN_LSE, LIN_DZ: C = A . B^T, A rows = label rows, B rows = classes, the reduction along the rows of both.
+// LIN_STORE: C = A . B or A^T . B, B [K][N] with its rows along the reduction, A [M][K] or (ta) [K][M].
+// Row starts are 16-byte aligned (fp32 B of LIN_STORE and both operands of the others may be odd).
 enum { LIN_LSE = 0, LIN_DZ = 1, LIN_STORE = 2 };
 
 // fp32 operands of large products as three bf16 planes: x = x0 + x1 + x2, each the rounding of what the ones before leave, so the sum holds
-// all 24 bits.  A row is [plane 0 | plane 1 | plane 2] of Kp (a multiple of 64) elements, zero behind the end.  A product runs over the six
-// pairs of planes whose weight is above 2^-24 (x1 y1, x2 y0, x0 y2, x1 y0, x0 y1, x0 y0, the small ones first, all into one fp32 sum): the
-// bf16 matrix rate is 16 times the fp32 one, so six products still gain 2.7.  FEA_PL is the form's dtype code inside these files.
+// all 24 bits.  A row is [plane 0 | plane 1 | plane 2], each of its length rounded up to 64 and zero behind the end.  A product runs over the
+// six pairs of planes whose weight is above 2^-24 (x1 y1, x2 y0, x0 y2, x1 y0, x0 y1, x0 y0, the small ones first, all into one fp32
+// sum): the bf16 matrix rate is 16 times the fp32 one, so six products still gain 2.7.  FEA_PL is the form's dtype code inside these files.
 #define FEA_PL 2
 __device__ __forceinline__ int lin_plane_a(int pair) { return (0x001021 >> (4 * pair)) & 15; }
 __device__ __forceinline__ int lin_plane_b(int pair) { return (0x010201 >> (4 * pair)) & 15; }
 
 struct LinGemm {
-    int Kp;                           // FEA_PL: elements of a plane; K = 6 Kp
     const void *a, *b;
     long long lda, ldb;
-    int M, N, K;                      // rows of A, rows of B, reduction
+    int M, N, K;                      // rows, columns, reduction
+    int ta;                           // LIN_STORE: A is [K][M]
+    int Kp, Kr, Pa, Pb;               // FEA_PL: reduction of one plane rounded up to 64 (K = 6 Kp) and as it is; planes of A / B rows that hold M / N elements
     // LIN_LSE, LIN_DZ: z = (a . b + bias) * inv_t
     const float* bias;                // [N], nullable
     float inv_t;
     float2* part;                     // LIN_LSE: [M][ntn] (max, sum of exp(z - max)) of one column tile
     const float2* stat;               // LIN_DZ: [M] (log sum exp, gate)
-    const float* gout; int gstride;   // LIN_DZ: upstream gradient, one value (stride 0) or one per row
-    const int* count;                 // LIN_DZ: rows that count (mean), nullable
-    float t;                          // LIN_DZ: temperature
-    void *dz, *dzt;                   // LIN_DZ: [M][lddz], [N][lddzt]; dzt nullable
-    long long lddz, lddzt;
-    int Npad, Mpad;                   // LIN_DZ: columns / rows written, zero behind N / M
+    const float* gout; int gstride;   // upstream gradient, one value (stride 0) or one per row
+    const int* count;                 // rows that count (mean), nullable
+    float t;                          // temperature
+    void* dz; long long lddz;         // LIN_DZ: [M][lddz]
+    int Npad;                         // LIN_DZ: columns written (FEA_PL: of each plane), zero behind N
     float* colsum;                    // LIN_DZ: [tiles of A rows][N], nullable: sums of row scale * softmax over the tile's rows
     long long ldcol;
     // LIN_STORE: split over K into `splits` parts of kper: direct store to out (splits == 1, slab == NULL) or fp32 slabs
     void* out; long long ldo;
     float* slab;                      // [splits][M][ldo], ldo a multiple of 4 (columns behind N hold nothing)
-    int scale;                        // 0: none, 1: times the row scale of A's row, 2: times the common scale (gout, count, t above)
+    int scale;                        // 0: none, 1: times the row scale of C's row, 2: times the common scale (gout, count, t above)
     int splits, kper;
     int ntm, ntn;
     // fea_lin_rows: selected logits a . b + bias of the entries index[M][sel] (nullable)

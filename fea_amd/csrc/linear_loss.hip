@@ -24,116 +24,51 @@ __device__ __forceinline__ void lin_split3(float v, __bf16& x0, __bf16& x1, __bf
     x2 = (__bf16)v;
 }
 
-// Copies of an operand in [R][ld]: `rows` [R][ldr] (zero for C <= c < Cpad) and `cols` [C][ldc] (zero for R <= r < Rpad), either nullable; Cpad and
-// Rpad are multiples of 64.  With planes (fp32 in, bf16 out) a row holds three of Cpad / Rpad elements.  In `cols`, rows whose gate is 0
-// count as zeros: what an ignored row holds (an infinity, a NaN) meets a zero gradient in the weight's product, and 0 x NaN must
-// not reach the weight; and with gout every row is multiplied by its own upstream gradient.  Two operands per launch, 64 x 64 tiles.
-struct LinCopy { const void* in; void *rows, *cols; long long ld, ldr, ldc, R, Rpad; int C, Cpad; const float2* stat; const float* gout; float t; long long tiles; };
-struct LinCopies { LinCopy a, b; };
+// Copies of an operand's rows [R][ld]: C elements in rows of Cpad (a multiple of 64, zero behind C); with planes (fp32 in, bf16 out) a row
+// holds three of Cpad.  With stat, rows whose gate is 0 count as zeros: what an ignored row holds (an infinity, a NaN) meets a zero
+// gradient in the weight's product, and 0 x NaN must not reach the weight; with gout every row is multiplied by its own
+// upstream gradient.  Up to three operands per launch, 64 x 64 elements per workgroup.
+struct LinCopy { const void* in; void* out; long long ld, ldo, R; int C, Cpad; const float2* stat; const float* gout; float t; long long tiles; };
+struct LinCopies { LinCopy j[3]; };
 
-__device__ __forceinline__ bool lin_copy_tile(const LinCopies& both, LinCopy& j, long long& r0, int& c0) {
-    const bool second = blockIdx.x >= both.a.tiles;
-    j = second ? both.b : both.a;
-    const long long tile = blockIdx.x - (second ? both.a.tiles : 0);
+template <typename T, bool PL, bool ALN>
+__global__ __launch_bounds__(256) void lin_copy_kernel(const LinCopies js) {
+    constexpr int EPC = Elem<T>::EPC, NV = 8 / EPC;
+    long long tile = blockIdx.x;
+    int n = 0;
+    while (n < 2 && tile >= js.j[n].tiles) tile -= js.j[n++].tiles;
+    const LinCopy j = js.j[n];
     const int nc = j.Cpad / 64;
-    r0 = tile / nc * 64;
-    c0 = (int)(tile % nc) * 64;
-    return j.in != nullptr;
-}
-__device__ __forceinline__ bool lin_copy_gate(const LinCopy& j, long long r) { return r < j.R && (!j.stat || j.stat[r].y != 0.f); }
-__device__ __forceinline__ float lin_copy_factor(const LinCopy& j, long long r) { return j.gout ? lin_row_scale(j.gout, 1, nullptr, j.t, 1.f, r) : 1.f; }
-
-// fp32 (out fp32, or three bf16 planes: PL)
-template <bool PL>
-__global__ __launch_bounds__(256) void lin_copy32_kernel(const LinCopies both) {
-    __shared__ float tile[64][65];
-    LinCopy j;
-    long long r0;
-    int c0;
-    if (!lin_copy_tile(both, j, r0, c0)) return;
-    const float* const in = (const float*)j.in;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6, hi = threadIdx.x >> 3, lo = (threadIdx.x & 7) * 8;
-#pragma unroll 4
-    for (int i = y; i < 64; i += 4) tile[i][x] = r0 + i < j.R && c0 + x < j.C ? in[(r0 + i) * j.ld + c0 + x] : 0.f;
-    __syncthreads();
-    if (j.rows)
+    const long long r0 = tile / nc * 64 + (threadIdx.x >> 3);
+    const int c = (int)(tile % nc) * 64 + (threadIdx.x & 7) * 8;
+    u32x4 v[2][NV];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = hi + 32 * i;
-            if (r0 + r >= j.R) continue;
-            if constexpr (PL) {
-                __bf16 v[3][8];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) lin_split3(tile[r][lo + e], v[0][e], v[1][e], v[2][e]);
-                __bf16* const o = (__bf16*)j.rows + (r0 + r) * j.ldr + c0 + lo;
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(o + (long long)p * j.Cpad) = *reinterpret_cast<const u32x4*>(v[p]);
-            } else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ((float*)j.rows)[(r0 + r) * j.ldr + c0 + lo + e] = tile[r][lo + e];
-        }
-    if (j.cols) {
-        if (j.stat) {
-            __syncthreads();
-#pragma unroll 4
-            for (int i = y; i < 64; i += 4) tile[i][x] = lin_copy_gate(j, r0 + i) ? tile[i][x] * lin_copy_factor(j, r0 + i) : 0.f;
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = hi + 32 * i;
-            if (c0 + c >= j.C) continue;
-            if constexpr (PL) {
-                __bf16 v[3][8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) lin_split3(tile[lo + e][c], v[0][e], v[1][e], v[2][e]);
-                __bf16* const o = (__bf16*)j.cols + (c0 + c) * j.ldc + r0 + lo;
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(o + p * j.Rpad) = *reinterpret_cast<const u32x4*>(v[p]);
-            } else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ((float*)j.cols)[(c0 + c) * j.ldc + r0 + lo + e] = tile[lo + e][c];
-        }
-    }
-}
-
-// bf16: 16-byte loads and stores; a thread turns 2 rows x 8 columns into 8 dwords (two rows of a column each) on the way into LDS
-template <bool ALN>
-__global__ __launch_bounds__(256) void lin_copy16_kernel(const LinCopies both) {
-    __shared__ __attribute__((aligned(16))) uint32_t tile[64][36];        // [column][row pair]
-    LinCopy j;
-    long long r0;
-    int c0;
-    if (!lin_copy_tile(both, j, r0, c0)) return;
-    const __bf16* const in = (const __bf16*)j.in;
-    const int hi = threadIdx.x >> 3, lo = threadIdx.x & 7;
-    u32x4 v[2];
+        for (int q = 0; q < NV; ++q)
+            v[i][q] = r0 + 32 * i < j.R ? lin_load16<T, ALN>((const T*)j.in + (r0 + 32 * i) * j.ld + c + q * EPC, j.C - c - q * EPC) : u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const long long r = r0 + 2 * hi + i;
-        v[i] = r < j.R ? lin_load16<__bf16, ALN>(in + r * j.ld + c0 + 8 * lo, j.C - c0 - 8 * lo) : u32x4{0, 0, 0, 0};
-        if (j.rows && r < j.R) *reinterpret_cast<u32x4*>((__bf16*)j.rows + r * j.ldr + c0 + 8 * lo) = v[i];
-        if (!lin_copy_gate(j, r)) v[i] = u32x4{0, 0, 0, 0};
-        else if (j.gout) {
-            const float f = lin_copy_factor(j, r);
-            __bf16 x[8];
-            *reinterpret_cast<u32x4*>(x) = v[i];
+        const long long r = r0 + 32 * i;
+        if (r >= j.R) continue;
+        T x[8];
+        const bool dead = j.stat && j.stat[r].y == 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (__bf16)((float)x[e] * f);
-            v[i] = *reinterpret_cast<const u32x4*>(x);
+        for (int q = 0; q < NV; ++q) *reinterpret_cast<u32x4*>(x + q * EPC) = dead ? u32x4{0, 0, 0, 0} : v[i][q];
+        if (j.gout) {
+            const float f = lin_row_scale(j.gout, 1, nullptr, j.t, 1.f, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = dead ? from_f32<T>(0.f) : from_f32<T>(to_f32(x[e]) * f);
         }
-    }
-    if (!j.cols) return;
+        if constexpr (PL) {
+            __bf16 y[3][8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        tile[8 * lo + 2 * q][hi] = __builtin_amdgcn_perm(v[1][q], v[0][q], 0x05040100u);
-        tile[8 * lo + 2 * q + 1][hi] = __builtin_amdgcn_perm(v[1][q], v[0][q], 0x07060302u);
-    }
-    __syncthreads();
+            for (int e = 0; e < 8; ++e) lin_split3(x[e], y[0][e], y[1][e], y[2][e]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int c = hi + 32 * i;
-        if (c0 + c < j.C) *reinterpret_cast<u32x4*>((__bf16*)j.cols + (c0 + c) * j.ldc + r0 + 8 * lo) = *reinterpret_cast<const u32x4*>(&tile[c][4 * lo]);
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>((__bf16*)j.out + r * j.ldo + p * j.Cpad + c) = *reinterpret_cast<const u32x4*>(y[p]);
+        } else
+#pragma unroll
+            for (int q = 0; q < NV; ++q) *reinterpret_cast<u32x4*>((T*)j.out + r * j.ldo + c + q * EPC) = *reinterpret_cast<const u32x4*>(x + q * EPC);
     }
 }
 
@@ -340,8 +275,7 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 // same class hold the same value.
 template <typename T, bool PL>
 __global__ __launch_bounds__(256) void lin_scatter_kernel(const long long* __restrict__ index, const float* __restrict__ dsel, int K,
-                                                          const float2* __restrict__ stat, T* dz, long long lddz, T* dzt, long long lddzt, long long v0, int N, long long entries,
-                                                          int Npad, long long Mpad) {
+                                                          const float2* __restrict__ stat, T* dz, long long lddz, long long v0, int N, long long entries, int Npad) {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= entries) return;
     const long long m = e / K, i = index[e] - v0;
@@ -350,15 +284,8 @@ __global__ __launch_bounds__(256) void lin_scatter_kernel(const long long* __res
     if constexpr (PL) {
         T x[3];
         lin_split3(dsel[e], x[0], x[1], x[2]);
-        for (int p = 0; p < 3; ++p) {
-            dz[m * lddz + (long long)p * Npad + i] = x[p];
-            if (dzt) dzt[i * lddzt + p * Mpad + m] = x[p];
-        }
-    } else {
-        const T v = from_f32<T>(dsel[e]);
-        dz[m * lddz + i] = v;
-        if (dzt) dzt[i * lddzt + m] = v;
-    }
+        for (int p = 0; p < 3; ++p) dz[m * lddz + (long long)p * Npad + i] = x[p];
+    } else dz[m * lddz + i] = from_f32<T>(dsel[e]);
 }
 
 // out = acc + slabs in split order, rows of N in slabs with rows of ld = N rounded up to 4; acc (nullable, rows of ld) is the fp32 sum of
@@ -461,11 +388,10 @@ struct LinDims {
     long long rows; int D, V, K, dtype, es, epc;
     bool odd() const { return D % epc != 0; }      // rows that are no multiple of 16 bytes
     bool straight() const { return !odd(); }       // gradients go straight to their rows (others through slabs, which have wide stores)
-    bool wide;                    // row strides of 2^21 elements or more (a slice of something very wide): the 128 tile, which has 64-bit offsets
 };
 
 static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
-    LinDims d{rows, D, V, K, dtype, dtype == FEA_BF16 ? 2 : 4, dtype == FEA_BF16 ? 8 : 4, false};
+    LinDims d{rows, D, V, K, dtype, dtype == FEA_BF16 ? 2 : 4, dtype == FEA_BF16 ? 8 : 4};
     return d;
 }
 
@@ -473,7 +399,7 @@ static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
 struct LinForm {
     int dt, es, mul, pad;         // dtype of the products, bytes of an element, elements of a row per channel, what a row is rounded up to
     long long row(long long k) const { return up(k, pad) * mul; }          // elements of a row of k channels
-    int K(long long k) const { return (int)(dt == FEA_PL ? 6 * up(k, 64) : up(k, pad)); }
+    int K(long long k) const { return (int)(dt == FEA_PL ? 6 * up(k, 64) : dt == FEA_BF16 ? up(k, 64) : k); }      // reduction over k channels
 };
 static LinForm lin_form(int dtype, bool planes) {
     if (planes) return LinForm{FEA_PL, 2, 3, 64};
@@ -494,7 +420,6 @@ static LinFwd lin_fwd_plan(const LinDims& d) {
         if (q.time + ((double)p.rc + d.V) * d.D * 10 / 4e12 + 6e-6 < t.time) { t = q; p.planes = true; }
     }
     p.tile = t.tile;
-    if (d.wide && !p.planes) p.tile = 128;
     if (d.rows <= 64) { p.tile = 64; p.planes = false; }
     p.ntn = (d.V + p.tile - 1) / p.tile;
     p.G = 1;
@@ -503,7 +428,7 @@ static LinFwd lin_fwd_plan(const LinDims& d) {
     return p;
 }
 
-// Backward: pieces of rc rows x vc classes.  dz and its transpose take rc x vc elements each: 2^28 at most
+// Backward: pieces of rc rows x vc classes.  dz takes rc x vc elements: 2^28 at most
 // (FEA_AMD_LINEAR_PIECE: tests, many pieces on small shapes).
 static long long lin_piece() {
     const char* e = getenv("FEA_AMD_LINEAR_PIECE");
@@ -530,12 +455,12 @@ static LinBwd lin_bwd_plan(const LinDims& d, int want) {
     };
     const double t = tiles(d.dtype, 1, tz, p.th, p.tw);
     p.planes = false;
-    if (d.dtype == FEA_F32 && 3 * up(p.rc > p.vc ? p.rc : p.vc, 64) < 1 << 21) {     // (the strides that the large tile takes)
+    if (d.dtype == FEA_F32 && 3 * up(p.vc, 64) < 1 << 21) {     // (the strides that the bf16 kernels take)
         LinTile z, h, w;
         const double q = tiles(FEA_PL, 6, z, h, w);
-        if (q + (((double)p.rc + p.vc) * d.D * 12 + 4.0 * p.rc * p.vc) / 4e12 + 6e-6 < t) { tz = z; p.th = h; p.tw = w; p.planes = true; }
+        if (q + (((double)p.rc + p.vc) * d.D * 10 + 2.0 * p.rc * p.vc) / 4e12 + 6e-6 < t) { tz = z; p.th = h; p.tw = w; p.planes = true; }
     }
-    p.tz = d.wide && !p.planes ? 128 : tz.tile;
+    p.tz = tz.tile;
     return p;
 }
 
@@ -548,8 +473,7 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
         w.bcnt = c.take<int>(fea_lin_few_blocks(d.rows, false));
         return c.at;
     }
-    const int t = p.tile == 64 ? 64 : 128;               // (not 256: wide row strides, which a size query does not know, ask for 128)
-    w.part = c.take<float2>(p.rc * ((d.V + t - 1) / t));
+    w.part = c.take<float2>(p.rc * p.ntn);
     w.zsel = c.take<float>(d.rows * d.K);
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
@@ -562,7 +486,7 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
     return c.at;
 }
 
-struct LinBwdWs { void *hp, *wp, *ht, *wt, *dz, *dzt; float *slab, *acch, *accw, *colsum; double* dbpart; };
+struct LinBwdWs { void *hp, *wp, *hg, *dz; float *slab, *acch, *accw, *colsum; double* dbpart; };
 static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* base, LinBwdWs& w) {
     LinCarve c{base};
     w = LinBwdWs{};
@@ -575,8 +499,7 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     const LinForm f = lin_form(d.dtype, p.planes);
     if (p.planes || (d.dtype == FEA_BF16 && d.odd())) { w.hp = c.take<char>(p.rc * f.row(d.D) * f.es); w.wp = c.take<char>(p.vc * f.row(d.D) * f.es); }
     w.dz = c.take<char>(p.rc * f.row(p.vc) * f.es);
-    if (want & 2) { w.dzt = c.take<char>(p.vc * f.row(p.rc) * f.es); w.ht = c.take<char>(d.D * f.row(p.rc) * f.es); }
-    if (want & 1) w.wt = c.take<char>(d.D * f.row(p.vc) * f.es);
+    if (want & 2) w.hg = c.take<char>(p.rc * f.row(d.D) * f.es);
     long long slab = 0;
     const long long ld = up(d.D, 4);
     if ((want & 1) && !(p.th.splits == 1 && p.nvc == 1 && d.straight())) slab = p.th.splits * p.rc * ld;
@@ -596,24 +519,25 @@ extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, 
     return lin_bwd_carve(d, lin_bwd_plan(d, grads), grads, nullptr, w);
 }
 
-// an operand of R rows and where its copies go
-static LinCopy lin_copy_of(const LinDims& d, const LinForm& f, const void* in, long long ld, long long R, void* rows, void* cols) {
+// an operand of R rows and where its copy goes (nullptr: none)
+static LinCopy lin_copy_of(const LinDims& d, const LinForm& f, const void* in, long long ld, long long R, void* out) {
     LinCopy j{};
-    j.in = rows || cols ? in : nullptr; j.rows = rows; j.cols = cols; j.ld = ld; j.R = R; j.Rpad = up(R, 64); j.C = d.D; j.Cpad = (int)up(d.D, 64);
-    j.ldr = f.row(d.D); j.ldc = f.row(R);
-    j.tiles = j.in ? j.Rpad / 64 * (j.Cpad / 64) : 0;
+    j.in = in; j.out = out; j.ld = ld; j.ldo = f.row(d.D); j.R = R; j.C = d.D; j.Cpad = (int)up(d.D, 64);
+    j.tiles = out ? (R + 63) / 64 * (j.Cpad / 64) : 0;
     return j;
 }
-static int lin_copy(const LinDims& d, const LinForm& f, const LinCopy& a, const LinCopy& b, hipStream_t s) {
-    const LinCopies both{a, b};
-    const long long n = a.tiles + b.tiles;
+static int lin_copy(const LinDims& d, const LinForm& f, const LinCopies& js, hipStream_t s) {
+    const long long n = js.j[0].tiles + js.j[1].tiles + js.j[2].tiles;
     if (!n) return FEA_OK;
-    FEA_CHECK(n < 1 << 24, FEA_E_UNSUPPORTED_SHAPE, "lin_copy: %lld tiles", n);
-    const dim3 grid((unsigned)n);
-    if (f.dt == FEA_PL)       hipLaunchKernelGGL(lin_copy32_kernel<true>, grid, dim3(256), 0, s, both);
-    else if (f.dt == FEA_F32) hipLaunchKernelGGL(lin_copy32_kernel<false>, grid, dim3(256), 0, s, both);
-    else if (d.odd())         hipLaunchKernelGGL(lin_copy16_kernel<false>, grid, dim3(256), 0, s, both);
-    else                      hipLaunchKernelGGL(lin_copy16_kernel<true>, grid, dim3(256), 0, s, both);
+    FEA_CHECK(n < INT_MAX, FEA_E_UNSUPPORTED_SHAPE, "lin_copy: %lld tiles", n);
+    const dim3 grid((unsigned)n), bl(256);
+    const bool aln = !d.odd();
+    if (f.dt == FEA_PL && aln)       hipLaunchKernelGGL((lin_copy_kernel<float, true, true>), grid, bl, 0, s, js);
+    else if (f.dt == FEA_PL)         hipLaunchKernelGGL((lin_copy_kernel<float, true, false>), grid, bl, 0, s, js);
+    else if (f.dt == FEA_F32 && aln) hipLaunchKernelGGL((lin_copy_kernel<float, false, true>), grid, bl, 0, s, js);
+    else if (f.dt == FEA_F32)        hipLaunchKernelGGL((lin_copy_kernel<float, false, false>), grid, bl, 0, s, js);
+    else if (aln)                    hipLaunchKernelGGL((lin_copy_kernel<__bf16, false, true>), grid, bl, 0, s, js);
+    else                             hipLaunchKernelGGL((lin_copy_kernel<__bf16, false, false>), grid, bl, 0, s, js);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
@@ -641,13 +565,14 @@ static int lin_check(const char* who, const LinDims& d, const void* h, long long
     if (!d.odd())
         FEA_CHECK(((uintptr_t)h | (uintptr_t)w) % 16 == 0 && ldh % d.epc == 0 && ldw % d.epc == 0, FEA_E_BADARG,
                   "%s: hidden and weight need 16-byte aligned rows when the features are a multiple of %d", who, d.epc);
+    if (!d.odd() && d.dtype == FEA_BF16)      // (32-bit offsets over a tile's rows)
+        FEA_CHECK(ldh < 1 << 21 && ldw < 1 << 21, FEA_E_UNSUPPORTED_SHAPE, "%s: bf16 row strides below %d are served (hidden %lld, weight %lld)", who, 1 << 21, ldh, ldw);
     return FEA_OK;
 }
 
 static int lin_forward(const char* who, LinDims d, const void* h, long long ldh, const void* w, long long ldw, const float* bias, LinJoin j,
                        float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
-    d.wide = !d.odd() && (ldh >= 1 << 21 || ldw >= 1 << 21);
     const LinFwd p = lin_fwd_plan(d);
     LinFwdWs b;
     const size_t need = lin_fwd_carve(d, p, (char*)ws, b);
@@ -685,7 +610,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
     for (long long r = 0; r < d.rows; r += p.rc) {
         const long long n = d.rows - r < p.rc ? d.rows - r : p.rc;
         const void* hr = (const char*)h + r * ldh * d.es;
-        if (pack) LIN_TRY(lin_copy(d, f, lin_copy_of(d, f, hr, ldh, n, b.hp, nullptr), lin_copy_of(d, f, w, ldw, d.V, r ? nullptr : b.wp, nullptr), s));
+        if (pack) LIN_TRY(lin_copy(d, f, LinCopies{{lin_copy_of(d, f, hr, ldh, n, b.hp), lin_copy_of(d, f, w, ldw, d.V, r ? nullptr : b.wp)}}, s));
         LinGemm g{};
         g.a = pack ? b.hp : hr; g.lda = pack ? f.row(d.D) : ldh; g.b = pack ? b.wp : w; g.ldb = pack ? f.row(d.D) : ldw;
         g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
@@ -746,7 +671,6 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     LinDims d = lin_dims(rows, D, V, K, dtype);
     hipStream_t s = (hipStream_t)stream;
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
-    d.wide = !d.odd() && (ldh >= 1 << 21 || ldw >= 1 << 21);
     FEA_CHECK(index && stat && dsel && gout, FEA_E_BADARG, "%s: null operand", who);
     FEA_CHECK(gout_stride == 0 || gout_stride == 1, FEA_E_BADARG, "%s: gout_stride %d", who, gout_stride);
     FEA_CHECK(dh || dw || db, FEA_E_BADARG, "%s: no gradient asked for", who);
@@ -777,25 +701,30 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             const long long v0 = (long long)iv * p.vc;
             const int nv = (int)(V - v0 < p.vc ? V - v0 : p.vc);
             const char* wr = (const char*)w + v0 * ldw * d.es;
-            // the operands' copies: hidden once for its rows, the weight's piece unless the only piece is there from the rows before
-            LinCopy jh = lin_copy_of(d, f, hr, ldh, n, pack && iv == 0 ? b.hp : nullptr, dw && iv == 0 ? b.ht : nullptr);
-            jh.stat = st; jh.gout = gout_stride ? go : nullptr; jh.t = temperature;
-            const bool fresh = ir == 0 || p.nvc > 1;
-            LIN_TRY(lin_copy(d, f, jh, lin_copy_of(d, f, wr, ldw, nv, pack && fresh ? b.wp : nullptr, dh && fresh ? b.wt : nullptr), s));
+            // the operands' copies: packed rows, and hidden as dw takes it (gated, times each row's own upstream gradient; gated alone, it is
+            // the packed one).  Hidden once for its rows, the weight's piece unless the only piece is there from the rows before
+            const bool gated = dw && (!pack || gout_stride);
+            LinCopies js{{lin_copy_of(d, f, hr, ldh, n, pack && iv == 0 ? b.hp : nullptr), lin_copy_of(d, f, wr, ldw, nv, pack && (ir == 0 || p.nvc > 1) ? b.wp : nullptr),
+                          lin_copy_of(d, f, hr, ldh, n, gated && iv == 0 ? b.hg : nullptr)}};
+            js.j[0].stat = js.j[2].stat = st;
+            if (gout_stride) { js.j[2].gout = go; js.j[2].t = temperature; }
+            LIN_TRY(lin_copy(d, f, js, s));
+            const void* const wk = pack ? b.wp : (const void*)wr;
+            const long long ldwk = pack ? f.row(D) : ldw;
             LinGemm g{};
-            g.a = pack ? b.hp : (const void*)hr; g.lda = pack ? f.row(D) : ldh; g.b = pack ? b.wp : (const void*)wr; g.ldb = pack ? f.row(D) : ldw;
+            g.a = pack ? b.hp : (const void*)hr; g.lda = pack ? f.row(D) : ldh; g.b = wk; g.ldb = ldwk;
             g.M = (int)n; g.N = nv; g.K = pack ? f.K(D) : D; g.Kp = (int)up(D, 64);
             g.bias = bias ? bias + v0 : nullptr; g.inv_t = 1.f / temperature; g.stat = st; g.gout = go; g.gstride = gout_stride;
             g.count = count; g.t = temperature;
-            g.dz = b.dz; g.lddz = f.row(nv); g.Npad = (int)up(nv, f.pad); g.dzt = dw ? b.dzt : nullptr; g.lddzt = f.row(n); g.Mpad = (int)up(n, f.pad);
+            g.dz = b.dz; g.lddz = f.row(nv); g.Npad = (int)up(nv, f.pad);
             g.colsum = db ? b.colsum : nullptr; g.ldcol = up(p.vc, 64);
             LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
             const unsigned sg = (unsigned)((entries + 255) / 256);
-            if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, (__bf16*)g.dzt, g.lddzt, v0, nv, entries, g.Npad, (long long)g.Mpad);
-            else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, (__bf16*)g.dzt, g.lddzt, v0, nv, entries, 0, 0ll);
-            else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, (float*)g.dzt, g.lddzt, v0, nv, entries, 0, 0ll);
+            if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, g.Npad);
+            else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, 0);
+            else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0);
             FEA_LAUNCH_CHECK();
             if (db) {
                 const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (int)((n + LIN_DB_ROWS - 1) / LIN_DB_ROWS);
@@ -804,11 +733,13 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);
                 FEA_LAUNCH_CHECK();
             }
-            // out (contiguous rows of D) = A . B^T over k channels: straight to out, or through fp32 slabs where the reduction is split
-            // or pieces before this one (acc) or behind it add to the sum
-            auto product = [&](const LinGemm& from, const void* A, const void* B, long long M, long long k, const LinTile& t, void* out, float* acc, bool first, bool last) {
-                LinGemm m = from;
-                m.a = A; m.b = B; m.lda = m.ldb = f.row(k); m.M = (int)M; m.N = D; m.K = f.K(k); m.Kp = (int)up(k, 64);
+            // out (contiguous rows of D) = dz . B or dz^T . B over k channels: straight to out, or through fp32 slabs where the reduction is
+            // split or pieces before this one (acc) or behind it add to the sum
+            auto product = [&](bool ta, int scale, const void* B, long long ldb, long long M, long long k, const LinTile& t, void* out, float* acc, bool first, bool last) {
+                LinGemm m{};
+                m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
+                m.a = b.dz; m.lda = f.row(nv); m.ta = ta; m.b = B; m.ldb = ldb; m.scale = scale;
+                m.M = (int)M; m.N = D; m.K = f.K(k); m.Kp = (int)up(k, 64); m.Kr = (int)k; m.Pa = (int)up(nv, 64); m.Pb = (int)up(D, 64);
                 m.splits = t.splits; m.kper = (int)up((m.K + t.splits - 1) / t.splits, 64);
                 const bool direct = t.splits == 1 && first && last && d.straight();
                 m.ldo = up(D, 4);
@@ -816,16 +747,8 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 LIN_TRY(fea_lin_gemm(LIN_STORE, f.dt, t.tile, m, s));
                 return direct ? FEA_OK : lin_reduce(d, b.slab, t.splits, M, first ? nullptr : acc, last ? nullptr : acc, last ? out : nullptr, s);
             };
-            LinGemm m{};
-            m.stat = st; m.gout = go; m.gstride = gout_stride; m.count = count; m.t = temperature;
-            if (dh) {
-                m.scale = 1;
-                LIN_TRY(product(m, b.dz, b.wt, n, nv, p.th, (char*)dh + r0 * D * d.es, b.acch, iv == 0, iv + 1 == p.nvc));
-            }
-            if (dw) {
-                m.scale = gout_stride ? 0 : 2;
-                LIN_TRY(product(m, b.dzt, b.ht, nv, n, p.tw, (char*)dw + v0 * D * d.es, b.accw ? b.accw + v0 * up(D, 4) : nullptr, ir == 0, ir + 1 == p.nrc));
-            }
+            if (dh) LIN_TRY(product(false, 1, wk, ldwk, n, nv, p.th, (char*)dh + r0 * D * d.es, b.acch, iv == 0, iv + 1 == p.nvc));
+            if (dw) LIN_TRY(product(true, gout_stride ? 0 : 2, gated ? b.hg : b.hp, f.row(D), nv, n, p.tw, (char*)dw + v0 * D * d.es, b.accw ? b.accw + v0 * up(D, 4) : nullptr, ir == 0, ir + 1 == p.nrc));
         }
     }
     return FEA_OK;

@@ -104,13 +104,13 @@ def iou_from_counts(inter: torch.Tensor, union: torch.Tensor):
 # ---- loss heads over many classes ---------------------------------------------------------------------------------------
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """[..., D] -> [rows, D] as the kernels read it: contiguous rows, 16-byte aligned where D allows it."""
+    """[..., D] -> [rows, D] as the kernels read it: contiguous rows, 16-byte aligned where D allows it, less than 2^21 elements apart."""
     t = t.detach()
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     epc = 16 // t.element_size()
     d = t.shape[1]
-    if (t.stride(1) != 1 and d > 1) or t.stride(0) < d or (d % epc == 0 and (t.data_ptr() % 16 or t.stride(0) % epc)):
+    if (t.stride(1) != 1 and d > 1) or t.stride(0) < d or t.stride(0) >= 1 << 21 or (d % epc == 0 and (t.data_ptr() % 16 or t.stride(0) % epc)):
         t = t.contiguous()
         if d % epc == 0 and t.data_ptr() % 16:         # contiguous already, but a view at an odd offset
             t = t.clone()
