@@ -16,7 +16,7 @@
 // serves what the planes' copies do not pay for.
 #include "linear_loss.h"
 
-static constexpr int LG_T = 128, LG_STAGE = 2 * LG_T * 128, LG_CK = 32;
+static constexpr int LG_T = 128, LG_CK = 32;
 
 __device__ __forceinline__ void lg_store4(float* p, const float (&v)[4], int n) {
     if (n >= 4 && ((uintptr_t)p & 15) == 0) *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
@@ -25,49 +25,51 @@ __device__ __forceinline__ void lg_store4(float* p, const float (&v)[4], int n) 
         for (int i = 0; i < 4; ++i) if (i < n) p[i] = v[i];
 }
 
-template <int EPI, bool ALN, bool TA>
+// TM: label rows of a tile, 128 or, for 64 rows and less in all, 64 with the four waves along the classes (64 x 32 each)
+template <int EPI, bool ALN, bool TA, int TM>
 __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     constexpr bool TB = EPI == LIN_STORE;
+    constexpr int WM = TM / 64, WN = 4 / WM, NJ = 4 / WN, WC = 32 * NJ, LG_STAGE = (TM + LG_T) * 128;      // waves along labels and classes, class tiles and classes of a wave
     __shared__ __attribute__((aligned(128))) char smem[2 * LG_STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave & 1, wn = wave >> 1, l32 = lane & 31, hf = lane >> 5;
+    const int wm = WM == 2 ? wave & 1 : 0, wn = WM == 2 ? wave >> 1 : wave, l32 = lane & 31, hf = lane >> 5;
     // consecutive tiles of an XCD share the class tile and walk the label rows: the larger operand is read once
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tm = id % g.ntm, rest = id / g.ntm, tn = rest % g.ntn, sp = rest / g.ntn;
-    const int m0 = tm * LG_T, n0 = tn * LG_T;
+    const int m0 = tm * TM, n0 = tn * LG_T;
     const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, k1 = EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K;
 
     // staging.  Rows along the tile: thread -> rows r + 32 i, 16-byte chunk c of 128 bytes, XOR-swizzled by the row.  Rows along the reduction:
-    // thread -> rows tr + 8 i of 32, 4 columns from 4 tc, columns XORed so that the two halves of a wave read different banks.
-    const int r = tid >> 3, c = tid & 7, tr = tid >> 5, tc = tid & 31;
+    // thread -> rows of 32, 4 columns each, columns XORed so that the two halves of a wave read different banks.
+    const int r = tid >> 3, c = tid & 7;
     const float *const ap = (const float*)g.a, *const bp = (const float*)g.b;
-    u32x4 ra[2][4], rb[2][4];          // two steps on the way: the first is needed a whole step after it was asked for
-    auto fetch1 = [&](const float* p, long long ld, int x0, int X, int k, int i, bool t) {
-        if (t) return k + tr + 8 * i < k1 ? lin_load16<float, ALN>(p + (k + tr + 8 * i) * ld + x0 + 4 * tc, X - x0 - 4 * tc) : u32x4{0, 0, 0, 0};
+    u32x4 ra[2][TM / 32], rb[2][4];          // two steps on the way: the first is needed a whole step after it was asked for
+    auto fetch1 = [&](const float* p, long long ld, int x0, int X, int k, int i, bool t, int W) {      // W: rows of the tile
+        const int kr = k + tid / (W / 4) + 1024 / W * i, x = x0 + tid % (W / 4) * 4;
+        if (t) return kr < k1 ? lin_load16<float, ALN>(p + kr * ld + x, X - x) : u32x4{0, 0, 0, 0};
         return x0 + r + 32 * i < X ? lin_load16<float, ALN>(p + (x0 + r + 32 * i) * ld + k + 4 * c, k1 - k - 4 * c) : u32x4{0, 0, 0, 0};
     };
     auto fetch = [&](int u, int k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ra[u][i] = fetch1(ap, g.lda, m0, g.M, k, i, TA);
-            rb[u][i] = fetch1(bp, g.ldb, n0, g.N, k, i, TB);
-        }
+        for (int i = 0; i < TM / 32; ++i) ra[u][i] = fetch1(ap, g.lda, m0, g.M, k, i, TA, TM);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rb[u][i] = fetch1(bp, g.ldb, n0, g.N, k, i, TB, LG_T);
     };
-    auto put1 = [&](char* op, const u32x4& v, int i, bool t) {
-        const int row = t ? tr + 8 * i : r + 32 * i;
-        *reinterpret_cast<u32x4*>(op + (t ? row * 512 + ((tc ^ (((row >> 2) & 1) << 3)) << 4) : row * 128 + ((c ^ (row & 7)) << 4))) = v;
+    auto put1 = [&](char* op, const u32x4& v, int i, bool t, int W) {
+        const int row = t ? tid / (W / 4) + 1024 / W * i : r + 32 * i;
+        *reinterpret_cast<u32x4*>(op + (t ? row * 4 * W + ((tid % (W / 4) ^ (((row >> 2) & 1) << 3)) << 4) : row * 128 + ((c ^ (row & 7)) << 4))) = v;
     };
     // fragment of 32 rows from x: lane l32 -> row, channels 8 s + 4 hf .. + 3
-    auto frag = [&](const char* op, int x, int s, bool t) {
+    auto frag = [&](const char* op, int x, int s, bool t, int W) {
         if (!t) return *reinterpret_cast<const u32x4*>(op + (x + l32) * 128 + (((2 * s + hf) ^ (l32 & 7)) << 4));
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(op) + (8 * s + 4 * hf) * 128 + ((x + l32) ^ (hf << 5));
-        return u32x4{p[0], p[128], p[256], p[384]};
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(op) + (8 * s + 4 * hf) * W + ((x + l32) ^ (hf << 5));
+        return u32x4{p[0], p[W], p[2 * W], p[3 * W]};
     };
-    f32x16 acc[2][2];                 // [label tile][class tile]
+    f32x16 acc[2][NJ];                 // [label tile][class tile]
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
@@ -76,17 +78,25 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
     const int live = g.M - m0 - __builtin_amdgcn_readfirstlane(wm) * 64;        // of few rows only the half or quarter that holds them is computed
     auto step = [&](int st, int k) {   // stage and register set of the same parity
         char* const sa = smem + st * LG_STAGE;
-        char* const sb = sa + LG_T * 128;
+        char* const sb = sa + TM * 128;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { put1(sa, ra[st][i], i, TA); put1(sb, rb[st][i], i, TB); }
+        for (int i = 0; i < TM / 32; ++i) put1(sa, ra[st][i], i, TA, TM);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put1(sb, rb[st][i], i, TB, LG_T);
         __syncthreads();              // one barrier per step: the other stage was last read in front of the previous one
         if (k + 2 * LG_CK < k1) fetch(st, k + 2 * LG_CK);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const u32x4 a0 = frag(sa, wm * 64, s, TA), a1 = frag(sa, wm * 64 + 32, s, TA);
-            const u32x4 b0 = frag(sb, wn * 64, s, TB), b1 = frag(sb, wn * 64 + 32, s, TB);
-            if (live > 0)  { mma16(acc[0][0], b0, a0, (const float*)nullptr); mma16(acc[0][1], b1, a0, (const float*)nullptr); }
-            if (live > 32) { mma16(acc[1][0], b0, a1, (const float*)nullptr); mma16(acc[1][1], b1, a1, (const float*)nullptr); }
+            u32x4 b[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) b[j] = frag(sb, wn * WC + j * 32, s, TB, LG_T);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (32 * i >= live) break;
+                const u32x4 a = frag(sa, wm * 64 + i * 32, s, TA, TM);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) mma16(acc[i][j], b[j], a, (const float*)nullptr);
+            }
         }
     };
     for (int k = k0; k < k1; k += 2 * LG_CK) {
@@ -97,7 +107,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
 
     // lane: label row mrow(i), register e of class tile j: class ncol(j, e)
     auto mrow = [&](int i) { return m0 + wm * 64 + i * 32 + l32; };
-    auto ncol = [&](int j, int e) { return n0 + wn * 64 + j * 32 + 8 * (e >> 2) + 4 * hf + (e & 3); };
+    auto ncol = [&](int j, int e) { return n0 + wn * WC + j * 32 + 8 * (e >> 2) + 4 * hf + (e & 3); };
 
     if constexpr (EPI == LIN_STORE) {
 #pragma unroll
@@ -108,7 +118,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
                            : g.scale == 2 ? lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0) : 1.f;
             float* const o = g.slab ? g.slab + ((long long)sp * g.M + m) * g.ldo : (float*)g.out + m * g.ldo;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const int n = ncol(j, e);
@@ -122,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
 
     // z in place; classes behind the last are -inf
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int n = ncol(j, e);
@@ -132,29 +142,33 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
         }
 
     if constexpr (EPI == LIN_LSE) {
-        float2* const red = reinterpret_cast<float2*>(smem);       // [wn][128 rows]
+        float2* const red = reinterpret_cast<float2*>(smem);       // [wn][rows]
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[i][j][e]);
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float base = mx == -INFINITY ? 0.f : mx;         // every class masked by a -inf bias: the sum is 0, not NaN
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum += __expf(acc[i][j][e] - base);
             sum += __shfl_xor(sum, 32);
-            if (hf == 0) red[wn * LG_T + wm * 64 + i * 32 + l32] = make_float2(mx, sum);
+            if (hf == 0) red[wn * TM + wm * 64 + i * 32 + l32] = make_float2(mx, sum);
         }
         __syncthreads();
-        if (tid < LG_T && m0 + tid < g.M) {
-            const float2 p = red[tid], q = red[LG_T + tid];
-            const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
-            g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, p.y * __expf(p.x - base) + q.y * __expf(q.x - base));
+        if (tid < TM && m0 + tid < g.M) {
+            float mx = red[tid].x, sum = 0.f;
+#pragma unroll
+            for (int w = 1; w < WN; ++w) mx = fmaxf(mx, red[w * TM + tid].x);
+            const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+            for (int w = 0; w < WN; ++w) sum += red[w * TM + tid].y * __expf(red[w * TM + tid].x - base);
+            g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, sum);
         }
     }
 
@@ -168,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             const float lse = st2.x;
             sc[i] = dead ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, st2.y, m);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float q = __expf(acc[i][j][e] - lse);
@@ -178,7 +192,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
         if (g.colsum) {
             float* const red = reinterpret_cast<float*>(smem);     // [wm][128 classes]
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     float s = acc[0][j][e] * sc[0] + acc[1][j][e] * sc[1];
@@ -187,13 +201,13 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
                     if (l32 == 0) red[wm * LG_T + ncol(j, e) - n0] = s;
                 }
             __syncthreads();
-            if (tid < LG_T && n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = red[tid] + red[LG_T + tid];
+            if (tid < LG_T && n0 + tid < g.N) g.colsum[tm * g.ldcol + n0 + tid] = WM == 2 ? red[tid] + red[LG_T + tid] : red[tid];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int m = mrow(i);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const int n = ncol(j, e);
@@ -207,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
 // Tile and split of a product: the one whose modelled time is least, from the rates that the kernels reach on full chips (fp32 100, bf16 700
 // and 1,300 TFLOP/s) and from the bytes of operands and result at 4 TB/s.  Both take whole rounds of the chip (256 workgroups of the large
 // tile, 512 of the small one); the parts of a split reduction are written and read once more, at least 512 (bf16) or 256 (fp32)
-// channels each.  dtype FEA_PL: K is six times the planes'.
+// channels each.  Of up to 64 or 32 rows the fp32 kernel computes no more.  dtype FEA_PL: K is six times the planes'.
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split) {
     LinTile best{128, 1, 1e30};
     const double size = dtype == FEA_F32 ? 4 : dtype == FEA_BF16 ? 2 : 1;      // bytes per element of K: a plane pair's share is 6 of 6 K
@@ -215,17 +229,28 @@ LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool spli
     for (int tile = 128; tile <= (dtype == FEA_F32 ? 128 : 256); tile += 128) {
         const double slots = tile == 256 ? 256 : 512;
         const double rate = dtype == FEA_F32 ? 100e12 : tile == 256 ? 1300e12 : 700e12;
+        const double rows = dtype == FEA_F32 && M <= 64 ? (M <= 32 ? 32 : 64) : tile;      // that are computed
         const long long tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
         for (int sp = 1; sp <= (split ? 32 : 1); ++sp) {
             if (sp > 1 && K / sp < (dtype == FEA_F32 ? 256 : 512)) break;
             const double rounds = (double)((tiles * sp + (long long)slots - 1) / (long long)slots);
-            double t = rounds * (2.0 * tile * tile * ((double)K / sp + 128) / (rate / slots));
+            double t = rounds * (2.0 * rows * tile * ((double)K / sp + 128) / (rate / slots));
             if (t < bytes / 4e12) t = bytes / 4e12;
             t += sp > 1 ? 2.0 * sp * M * N * 4 / 4e12 + 3e-6 : 0.0;
             if (t < best.time * 0.999) best = LinTile{tile, sp, t};
         }
     }
     return best;
+}
+
+template <int EPI, bool TA> static void lg_launch(const LinGemm& g, bool aln, unsigned grid, hipStream_t s) {
+    if (g.M <= 64) {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<EPI, true, TA, 64>), dim3(grid), dim3(256), 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<EPI, false, TA, 64>), dim3(grid), dim3(256), 0, s, g);
+    } else {
+        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<EPI, true, TA, 128>), dim3(grid), dim3(256), 0, s, g);
+        else     hipLaunchKernelGGL((lin_gemm_kernel<EPI, false, TA, 128>), dim3(grid), dim3(256), 0, s, g);
+    }
 }
 
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
@@ -241,21 +266,11 @@ int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }
     const long long grid = (long long)g.ntm * g.ntn * g.splits;
     FEA_CHECK(grid > 0 && grid <= (1 << 23), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: %lld tiles", grid);
-    const dim3 gr((unsigned)grid), bl(256);
     if (dtype != FEA_F32) fea_lin_gemm256(epi, tile, dtype == FEA_PL, g, (unsigned)grid, s);
-    else if (epi == LIN_LSE) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_LSE, true, false>), gr, bl, 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_LSE, false, false>), gr, bl, 0, s, g);
-    } else if (epi == LIN_DZ) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_DZ, true, false>), gr, bl, 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_DZ, false, false>), gr, bl, 0, s, g);
-    } else if (g.ta) {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, true, true>), gr, bl, 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, false, true>), gr, bl, 0, s, g);
-    } else {
-        if (aln) hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, true, false>), gr, bl, 0, s, g);
-        else     hipLaunchKernelGGL((lin_gemm_kernel<LIN_STORE, false, false>), gr, bl, 0, s, g);
-    }
+    else if (epi == LIN_LSE) lg_launch<LIN_LSE, false>(g, aln, (unsigned)grid, s);
+    else if (epi == LIN_DZ)  lg_launch<LIN_DZ, false>(g, aln, (unsigned)grid, s);
+    else if (g.ta)           lg_launch<LIN_STORE, true>(g, aln, (unsigned)grid, s);
+    else                     lg_launch<LIN_STORE, false>(g, aln, (unsigned)grid, s);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
