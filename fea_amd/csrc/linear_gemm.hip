@@ -170,6 +170,18 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             for (int w = 0; w < WN; ++w) sum += red[w * TM + tid].y * __expf(red[w * TM + tid].x - base);
             g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, sum);
         }
+        if (g.keep)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int m = mrow(i);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const int n = ncol(j, e);
+                        if (m < g.M && n < g.ldkeep) *reinterpret_cast<f32x4*>((float*)g.keep + m * g.ldkeep + n) = f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                    }
+            }
     }
 
     if constexpr (EPI == LIN_DZ) {

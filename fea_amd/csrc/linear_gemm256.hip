@@ -312,6 +312,30 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
             g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, p.y * __expf(p.x - base) + q.y * __expf(q.x - base));
         }
+        if (g.keep)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int m = mrow(i), l = wm * LB_W + i * 16 + r16;
+                if constexpr (PL) {
+                    float* const o = (float*)g.keep + m * g.ldkeep;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        if (m < g.M && ncol(j) < g.ldkeep) *reinterpret_cast<f32x4*>(o + ncol(j)) = acc[i][j];
+                } else {
+                    const float mx = fmaxf(red[l].x, red[LB_T + l].x), top = mx == -INFINITY ? 0.f : mx / LIN_RANGE;
+                    uint16_t* const o = (uint16_t*)g.keep + m * g.ldkeep;
+#pragma unroll
+                    for (int p = 0; p < NT / 2; ++p) {
+                        u32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const f32x4& x = acc[i][2 * p + (e >> 1)];
+                            v[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(top - x[2 * (e & 1)] / LIN_RANGE, top - x[2 * (e & 1) + 1] / LIN_RANGE));
+                        }
+                        if (m < g.M && pcol + 32 * p < g.ldkeep) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
+                    }
+                }
+            }
     }
 
     if constexpr (EPI == LIN_DZ) {

@@ -271,6 +271,92 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 
+// dz of the piece from the logits that the forward kept: exp(z - lse), 0 in rows that do not count.  Workgroup: 128 rows x 128 classes, a thread
+// 8 classes of 8 rows.  Bound by memory: reads z, writes dz.
+struct LinDecode {
+    const void* z; long long ldz;         // at the piece's first row and class
+    const float2* part; int ntn, shift;   // bf16: the tiles' maxima, at the first row; class >> shift is the tile
+    const float2* stat; const float* gout; int gstride; const int* count; float t;
+    void* dz; long long lddz; int Npad;
+    float* colsum; long long ldcol;       // fp32, nullable: [tiles of 128 rows][classes] sums of row scale * softmax
+    int n, nv, v0, nct;                   // rows, classes, first class, tiles of 128 columns
+};
+template <bool CODES, bool PL>
+__global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
+    __shared__ float ref[128], none[128], scale[128], red[16][128];
+    const int id = blockIdx.x, tc = id % g.nct, tm = id / g.nct, tid = threadIdx.x;
+    const int r0 = tm * 128, c = tc * 128 + (tid & 15) * 8, y = tid >> 4;
+    const bool in = c < g.Npad;
+    constexpr float L2E = 1.4426950408889634f;
+    u32x4 z[8][CODES ? 1 : 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int q = 0; q < (CODES ? 1 : 2); ++q) {
+            const long long m = r0 + y + 16 * i;
+            z[i][q] = in && m < g.n ? *reinterpret_cast<const u32x4*>((const char*)g.z + (m * g.ldz + c) * (CODES ? 2 : 4) + 16 * q) : u32x4{0, 0, 0, 0};
+        }
+    if (tid < 128) {
+        const int m = r0 + tid;
+        const float2 s = m < g.n ? g.stat[m] : make_float2(0.f, 0.f);
+        const bool dead = s.y == 0.f;
+        // what 0 becomes where the sum is a NaN or an infinity: a NaN, as exp(z - lse) would
+        none[tid] = dead ? 0.f : s.x - s.x;
+        ref[tid] = dead ? CODES ? -INFINITY : INFINITY : CODES ? (g.part[(long long)m * g.ntn + ((g.v0 + tc * 128) >> g.shift)].x - s.x) * L2E : s.x;
+        scale[tid] = dead || !g.colsum ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, s.y, m);
+    }
+    __syncthreads();
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int l = y + 16 * i, m = r0 + l;
+        float v[8];
+        if constexpr (CODES) {
+            const float top = ref[l], nil = none[l];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t u = e & 1 ? z[i][0][e >> 1] >> 16 : z[i][0][e >> 1] & 0xffffu;
+                v[e] = u == 0xffffu ? nil : __builtin_amdgcn_exp2f(fmaf((float)u, -LIN_STEP * L2E, top));
+            }
+        } else {
+            const bool dead = ref[l] == INFINITY && none[l] == 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = dead ? 0.f : __expf(__builtin_bit_cast(f32x4, z[i][e >> 2])[e & 3] - ref[l]);
+                sum[e] += v[e] * scale[l];
+            }
+        }
+        if (!in || m >= g.n) continue;
+        if constexpr (CODES) {
+            __bf16 x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (__bf16)v[e];
+            *reinterpret_cast<u32x4*>((__bf16*)g.dz + m * g.lddz + c) = *reinterpret_cast<const u32x4*>(x);
+        } else if constexpr (PL) {
+            __bf16 x[3][8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) lin_split3(v[e], x[0][e], x[1][e], x[2][e]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>((__bf16*)g.dz + m * g.lddz + (long long)p * g.Npad + c) = *reinterpret_cast<const u32x4*>(x[p]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) *reinterpret_cast<f32x4*>((float*)g.dz + m * g.lddz + c + 4 * q) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        }
+    }
+    if constexpr (!CODES) {
+        if (!g.colsum) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) red[y][(tid & 15) * 8 + e] = sum[e];
+        __syncthreads();
+        if (tid < 128 && tc * 128 + tid < g.nv) {
+            float s = 0.f;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) s += red[q][tid];
+            g.colsum[tm * g.ldcol + tc * 128 + tid] = s;
+        }
+    }
+}
+
 // dz at the selected classes of the piece [v0, v0 + N): softmax - teacher, from the forward's fp32 values.  Entries that name the
 // same class hold the same value.
 template <typename T, bool PL>
@@ -436,7 +522,7 @@ static long long lin_piece() {
     return v >= 1 << 14 && v < 1 << 28 ? v : 1ll << 28;
 }
 struct LinBwd { long long rc; int vc, nrc, nvc, tz; bool planes; LinTile th, tw; };
-static LinBwd lin_bwd_plan(const LinDims& d, int want) {
+static LinBwd lin_bwd_plan(const LinDims& d, int want) {       // want: 1 dh, 2 dw, 4 db, 8 with the kept logits
     LinBwd p;
     const long long piece = lin_piece();
     p.rc = d.rows < 32768 ? d.rows : 32768;
@@ -451,7 +537,7 @@ static LinBwd lin_bwd_plan(const LinDims& d, int want) {
         z = fea_lin_tile(dt, p.rc, p.vc, mul * up(d.D, 64), false);
         h = fea_lin_tile(dt, p.rc, d.D, mul * up(p.vc, 64), true);
         w = fea_lin_tile(dt, p.vc, d.D, mul * up(p.rc, 64), true);
-        return z.time + (want & 1 ? h.time : 0.0) + (want & 2 ? w.time : 0.0);
+        return (want & 8 ? 0.0 : z.time) + (want & 1 ? h.time : 0.0) + (want & 2 ? w.time : 0.0);
     };
     const double t = tiles(d.dtype, 1, tz, p.th, p.tw);
     p.planes = false;
@@ -509,6 +595,16 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     if ((want & 2) && p.nrc > 1) w.accw = c.take<float>(d.V * ld);
     if (want & 4) { const long long t = (p.rc + 127) / 128; w.colsum = c.take<float>(t * up(p.vc, 64)); w.dbpart = c.take<double>((p.rc + LIN_DB_ROWS - 1) / LIN_DB_ROWS * p.vc); }
     return c.at;
+}
+
+// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16) or fp32, then (bf16) the forward's table of the tiles' maxima.  Not for the heads that
+// read no more for recomputing them: few rows (the weight once more) and few classes (nothing).
+static long long lin_keep_ld(const LinDims& d) { return up(d.V, 64); }
+static size_t lin_keep_table(const LinDims& d) { return (size_t)up(d.rows * lin_keep_ld(d) * d.es, 256); }
+extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype) {
+    if (rows <= 64 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
+    const LinDims d = lin_dims(rows, D, V, 1, dtype);
+    return lin_keep_table(d) + (dtype == FEA_BF16 ? (size_t)rows * lin_fwd_plan(d).ntn * sizeof(float2) : 0);
 }
 
 extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads) {
@@ -571,12 +667,13 @@ static int lin_check(const char* who, const LinDims& d, const void* h, long long
 }
 
 static int lin_forward(const char* who, LinDims d, const void* h, long long ldh, const void* w, long long ldw, const float* bias, LinJoin j,
-                       float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
+                       void* keep, float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
     const LinFwd p = lin_fwd_plan(d);
     LinFwdWs b;
     const size_t need = lin_fwd_carve(d, p, (char*)ws, b);
     FEA_CHECK(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, FEA_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, need, ws_bytes);
+    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(d.rows, d.D, d.V, (int)d.dtype) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
     FEA_CHECK(!loss == !count, FEA_E_BADARG, "%s: loss and count go together", who);
     FEA_CHECK(loss || j.loss_rows, FEA_E_BADARG, "%s: nothing to write", who);
 
@@ -615,11 +712,15 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         g.a = pack ? b.hp : hr; g.lda = pack ? f.row(d.D) : ldh; g.b = pack ? b.wp : w; g.ldb = pack ? f.row(d.D) : ldw;
         g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
+        if (keep) {
+            g.keep = (char*)keep + r * lin_keep_ld(d) * d.es; g.ldkeep = lin_keep_ld(d);
+            if (d.dtype == FEA_BF16) g.part = (float2*)((char*)keep + lin_keep_table(d)) + r * p.ntn;
+        }
         if (inner) { g.zsel = b.zsel; g.index = j.index; g.sel = d.K; }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
         else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;
-        q.part = b.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
+        q.part = g.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
         q.zsel = b.zsel + r * d.K; q.index = j.index + r * d.K;
         if (q.tlog) q.tlog = (const char*)j.tlog + r * d.K * (j.tdt == FEA_BF16 ? 2 : 4);
         if (q.stat) q.stat += r;
@@ -641,18 +742,18 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
 }
 
 extern "C" int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
-                                 long long ignore_index, float* stat, float* dsel, float* loss_rows, float* loss, int* count, int mean,
-                                 void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream) {
+                                 long long ignore_index, float* stat, float* dsel, void* keep, float* loss_rows, float* loss, int* count,
+                                 int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream) {
     FEA_CHECK(target, FEA_E_BADARG, "fea_linear_ce_fwd: null target");
     LinJoin j{};
     j.index = target; j.ignore = ignore_index; j.t = j.inv_t = 1.f;
     j.stat = (float2*)stat; j.dsel = dsel; j.loss_rows = loss_rows;
-    return lin_forward("fea_linear_ce_fwd", lin_dims(rows, D, V, 1, dtype), h, ldh, w, ldw, bias, j, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
+    return lin_forward("fea_linear_ce_fwd", lin_dims(rows, D, V, 1, dtype), h, ldh, w, ldw, bias, j, keep, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const void* teacher_logits,
                                  int teacher_dtype, const long long* teacher_index, int K, float temperature, float* stat, float* dsel, float* psel,
-                                 float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                                 void* keep, float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
                                  int dtype, void* stream) {
     FEA_CHECK(teacher_logits && teacher_index, FEA_E_BADARG, "fea_linear_kd_fwd: null teacher");
     FEA_CHECK(teacher_dtype == FEA_F32 || teacher_dtype == FEA_BF16, FEA_E_BADARG, "fea_linear_kd_fwd: teacher dtype %d", teacher_dtype);
@@ -660,12 +761,12 @@ extern "C" int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, lo
     LinJoin j{};
     j.index = teacher_index; j.tlog = teacher_logits; j.tdt = teacher_dtype; j.t = temperature; j.inv_t = 1.f / temperature;
     j.stat = (float2*)stat; j.dsel = dsel; j.psel = psel; j.loss_rows = loss_rows;
-    return lin_forward("fea_linear_kd_fwd", lin_dims(rows, D, V, K, dtype), h, ldh, w, ldw, bias, j, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
+    return lin_forward("fea_linear_kd_fwd", lin_dims(rows, D, V, K, dtype), h, ldh, w, ldw, bias, j, keep, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* index, int K,
-                                   const float* stat, const float* dsel, const float* psel, const int* count, const float* gout, int gout_stride,
-                                   float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                                   const float* stat, const float* dsel, const float* psel, const void* keep, const int* count, const float* gout,
+                                   int gout_stride, float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
                                    int dtype, void* stream) {
     const char* who = "fea_linear_loss_bwd";
     LinDims d = lin_dims(rows, D, V, K, dtype);
@@ -677,7 +778,9 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     FEA_CHECK(((uintptr_t)dh | (uintptr_t)dw) % 16 == 0 && (uintptr_t)db % 4 == 0, FEA_E_BADARG, "%s: misaligned gradient", who);
     FEA_CHECK(K == 1 || !db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
     FEA_CHECK(temperature > 0.f && isfinite(temperature) && isfinite(1.f / temperature), FEA_E_BADARG, "%s: temperature %g", who, (double)temperature);
-    const int want = (dh ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0);
+    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(rows, D, V, dtype) > 0 && !(db && dtype == FEA_BF16)), FEA_E_BADARG,
+              "%s: no logits are kept of these sizes (or, bf16, for a bias gradient), or misaligned", who);
+    const int want = (dh ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0) | (keep ? 8 : 0);
     const LinBwd p = lin_bwd_plan(d, want);
     LinBwdWs b;
     const size_t need = lin_bwd_carve(d, p, want, (char*)ws, b);
@@ -692,6 +795,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     }
     const LinForm f = lin_form(dtype, p.planes);
     const bool pack = p.planes || (dtype == FEA_BF16 && d.odd());
+    const LinFwd kp = lin_fwd_plan(d);              // (its tiles are the kept table's)
     for (int ir = 0; ir < p.nrc; ++ir) {
         const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc;
         const char* hr = (const char*)h + r0 * ldh * d.es;
@@ -704,7 +808,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             // the operands' copies: packed rows, and hidden as dw takes it (gated, times each row's own upstream gradient; gated alone, it is
             // the packed one).  Hidden once for its rows, the weight's piece unless the only piece is there from the rows before
             const bool gated = dw && (!pack || gout_stride);
-            LinCopies js{{lin_copy_of(d, f, hr, ldh, n, pack && iv == 0 ? b.hp : nullptr), lin_copy_of(d, f, wr, ldw, nv, pack && (ir == 0 || p.nvc > 1) ? b.wp : nullptr),
+            LinCopies js{{lin_copy_of(d, f, hr, ldh, n, pack && iv == 0 && (!keep || (dw && !gated)) ? b.hp : nullptr), lin_copy_of(d, f, wr, ldw, nv, pack && (ir == 0 || p.nvc > 1) && (!keep || dh) ? b.wp : nullptr),
                           lin_copy_of(d, f, hr, ldh, n, gated && iv == 0 ? b.hg : nullptr)}};
             js.j[0].stat = js.j[2].stat = st;
             if (gout_stride) { js.j[2].gout = go; js.j[2].t = temperature; }
@@ -718,7 +822,19 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             g.count = count; g.t = temperature;
             g.dz = b.dz; g.lddz = f.row(nv); g.Npad = (int)up(nv, f.pad);
             g.colsum = db ? b.colsum : nullptr; g.ldcol = up(p.vc, 64);
-            LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
+            if (keep) {
+                LinDecode x{};
+                x.z = (const char*)keep + (r0 * lin_keep_ld(d) + v0) * d.es; x.ldz = lin_keep_ld(d);
+                x.part = (const float2*)((const char*)keep + lin_keep_table(d)) + r0 * kp.ntn; x.ntn = kp.ntn; x.shift = kp.tile == 256 ? 8 : 7;
+                x.stat = st; x.gout = go; x.gstride = gout_stride; x.count = count; x.t = temperature;
+                x.dz = b.dz; x.lddz = g.lddz; x.Npad = g.Npad; x.colsum = g.colsum; x.ldcol = g.ldcol;
+                x.n = (int)n; x.nv = nv; x.v0 = (int)v0; x.nct = (nv + 127) / 128;
+                const unsigned blocks = (unsigned)((n + 127) / 128 * x.nct);
+                if (dtype == FEA_BF16) hipLaunchKernelGGL((lin_decode_kernel<true, false>), dim3(blocks), dim3(256), 0, s, x);
+                else if (p.planes)     hipLaunchKernelGGL((lin_decode_kernel<false, true>), dim3(blocks), dim3(256), 0, s, x);
+                else                   hipLaunchKernelGGL((lin_decode_kernel<false, false>), dim3(blocks), dim3(256), 0, s, x);
+                FEA_LAUNCH_CHECK();
+            } else LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
             const unsigned sg = (unsigned)((entries + 255) / 256);
@@ -727,7 +843,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0);
             FEA_LAUNCH_CHECK();
             if (db) {
-                const int tm = p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (int)((n + LIN_DB_ROWS - 1) / LIN_DB_ROWS);
+                const int tm = keep ? 128 : p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (int)((n + LIN_DB_ROWS - 1) / LIN_DB_ROWS);
                 hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(64 * LIN_DB_WAVES), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, LIN_DB_ROWS / tm, (long long)LIN_DB_ROWS * K, b.dbpart);
                 FEA_LAUNCH_CHECK();
                 hipLaunchKernelGGL(lin_dbias_join_kernel, dim3((unsigned)((nv + 255) / 256)), dim3(256), 0, s, (const double*)b.dbpart, chunks, nv, db + v0, ir > 0 ? 1 : 0);

@@ -3,6 +3,8 @@
 `linear_cross_entropy`, `linear_distillation`."""
 from __future__ import annotations
 
+import os
+
 import torch
 
 from . import _lib as L
@@ -129,11 +131,14 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     ix = ix.contiguous()
     b = None if bias is None else bias.detach().contiguous()
     dt = L.dt_code(h.dtype)
-    stat = dsel = psel = count = None
+    stat = dsel = psel = count = keep = None
     if grads:
         stat = torch.empty((rows, 2), dtype=torch.float32, device=dev)
         dsel = torch.empty((rows, k), dtype=torch.float32, device=dev)
         psel = torch.empty((rows, k), dtype=torch.float32, device=dev) if tlog is not None else None
+        n = 0 if grads & 4 and dt == L.BF16 else L.load().fea_linear_loss_keep_bytes(rows, d, v, dt)
+        if 0 < n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33)):
+            keep = torch.empty(n, dtype=torch.uint8, device=dev)
     if reduction == "none":
         loss = torch.empty(index.shape if tlog is None else index.shape[:-1], dtype=torch.float32, device=dev)
         outs = (loss, None, None, 0)
@@ -144,28 +149,28 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     if tlog is None:
-        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, *outs, ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
+        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, keep, *outs, ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
     else:
         tl = tlog.detach().contiguous()
-        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, *outs,
+        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, keep, *outs,
                ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
-    return loss, (ix, stat, dsel, psel, count)
+    return loss, (ix, stat, dsel, psel, keep, count)
 
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
         grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want)
-        loss, (ix, stat, dsel, psel, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
+        loss, (ix, stat, dsel, psel, keep, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
         # the operands themselves are saved, so that autograd sees a change in place between forward and backward
-        ctx.save_for_backward(hidden, weight, bias, ix, stat, dsel, psel, count if reduction == "mean" else None)
+        ctx.save_for_backward(hidden, weight, bias, ix, stat, dsel, psel, keep, count if reduction == "mean" else None)
         ctx.how = (temperature, reduction, dsel.shape[1], grads)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
-        hidden, weight, bias, ix, stat, dsel, psel, count = ctx.saved_tensors
+        hidden, weight, bias, ix, stat, dsel, psel, keep, count = ctx.saved_tensors
         temperature, reduction, k, grads = ctx.how
         # (the autograd engine runs this on the forward's device and stream)
         h, w = _aligned_rows(hidden), _aligned_rows(weight)
@@ -176,9 +181,9 @@ class _LinearLoss(torch.autograd.Function):
         dw = torch.empty(weight.shape, dtype=w.dtype, device=w.device) if grads & 2 else None
         db = torch.empty(v, dtype=torch.float32, device=h.device) if grads & 4 else None
         go = gout.detach().contiguous()
-        n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, grads)
+        n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, grads | (8 if keep is not None else 0))
         ws = torch.empty(n, dtype=torch.uint8, device=h.device)
-        L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, count, go, int(reduction == "none"),
+        L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, keep, count, go, int(reduction == "none"),
                temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr(h.device.index))
         return dh, dw, db, None, None, None, None, None
 

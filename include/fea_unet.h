@@ -356,25 +356,29 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * teacher logit that is NaN or +inf: the row's loss and the gradients it reaches are NaN (nothing is read out of range).
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
- * psel[rows][K] (all nullable).
- *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): recomputes the logits in pieces of the
- *     classes and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
+ * psel[rows][K] (all nullable), and keep (nullable): fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned, for the logits: fp32, or with bf16
+ * operands 16 bits (z below its tile's maximum in steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0).
+ * 0 bytes = none are kept (rows <= 64, few classes with few features: recomputing them reads next to nothing more).
+ *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the
+ *     logits from the forward's keep, or (NULL; with bf16 operands a bias gradient asks for it) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
  *     value (gout_stride 0) or one per row (1); count: divide it by count[0] (mean) or NULL.
  * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are taken at any alignment.
  * fp32: products of a certain size run as six products of bf16 planes (24 bits in three), the others on the fp32 matrix rate.
- * ws: fea_linear_loss_ws_bytes(..., grads) bytes, 256-byte aligned; grads = 0 for the forwards, 1 dh + 2 dw + 4 db for the backward
+ * ws: fea_linear_loss_ws_bytes(..., grads) bytes, 256-byte aligned; grads = 0 for the forwards, 1 dh + 2 dw + 4 db for the
+ * backward, + 8 with keep
  * (0 bytes = sizes that are refused).  Results are the same from run to run. */
 size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);
+size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype);
 int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
-                      long long ignore_index, float* stat, float* dsel, float* loss_rows, float* loss, int* count, int mean,
-                      void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
+                      long long ignore_index, float* stat, float* dsel, void* keep, float* loss_rows, float* loss,
+                      int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
 int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const void* teacher_logits,
                       int teacher_dtype, const long long* teacher_index, int K, float temperature, float* stat, float* dsel, float* psel,
-                      float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                      void* keep, float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
                       int dtype, void* stream);
 int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* index, int K,
-                        const float* stat, const float* dsel, const float* psel, const int* count, const float* gout, int gout_stride,
-                        float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                        const float* stat, const float* dsel, const float* psel, const void* keep, const int* count, const float* gout,
+                        int gout_stride, float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
                         int dtype, void* stream);
 
 /* ---- input pipeline ------------------------------------------------

@@ -3,6 +3,11 @@
 u = torch.finfo(dtype).eps / 2 (a rounding to the storage type), e = 2^-24 (a rounding in 32 bits), with B = max_v sum_d |h_d w_d| + |b_v|:
   a logit is off by dz <= (D + 4) e B / T (D products and sums, bias, scale), an exponential by 3 e more and e |z - lse| for its argument;
   log-sum-exp by the largest of these and the sum's (16 + V / 64) e;  so a loss by 2 of them, a softmax value q by the same relative to q.
+  A teacher's share p = exp(x_k) / sum exp(x_k), x_k = (a_k - max a) / T in 32 bits: a and 1 / T are rounded and multiplied on either side of the
+  difference (4 e A with A = max |a| / T), the difference is (2 e A) and its exponential's argument (2 x 2 e A): 10 e A of itself, the sum the
+  same, so p is off by 20 e A of itself and log p by 20 e A.
+  With bf16 operands the backward takes z from 16 bits that the forward kept (more than 64 rows, no bias gradient): half a step of
+  64 / 65535 off, so q by up to exp(32 / 65535) - 1 < 4.89e-4 of itself (and by the e^-64 that counts as 0).
   dz = g (q - p) is rounded once to the storage type; dh and dw add the products' fp32 sums and one rounding to the storage type.
   Where every row has its own upstream gradient, dw's product takes rnd(q - p) and rnd(g h), two operands rounded once each:
   |rnd(x) rnd(y) - x y| <= (2 u + u^2) |x y|, so its terms |dz| |h| are off by u (1 + u) more than with one upstream gradient
@@ -46,7 +51,7 @@ def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, redu
         p[on, ix[on]] = 1.0
         loss = torch.where(on, lse - z.gather(1, torch.where(on, ix, 0)[:, None])[:, 0], 0.0)
         scale = 1.0
-        spread = torch.zeros(rows, dtype=torch.float64)
+        spread, arg = torch.zeros(rows, dtype=torch.float64), torch.zeros(rows, dtype=torch.float64)
     else:
         ix, a = index.reshape(rows, -1), tlog.double().reshape(rows, -1) / t
         a = a.masked_fill(ix < 0, -torch.inf)
@@ -56,11 +61,12 @@ def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, redu
         zk = z.gather(1, ix.clamp(min=0))
         loss = t * t * torch.where(pk > 0, pk * (torch.log(pk.clamp(min=1e-300)) - zk + lse[:, None]), 0.0).sum(1)
         scale = t * t
+        arg = 20 * E * torch.where(torch.isfinite(a), a, 0.0).abs().amax(1)
         spread = (pk * (torch.log(pk.clamp(min=1e-300)).abs() + zk.abs() + lse.abs()[:, None])).nan_to_num(0.0, 0.0, 0.0).sum(1)
     n = max(1, int(on.sum()))
     big = (hd.abs() @ wd.abs().T + torch.where(bd > -1e30, bd, 0.0).abs()).amax(1)
     dz_log = ((dim + 4) * E * big / t + (16 + v / 64) * E + 3 * E + E * (z - lse[:, None]).masked_fill(z < -1e30, 0).abs().amax(1)).masked_fill(~on, 0.0)
-    loss_off = scale * (2 * dz_log + E * lse.abs().masked_fill(~on, 0.0) + (8 + (0 if tlog is None else index.shape[-1])) * E * (spread + 1))
+    loss_off = scale * (2 * dz_log + E * lse.abs().masked_fill(~on, 0.0) + ((8 + (0 if tlog is None else index.shape[-1])) * E + arg) * (spread + 1))
     loss = torch.where(on, loss, 0.0)
     if reduction == "none":
         g = torch.ones(rows, dtype=torch.float64) if gout is None else gout.double().reshape(-1)
@@ -74,12 +80,13 @@ def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, redu
     q = q.nan_to_num(0.0) if not on.all() else q
     hd = torch.where(on[:, None], hd, 0.0)
     dz = g[:, None] * (q - p)
-    off = g.abs()[:, None] * (q * 2 * dz_log[:, None] + (8 + (0 if tlog is None else index.shape[-1])) * E * (p + q)) + u * dz.abs() + 2 * E * dz.abs()
+    kept = 4.89e-4 if dtype == torch.bfloat16 and rows > 64 and b is None and not (v <= 32 and dim <= 64 and rows >= 4096) else 0.0
+    off = g.abs()[:, None] * (q * kept * (1 + u) + (1.7e-28 if kept else 0.0) + q * 2 * dz_log[:, None] + (8 + (0 if tlog is None else index.shape[-1])) * E * (p + q) + p * arg[:, None]) + u * dz.abs() + 2 * E * dz.abs()
     dh, dw = dz @ wd, dz.T @ hd
     out["hidden"] = (dh, off @ wd.abs() + (v + 8) * E * (dz.abs() @ wd.abs()) + u * dh.abs() + 1e-37)
     own = u * (1 + u) if reduction == "none" else 0.0
     out["weight"] = (dw, off.T @ hd.abs() + own * (dz.abs().T @ hd.abs()) + (rows + 8) * E * (dz.abs().T @ hd.abs()) + u * dw.abs() + 1e-37)
-    offb = g.abs()[:, None] * (q * 2 * dz_log[:, None] + 8 * E * (p + q)) + 4 * E * g.abs()[:, None] * (q + p)
+    offb = g.abs()[:, None] * (q * 2 * dz_log[:, None] + 8 * E * (p + q) + p * arg[:, None]) + 4 * E * g.abs()[:, None] * (q + p)
     out["bias"] = (dz.sum(0), offb.sum(0) + 20 * E * (g.abs()[:, None] * (q + p)).sum(0) + 1e-37)
     return out
 

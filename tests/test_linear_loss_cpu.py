@@ -47,6 +47,16 @@ def test_workspace_sizes():
             sizes = [ws(rows, d, v, k, dt, g) for g in (1, 2, 3, 7)]
             assert sizes[0] <= sizes[2] <= sizes[3] and sizes[1] <= sizes[2], (rows, d, v)
             assert sizes[3] < 24 << 30, (rows, d, v)
+            assert 0 < ws(rows, d, v, k, dt, 11) <= max(sizes[3], ws(rows, d, v, k, dt, 3)) * 2
+
+
+def test_kept_sizes():
+    keep = L.load().fea_linear_loss_keep_bytes
+    assert keep(0, 8, 8, 0) == 0 and keep(64, 64, 1000, 0) == 0 and keep(1 << 20, 64, 6, 1) == 0 and keep(100, 64, 1000, 5) == 0
+    for rows, d, v in ((65, 8, 1), (100, 64, 1000), (8192, 4096, 131072), (1 << 20, 65, 6)):
+        ld = (v + 63) // 64 * 64
+        assert rows * ld * 4 <= keep(rows, d, v, L.F32) < rows * ld * 4 + 256
+        assert rows * ld * 2 < keep(rows, d, v, L.BF16) <= rows * ld * 2 + 256 + rows * ((v + 127) // 128) * 8
 
 
 @pytest.mark.parametrize("top", [0, 4])

@@ -89,6 +89,59 @@ def test_large_tiles(shape, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(65, 8, 64), (130, 33, 257), (258, 200, 333), (514, 640, 1537), (2050, 1096, 2310)])
+@pytest.mark.parametrize("top", [0, 5])
+@pytest.mark.parametrize("keep", [0, 1 << 30])
+def test_logits_kept_or_recomputed(shape, dtype, top, keep, monkeypatch):
+    """A head without bias keeps its logits for the backward, within a limit; recomputed ones hold the same bounds."""
+    monkeypatch.setenv("FEA_AMD_LINEAR_KEEP", str(keep))
+    c = O.case(*shape, dtype, seed=sum(shape) + 1, top=top, ignored=0.2, short=0.3)
+    _compare(_run(*c), O.evaluate(*c))
+    x = [_leaf(t) for t in c[:2]]
+    loss = F.linear_distillation(*x, c[4].to(DEV), c[3].to(DEV)) if top else F.linear_cross_entropy(*x, c[3].to(DEV))
+    held = [t.numel() for t in loss.grad_fn.saved_tensors if t is not None and t.dtype == torch.uint8]
+    assert [n >= shape[0] * shape[2] * c[0].element_size() for n in held] == [True] * (keep > 0)
+    want = torch.autograd.grad(loss, x, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, x), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1.0, 0.02])
+def test_logits_far_apart(dtype, temperature):
+    """Logits that lie hundreds below their tile's largest count as a share of 0, others down to e^-64 as they are."""
+    h, w, _, i, a = O.case(200, 64, 700, dtype, seed=50, top=4, ignored=0.1, short=0.2)
+    h = (h.float() * torch.logspace(0, 1.5, 200)[:, None]).to(dtype)
+    _compare(_run(h, w, None, i, a, temperature=temperature), O.evaluate(h, w, None, i, a, temperature=temperature))
+
+
+def test_far_kept_logits(monkeypatch):
+    """More than 2^31 kept logits, from two chunks of the rows, against recomputed ones.  Either side's shares of the softmax are off by 2^-8 and
+    4.9e-4 of themselves at most; a row's shares and its label's add up to 2 at most, and the fp32 sums over a million classes to 1e-3 of that."""
+    g = torch.Generator().manual_seed(51)
+    rows, v, d = 2400, 1000003, 16
+    h, w = torch.randn(rows, d, generator=g).bfloat16(), torch.randn(v, d, generator=g).bfloat16()
+    t = torch.randint(0, v, (rows,), generator=g)
+    assert rows * v > 1 << 31
+    kept = _run(h, w, None, t, reduction="sum")
+    monkeypatch.setenv("FEA_AMD_LINEAR_KEEP", "0")
+    again = _run(h, w, None, t, reduction="sum")
+    assert torch.equal(kept["loss"], again["loss"])
+    top = float(w.float().abs().max())
+    off = (kept["hidden"].float() - again["hidden"].float()).abs()
+    assert bool((off <= 2 * (2 * 2.0 ** -8 + 4.9e-4 + 1e-3) * top + 2 * 2.0 ** -8 * again["hidden"].float().abs()).all())
+    # a class's gradient: its shares of all rows, at most 2 |h| of its labels' rows in sum; classes that no label names are compared to their own size
+    free = torch.ones(v, dtype=torch.bool)
+    free[t] = False
+    a, b = kept["weight"].float().cpu()[free], again["weight"].float().cpu()[free]
+    q = torch.zeros(v, dtype=torch.float64)
+    for k in range(0, rows, 240):
+        z = h[k:k + 240].float() @ w.float().T
+        q += torch.softmax(z, 1).double().sum(0)
+    bound = q[free].float()[:, None] * float(h.float().abs().max()) * (2 * 2.0 ** -8 + 4.9e-4 + 1e-3) + 2 * 2.0 ** -8 * b.abs()
+    assert bool(((a - b).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [9, 4100])
 def test_nothing_counts(dtype, rows):
     h, w, b, t = O.case(rows, 16, 20, dtype, bias=True)
@@ -399,11 +452,11 @@ def test_workspace_and_operands_are_checked():
     ws = torch.empty(n, dtype=torch.uint8, device=DEV)
     out = torch.empty(16, device=DEV)
 
-    def fwd(h=h, ldh=32, ws=ws, n=n, rows=16, d=32, v=40, dt=L.F32):
-        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
+    def fwd(h=h, ldh=32, ws=ws, n=n, rows=16, d=32, v=40, dt=L.F32, keep=None):
+        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, keep, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
     fwd()
     for bad in ({"n": n - 1}, {"ws": None}, {"ldh": 31}, {"ldh": 33}, {"h": None}, {"dt": 7}, {"rows": 0}, {"v": 0}, {"d": 0}, {"h": h.data_ptr() + 4},
-                {"ws": ws.data_ptr() + 16}, {"d": 1 << 17, "ldh": 1 << 17}):
+                {"ws": ws.data_ptr() + 16}, {"d": 1 << 17, "ldh": 1 << 17}, {"keep": ws}):
         with pytest.raises(L.FeaError):
             fwd(**bad)
     torch.cuda.synchronize()
