@@ -1,15 +1,22 @@
-// The product of the many-class loss heads for large bf16 operands: 256 x 256 tiles, with the epilogues of linear_gemm.hip.
+// The products of the many-class loss heads on the bf16 matrix rate, 256 x 256 and 128 x 128 tiles, with the epilogues of linear_gemm.hip.
 //
 // A tile of T x T takes T T / (2 T) = T / 2 multiply-adds per operand element it reads: at 256 a CU at full matrix rate asks for
 // 32 B per cycle from L2 (128: 64 B, twice what L2 gives) and for 64 KB of LDS reads per 32-channel step of 1,024 cycles.  Four waves of
 // 128 x 128 read each operand twice (8 fragments of each per step and wave: half the LDS rate); eight waves of 128 x 64 would read
 // 96 KB, with the fill the whole LDS rate.  So: one workgroup of 4 waves per CU, one wave per SIMD, 8 x 8 accumulators of
-// v_mfma_f32_16x16x32_bf16 in the 256 accumulation registers, the rest in the other 256.
+// v_mfma_f32_16x16x32_bf16 in the 256 accumulation registers, fragments and addresses in the other 256.
 //
-// Reduction in chunks of 64 channels (whole 128-byte lines), two LDS stages.  In the first half of chunk c every fourth MFMA is
-// followed by one fragment read (second half of c), one LDS write of chunk c + 1 from the registers and one load of chunk c + 2 (c + 3 in
-// the 128 tile, which has registers for two chunks) into the registers just freed; one barrier; in the second half the fragments of chunk c + 1 are read.  Loads are buffer loads with
-// every bound in the lane's offset, so rows, classes and channels behind the end arrive as zeros without a branch.
+// 256 tile: chunks of 64 channels (whole 128-byte lines) go from memory to LDS without a register in between, a wave's 1,024 bytes per load, in
+// a ring of five operand chunks of 32 KB (all of the CU's 160 KB): 16 loads per chunk, one per 8 MFMA, 1 to 1.5 chunks ahead; one
+// barrier per chunk.  128 tile (two workgroups per CU): through registers, two chunks on the way, two LDS stages.
+// Loads are buffer loads with every bound in the descriptor or the lane's offset: rows, classes and channels behind the end arrive as zeros
+// without a branch.
+//
+// Measured on 4,096 x 4,096 x 131,072 (a third of a training step each): h w^T with softmax sums and kept logits 3.6 ms (1.21 PFLOP/s;
+// 3.36 without keeping), dz w 3.25 ms (1.35), dz^T h 3.9 ms (1.13); a library's plain products 2.98, 3.16 and 3.85 ms.  Bound by power:
+// at 60 % of the matrix pipes' cycles the clock is down to 1.9 GHz, and a loop of nothing but these MFMA on normally distributed
+// operands reaches 2.1 PFLOP/s (32 x 32 x 16 MFMA: 1.85), so what helps is less traffic and an even one: through registers and with LDS
+// writes the step took 4 % longer, with the same direct loads in bursts 5 %.
 #include "linear_loss.h"
 
 
@@ -30,9 +37,10 @@ __device__ __forceinline__ uint32_t lb_pack(float a, float b) {
 template <int EPI, bool PL, int NT, bool TA, bool TB>
 __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const LinGemm g) {
     constexpr int LB_T = 32 * NT, LB_W = 16 * NT, NL = 2 * NT;
-    constexpr int RB = 2 * LB_T + 32, TOP = 64 * RB + 8 * 128;                       // a row along the reduction, an operand of them
+    constexpr bool DL = NT == 8;                          // loads go to LDS by themselves
+    constexpr int RB = DL ? 2 * LB_T : 2 * LB_T + 32, TOP = DL ? 64 * RB : 64 * RB + 8 * 128;     // a row along the reduction, an operand of them
     constexpr int LB_OP = TA ? TOP : LB_T * 128, LB_STAGE = LB_OP + (TB ? TOP : LB_T * 128);
-    __shared__ __attribute__((aligned(128))) char smem[2 * LB_STAGE];
+    __shared__ __attribute__((aligned(128))) char smem[DL ? 5 * LB_OP : 2 * LB_STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave & 1, wn = wave >> 1, r16 = lane & 15, q16 = lane >> 4;
     // tiles in groups of 8 row tiles, walked along the classes: the 32 tiles that an XCD has in flight are 8 x 4
@@ -46,55 +54,79 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     const int nc = (K + 63) >> 6;
 
     auto rsrc = [&](const __bf16* p, long long ld, int rows, int cols) {       // rows x cols of a matrix; 0 rows: nothing is read
-        return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, rows > 0 ? (int)(((rows - 1) * ld + cols) * 2) : 0, 0x00020000);
+        const int bytes = rows > 0 ? (int)(((rows - 1) * ld + cols) * 2) : 0;
+        if constexpr (DL) return u32x4{(uint32_t)(uintptr_t)p, (uint32_t)((uintptr_t)p >> 32) & 0xffffu, (uint32_t)bytes, 0x00020000u};
+        else return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00020000);
     };
-    const int kb = PL ? 0 : k0, kl = PL ? 3 * g.Kp : K;      // first channel and length of a row along the reduction
+    const int kf = PL ? 0 : k0, kl = PL ? 3 * g.Kp : K;      // first channel and length of a row along the reduction
     const __bf16 *const a = (const __bf16*)g.a, *const b = (const __bf16*)g.b;
-    __amdgpu_buffer_rsrc_t rsa = rsrc(a + m0 * g.lda + kb, g.lda, K ? min(LB_T, g.M - m0) : 0, kl);
-    __amdgpu_buffer_rsrc_t rsb = rsrc(b + n0 * g.ldb + kb, g.ldb, K ? min(LB_T, g.N - n0) : 0, kl);
+    auto rsa = rsrc(a + m0 * g.lda + kf, g.lda, K ? min(LB_T, g.M - m0) : 0, kl);
+    auto rsb = rsrc(b + n0 * g.ldb + kf, g.ldb, K ? min(LB_T, g.N - n0) : 0, kl);
 
     // Staging, rows along the tile: thread -> LDS rows r + 32 i, 16-byte chunk c.  Which class lies in which LDS row is chosen for the
     // epilogue: the lane that ends up with column r16 of the products holds, over tiles 2 p and 2 p + 1, 8 consecutive classes.
-    const int r = tid >> 3, c = tid & 7;
+    const int r = tid >> 3, c = DL ? (tid & 7) ^ lb_swz(r) : tid & 7;
     const int rb = ((r >> 4) & 1) * 4 + ((r >> 2) & 3) * 8 + (r & 3);
     const int wofs = r * 128 + ((c ^ lb_swz(r)) << 4);
-    // Rows along the reduction: thread -> rows tr + RPP i of the chunk's 64, 16-byte piece tc.  A row is 32 bytes longer than its data and every
-    // 8 rows have 128 more: the 8 rows x 32 bytes that half a wave takes in one transposing read lie in different banks, and
-    // tiles, steps and loads are constant offsets.
+    // Rows along the reduction: thread -> rows tr + RPP i of the chunk's 64, 16-byte piece tc.  The 8 rows x 32 bytes that half a wave takes in
+    // one transposing read have to lie in different banks.  256 tile: the 32-byte pieces of a row are XORed by fr of the row (its bits 0, 1
+    // and 3), on the way in by which piece a lane loads (odd i: the row's bit 3 is set).  128 tile: a row is 32 bytes longer than its
+    // data and every 8 rows have 128 more, so that tiles, steps and loads are constant offsets.
     constexpr int CPR = LB_T / 8, RPP = 256 / CPR;
-    const int tr = tid / CPR, tc = tid % CPR;
+    const int tr = tid / CPR, tc = DL ? (tid % CPR) ^ ((tr & 3) << 1) : tid % CPR;
     const int tofs = tr * RB + (tr >> 3) * 128 + tc * 16;
-    const unsigned va = TA ? (unsigned)(tr * (int)g.lda * 2 + tc * 16) : (unsigned)(r * (int)g.lda * 2 + c * 16);
-    const unsigned vb = TB ? (unsigned)(tr * (int)g.ldb * 2 + tc * 16) : (unsigned)(rb * (int)g.ldb * 2 + c * 16);
+    const unsigned va = TA ? (unsigned)(tr * (int)g.lda * 2 + tc * 16) : (unsigned)(r * (int)g.lda * 2 + c * 16), va1 = DL && TA ? va + ((tc ^ 8) - tc) * 16 : va;
+    const unsigned vb = TB ? (unsigned)(tr * (int)g.ldb * 2 + tc * 16) : (unsigned)(rb * (int)g.ldb * 2 + c * 16), vb1 = DL && TB ? vb + ((tc ^ 8) - tc) * 16 : vb;
     const unsigned sa = 2 * (TA ? RPP : 32) * (unsigned)g.lda, sb = 2 * (TB ? RPP : 32) * (unsigned)g.ldb;      // bytes from load i to i + 1
-    constexpr int SETS = NT == 8 ? 1 : 2;      // chunks on the way in registers (two where there is room: a chunk is then shorter than a load)
-    u32x4 st[SETS][NL];
+    constexpr int SETS = 2;           // 128 tile: chunks on the way in registers
+    u32x4 st[DL ? 1 : SETS][DL ? 1 : NL];
     // the XCDs start their reduction an eighth apart (it ends where it began): in step, every workgroup of the chip would ask for the
     // same columns of its rows at a time.  Within an XCD all are in step: they share operands in its L2.
-    int at = (int)(blockIdx.x & 7) * nc >> 3;
-    int pair = PL ? (k0 + at * 64) / g.Kp : 0, pk = PL ? k0 + at * 64 - pair * g.Kp : 0;       // FEA_PL: the pair of planes and the channel that are loaded next
-    unsigned ka = 0, kc = 0;
-    bool kin = false;
+    // (FEA_PL: a pair of planes and a channel)
+    struct Pos { int at, pair, pk; };
+    const int start = (int)(blockIdx.x & 7) * nc >> 3;
+    Pos pa{start, PL ? (k0 + start * 64) / g.Kp : 0, 0};
+    if constexpr (PL) pa.pk = k0 + start * 64 - pa.pair * g.Kp;
+    Pos pb = pa;
+    unsigned ka = 0, kb = 0;
+    bool ina = false, inb = false;
     const int ca = min(LB_T, (g.M - m0 + 7) & ~7), cb = min(LB_T, (g.N - n0 + 7) & ~7);        // (whole 16-byte pieces: rows are padded)
-    auto advance = [&](int ch) {      // where the chunk that is loaded ch-th lies in either operand
-        const bool live = ch < nc;
-        kin = live && at * 64 + c * 8 < K;
-        const int first = PL ? pk : k0 + at * 64, rows = live ? min(64, g.Kr - first) : 0;
-        if constexpr (TA) rsa = rsrc(a + first * g.lda + m0 + (PL ? lin_plane_a(pair) * g.Pa : 0), g.lda, rows, ca);
-        else ka = PL ? 2u * (unsigned)(lin_plane_a(pair) * g.Kp + pk) : at * 128;
-        if constexpr (TB) rsb = rsrc(b + first * g.ldb + n0 + (PL ? lin_plane_b(pair) * g.Pb : 0), g.ldb, rows, cb);
-        else kc = PL ? 2u * (unsigned)(lin_plane_b(pair) * g.Kp + pk) : at * 128;
-        if (++at == nc) {
-            at = 0;
-            if constexpr (PL) { pair = k0 / g.Kp; pk = k0 - pair * g.Kp; }
+    auto next = [&](Pos& p) {
+        if (++p.at == nc) {
+            p.at = 0;
+            if constexpr (PL) { p.pair = k0 / g.Kp; p.pk = k0 - p.pair * g.Kp; }
         } else if constexpr (PL) {
-            pk += 64;
-            if (pk >= g.Kp) { pk = 0; ++pair; }
+            p.pk += 64;
+            if (p.pk >= g.Kp) { p.pk = 0; ++p.pair; }
         }
     };
+    auto first = [&](const Pos& p) { return PL ? p.pk : k0 + p.at * 64; };
+    auto advance_a = [&](int ch) {      // where A's chunk that is loaded ch-th lies (behind the last: nowhere, zeros)
+        const bool live = ch < nc;
+        ina = live && pa.at * 64 + c * 8 < K;
+        if constexpr (TA) rsa = rsrc(a + first(pa) * g.lda + m0 + (PL ? lin_plane_a(pa.pair) * g.Pa : 0), g.lda, live ? min(64, g.Kr - first(pa)) : 0, ca);
+        else ka = PL ? 2u * (unsigned)(lin_plane_a(pa.pair) * g.Kp + pa.pk) : pa.at * 128;
+        next(pa);
+    };
+    auto advance_b = [&](int ch) {
+        const bool live = ch < nc;
+        inb = live && pb.at * 64 + c * 8 < K;
+        if constexpr (TB) rsb = rsrc(b + first(pb) * g.ldb + n0 + (PL ? lin_plane_b(pb.pair) * g.Pb : 0), g.ldb, live ? min(64, g.Kr - first(pb)) : 0, cb);
+        else kb = PL ? 2u * (unsigned)(lin_plane_b(pb.pair) * g.Kp + pb.pk) : pb.at * 128;
+        next(pb);
+    };
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 1024;
+    auto address = [&](int i) {        // of the lane's 16 bytes of load i (A's, then B's); 0x7fffff00: behind any end
+        const int q = i % NT;
+        return i < NT ? TA || ina ? (q & 1 ? va1 : va) + ka + q * sa : 0x7fffff00u : TB || inb ? (q & 1 ? vb1 : vb) + kb + q * sb : 0x7fffff00u;
+    };
+    auto dload = [&](int slot, int i) {     // a wave's 1,024 bytes straight to LDS: nothing lands in a register, and `landed` waits
+        const uint32_t m = lds + slot * LB_OP + i % NT * 4096;
+        if (i < NT) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m), "v"(address(i)), "s"(rsa) : "memory");
+        else        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m), "v"(address(i)), "s"(rsb) : "memory");
+    };
     auto gload = [&](int u, int i) {
-        if (i < NT) st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsa, TA || kin ? va + ka + i * sa : 0x7fffff00u, 0, 0));
-        else        st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsb, TB || kin ? vb + kc + (i - NT) * sb : 0x7fffff00u, 0, 0));
+        if constexpr (!DL) st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(i < NT ? rsa : rsb, address(i), 0, 0));
     };
     auto lput = [&](int u, int stage, int i) {
         const int ofs = (i < NT ? TA : TB) ? tofs + (i % NT) * (RPP * RB + RPP / 8 * 128) : wofs + (i % NT) * 32 * 128;
@@ -103,39 +135,94 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
 
     // fragments: lane -> row r16 of tile i, channels 8 q16 .. + 7 of the 32 of step ks
     const int fofs0 = r16 * 128 + ((q16 ^ lb_swz(r16)) << 4), fofs1 = fofs0 ^ 64;
-    const int fofst = (8 * q16 + (r16 >> 2)) * RB + q16 * 128 + (r16 & 3) * 8;       // 16 lanes: 4 rows of 16 columns
+    const int fofst = (8 * q16 + (r16 >> 2)) * RB + (DL ? 0 : q16 * 128) + (r16 & 3) * 8, fr = (r16 >> 2) | (q16 & 1) << 2;      // 16 lanes: 4 rows of 16 columns
     u32x4 A[2][NT], B[2][NT];
     auto frag = [&](const char* op, int w, int ks, int i, bool t) {
         if (!t) return *reinterpret_cast<const u32x4*>(op + (ks ? fofs1 : fofs0) + (w * LB_W + i * 16) * 128);
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4_t;
-        const char* p = op + fofst + w * (2 * LB_W) + i * 32 + ks * (32 * RB + 4 * 128);
+        const char* p = op + fofst + w * (2 * LB_W) + (DL ? (i ^ fr) * 32 + ks * (32 * RB) : i * 32 + ks * (32 * RB + 4 * 128));
         const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)p));
         const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p + 4 * RB)));
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
-    auto frd = [&](int stage, int ks, int i) {
-        if (i < NT) A[ks][i] = frag(smem + stage * LB_STAGE, wm, ks, i, TA);
-        else        B[ks][i - NT] = frag(smem + stage * LB_STAGE + LB_OP, wn, ks, i - NT, TB);
+    auto fread = [&](const char* sa_, const char* sb_, int ks, int i) {
+        if (i < NT) A[ks][i] = frag(sa_, wm, ks, i, TA);
+        else        B[ks][i - NT] = frag(sb_, wn, ks, i - NT, TB);
     };
+    auto frd = [&](int stage, int ks, int i) { fread(smem + stage * LB_STAGE, smem + stage * LB_STAGE + LB_OP, ks, i); };
     f32x4 acc[NT][NT];                // [label tile][class tile]
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto mma = [&](int ks, int i, int j) {
-        // (as inline asm where fragments come in halves: there the compiler moves accumulators between the register files in every step)
-        if constexpr (NT == 8 && (TA || TB)) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(B[ks][j]), "v"(A[ks][i]));
+        // (as inline asm where all 256 are taken: the compiler would move accumulators between the register files in every step)
+        if constexpr (DL) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(B[ks][j]), "v"(A[ks][i]));
         else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
     };
 
-    advance(0);
+    if constexpr (DL) {
+        // A ring of five operand chunks: A(c) in slot 2 c mod 5, B(c) in 2 c + 1 mod 5.  Half-way through chunk c its fragments are all in registers, so
+        // B(c + 2) goes where A(c) was, and in the next half A(c + 3) where B(c) was.  Loads are spread evenly (one per 8 MFMA): the
+        // same loads in bursts of the second half cost 3 to 5 % of the product.
+        auto landed = [&](bool all) {       // everything but A's 8 loads of the chunk after the next is there, and read by nobody any more
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            if (all) __builtin_amdgcn_s_waitcnt(0x0070);       // vmcnt(0) lgkmcnt(0)
+            else     __builtin_amdgcn_s_waitcnt(0x0078);       // vmcnt(8) lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        int a0 = 0, b0 = 1, a1 = 2, b1 = 3, a2 = 4;
+        advance_a(0); advance_b(0);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) dload(i < NT ? a0 : b0, i);
+        landed(true);
+        advance_a(1); advance_b(1);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) dload(i < NT ? a1 : b1, i);
+        advance_a(2);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) fread(smem + a0 * LB_OP, smem + b0 * LB_OP, 0, i < NT ? i + NT : i - NT);
+        for (int ch = 0; ch < nc; ++ch) {
+            // in slots of half a row of MFMAs.  First half: the second half's fragments, and A(ch + 2)
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+#pragma unroll
+                for (int j = 0; j < NT / 2; ++j) mma(0, q / 2, (q & 1) * (NT / 2) + j);
+                if (q < NT) { fread(smem + a0 * LB_OP, smem + b0 * LB_OP, 1, NT + q); fread(smem + a0 * LB_OP, smem + b0 * LB_OP, 1, q); }
+                if (q & 1) dload(a2, q / 2);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance_b(ch + 2);
+            landed(false);
+            // second half: the first fragments of chunk ch + 1 (done early: the loop's head waits for all), and B(ch + 2)
+#pragma unroll
+            for (int q = 0; q < NL; ++q) {
+#pragma unroll
+                for (int j = 0; j < NT / 2; ++j) mma(1, q / 2, (q & 1) * (NT / 2) + j);
+                if (!(q & 1)) dload(a0, NT + q / 2);
+                if (q < NT + 4) fread(smem + a1 * LB_OP, smem + b1 * LB_OP, 0, q < NT ? q + NT : q - NT);
+                if (q >= NT && q < NT + 4) fread(smem + a1 * LB_OP, smem + b1 * LB_OP, 0, q - NT + 4);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            advance_a(ch + 3);
+            const int fa = a0, fb = b0;
+            a0 = a1; b0 = b1; a1 = a2; b1 = fa; a2 = fb;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // (the loads behind the last chunk, zeros, are in LDS too)
+        // (the compiler does not know that inline asm has written the accumulators that are read from here on)
+        asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");
+    } else {
+    advance_a(0); advance_b(0);
 #pragma unroll
     for (int i = 0; i < NL; ++i) gload(0, i);
 #pragma unroll
     for (int i = 0; i < NL; ++i) lput(0, 0, i);
 #pragma unroll
     for (int u = 0; u < SETS; ++u) {
-        advance(1 + u);
+        advance_a(1 + u); advance_b(1 + u);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {        // (in the loop's order: its waits are counted for both ways in)
             gload((1 + u) % SETS, i);
@@ -158,7 +245,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
         };
-        advance(ch + 1 + SETS);
+        advance_a(ch + 1 + SETS); advance_b(ch + 1 + SETS);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (TA || TB) {
             // slots: half a row of MFMAs, then a fragment of the second half (in every second slot one of this half, three tiles ahead), an
@@ -213,15 +300,10 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             }
         }
     };
-    if constexpr (SETS == 1) {
-        for (int ch = 0; ch < nc; ++ch) step(ch, ch & 1, 0);
-        // (the compiler does not know that inline asm has written the accumulators that are read from here on)
-        if constexpr (TA || TB) asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");
-    } else {
-        for (int ch = 0; ch < nc; ch += 2) {
-            step(ch, 0, 1);
-            if (ch + 1 < nc) step(ch + 1, 1, 0);
-        }
+    for (int ch = 0; ch < nc; ch += 2) {
+        step(ch, 0, 1);
+        if (ch + 1 < nc) step(ch + 1, 1, 0);
+    }
     }
     __syncthreads();
 
@@ -273,69 +355,84 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                 }
             }
         }
-    } else {
-        // z in place; classes behind the last are -inf
-        const bool edge = n0 + LB_T > g.N;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = ncol(j) + e;
-                const float b = g.bias && n < g.N ? g.bias[n] : 0.f;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) acc[i][j][e] = edge && n >= g.N ? -INFINITY : (acc[i][j][e] + b) * g.inv_t;
-            }
     }
-
-    if constexpr (EPI == LIN_LSE) {
-        float2* const red = reinterpret_cast<float2*>(smem);       // [wn][256 labels]
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < NT; ++j) mx = fmaxf(fmaxf(mx, fmaxf(acc[i][j][0], acc[i][j][1])), fmaxf(acc[i][j][2], acc[i][j][3]));
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float sum = 0.f;
+    // z of a lane's 4 classes of tile j, label tile i; classes behind the last are -inf (whatever 0 times the label's row gave)
+    f32x4 bias[EPI == LIN_STORE ? 1 : NT];
+    if constexpr (EPI != LIN_STORE) {
+        if (n0 + LB_T > g.N)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum += __expf(acc[i][j][e] - base);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (q16 == 0) red[wn * LB_T + wm * LB_W + i * 16 + r16] = make_float2(mx, sum);
-        }
-        __syncthreads();
-        if (tid < LB_T && m0 + tid < g.M) {
-            const float2 p = red[tid], q = red[LB_T + tid];
-            const float mx = fmaxf(p.x, q.x), base = mx == -INFINITY ? 0.f : mx;
-            g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, p.y * __expf(p.x - base) + q.y * __expf(q.x - base));
-        }
-        if (g.keep)
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int m = mrow(i), l = wm * LB_W + i * 16 + r16;
+                    for (int i = 0; i < NT; ++i) acc[i][j][e] = ncol(j) + e < g.N ? acc[i][j][e] : 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[j][e] = ncol(j) + e >= g.N ? -INFINITY : g.bias ? g.bias[ncol(j) + e] * g.inv_t : 0.f;
+    }
+    auto logits = [&](int i, int j) {
+        f32x4 z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = fmaf(acc[i][j][e], g.inv_t, bias[j][e]);
+        return z;
+    };
+
+    if constexpr (EPI == LIN_LSE) {
+        // every lane's own maximum and sum of a label's 4 NT classes, joined in LDS: nothing goes across lanes on the way, and a label's kept
+        // logits leave while the next one's exponentials run
+        float2* const red = reinterpret_cast<float2*>(smem);       // [wn, q16][labels of the tile]
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int m = mrow(i);
+            f32x4 z[NT];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                z[j] = logits(i, j);
+                mx = fmaxf(fmaxf(mx, fmaxf(z[j][0], z[j][1])), fmaxf(z[j][2], z[j][3]));
+            }
+            const float base = mx == -INFINITY ? 0.f : mx;         // every class masked by a -inf bias: the sum is 0, not NaN
+            if (g.keep && m < g.M) {
                 if constexpr (PL) {
                     float* const o = (float*)g.keep + m * g.ldkeep;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        if (m < g.M && ncol(j) < g.ldkeep) *reinterpret_cast<f32x4*>(o + ncol(j)) = acc[i][j];
+                    for (int j = 0; j < NT; ++j) if (ncol(j) < g.ldkeep) *reinterpret_cast<f32x4*>(o + ncol(j)) = z[j];
                 } else {
-                    const float mx = fmaxf(red[l].x, red[LB_T + l].x), top = mx == -INFINITY ? 0.f : mx / LIN_RANGE;
                     uint16_t* const o = (uint16_t*)g.keep + m * g.ldkeep;
+                    const float t = base / LIN_RANGE;
+                    g.top[m * g.ldtop + (n0 / LB_W + wn) * 4 + q16] = base;
 #pragma unroll
                     for (int p = 0; p < NT / 2; ++p) {
                         u32x4 v;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const f32x4& x = acc[i][2 * p + (e >> 1)];
-                            v[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(top - x[2 * (e & 1)] / LIN_RANGE, top - x[2 * (e & 1) + 1] / LIN_RANGE));
+                            const float x = z[2 * p + (e >> 1)][2 * (e & 1)], y = z[2 * p + (e >> 1)][2 * (e & 1) + 1];
+                            v[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(t - x / LIN_RANGE, t - y / LIN_RANGE));
                         }
-                        if (m < g.M && pcol + 32 * p < g.ldkeep) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
+                        if (pcol + 32 * p < g.ldkeep) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
                     }
                 }
             }
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += __expf(z[j][e] - base);
+            red[(wn * 4 + q16) * LB_T + wm * LB_W + i * 16 + r16] = make_float2(mx, sum);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        if (tid < LB_T && m0 + tid < g.M) {
+            float2 p[8];
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) { p[w] = red[w * LB_T + tid]; mx = fmaxf(mx, p[w].x); }
+            const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) sum += p[w].y * __expf(p[w].x - base);
+            g.part[(long long)(m0 + tid) * g.ntn + tn] = make_float2(mx, sum);
+        }
     }
 
     if constexpr (EPI == LIN_DZ) {
@@ -347,12 +444,14 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             const bool dead = s2.y == 0.f;
             sc[i] = dead || !g.colsum ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, s2.y, m);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j) {
+                const f32x4 z = logits(i, j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float q = __expf(acc[i][j][e] - s2.x);
+                    const float q = __expf(z[e] - s2.x);
                     acc[i][j][e] = dead || (n0 + LB_T > g.N && ncol(j) + e >= g.N) ? 0.f : q;
                 }
+            }
         }
         if (g.colsum) {
             float* const red = reinterpret_cast<float*>(smem);     // [wm][256 classes]

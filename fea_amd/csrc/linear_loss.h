@@ -17,7 +17,8 @@ __device__ __forceinline__ int lin_plane_a(int pair) { return (0x001021 >> (4 * 
 __device__ __forceinline__ int lin_plane_b(int pair) { return (0x010201 >> (4 * pair)) & 15; }
 
 // Kept logits of a bf16 head: 16 bits each.  exp(z - lse) goes to bf16 next, which rounds it by up to 2^-8 of itself; a fixed-point z is off by
-// half a step, 4.9e-4 of exp(z - lse), whatever z is.  Entries e^-64 times the largest of their tile and less count as 0.
+// half a step, 4.9e-4 of exp(z - lse), whatever z is.  Entries e^-64 times the largest of their
+// group and less count as 0.
 #define LIN_RANGE 64.f
 #define LIN_STEP (LIN_RANGE / 65535.f)
 
@@ -32,7 +33,8 @@ struct LinGemm {
     float inv_t;
     float2* part;                     // LIN_LSE: [M][ntn] (max, sum of exp(z - max)) of one column tile
     void* keep; long long ldkeep;     // LIN_LSE, nullable: the logits kept for the backward, rows of ldkeep (classes rounded up to 64): fp32 z, or (bf16) how far
-                                      // z lies below part's maximum of its tile, in steps of LIN_STEP (65535: LIN_RANGE and more, and classes behind the last)
+                                      // z lies below the largest of its group, in steps of LIN_STEP (65535: LIN_RANGE and more, and classes behind the last)
+    float* top; long long ldtop;      // with bf16 keep: the groups' largest, rows of ldtop; a group: every fourth 8 classes of half a tile's (what a lane holds of a row)
     const float2* stat;               // LIN_DZ: [M] (log sum exp, gate)
     const float* gout; int gstride;   // upstream gradient, one value (stride 0) or one per row
     const int* count;                 // rows that count (mean), nullable

@@ -275,7 +275,7 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 // 8 classes of 8 rows.  Bound by memory: reads z, writes dz.
 struct LinDecode {
     const void* z; long long ldz;         // at the piece's first row and class
-    const float2* part; int ntn, shift;   // bf16: the tiles' maxima, at the first row; class >> shift is the tile
+    const float* top; long long ldtop; int shift;   // bf16: the groups' largest at the first row; a class's: 4 (class >> shift) + (class >> 3 & 3)
     const float2* stat; const float* gout; int gstride; const int* count; float t;
     void* dz; long long lddz; int Npad;
     float* colsum; long long ldcol;       // fp32, nullable: [tiles of 128 rows][classes] sums of row scale * softmax
@@ -289,12 +289,14 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
     const bool in = c < g.Npad;
     constexpr float L2E = 1.4426950408889634f;
     u32x4 z[8][CODES ? 1 : 2];
+    float top[CODES ? 8 : 1];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int q = 0; q < (CODES ? 1 : 2); ++q) {
             const long long m = r0 + y + 16 * i;
             z[i][q] = in && m < g.n ? *reinterpret_cast<const u32x4*>((const char*)g.z + (m * g.ldz + c) * (CODES ? 2 : 4) + 16 * q) : u32x4{0, 0, 0, 0};
+            if constexpr (CODES) top[i] = in && m < g.n ? g.top[m * g.ldtop + 4 * ((g.v0 + c) >> g.shift) + (c >> 3 & 3)] : 0.f;
         }
     if (tid < 128) {
         const int m = r0 + tid;
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
         const bool dead = s.y == 0.f;
         // what 0 becomes where the sum is a NaN or an infinity: a NaN, as exp(z - lse) would
         none[tid] = dead ? 0.f : s.x - s.x;
-        ref[tid] = dead ? CODES ? -INFINITY : INFINITY : CODES ? (g.part[(long long)m * g.ntn + ((g.v0 + tc * 128) >> g.shift)].x - s.x) * L2E : s.x;
+        ref[tid] = dead ? INFINITY : s.x;
         scale[tid] = dead || !g.colsum ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, s.y, m);
     }
     __syncthreads();
@@ -311,15 +313,15 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
     for (int i = 0; i < 8; ++i) {
         const int l = y + 16 * i, m = r0 + l;
         float v[8];
+        const bool dead = ref[l] == INFINITY && none[l] == 0.f;
         if constexpr (CODES) {
-            const float top = ref[l], nil = none[l];
+            const float low = dead ? -INFINITY : (top[i] - ref[l]) * L2E, nil = none[l];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t u = e & 1 ? z[i][0][e >> 1] >> 16 : z[i][0][e >> 1] & 0xffffu;
-                v[e] = u == 0xffffu ? nil : __builtin_amdgcn_exp2f(fmaf((float)u, -LIN_STEP * L2E, top));
+                v[e] = u == 0xffffu ? nil : __builtin_amdgcn_exp2f(fmaf((float)u, -LIN_STEP * L2E, low));
             }
         } else {
-            const bool dead = ref[l] == INFINITY && none[l] == 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 v[e] = dead ? 0.f : __expf(__builtin_bit_cast(f32x4, z[i][e >> 2])[e & 3] - ref[l]);
@@ -484,7 +486,7 @@ static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
 // The form that a call's products take: the operands as they are, or fp32 as three bf16 planes where the copies pay.
 struct LinForm {
     int dt, es, mul, pad;         // dtype of the products, bytes of an element, elements of a row per channel, what a row is rounded up to
-    long long row(long long k) const { return up(k, pad) * mul; }          // elements of a row of k channels
+    long long row(long long k) const { const long long r = up(k, pad) * mul; return r % 128 ? r : r + 64; }          // elements of a row of k channels
     int K(long long k) const { return (int)(dt == FEA_PL ? 6 * up(k, 64) : dt == FEA_BF16 ? up(k, 64) : k); }      // reduction over k channels
 };
 static LinForm lin_form(int dtype, bool planes) {
@@ -597,14 +599,14 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     return c.at;
 }
 
-// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16) or fp32, then (bf16) the forward's table of the tiles' maxima.  Not for the heads that
+// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16) or fp32, then (bf16) the groups' largest.  Not for the heads that
 // read no more for recomputing them: few rows (the weight once more) and few classes (nothing).
 static long long lin_keep_ld(const LinDims& d) { return up(d.V, 64); }
 static size_t lin_keep_table(const LinDims& d) { return (size_t)up(d.rows * lin_keep_ld(d) * d.es, 256); }
 extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype) {
     if (rows <= 64 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
     const LinDims d = lin_dims(rows, D, V, 1, dtype);
-    return lin_keep_table(d) + (dtype == FEA_BF16 ? (size_t)rows * lin_fwd_plan(d).ntn * sizeof(float2) : 0);
+    return lin_keep_table(d) + (dtype == FEA_BF16 ? (size_t)rows * lin_fwd_plan(d).ntn * 8 * sizeof(float) : 0);
 }
 
 extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads) {
@@ -714,13 +716,13 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
         if (keep) {
             g.keep = (char*)keep + r * lin_keep_ld(d) * d.es; g.ldkeep = lin_keep_ld(d);
-            if (d.dtype == FEA_BF16) g.part = (float2*)((char*)keep + lin_keep_table(d)) + r * p.ntn;
+            if (d.dtype == FEA_BF16) { g.ldtop = p.ntn * 8; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * g.ldtop; }
         }
         if (inner) { g.zsel = b.zsel; g.index = j.index; g.sel = d.K; }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
         else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;
-        q.part = g.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
+        q.part = b.part; q.ntn = p.ntn; q.rows = n; q.K = d.K; q.V = d.V; q.G = p.G;
         q.zsel = b.zsel + r * d.K; q.index = j.index + r * d.K;
         if (q.tlog) q.tlog = (const char*)j.tlog + r * d.K * (j.tdt == FEA_BF16 ? 2 : 4);
         if (q.stat) q.stat += r;
@@ -795,7 +797,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     }
     const LinForm f = lin_form(dtype, p.planes);
     const bool pack = p.planes || (dtype == FEA_BF16 && d.odd());
-    const LinFwd kp = lin_fwd_plan(d);              // (its tiles are the kept table's)
+    const LinFwd kp = lin_fwd_plan(d);              // (its tiles make the kept groups)
     for (int ir = 0; ir < p.nrc; ++ir) {
         const long long r0 = ir * p.rc, n = rows - r0 < p.rc ? rows - r0 : p.rc;
         const char* hr = (const char*)h + r0 * ldh * d.es;
@@ -825,7 +827,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             if (keep) {
                 LinDecode x{};
                 x.z = (const char*)keep + (r0 * lin_keep_ld(d) + v0) * d.es; x.ldz = lin_keep_ld(d);
-                x.part = (const float2*)((const char*)keep + lin_keep_table(d)) + r0 * kp.ntn; x.ntn = kp.ntn; x.shift = kp.tile == 256 ? 8 : 7;
+                x.ldtop = kp.ntn * 8; x.top = (const float*)((const char*)keep + lin_keep_table(d)) + r0 * x.ldtop; x.shift = kp.tile == 256 ? 7 : 6;
                 x.stat = st; x.gout = go; x.gstride = gout_stride; x.count = count; x.t = temperature;
                 x.dz = b.dz; x.lddz = g.lddz; x.Npad = g.Npad; x.colsum = g.colsum; x.ldcol = g.ldcol;
                 x.n = (int)n; x.nv = nv; x.v0 = (int)v0; x.nct = (nv + 127) / 128;

@@ -357,7 +357,7 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
  * psel[rows][K] (all nullable), and keep (nullable): fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned, for the logits: fp32, or with bf16
- * operands 16 bits (z below its tile's maximum in steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0).
+ * operands 16 bits (z below the largest of its 16 or 32 in steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0).
  * 0 bytes = none are kept (rows <= 64, few classes with few features: recomputing them reads next to nothing more).
  *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the
  *     logits from the forward's keep, or (NULL; with bf16 operands a bias gradient asks for it) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one

@@ -32,9 +32,10 @@ def case(rows, dim, classes, dtype, seed=0, top=0, ignored=0.0, short=0.0, bias=
     return h, w, b, i, (torch.randn(rows, top, generator=g) * 2 + 5).to(dtype)
 
 
-def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, reduction="mean", gout=None):
+def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, reduction="mean", gout=None, kept=None):
     """{"loss", "hidden", "weight", "bias"}: values and bounds, as (value, bound) pairs in 64 bits.  gout: upstream gradient of the losses
-    (rows) for "none", else of the result."""
+    (rows) for "none", else of the result.  kept: the
+    backward had the forward's logits (None: as a head whose every operand has a gradient would)."""
     dtype, t = h.dtype, temperature
     u = torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else E
     hd, wd = h.double().reshape(-1, h.shape[-1]), w.double()
@@ -80,7 +81,8 @@ def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, redu
     q = q.nan_to_num(0.0) if not on.all() else q
     hd = torch.where(on[:, None], hd, 0.0)
     dz = g[:, None] * (q - p)
-    kept = 4.89e-4 if dtype == torch.bfloat16 and rows > 64 and b is None and not (v <= 32 and dim <= 64 and rows >= 4096) else 0.0
+    kept = kept if kept is not None else rows > 64 and b is None and not (v <= 32 and dim <= 64 and rows >= 4096)
+    kept = 4.89e-4 if kept and dtype == torch.bfloat16 else 0.0
     off = g.abs()[:, None] * (q * kept * (1 + u) + (1.7e-28 if kept else 0.0) + q * 2 * dz_log[:, None] + (8 + (0 if tlog is None else index.shape[-1])) * E * (p + q) + p * arg[:, None]) + u * dz.abs() + 2 * E * dz.abs()
     dh, dw = dz @ wd, dz.T @ hd
     out["hidden"] = (dh, off @ wd.abs() + (v + 8) * E * (dz.abs() @ wd.abs()) + u * dh.abs() + 1e-37)

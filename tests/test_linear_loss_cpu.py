@@ -56,7 +56,7 @@ def test_kept_sizes():
     for rows, d, v in ((65, 8, 1), (100, 64, 1000), (8192, 4096, 131072), (1 << 20, 65, 6)):
         ld = (v + 63) // 64 * 64
         assert rows * ld * 4 <= keep(rows, d, v, L.F32) < rows * ld * 4 + 256
-        assert rows * ld * 2 < keep(rows, d, v, L.BF16) <= rows * ld * 2 + 256 + rows * ((v + 127) // 128) * 8
+        assert rows * ld * 2 < keep(rows, d, v, L.BF16) <= rows * ld * 2 + 256 + rows * ((v + 127) // 128) * 32
 
 
 @pytest.mark.parametrize("top", [0, 4])

@@ -170,6 +170,37 @@ def test_ignored_rows_may_hold_anything(shape, dtype, top, bad):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -1e30])
+def test_ignored_rows_of_kept_logits_may_hold_anything(dtype, top, bad):
+    c = list(O.case(90, 64, 200, dtype, seed=3, top=top, ignored=0.4))
+    want = O.evaluate(*c)
+    gone = c[3] == -100 if not top else (c[3] < 0).all(1)
+    assert 5 < int(gone.sum()) < 85
+    c[0] = c[0].clone()
+    c[0][gone] = bad
+    _compare(_run(*c), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_classes_of_kept_logits(dtype):
+    """A bias without a gradient masks classes: their kept logits are a share of 0, and gradient 0."""
+    h, w, b, t = O.case(65, 48, 400, dtype, seed=4, bias=True)
+    b[100:228] = -torch.inf
+    b[256:384] = torch.finfo(torch.float32).min
+    t = t % 100
+    want = O.evaluate(h, w, b, t)
+    x, y = _leaf(h), _leaf(w)
+    loss = F.linear_cross_entropy(x, y, t.to(DEV), bias=b.to(DEV))
+    assert any(s is not None and s.dtype == torch.uint8 for s in loss.grad_fn.saved_tensors)
+    gh, gw = torch.autograd.grad(loss, [x, y])
+    assert float(gw[100:228].abs().max()) == 0.0 and float(gw[256:384].abs().max()) == 0.0
+    kept = O.evaluate(h, w, b, t, kept=True)
+    _compare({"loss": loss, "hidden": gh, "weight": gw}, kept)
+    assert torch.equal(kept["hidden"][0], want["hidden"][0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_masked_classes(dtype):
     """Classes masked by a bias of -inf or of the type's lowest value: softmax 0 and gradient 0 there."""
     h, w, b, t = O.case(65, 48, 400, dtype, seed=4, bias=True)
