@@ -12,6 +12,7 @@
 // fp32 values, then two products.  The workspace is bounded by the piece, not by rows x classes.
 #include "linear_loss.h"
 #include <limits.h>
+#include <type_traits>
 #include <math.h>
 #include <stdlib.h>
 
@@ -32,9 +33,8 @@ struct LinCopy { const void* in; void* out; long long ld, ldo, R; int C, Cpad; c
 struct LinCopies { LinCopy j[3]; };
 
 template <typename T, bool PL, bool ALN>
-__global__ __launch_bounds__(256) void lin_copy_kernel(const LinCopies js) {
+__device__ __forceinline__ void lin_copy_tile(const LinCopies& js, long long tile) {
     constexpr int EPC = Elem<T>::EPC, NV = 8 / EPC;
-    long long tile = blockIdx.x;
     int n = 0;
     while (n < 2 && tile >= js.j[n].tiles) tile -= js.j[n++].tiles;
     const LinCopy j = js.j[n];
@@ -71,6 +71,9 @@ __global__ __launch_bounds__(256) void lin_copy_kernel(const LinCopies js) {
             for (int q = 0; q < NV; ++q) *reinterpret_cast<u32x4*>((T*)j.out + r * j.ldo + c + q * EPC) = *reinterpret_cast<const u32x4*>(x + q * EPC);
     }
 }
+
+template <typename T, bool PL, bool ALN>
+__global__ __launch_bounds__(256) void lin_copy_kernel(const LinCopies js) { lin_copy_tile<T, PL, ALN>(js, blockIdx.x); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
 
@@ -272,18 +275,24 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 // ---- backward -----------------------------------------------------------------------------------------------------------
 
 // dz of the piece from the logits that the forward kept: exp(z - lse), 0 in rows that do not count.  Workgroup: 128 rows x 128 classes, a thread
-// 8 classes of 8 rows.  Bound by memory: reads z, writes dz.
+// 8 classes of 8 rows.  Bound by memory: reads z, writes dz.  A cross entropy's labels are set on the way, and the operands' copies for the
+// products go along.
 struct LinDecode {
     const void* z; long long ldz;         // at the piece's first row and class
     const float* top; long long ldtop; int shift;   // bf16: the groups' largest at the first row; a class's: 4 (class >> shift) + (class >> 3 & 3)
     const float2* stat; const float* gout; int gstride; const int* count; float t;
     void* dz; long long lddz; int Npad;
     float* colsum; long long ldcol;       // fp32, nullable: [tiles of 128 rows][classes] sums of row scale * softmax
+    const long long* index; const float* dsel;      // nullable: one selected class per row, and dz there
     int n, nv, v0, nct;                   // rows, classes, first class, tiles of 128 columns
+    unsigned blocks;                      // of this; the ones behind it copy operands
+    LinCopies copies;
 };
-template <bool CODES, bool PL>
+template <bool CODES, bool PL, bool ALN>
 __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
-    __shared__ float ref[128], none[128], scale[128], red[16][128];
+    __shared__ float ref[128], none[128], scale[128], dpick[128], red[16][128];
+    __shared__ int pick[128];
+    if (blockIdx.x >= g.blocks) return lin_copy_tile<std::conditional_t<CODES, __bf16, float>, PL, ALN>(g.copies, blockIdx.x - g.blocks);
     const int id = blockIdx.x, tc = id % g.nct, tm = id / g.nct, tid = threadIdx.x;
     const int r0 = tm * 128, c = tc * 128 + (tid & 15) * 8, y = tid >> 4;
     const bool in = c < g.Npad;
@@ -306,6 +315,9 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
         none[tid] = dead ? 0.f : s.x - s.x;
         ref[tid] = dead ? INFINITY : s.x;
         scale[tid] = dead || !g.colsum ? 0.f : lin_row_scale(g.gout, g.gstride, g.count, g.t, s.y, m);
+        const long long i = g.index && !dead ? g.index[m] - g.v0 : -1;
+        pick[tid] = i >= 0 && i < g.nv ? (int)i : -8;
+        dpick[tid] = g.index && !dead ? g.dsel[m] : 0.f;
     }
     __syncthreads();
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -329,6 +341,9 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
             }
         }
         if (!in || m >= g.n) continue;
+        if ((unsigned)(pick[l] - c) < 8u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) if (pick[l] - c == e) v[e] = dpick[l];
         if constexpr (CODES) {
             __bf16 x[8];
 #pragma unroll
@@ -693,6 +708,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
     }
     const long long entries = d.rows * d.K;
     // selected logits: in the few-rows kernel's epilogue, where every workgroup looks through all entries, or by gathered dot products
+    // (2,048 labels of 2,048 features: 8 us; the large product's epilogue took 10 us longer for them)
     const bool inner = p.tile == 64 && entries <= 2048;
     if (!inner) {
         int lanes = 1;
@@ -814,7 +830,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                           lin_copy_of(d, f, hr, ldh, n, gated && iv == 0 ? b.hg : nullptr)}};
             js.j[0].stat = js.j[2].stat = st;
             if (gout_stride) { js.j[2].gout = go; js.j[2].t = temperature; }
-            LIN_TRY(lin_copy(d, f, js, s));
+            if (!keep) LIN_TRY(lin_copy(d, f, js, s));
             const void* const wk = pack ? b.wp : (const void*)wr;
             const long long ldwk = pack ? f.row(D) : ldw;
             LinGemm g{};
@@ -831,19 +847,25 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 x.stat = st; x.gout = go; x.gstride = gout_stride; x.count = count; x.t = temperature;
                 x.dz = b.dz; x.lddz = g.lddz; x.Npad = g.Npad; x.colsum = g.colsum; x.ldcol = g.ldcol;
                 x.n = (int)n; x.nv = nv; x.v0 = (int)v0; x.nct = (nv + 127) / 128;
-                const unsigned blocks = (unsigned)((n + 127) / 128 * x.nct);
-                if (dtype == FEA_BF16) hipLaunchKernelGGL((lin_decode_kernel<true, false>), dim3(blocks), dim3(256), 0, s, x);
-                else if (p.planes)     hipLaunchKernelGGL((lin_decode_kernel<false, true>), dim3(blocks), dim3(256), 0, s, x);
-                else                   hipLaunchKernelGGL((lin_decode_kernel<false, false>), dim3(blocks), dim3(256), 0, s, x);
+                if (K == 1) { x.index = index + r0; x.dsel = dsel + r0; }
+                x.blocks = (unsigned)((n + 127) / 128 * x.nct); x.copies = js;
+                const long long blocks = x.blocks + js.j[0].tiles + js.j[1].tiles + js.j[2].tiles;
+                FEA_CHECK(blocks < INT_MAX, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld tiles", who, blocks);
+                const dim3 grid((unsigned)blocks), bl(256);
+                if (dtype == FEA_BF16) { if (d.odd()) hipLaunchKernelGGL((lin_decode_kernel<true, false, false>), grid, bl, 0, s, x); else hipLaunchKernelGGL((lin_decode_kernel<true, false, true>), grid, bl, 0, s, x); }
+                else if (p.planes)     { if (d.odd()) hipLaunchKernelGGL((lin_decode_kernel<false, true, false>), grid, bl, 0, s, x); else hipLaunchKernelGGL((lin_decode_kernel<false, true, true>), grid, bl, 0, s, x); }
+                else                   { if (d.odd()) hipLaunchKernelGGL((lin_decode_kernel<false, false, false>), grid, bl, 0, s, x); else hipLaunchKernelGGL((lin_decode_kernel<false, false, true>), grid, bl, 0, s, x); }
                 FEA_LAUNCH_CHECK();
             } else LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
             const unsigned sg = (unsigned)((entries + 255) / 256);
-            if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, g.Npad);
-            else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, 0);
-            else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0);
-            FEA_LAUNCH_CHECK();
+            if (!keep || K > 1) {
+                if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, g.Npad);
+                else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, 0);
+                else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0);
+                FEA_LAUNCH_CHECK();
+            }
             if (db) {
                 const int tm = keep ? 128 : p.tz, tiles = (int)((n + tm - 1) / tm), chunks = (int)((n + LIN_DB_ROWS - 1) / LIN_DB_ROWS);
                 hipLaunchKernelGGL(lin_dbias_kernel, dim3((unsigned)((nv + 255) / 256), (unsigned)chunks), dim3(64 * LIN_DB_WAVES), 0, s, (const float*)b.colsum, tiles, (long long)g.ldcol, ix, psel ? psel + r0 * K : nullptr, K, st, go, gout_stride, count, temperature, v0, nv, entries, LIN_DB_ROWS / tm, (long long)LIN_DB_ROWS * K, b.dbpart);
