@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                 } else {
                     uint16_t* const o = (uint16_t*)g.keep + m * g.ldkeep;
                     const float t = base / LIN_RANGE;
-                    g.top[m * g.ldtop + (n0 / LB_W + wn) * 4 + q16] = base;
+                    g.top[((n0 / LB_W + wn) * g.ldtop + m) * 4 + q16] = base;
 #pragma unroll
                     for (int p = 0; p < NT / 2; ++p) {
                         u32x4 v;

@@ -279,7 +279,7 @@ __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, con
 // products go along.
 struct LinDecode {
     const void* z; long long ldz;         // at the piece's first row and class
-    const float* top; long long ldtop; int shift;   // bf16: the groups' largest at the first row; a class's: 4 (class >> shift) + (class >> 3 & 3)
+    const float* top; long long ldtop; int shift;   // bf16: the groups' largest at the first row; a class's half tile is class >> shift
     const float2* stat; const float* gout; int gstride; const int* count; float t;
     void* dz; long long lddz; int Npad;
     float* colsum; long long ldcol;       // fp32, nullable: [tiles of 128 rows][classes] sums of row scale * softmax
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
         for (int q = 0; q < (CODES ? 1 : 2); ++q) {
             const long long m = r0 + y + 16 * i;
             z[i][q] = in && m < g.n ? *reinterpret_cast<const u32x4*>((const char*)g.z + (m * g.ldz + c) * (CODES ? 2 : 4) + 16 * q) : u32x4{0, 0, 0, 0};
-            if constexpr (CODES) top[i] = in && m < g.n ? g.top[m * g.ldtop + 4 * ((g.v0 + c) >> g.shift) + (c >> 3 & 3)] : 0.f;
+            if constexpr (CODES) top[i] = in && m < g.n ? g.top[(((g.v0 + c) >> g.shift) * g.ldtop + m) * 4 + (c >> 3 & 3)] : 0.f;
         }
     if (tid < 128) {
         const int m = r0 + tid;
@@ -732,7 +732,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
         if (keep) {
             g.keep = (char*)keep + r * lin_keep_ld(d) * d.es; g.ldkeep = lin_keep_ld(d);
-            if (d.dtype == FEA_BF16) { g.ldtop = p.ntn * 8; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * g.ldtop; }
+            if (d.dtype == FEA_BF16) { g.ldtop = d.rows; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * 4; }
         }
         if (inner) { g.zsel = b.zsel; g.index = j.index; g.sel = d.K; }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
@@ -843,7 +843,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             if (keep) {
                 LinDecode x{};
                 x.z = (const char*)keep + (r0 * lin_keep_ld(d) + v0) * d.es; x.ldz = lin_keep_ld(d);
-                x.ldtop = kp.ntn * 8; x.top = (const float*)((const char*)keep + lin_keep_table(d)) + r0 * x.ldtop; x.shift = kp.tile == 256 ? 7 : 6;
+                x.ldtop = rows; x.top = (const float*)((const char*)keep + lin_keep_table(d)) + r0 * 4; x.shift = kp.tile == 256 ? 7 : 6;
                 x.stat = st; x.gout = go; x.gstride = gout_stride; x.count = count; x.t = temperature;
                 x.dz = b.dz; x.lddz = g.lddz; x.Npad = g.Npad; x.colsum = g.colsum; x.ldcol = g.ldcol;
                 x.n = (int)n; x.nv = nv; x.v0 = (int)v0; x.nct = (nv + 127) / 128;
