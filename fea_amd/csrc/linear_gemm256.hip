@@ -161,6 +161,19 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
     };
 
+    // LIN_LSE: the selected classes of the tile's row tid (asked for behind the first chunk's loads, wanted in the epilogue)
+    uint2 where = make_uint2(~0u, ~0u);
+    auto look = [&]() {
+        if constexpr (EPI == LIN_LSE)
+            if (g.zsel && tid < LB_T && m0 + tid < g.M) {
+                if (g.where) where = g.where[(long long)(m0 + tid) * g.ntn + tn];
+                else {
+                    const long long t = g.index[m0 + tid];
+                    if (t >= n0 && t < min(n0 + LB_T, g.N)) where.x = 0xffff0000u | (unsigned)(t - n0);
+                }
+            }
+    };
+
     if constexpr (DL) {
         // A ring of five operand chunks: A(c) in slot 2 c mod 5, B(c) in 2 c + 1 mod 5.  Half-way through chunk c its fragments are all in registers, so
         // B(c + 2) goes where A(c) was, and in the next half A(c + 3) where B(c) was.  Loads are spread evenly (one per 8 MFMA): the
@@ -178,6 +191,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         advance_a(0); advance_b(0);
 #pragma unroll
         for (int i = 0; i < NL; ++i) dload(i < NT ? a0 : b0, i);
+        look();
         landed(true);
         advance_a(1); advance_b(1);
 #pragma unroll
@@ -218,6 +232,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     advance_a(0); advance_b(0);
 #pragma unroll
     for (int i = 0; i < NL; ++i) gload(0, i);
+    look();
 #pragma unroll
     for (int i = 0; i < NL; ++i) lput(0, 0, i);
 #pragma unroll
@@ -382,6 +397,11 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         // every lane's own maximum and sum of a label's 4 NT classes, joined in LDS: nothing goes across lanes on the way, and a label's kept
         // logits leave while the next one's exponentials run
         float2* const red = reinterpret_cast<float2*>(smem);       // [wn, q16][labels of the tile]
+        uint2* const wanted = reinterpret_cast<uint2*>(red + 8 * LB_T);
+        if (g.zsel) {
+            if (tid < LB_T) wanted[tid] = where;
+            __syncthreads();
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int m = mrow(i);
@@ -413,6 +433,27 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                         if (pcol + 32 * p < g.ldkeep) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
                     }
                 }
+            }
+            if (g.zsel) {
+                // one lane of the chip has a selected logit: out of its 4 NT
+                auto give = [&](unsigned col, int k) {
+                    if (col / LB_W != (unsigned)wn || ((col >> 3) & 3) != (unsigned)q16) return;
+                    const unsigned at = (col % LB_W >> 5) * 8 + (col & 7);
+                    float x = z[0][0];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x = at == 4 * j + e ? z[j][e] : x;
+                    g.zsel[(long long)m * g.sel + k] = x;
+                };
+                const uint2 w = wanted[wm * LB_W + i * 16 + r16];
+                if ((w.x & 0xffffu) == LIN_MANY)
+                    for (int k = 0; k < g.sel; ++k) {
+                        const long long t = g.index[(long long)m * g.sel + k];
+                        if (t >= n0 && t < min(n0 + LB_T, g.N)) give((unsigned)(t - n0), k);
+                    }
+                else
+                    for (uint64_t h = w.x | (uint64_t)w.y << 32; (h & 0xffffu) != LIN_NONE; h = h >> 16 | (uint64_t)LIN_NONE << 48) give((unsigned)h & 255u, (int)(h >> 8) & 255);
             }
             float sum = 0.f;
 #pragma unroll

@@ -22,6 +22,13 @@ __device__ __forceinline__ int lin_plane_b(int pair) { return (0x010201 >> (4 * 
 #define LIN_RANGE 64.f
 #define LIN_STEP (LIN_RANGE / 65535.f)
 
+// Where a row's selected classes lie: for every row and column tile up to four entries of 16 bits (column of the tile, k << 8), LIN_NONE behind
+// them; LIN_MANY in the first: more than four, look through all.  At most LIN_WHERE_K entries per row, LIN_WHERE_T tiles.
+#define LIN_NONE 0xffffu
+#define LIN_MANY 0xfffeu
+#define LIN_WHERE_K 254
+#define LIN_WHERE_T 1280
+
 struct LinGemm {
     const void *a, *b;
     long long lda, ldb;
@@ -49,8 +56,9 @@ struct LinGemm {
     int scale;                        // 0: none, 1: times the row scale of C's row, 2: times the common scale (gout, count, t above)
     int splits, kper;
     int ntm, ntn;
-    // fea_lin_rows: selected logits a . b + bias of the entries index[M][sel] (nullable)
+    // LIN_LSE: selected z of the entries index[M][sel] (nullable); with bf16 or FEA_PL tiles and sel > 1 also where they are (lin_where_kernel)
     float* zsel; const long long* index; int sel;
+    const uint2* where;
 };
 
 // gradient scale of a row: d loss / d (row loss) times the temperature; 0 for a row that does not count

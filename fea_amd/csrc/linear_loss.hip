@@ -96,12 +96,12 @@ __device__ __forceinline__ float lin_dot(const T* a, const T* b, int D, int lane
     return s;
 }
 
-// zsel[n][k] = h_n . w_{index[n][k]} + b: L lanes (a power of two that covers the row in 16-byte loads, 64 at most) per entry.
+// zsel[n][k] = (h_n . w_{index[n][k]} + b) / T: L lanes (a power of two that covers the row in 16-byte loads, 64 at most) per entry.
 // Absent entries (index < 0 or >= V) are not read.
 template <typename T>
 __global__ __launch_bounds__(256) void lin_select_kernel(const T* __restrict__ h, long long ldh, const T* __restrict__ w, long long ldw,
                                                          const float* __restrict__ bias, const long long* __restrict__ index, int K,
-                                                         float* __restrict__ zsel, long long entries, int D, int V, int L, int vec) {
+                                                         float* __restrict__ zsel, long long entries, int D, int V, int L, int vec, float inv_t) {
     const int lane = threadIdx.x & (L - 1), per = 256 / L;
     for (long long b0 = (long long)blockIdx.x * per; b0 < entries; b0 += (long long)gridDim.x * per) {
         const long long e = b0 + threadIdx.x / L;
@@ -109,8 +109,30 @@ __global__ __launch_bounds__(256) void lin_select_kernel(const T* __restrict__ h
         if (i < 0 || i >= V) continue;                       // (the L lanes of an entry go together)
         const T* a = h + e / K * ldh;
         const float s = vec ? lin_dot<T, true>(a, w + i * ldw, D, lane, L) : lin_dot<T, false>(a, w + i * ldw, D, lane, L);
-        if (lane == 0) zsel[e] = bias ? s + bias[i] : s;
+        if (lane == 0) zsel[e] = (bias ? s + bias[i] : s) * inv_t;
     }
+}
+
+// The tiles of T columns that hold a row's selected classes (linear_loss.h), a wave per row.  Which entry comes first in a tile is left
+// open: each has its own place in zsel.
+__global__ __launch_bounds__(256) void lin_where_kernel(const long long* __restrict__ index, int K, long long rows, int V, int T, int ntn, uint2* __restrict__ where) {
+    extern __shared__ uint32_t tab[];                    // per row: two dwords and a count for each tile
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long row = (long long)blockIdx.x * 4 + wave;
+    uint32_t* const slot = tab + wave * 3 * ntn;
+    int* const n = (int*)(slot + 2 * ntn);
+    for (int i = lane; i < ntn; i += 64) { slot[2 * i] = slot[2 * i + 1] = ~0u; n[i] = 0; }
+    __syncthreads();
+    if (row < rows)
+        for (int k = lane; k < K; k += 64) {
+            const long long i = index[row * K + k];
+            if (i < 0 || i >= V) continue;
+            const int tile = (int)i / T, at = atomicAdd(n + tile, 1);
+            if (at < 4) reinterpret_cast<uint16_t*>(slot + 2 * tile)[at] = (uint16_t)((int)i % T | k << 8);
+        }
+    __syncthreads();
+    if (row < rows)
+        for (int i = lane; i < ntn; i += 64) where[row * ntn + i] = n[i] > 4 ? make_uint2(0xffff0000u | LIN_MANY, ~0u) : make_uint2(slot[2 * i], slot[2 * i + 1]);
 }
 
 struct LinJoin {
@@ -188,7 +210,7 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
                 if (counts && ix[q] >= 0) {
                     if (bad) { loss = ds = ps = NAN; }
                     else {
-                        const float zq = j.zsel[e0 + k] * j.inv_t - lse;
+                        const float zq = j.zsel[e0 + k] - lse;
                         if (p[q] > 0.f) loss += p[q] * (tv[q] - tb - lt - zq);
                         ds = expf(zq) - all[q];
                         ps = p[q];
@@ -510,7 +532,7 @@ static LinForm lin_form(int dtype, bool planes) {
 }
 
 // Forward: rows in chunks that bound the partial table to 128 MB.
-struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; };
+struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; int pick; };   // pick: 0 selected logits by dot products, 1 out of the product, 2 with lin_where_kernel
 static LinFwd lin_fwd_plan(const LinDims& d) {
     LinFwd p;
     const long long cap = (1ll << 24) / ((d.V + 127) / 128);
@@ -525,6 +547,9 @@ static LinFwd lin_fwd_plan(const LinDims& d) {
     p.tile = t.tile;
     if (d.rows <= 64) { p.tile = 64; p.planes = false; }
     p.ntn = (d.V + p.tile - 1) / p.tile;
+    // selected logits come out of the product where it can give them
+    const bool tiles = p.tile != 64 && (d.dtype == FEA_BF16 || p.planes);
+    p.pick = p.tile == 64 ? d.rows * d.K <= 2048 : !tiles ? 0 : d.K == 1 ? 1 : d.K <= LIN_WHERE_K && p.ntn <= LIN_WHERE_T ? 2 : 0;
     p.G = 1;
     while (p.G < 64 && (p.G < (d.V + 127) / 128 || p.G < d.K)) p.G *= 2;
     p.blocks = p.tile == 64 ? d.rows : (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
@@ -567,7 +592,7 @@ static LinBwd lin_bwd_plan(const LinDims& d, int want) {       // want: 1 dh, 2 
     return p;
 }
 
-struct LinFwdWs { void *hp, *wp; float2* part; float* zsel; double* bsum; int* bcnt; };
+struct LinFwdWs { void *hp, *wp; float2* part; float* zsel; uint2* where; double* bsum; int* bcnt; };
 static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFwdWs& w) {
     LinCarve c{base};
     if (fea_lin_few(d.rows, d.D, d.V)) {
@@ -581,6 +606,7 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
     w.hp = w.wp = nullptr;
+    w.where = p.pick == 2 ? c.take<uint2>(p.rc * p.ntn) : nullptr;
     if (p.planes || (d.dtype == FEA_BF16 && d.odd() && p.tile != 64)) {
         const LinForm f = lin_form(d.dtype, p.planes);
         w.hp = c.take<char>(p.rc * f.row(d.D) * f.es);
@@ -707,16 +733,13 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         return FEA_OK;
     }
     const long long entries = d.rows * d.K;
-    // selected logits: in the few-rows kernel's epilogue, where every workgroup looks through all entries, or by gathered dot products
-    // (2,048 labels of 2,048 features: 8 us; the large product's epilogue took 10 us longer for them)
-    const bool inner = p.tile == 64 && entries <= 2048;
-    if (!inner) {
+    if (!p.pick) {
         int lanes = 1;
         while (lanes < 64 && lanes * d.epc < d.D) lanes *= 2;
         const long long blocks = (entries * lanes + 255) / 256;
         const unsigned grid = (unsigned)(blocks < 1 << 16 ? blocks : 1 << 16);
-        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.odd() ? 0 : 1);
-        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.odd() ? 0 : 1);
+        if (d.dtype == FEA_BF16) hipLaunchKernelGGL(lin_select_kernel<__bf16>, dim3(grid), dim3(256), 0, s, (const __bf16*)h, ldh, (const __bf16*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.odd() ? 0 : 1, j.inv_t);
+        else                     hipLaunchKernelGGL(lin_select_kernel<float>, dim3(grid), dim3(256), 0, s, (const float*)h, ldh, (const float*)w, ldw, bias, j.index, d.K, b.zsel, entries, d.D, d.V, lanes, d.odd() ? 0 : 1, j.inv_t);
         FEA_LAUNCH_CHECK();
     }
     const LinForm f = lin_form(d.dtype, p.planes);
@@ -734,7 +757,12 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
             g.keep = (char*)keep + r * lin_keep_ld(d) * d.es; g.ldkeep = lin_keep_ld(d);
             if (d.dtype == FEA_BF16) { g.ldtop = d.rows; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * 4; }
         }
-        if (inner) { g.zsel = b.zsel; g.index = j.index; g.sel = d.K; }
+        if (p.pick) { g.zsel = b.zsel + r * d.K; g.index = j.index + r * d.K; g.sel = d.K; }
+        if (p.pick == 2) {
+            g.where = b.where;
+            hipLaunchKernelGGL(lin_where_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 4 * 3 * p.ntn * sizeof(uint32_t), s, g.index, d.K, n, d.V, p.tile, p.ntn, b.where);
+            FEA_LAUNCH_CHECK();
+        }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
         else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;

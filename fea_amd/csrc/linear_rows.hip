@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float raw = acc[i][e] + bias[e];
-            if (g.zsel) zt[wave * 16 + 4 * q16 + e][16 * i + r16] = raw;
+            if (g.zsel) zt[wave * 16 + 4 * q16 + e][16 * i + r16] = raw * g.inv_t;
             z[e] = n0 + 4 * q16 + e < g.N ? raw * g.inv_t : -INFINITY;
             mx = fmaxf(mx, z[e]);
         }

@@ -58,6 +58,16 @@ def test_most_entries(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,top", [((100, 64, 300), 254), ((100, 64, 300), 255), ((70, 8, 170000), 5), ((300, 72, 2000), 4), ((300, 72, 2000), 40)])
+def test_where_the_entries_are(shape, top, dtype):
+    """Selected logits out of the product: four entries in a column tile and more, all in one tile, in too many tiles, too many entries."""
+    h, w, _, i, a = O.case(*shape, dtype, seed=61, top=top, ignored=0.1, short=0.1)
+    i[::3] = i[::3] % 120                                      # all in the first tile
+    i[1] = shape[2] - 1                                        # one class, every time
+    _compare(_run(h, w, None, i, a, temperature=1.5), O.evaluate(h, w, None, i, a, temperature=1.5))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", ["sum", "none"])
 @pytest.mark.parametrize("top", [0, 3])
 @pytest.mark.parametrize("shape", [(77, 40, 300), (4500, 24, 11)])
