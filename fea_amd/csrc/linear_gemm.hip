@@ -12,8 +12,9 @@
 // of the MFMA are swapped (classes as its rows), so a lane holds one label row and 32 of its classes: the softmax sums are
 // in-lane sums and one exchange between wave halves.  An operand with its rows along the reduction keeps them in LDS, and a
 // fragment is four reads down a column.
-// Bound by the fp32 matrix rate: 1,531 x 643 x 10,007 takes 204 us (96 TFLOP/s), as planes (linear_gemm256.hip) 107 us; this kernel
-// serves what the planes' copies do not pay for.
+// Bound by the fp32 matrix rate: 1,531 x 643 x 10,007 takes 204 us (96 TFLOP/s), as planes (linear_gemm256.hip) 120 us and 19 us of copies;
+// this kernel serves what the planes' copies do not pay for: with 2 rows x 1,472 x 119,936 the products take 180 to 220 us each, bound
+// by the weight's bytes (706 MB), as planes 400 us and 290 us of copies.
 #include "linear_loss.h"
 
 static constexpr int LG_T = 128, LG_CK = 32;

@@ -122,8 +122,8 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     };
     auto dload = [&](int slot, int i) {     // a wave's 1,024 bytes straight to LDS: nothing lands in a register, and `landed` waits
         const uint32_t m = lds + slot * LB_OP + i % NT * 4096;
-        if (i < NT) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m), "v"(address(i)), "s"(rsa) : "memory");
-        else        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m), "v"(address(i)), "s"(rsb) : "memory");
+        if (i < NT) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m), "v"(address(i)), "s"(rsa) : "memory", "m0");
+        else        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(m), "v"(address(i)), "s"(rsb) : "memory", "m0");
     };
     auto gload = [&](int u, int i) {
         if constexpr (!DL) st[u][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(i < NT ? rsa : rsb, address(i), 0, 0));

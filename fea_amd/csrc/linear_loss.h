@@ -1,5 +1,5 @@
-// Shared between the files of the many-class loss heads (linear_loss.hip: entry points, statistics, layouts;
-// linear_gemm.hip: the tiled product and its epilogues).
+// Shared between the files of the many-class loss heads: linear_loss.hip (entry points, statistics, layouts), linear_gemm256.hip (bf16 products),
+// linear_gemm.hip (fp32 products, the choice of a tile), linear_rows.hip (few rows), linear_few.hip (few classes).
 #pragma once
 #include "common.h"
 
@@ -107,7 +107,7 @@ int fea_lin_few_blocks(long long rows, bool bwd);
 int fea_lin_few_fwd(const LinFew& g, int dtype, hipStream_t s);
 int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 
-// linear_gemm.hip: which tile a product takes (256: linear_gemm256.hip, 128: linear_gemm.hip) and into how many parts its reduction is split
+// linear_gemm.hip: which tile a product takes and into how many parts its reduction is split
 struct LinTile { int tile, splits; double time; };
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split);
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s);

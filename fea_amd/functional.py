@@ -230,13 +230,15 @@ def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperatu
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor = None,
                          ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
-    """Softmax cross entropy of `hidden @ weight.T + bias` against one label per row, without keeping the logits.
+    """Softmax cross entropy of `hidden @ weight.T + bias` against one label per row.
 
     hidden [..., D] and weight [classes, D]: both float32 or both bfloat16 (sums, softmax and loss in 32 bits); target [...]
     integers; bias [classes], float32 or the weight's type.  Rows whose target is `ignore_index` do not count: loss 0 and
     gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
-    Differentiable once, in hidden, weight and bias; the backward recomputes the logits in pieces of the classes.
+    Differentiable once, in hidden, weight and bias.  The logits are never there in full precision and shape: for a backward
+    the forward keeps 2 bytes of each (4 in float32) if that is 8 GiB or less (FEA_AMD_LINEAR_KEEP: another limit in bytes,
+    0 for none); beyond it, with a bias gradient in bfloat16, and for up to 64 rows the backward recomputes them in pieces.
     An NHWC feature map and a 1x1 convolution's weight viewed [classes, channels] are taken as they are."""
     ignore_index = int(ignore_index)
     if not -(1 << 63) <= ignore_index < 1 << 63:
@@ -246,14 +248,14 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
                         bias: torch.Tensor = None, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
-    """Distillation of `hidden @ weight.T + bias` from a teacher's top logits, without keeping the student's logits.
+    """Distillation of `hidden @ weight.T + bias` from a teacher's top logits.
 
     teacher_logits [..., K] (float32 or bfloat16) and teacher_index [..., K] (integers): the teacher's K (1..256) largest logits of
     a row and their classes; a negative index is no entry.  With p = softmax(teacher_logits / T) over a row's entries and
     q = softmax of all the student's logits / T, the loss of a row is T^2 sum_k p_k (log p_k - log q_{index_k}).  Rows without
     an entry (or with -inf logits alone) do not count.  A class named twice in a row has the sum of both shares; an index
     beyond the classes, a NaN or +inf teacher logit make the loss and the gradients NaN.  The teacher has no gradient.
-    hidden, weight, bias, reduction and the result as in `linear_cross_entropy`."""
+    hidden, weight, bias, reduction, the result and what is kept for the backward as in `linear_cross_entropy`."""
     who = "linear_distillation"
     if not isinstance(teacher_logits, torch.Tensor) or not isinstance(teacher_index, torch.Tensor):
         raise ValueError(f"{who}: teacher_logits and teacher_index are tensors")

@@ -403,6 +403,64 @@ def test_same_result_every_time_and_on_another_stream():
             assert torch.equal(got[k], want[k]) and torch.equal(other[k], want[k]), k
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [0, 3])
+def test_kept_logits_captured_and_on_other_streams(dtype, top):
+    """Two steps at once on two streams, and a captured one replayed with other inputs, each with its own kept logits."""
+    cases = [O.case(300, 64, 700, dtype, seed=s, top=top, ignored=0.1) for s in (1, 2, 3)]
+    kw = {"temperature": 2.0} if top else {}
+    wants = [_run(*c, **kw) for c in cases]
+    torch.cuda.synchronize()
+    streams, gots = [torch.cuda.Stream() for _ in cases], []
+    for c, s in zip(cases, streams):
+        with torch.cuda.stream(s):
+            gots.append(_run(*c, **kw))
+    torch.cuda.synchronize()
+    for got, want in zip(gots, wants):
+        assert all(torch.equal(got[k], want[k]) for k in want)
+    x = [None if t is None else t.to(DEV) for t in cases[0]]
+    for t in x[:2]:
+        t.requires_grad_(True)
+
+    def step():
+        loss = F.linear_distillation(x[0], x[1], x[4], x[3], **kw) if top else F.linear_cross_entropy(x[0], x[1], x[3])
+        assert any(t is not None and t.dtype == torch.uint8 for t in loss.grad_fn.saved_tensors)
+        return [loss.detach(), *torch.autograd.grad(loss, x[:2])]
+
+    with torch.cuda.stream(streams[0]):
+        step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for c, want in list(zip(cases, wants))[::-1] + [(cases[0], wants[0])]:
+        with torch.no_grad():
+            for dst, src in zip(x, c):
+                if dst is not None:
+                    dst.copy_(src.to(DEV))
+        g.replay()
+        other = _run(*cases[1], **kw)                       # the program's own work in between
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, want[k]) for a, k in zip(out, ("loss", "hidden", "weight")))
+        assert all(torch.equal(other[k], wants[1][k]) for k in other)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_logits_kept_or_not(dtype, monkeypatch):
+    """A class at +inf has no softmax (inf - inf): the loss and the gradients it reaches are NaN, kept or recomputed."""
+    h, w, b, t = O.case(130, 64, 300, dtype, seed=5, bias=True)
+    b[200] = torch.inf
+    got = []
+    for keep in ("0", str(1 << 30)):
+        monkeypatch.setenv("FEA_AMD_LINEAR_KEEP", keep)
+        x, y = _leaf(h), _leaf(w)
+        loss = F.linear_cross_entropy(x, y, t.to(DEV), bias=b.to(DEV), reduction="sum")
+        got.append([loss.detach(), *torch.autograd.grad(loss, [x, y])])
+    assert bool(torch.isnan(got[0][0]))
+    for a, c in zip(*got):
+        assert torch.equal(torch.isnan(a), torch.isnan(c))
+
+
 @pytest.mark.parametrize("top", [0, 3])
 def test_captured_and_replayed(top):
     """Forward and backward in one captured graph, replayed with other inputs, the program's own work in between; a second graph
@@ -500,4 +558,15 @@ def test_workspace_and_operands_are_checked():
                 {"ws": ws.data_ptr() + 16}, {"d": 1 << 17, "ldh": 1 << 17}, {"keep": ws}):
         with pytest.raises(L.FeaError):
             fwd(**bad)
+    far = torch.zeros(1, device=DEV)                        # (refused before anything is read)
+    with pytest.raises(L.FeaError, match="strides"):
+        fwd(h=far, ldh=1 << 21, dt=L.BF16)
+    n = L.load().fea_linear_loss_keep_bytes(80, 32, 40, L.BF16)
+    keep, back = torch.empty(n, dtype=torch.uint8, device=DEV), torch.empty(1 << 24, dtype=torch.uint8, device=DEV)
+    x = torch.zeros(80, 32, dtype=torch.bfloat16, device=DEV)
+    f = torch.zeros(160, device=DEV)
+    for kp, db in ((keep, f), (keep.data_ptr() + 64, None)):
+        with pytest.raises(L.FeaError, match="kept"):
+            L.call("fea_linear_loss_bwd", x, 32, x, 32, None, t.repeat(5), 1, f, f, None, kp, None, f, 0, 1.0, x, None, db, back, back.numel(), 80, 32, 40,
+                   L.BF16, L.stream_ptr())
     torch.cuda.synchronize()
