@@ -403,10 +403,12 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
 }
 
 // dz at the selected classes of the piece [v0, v0 + N): softmax - teacher, from the forward's fp32 values.  Entries that name the
-// same class hold the same value.
-template <typename T, bool PL>
+// same class hold the same value.  Workgroups from `blocks` on copy operands.
+template <typename T, bool PL, bool ALN>
 __global__ __launch_bounds__(256) void lin_scatter_kernel(const long long* __restrict__ index, const float* __restrict__ dsel, int K,
-                                                          const float2* __restrict__ stat, T* dz, long long lddz, long long v0, int N, long long entries, int Npad) {
+                                                          const float2* __restrict__ stat, T* dz, long long lddz, long long v0, int N, long long entries, int Npad,
+                                                          unsigned blocks, const LinCopies copies) {
+    if constexpr (!PL) if (blockIdx.x >= blocks) return lin_copy_tile<T, false, ALN>(copies, blockIdx.x - blocks);
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= entries) return;
     const long long m = e / K, i = index[e] - v0;
@@ -864,7 +866,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                           lin_copy_of(d, f, hr, ldh, n, gated && iv == 0 ? b.hg : nullptr)}};
             js.j[0].stat = js.j[2].stat = st;
             if (gout_stride) { js.j[2].gout = go; js.j[2].t = temperature; }
-            if (!keep) LIN_TRY(lin_copy(d, f, js, s));
+            if (pack && !keep) LIN_TRY(lin_copy(d, f, js, s));       // (else they go along with a kernel below)
             const void* const wk = pack ? b.wp : (const void*)wr;
             const long long ldwk = pack ? f.row(D) : ldw;
             LinGemm g{};
@@ -893,11 +895,17 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             } else LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
             const long long entries = n * K;
             const long long* ix = index + r0 * K;
-            const unsigned sg = (unsigned)((entries + 255) / 256);
             if (!keep || K > 1) {
-                if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, g.Npad);
-                else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, 0);
-                else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false>), dim3(sg), dim3(256), 0, s, ix, dsel + r0 * K, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0);
+                const unsigned sg = (unsigned)((entries + 255) / 256);
+                if (pack || keep) js = LinCopies{};
+                const long long blocks = sg + js.j[0].tiles + js.j[1].tiles + js.j[2].tiles;
+                FEA_CHECK(blocks < INT_MAX, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld tiles", who, blocks);
+                const dim3 grid((unsigned)blocks), bl(256);
+                const float* ds = dsel + r0 * K;
+                if (f.dt == FEA_PL)        hipLaunchKernelGGL((lin_scatter_kernel<__bf16, true, true>), grid, bl, 0, s, ix, ds, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, g.Npad, sg, js);
+                else if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_scatter_kernel<__bf16, false, true>), grid, bl, 0, s, ix, ds, K, st, (__bf16*)b.dz, g.lddz, v0, nv, entries, 0, sg, js);
+                else if (d.odd())          hipLaunchKernelGGL((lin_scatter_kernel<float, false, false>), grid, bl, 0, s, ix, ds, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0, sg, js);
+                else                       hipLaunchKernelGGL((lin_scatter_kernel<float, false, true>), grid, bl, 0, s, ix, ds, K, st, (float*)b.dz, g.lddz, v0, nv, entries, 0, sg, js);
                 FEA_LAUNCH_CHECK();
             }
             if (db) {

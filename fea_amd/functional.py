@@ -119,6 +119,12 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _row_state(row, rows, k, teacher):
+    """Addresses of stat [rows, 2], dsel [rows, k] and, with a teacher, psel [rows, k] in the one tensor that holds them."""
+    at = row.data_ptr()
+    return at, at + rows * 8, at + rows * (8 + 4 * k) if teacher else None
+
+
 def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads):
     """One forward call.  grads: 0, or what the backward will want (1 hidden, 2 weight, 4 bias).  Returns (loss, saved)."""
     dev = hidden.device
@@ -131,16 +137,16 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     ix = ix.contiguous()
     b = None if bias is None else bias.detach().contiguous()
     dt = L.dt_code(h.dtype)
-    stat = dsel = psel = count = keep = None
+    row = keep = None
+    stat = dsel = psel = None
     if grads:
-        stat = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-        dsel = torch.empty((rows, k), dtype=torch.float32, device=dev)
-        psel = torch.empty((rows, k), dtype=torch.float32, device=dev) if tlog is not None else None
+        row = torch.empty(rows * (2 + k * (1 if tlog is None else 2)), dtype=torch.float32, device=dev)
+        stat, dsel, psel = _row_state(row, rows, k, tlog is not None)
         n = 0 if grads & 4 and dt == L.BF16 else L.load().fea_linear_loss_keep_bytes(rows, d, v, dt)
         if 0 < n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33)):
             keep = torch.empty(n, dtype=torch.uint8, device=dev)
     if reduction == "none":
-        loss = torch.empty(index.shape if tlog is None else index.shape[:-1], dtype=torch.float32, device=dev)
+        loss, count = torch.empty(index.shape if tlog is None else index.shape[:-1], dtype=torch.float32, device=dev), None
         outs = (loss, None, None, 0)
     else:
         loss = torch.empty((), dtype=torch.float32, device=dev)
@@ -154,29 +160,30 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
         tl = tlog.detach().contiguous()
         L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, keep, *outs,
                ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
-    return loss, (ix, stat, dsel, psel, keep, count)
+    return loss, (ix, row, keep, count)
 
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
         grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want)
-        loss, (ix, stat, dsel, psel, keep, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
+        loss, (ix, row, keep, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
         # the operands themselves are saved, so that autograd sees a change in place between forward and backward
-        ctx.save_for_backward(hidden, weight, bias, ix, stat, dsel, psel, keep, count if reduction == "mean" else None)
-        ctx.how = (temperature, reduction, dsel.shape[1], grads)
+        ctx.save_for_backward(hidden, weight, bias, ix, row, keep, count if reduction == "mean" else None)
+        ctx.how = (temperature, reduction, 1 if tlog is None else index.shape[-1], tlog is not None, grads)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):
-        hidden, weight, bias, ix, stat, dsel, psel, keep, count = ctx.saved_tensors
-        temperature, reduction, k, grads = ctx.how
+        hidden, weight, bias, ix, row, keep, count = ctx.saved_tensors
+        temperature, reduction, k, teacher, grads = ctx.how
         # (the autograd engine runs this on the forward's device and stream)
         h, w = _aligned_rows(hidden), _aligned_rows(weight)
         b = None if bias is None else bias.detach().contiguous()
         (rows, d), v = h.shape, w.shape[0]
         dt = L.dt_code(h.dtype)
+        stat, dsel, psel = _row_state(row, rows, k, teacher)
         dh = torch.empty(hidden.shape, dtype=h.dtype, device=h.device) if grads & 1 else None
         dw = torch.empty(weight.shape, dtype=w.dtype, device=w.device) if grads & 2 else None
         db = torch.empty(v, dtype=torch.float32, device=h.device) if grads & 4 else None
