@@ -89,7 +89,7 @@ SIGNATURES = {
     "fea_mask_iou": (I, [P, P, P, P, P, I, I, L, P]),
     "fea_binarise": (I, [P, P, L, P]),
     "fea_linear_loss_ws_bytes": (Z, [L, I, I, I, I, I]),
-    "fea_linear_loss_keep_bytes": (Z, [L, I, I, I]),
+    "fea_linear_loss_keep_bytes": (Z, [L, I, I, I, I]),
     "fea_linear_ce_fwd": (I, [P, L, P, L, P, P, L, P, P, P, P, P, P, I, P, Z, L, I, I, I, P]),
     "fea_linear_kd_fwd": (I, [P, L, P, L, P, P, I, P, I, F, P, P, P, P, P, P, P, I, P, Z, L, I, I, I, P]),
     "fea_linear_loss_bwd": (I, [P, L, P, L, P, P, I, P, P, P, P, P, P, I, F, P, P, P, P, Z, L, I, I, I, P]),

@@ -316,11 +316,12 @@ struct LinDecode {
     unsigned blocks;                      // of this; the ones behind it copy operands
     LinCopies copies;
 };
-template <bool CODES, bool PL, bool ALN>
+// T: what the products take; CODES: 16 bits are kept, else fp32; PL: planes
+template <typename T, bool CODES, bool PL, bool ALN>
 __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
     __shared__ float ref[128], none[128], scale[128], dpick[128], red[16][128];
     __shared__ int pick[128], counts[128];
-    if (blockIdx.x >= g.blocks) return lin_copy_tile<std::conditional_t<CODES, __bf16, float>, PL, ALN>(g.copies, blockIdx.x - g.blocks);
+    if (blockIdx.x >= g.blocks) return lin_copy_tile<std::conditional_t<PL, float, T>, PL, ALN>(g.copies, blockIdx.x - g.blocks);
     const int id = blockIdx.x, tc = id % g.nct, tm = id / g.nct, tid = threadIdx.x;
     const int r0 = tm * 128, c = tc * 128 + (tid & 15) * 8, y = tid >> 4;
     const bool in = c < g.Npad;
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(256) void lin_decode_kernel(const LinDecode g) {
         if ((unsigned)(pick[l] - c) < 8u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) if (pick[l] - c == e) v[e] = dpick[l];
-        if constexpr (CODES) {
+        if constexpr (sizeof(T) == 2 && !PL) {
             __bf16 x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = (__bf16)v[e];
@@ -648,14 +649,17 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     return c.at;
 }
 
-// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16) or fp32, then (bf16) the groups' largest.  Not for the heads that
-// read no more for recomputing them: few rows (the weight once more) and few classes (nothing).
+// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16 operands) or fp32 (fp32, and the few rows of linear_rows.hip), then, with 16 bits, the
+// groups' largest.  Not for few classes, where recomputing reads no more, and not in 16 bits for a bias gradient, which is fp32.
+static bool lin_keep_codes(const LinDims& d) { return d.dtype == FEA_BF16 && d.rows > 64; }
 static long long lin_keep_ld(const LinDims& d) { return up(d.V, 64); }
-static size_t lin_keep_table(const LinDims& d) { return (size_t)up(d.rows * lin_keep_ld(d) * d.es, 256); }
-extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype) {
-    if (rows <= 64 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
+static int lin_keep_es(const LinDims& d) { return lin_keep_codes(d) ? 2 : 4; }
+static size_t lin_keep_table(const LinDims& d) { return (size_t)up(d.rows * lin_keep_ld(d) * lin_keep_es(d), 256); }
+extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int grads) {
+    if (rows <= 0 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
     const LinDims d = lin_dims(rows, D, V, 1, dtype);
-    return lin_keep_table(d) + (dtype == FEA_BF16 ? (size_t)rows * lin_fwd_plan(d).ntn * 8 * sizeof(float) : 0);
+    if (lin_keep_codes(d) && grads & 4) return 0;
+    return lin_keep_table(d) + (lin_keep_codes(d) ? (size_t)rows * lin_fwd_plan(d).ntn * 8 * sizeof(float) : 0);
 }
 
 extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads) {
@@ -724,7 +728,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
     LinFwdWs b;
     const size_t need = lin_fwd_carve(d, p, (char*)ws, b);
     FEA_CHECK(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, FEA_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, need, ws_bytes);
-    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(d.rows, d.D, d.V, (int)d.dtype) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
+    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(d.rows, d.D, d.V, (int)d.dtype, 0) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
     FEA_CHECK(!loss == !count, FEA_E_BADARG, "%s: loss and count go together", who);
     FEA_CHECK(loss || j.loss_rows, FEA_E_BADARG, "%s: nothing to write", who);
 
@@ -762,8 +766,8 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
         if (keep) {
-            g.keep = (char*)keep + r * lin_keep_ld(d) * d.es; g.ldkeep = lin_keep_ld(d);
-            if (d.dtype == FEA_BF16) { g.ldtop = d.rows; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * 4; }
+            g.keep = (char*)keep + r * lin_keep_ld(d) * lin_keep_es(d); g.ldkeep = lin_keep_ld(d);
+            if (lin_keep_codes(d)) { g.ldtop = d.rows; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * 4; }
         }
         if (p.pick) { g.zsel = b.zsel + r * d.K; g.index = j.index + r * d.K; g.sel = d.K; }
         if (p.pick == 2) {
@@ -832,8 +836,8 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     FEA_CHECK(((uintptr_t)dh | (uintptr_t)dw) % 16 == 0 && (uintptr_t)db % 4 == 0, FEA_E_BADARG, "%s: misaligned gradient", who);
     FEA_CHECK(K == 1 || !db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
     FEA_CHECK(temperature > 0.f && isfinite(temperature) && isfinite(1.f / temperature), FEA_E_BADARG, "%s: temperature %g", who, (double)temperature);
-    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(rows, D, V, dtype) > 0 && !(db && dtype == FEA_BF16)), FEA_E_BADARG,
-              "%s: no logits are kept of these sizes (or, bf16, for a bias gradient), or misaligned", who);
+    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(rows, D, V, dtype, db ? 4 : 0) > 0), FEA_E_BADARG,
+              "%s: no logits are kept of these sizes (or, in 16 bits, for a bias gradient), or misaligned", who);
     const int want = (dh ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0) | (keep ? 8 : 0);
     const LinBwd p = lin_bwd_plan(d, want);
     LinBwdWs b;
@@ -878,7 +882,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             g.colsum = db ? b.colsum : nullptr; g.ldcol = up(p.vc, 64);
             if (keep) {
                 LinDecode x{};
-                x.z = (const char*)keep + (r0 * lin_keep_ld(d) + v0) * d.es; x.ldz = lin_keep_ld(d);
+                x.z = (const char*)keep + (r0 * lin_keep_ld(d) + v0) * lin_keep_es(d); x.ldz = lin_keep_ld(d);
                 x.ldtop = rows; x.top = (const float*)((const char*)keep + lin_keep_table(d)) + r0 * 4; x.shift = kp.tile == 256 ? 7 : 6;
                 x.stat = st; x.gout = go; x.gstride = gout_stride; x.count = count; x.t = temperature;
                 x.dz = b.dz; x.lddz = g.lddz; x.Npad = g.Npad; x.colsum = g.colsum; x.ldcol = g.ldcol;
@@ -888,9 +892,11 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 const long long blocks = x.blocks + js.j[0].tiles + js.j[1].tiles + js.j[2].tiles;
                 FEA_CHECK(blocks < INT_MAX, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld tiles", who, blocks);
                 const dim3 grid((unsigned)blocks), bl(256);
-                if (dtype == FEA_BF16) { if (d.odd()) hipLaunchKernelGGL((lin_decode_kernel<true, false, false>), grid, bl, 0, s, x); else hipLaunchKernelGGL((lin_decode_kernel<true, false, true>), grid, bl, 0, s, x); }
-                else if (p.planes)     { if (d.odd()) hipLaunchKernelGGL((lin_decode_kernel<false, true, false>), grid, bl, 0, s, x); else hipLaunchKernelGGL((lin_decode_kernel<false, true, true>), grid, bl, 0, s, x); }
-                else                   { if (d.odd()) hipLaunchKernelGGL((lin_decode_kernel<false, false, false>), grid, bl, 0, s, x); else hipLaunchKernelGGL((lin_decode_kernel<false, false, true>), grid, bl, 0, s, x); }
+                auto launch = [&](auto even, auto odd) { if (d.odd()) hipLaunchKernelGGL(odd, grid, bl, 0, s, x); else hipLaunchKernelGGL(even, grid, bl, 0, s, x); };
+                if (lin_keep_codes(d))      launch(lin_decode_kernel<__bf16, true, false, true>, lin_decode_kernel<__bf16, true, false, false>);
+                else if (dtype == FEA_BF16) launch(lin_decode_kernel<__bf16, false, false, true>, lin_decode_kernel<__bf16, false, false, false>);
+                else if (p.planes)          launch(lin_decode_kernel<float, false, true, true>, lin_decode_kernel<float, false, true, false>);
+                else                        launch(lin_decode_kernel<float, false, false, true>, lin_decode_kernel<float, false, false, false>);
                 FEA_LAUNCH_CHECK();
             } else LIN_TRY(fea_lin_gemm(LIN_DZ, f.dt, p.tz, g, s));
             const long long entries = n * K;

@@ -102,6 +102,8 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
             z[e] = n0 + 4 * q16 + e < g.N ? raw * g.inv_t : -INFINITY;
             mx = fmaxf(mx, z[e]);
         }
+        if (g.keep && 16 * i + r16 < g.M)
+            *reinterpret_cast<f32x4*>((float*)g.keep + (16 * i + r16) * g.ldkeep + n0 + 4 * q16) = f32x4{z[0], z[1], z[2], z[3]};
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
         const float base = mx == -INFINITY ? 0.f : mx;

@@ -142,7 +142,7 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     if grads:
         row = torch.empty(rows * (2 + k * (1 if tlog is None else 2)), dtype=torch.float32, device=dev)
         stat, dsel, psel = _row_state(row, rows, k, tlog is not None)
-        n = 0 if grads & 4 and dt == L.BF16 else L.load().fea_linear_loss_keep_bytes(rows, d, v, dt)
+        n = L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, grads)
         if 0 < n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33)):
             keep = torch.empty(n, dtype=torch.uint8, device=dev)
     if reduction == "none":
@@ -244,8 +244,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
     Differentiable once, in hidden, weight and bias.  The logits are never there in full precision and shape: for a backward
-    the forward keeps 2 bytes of each (4 in float32) if that is 8 GiB or less (FEA_AMD_LINEAR_KEEP: another limit in bytes,
-    0 for none); beyond it, with a bias gradient in bfloat16, and for up to 64 rows the backward recomputes them in pieces.
+    the forward keeps 2 bytes of each (4 in float32 and for up to 64 rows) if that is 8 GiB or less (FEA_AMD_LINEAR_KEEP:
+    another limit in bytes, 0 for none); beyond it, and with a bias gradient in bfloat16, the backward recomputes them in pieces.
     An NHWC feature map and a 1x1 convolution's weight viewed [classes, channels] are taken as they are."""
     ignore_index = int(ignore_index)
     if not -(1 << 63) <= ignore_index < 1 << 63:

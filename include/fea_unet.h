@@ -357,10 +357,10 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
  * psel[rows][K] (all nullable), and keep (nullable): fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned, for the logits: fp32, or with bf16
- * operands 16 bits (z below the largest of its 16 or 32 in steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0).
- * 0 bytes = none are kept (rows <= 64, few classes with few features: recomputing them reads next to nothing more).
+ * operands and more than 64 rows 16 bits (z below the largest of its 16 or 32 in steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0).
+ * 0 bytes = none are kept (few classes with few features: recomputing them reads no more; 16 bits where grads holds a bias gradient).
  *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the
- *     logits from the forward's keep, or (NULL; with bf16 operands a bias gradient asks for it) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
+ *     logits from the forward's keep, or (NULL) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
  *     value (gout_stride 0) or one per row (1); count: divide it by count[0] (mean) or NULL.
  * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are taken at any alignment.
  * fp32: products of a certain size run as six products of bf16 planes (24 bits in three), the others on the fp32 matrix rate.
@@ -368,7 +368,7 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * backward, + 8 with keep
  * (0 bytes = sizes that are refused).  Results are the same from run to run. */
 size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);
-size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype);
+size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int grads);
 int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
                       long long ignore_index, float* stat, float* dsel, void* keep, float* loss_rows, float* loss,
                       int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
