@@ -111,7 +111,8 @@ int fea_lin_few_bwd(LinFew g, int dtype, void* dw, float* db, hipStream_t s);
 struct LinTile { int tile, splits; double time; };
 LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool split);
 int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s);
-// linear_rows.hip: LIN_LSE of up to 64 label rows; g.part [M][classes / 64]
+// linear_rows.hip: LIN_LSE of up to 64 label rows; g.part [M][classes / 64], or, with g.splits > 1, sums g.slab [splits][M][ldo]
+int fea_lin_rows_splits(int dtype, int V, int D);
 int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s);
 // linear_gemm256.hip
 void fea_lin_gemm256(int epi, int tile, bool planes, const LinGemm& g, unsigned grid, hipStream_t s);

@@ -281,6 +281,35 @@ __global__ __launch_bounds__(256) void lin_join_rows_kernel(const LinJoin j) {
     lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64, lin_lse_of(lin_merge(lin_merge(red[0], red[1]), lin_merge(red[2], red[3]))));
 }
 
+// Few rows whose reduction is split: the parts' sums make z, one workgroup per row.
+struct LinParts { const float* slab; int parts; long long ld; const float* bias; float* keep; };      // keep (nullable): rows of ld
+__global__ __launch_bounds__(256) void lin_join_split_kernel(const LinJoin j, const LinParts t) {
+    __shared__ float2 red[4];
+    const long long row = blockIdx.x, next = j.rows * t.ld;
+    const float* const s = t.slab + row * t.ld;
+    float2 a = make_float2(-INFINITY, 0.f);
+    for (int v = 4 * threadIdx.x; v < t.ld; v += 1024) {
+        f32x4 z = *reinterpret_cast<const f32x4*>(s + v);
+        for (int p = 1; p < t.parts; ++p) z += *reinterpret_cast<const f32x4*>(s + p * next + v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = v + e < j.V ? (z[e] + (t.bias ? t.bias[v + e] : 0.f)) * j.inv_t : -INFINITY;
+        if (t.keep) *reinterpret_cast<f32x4*>(t.keep + row * t.ld + v) = z;
+        const float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), base = mx == -INFINITY ? 0.f : mx;
+        a = lin_merge(a, make_float2(mx, expf(z[0] - base) + expf(z[1] - base) + expf(z[2] - base) + expf(z[3] - base)));
+    }
+    for (int k = threadIdx.x; k < j.K; k += 256) {
+        const long long i = j.index[row * j.K + k];
+        if (i < 0 || i >= j.V) continue;
+        float z = s[i];
+        for (int p = 1; p < t.parts; ++p) z += s[p * next + i];
+        j.zsel[row * j.K + k] = (z + (t.bias ? t.bias[i] : 0.f)) * j.inv_t;
+    }
+    a = lin_merge_lanes(a, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64, lin_lse_of(lin_merge(lin_merge(red[0], red[1]), lin_merge(red[2], red[3]))));
+}
+
 // loss[0] = sum, or sum / rows that count (0 where none does); count[0] = rows that count
 __global__ __launch_bounds__(1024) void lin_total_kernel(const double* bsum, const int* bcnt, long long n, int mean, float* loss, int* count) {
     __shared__ double ls[1024];
@@ -541,7 +570,7 @@ static LinForm lin_form(int dtype, bool planes) {
 }
 
 // Forward: rows in chunks that bound the partial table to 128 MB.
-struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; int pick; };   // pick: 0 selected logits by dot products, 1 out of the product, 2 with lin_where_kernel
+struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; int pick, parts; };   // pick: 0 selected logits by dot products, 1 out of the product, 2 with lin_where_kernel; parts: of few rows' reduction
 static LinFwd lin_fwd_plan(const LinDims& d) {
     LinFwd p;
     const long long cap = (1ll << 24) / ((d.V + 127) / 128);
@@ -558,7 +587,8 @@ static LinFwd lin_fwd_plan(const LinDims& d) {
     p.ntn = (d.V + p.tile - 1) / p.tile;
     // selected logits come out of the product where it can give them
     const bool tiles = p.tile != 64 && (d.dtype == FEA_BF16 || p.planes);
-    p.pick = p.tile == 64 ? d.rows * d.K <= 2048 : !tiles ? 0 : d.K == 1 ? 1 : d.K <= LIN_WHERE_K && p.ntn <= LIN_WHERE_T ? 2 : 0;
+    p.parts = p.tile == 64 ? fea_lin_rows_splits((int)d.dtype, d.V, d.D) : 1;
+    p.pick = p.tile == 64 ? p.parts > 1 || d.rows * d.K <= 2048 : !tiles ? 0 : d.K == 1 ? 1 : d.K <= LIN_WHERE_K && p.ntn <= LIN_WHERE_T ? 2 : 0;
     p.G = 1;
     while (p.G < 64 && (p.G < (d.V + 127) / 128 || p.G < d.K)) p.G *= 2;
     p.blocks = p.tile == 64 ? d.rows : (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
@@ -601,7 +631,7 @@ static LinBwd lin_bwd_plan(const LinDims& d, int want) {       // want: 1 dh, 2 
     return p;
 }
 
-struct LinFwdWs { void *hp, *wp; float2* part; float* zsel; uint2* where; double* bsum; int* bcnt; };
+struct LinFwdWs { void *hp, *wp; float2* part; float *zsel, *slab; uint2* where; double* bsum; int* bcnt; };
 static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFwdWs& w) {
     LinCarve c{base};
     if (fea_lin_few(d.rows, d.D, d.V)) {
@@ -615,6 +645,7 @@ static size_t lin_fwd_carve(const LinDims& d, const LinFwd& p, char* base, LinFw
     w.bsum = c.take<double>(p.blocks);
     w.bcnt = c.take<int>(p.blocks);
     w.hp = w.wp = nullptr;
+    w.slab = p.parts > 1 ? c.take<float>(p.parts * d.rows * up(d.V, 64)) : nullptr;
     w.where = p.pick == 2 ? c.take<uint2>(p.rc * p.ntn) : nullptr;
     if (p.planes || (d.dtype == FEA_BF16 && d.odd() && p.tile != 64)) {
         const LinForm f = lin_form(d.dtype, p.planes);
@@ -775,6 +806,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
             hipLaunchKernelGGL(lin_where_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 4 * 3 * p.ntn * sizeof(uint32_t), s, g.index, d.K, n, d.V, p.tile, p.ntn, b.where);
             FEA_LAUNCH_CHECK();
         }
+        if (p.parts > 1) { g.zsel = nullptr; g.slab = b.slab; g.ldo = up(d.V, 64); g.splits = p.parts; }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
         else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;
@@ -787,7 +819,8 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         if (q.loss_rows) q.loss_rows += r;
         q.bsum = loss ? b.bsum + blk : nullptr; q.bcnt = b.bcnt + blk;
         const long long grid = p.tile == 64 ? n : (n + 256 / p.G - 1) / (256 / p.G);
-        if (p.tile == 64) hipLaunchKernelGGL(lin_join_rows_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
+        if (p.parts > 1)       hipLaunchKernelGGL(lin_join_split_kernel, dim3((unsigned)grid), dim3(256), 0, s, q, (LinParts{b.slab, p.parts, up(d.V, 64), bias, (float*)keep}));
+        else if (p.tile == 64) hipLaunchKernelGGL(lin_join_rows_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
         else              hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
         FEA_LAUNCH_CHECK();
         blk += grid;

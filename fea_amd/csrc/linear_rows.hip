@@ -33,12 +33,13 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
     const int n0 = blockIdx.x * CLS + wave * 16;
     const T* const w = (const T*)g.b + (long long)min(n0 + r16, g.N - 1) * g.ldb;
     const T* const h = (const T*)g.a;
+    const int kb = blockIdx.y * g.kper, K = min(kb + g.kper, g.K);       // part of a split reduction
     u32x4 wv[RING][NS];
     auto wload = [&](int buf, int k0) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             const int k = k0 + (4 * s + q16) * EPC;
-            wv[buf][s] = lin_load16<T, ALN>(w + k, g.K - k);
+            wv[buf][s] = lin_load16<T, ALN>(w + k, K - k);
         }
     };
     constexpr int HP = NR * 16 * PR / NT;           // 16-byte pieces of the labels' chunk per thread
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
 #pragma unroll
         for (int i = 0; i < HP; ++i) {
             const int p = tid + NT * i, row = p / PR, k = k0 + (p % PR) * EPC;
-            hv[buf][i] = row < g.M ? lin_load16<T, ALN>(h + row * g.lda + k, g.K - k) : u32x4{0, 0, 0, 0};
+            hv[buf][i] = row < g.M ? lin_load16<T, ALN>(h + row * g.lda + k, K - k) : u32x4{0, 0, 0, 0};
         }
     };
     auto hput = [&](int buf) {
@@ -62,9 +63,9 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
     for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     // The workgroups start their reduction at different chunks (it ends where it began): in step they would all ask for the same
     // columns of rows that lie a power of two apart, that is for a few of the memory channels at a time.
-    const int rounds = (g.K + RING * CE - 1) / (RING * CE), nch = rounds * RING;
+    const int rounds = (K - kb + RING * CE - 1) / (RING * CE), nch = rounds * RING;
     int at = (int)(3u * blockIdx.x % (unsigned)nch);
-    auto chunk = [&](int ahead) { int c = at + ahead; return (c >= nch ? c - nch : c) * CE; };
+    auto chunk = [&](int ahead) { int c = at + ahead; return kb + (c >= nch ? c - nch : c) * CE; };
     hload(0, chunk(0));
     wload(0, chunk(0));
     hload(1, chunk(1));
@@ -84,6 +85,12 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
                 for (int i = 0; i < NR; ++i)
                     mma16x16(acc[i], wv[c][s], *reinterpret_cast<const u32x4*>(hs[c & 1] + (16 * i + r16) * LD + (4 * s + q16) * 16), (const T*)nullptr);
         }
+    }
+    if (g.slab) {            // split: the sums as they are, joined by lin_join_split_kernel
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            if (16 * i + r16 < g.M) *reinterpret_cast<f32x4*>(g.slab + ((long long)blockIdx.y * g.M + 16 * i + r16) * g.ldo + n0 + 4 * q16) = acc[i];
+        return;
     }
     // the selected logits: every workgroup looks for its own classes among the entries
     __syncthreads();
@@ -130,19 +137,36 @@ __global__ __launch_bounds__(256, NR == 4 ? 3 : 4) void lin_rows_kernel(const Li
     }
 }
 
-template <typename T, bool ALN> static void rows_launch(const LinGemm& g, unsigned grid, hipStream_t s) {
-    if (g.M <= 16)      hipLaunchKernelGGL((lin_rows_kernel<T, 1, ALN>), dim3(grid), dim3(256), 0, s, g);
-    else if (g.M <= 32) hipLaunchKernelGGL((lin_rows_kernel<T, 2, ALN>), dim3(grid), dim3(256), 0, s, g);
-    else if (g.M <= 48) hipLaunchKernelGGL((lin_rows_kernel<T, 3, ALN>), dim3(grid), dim3(256), 0, s, g);
-    else                hipLaunchKernelGGL((lin_rows_kernel<T, 4, ALN>), dim3(grid), dim3(256), 0, s, g);
+template <typename T, bool ALN> static void rows_launch(const LinGemm& g, dim3 grid, hipStream_t s) {
+    if (g.M <= 16)      hipLaunchKernelGGL((lin_rows_kernel<T, 1, ALN>), grid, dim3(256), 0, s, g);
+    else if (g.M <= 32) hipLaunchKernelGGL((lin_rows_kernel<T, 2, ALN>), grid, dim3(256), 0, s, g);
+    else if (g.M <= 48) hipLaunchKernelGGL((lin_rows_kernel<T, 3, ALN>), grid, dim3(256), 0, s, g);
+    else                hipLaunchKernelGGL((lin_rows_kernel<T, 4, ALN>), grid, dim3(256), 0, s, g);
 }
 
+
+// Parts of the reduction: few classes make few workgroups, and one of them reads its 64 classes no faster for that.  Below 256 of them (bf16: 128)
+// about 512 in all, each with at least 8 chunks.  A loss of 30 rows x 3,840 x 3,840, one part and split: fp32 61 and 36 us, bf16 31 and
+// 21.5; 64 x 2,048 x 300: 57 and 23, 23 and 17; 64 x 1,024 x 8,192 (128 workgroups): 35 and 29, 18.5 and 18; 16 x 8,192 x 16,000 (250):
+// 119 and 108, 52 and 60.
+int fea_lin_rows_splits(int dtype, int V, int D) {
+    const int tiles = (V + 63) / 64, chunks = (D + (dtype == FEA_BF16 ? 127 : 63)) / (dtype == FEA_BF16 ? 128 : 64);
+    if (tiles >= (dtype == FEA_BF16 ? 128 : 256)) return 1;
+    const int want = 512 / tiles, most = chunks / 8;
+    const int parts = most < 1 ? 1 : want < most ? want : most, per = (chunks + parts - 1) / parts;
+    return (chunks + per - 1) / per;                            // (no part is empty)
+}
 
 // LIN_LSE of at most 64 label rows, operands of any alignment
 int fea_lin_rows(int dtype, bool aligned, LinGemm g, hipStream_t s) {
     FEA_CHECK(g.M > 0 && g.M <= 64 && g.N > 0 && g.K > 0, FEA_E_BADARG, "lin_rows: %d x %d x %d", g.M, g.N, g.K);
+    FEA_CHECK((g.slab != nullptr) == (g.splits > 1), FEA_E_BADARG, "lin_rows: %d parts", g.splits);
     g.ntn = (g.N + 63) / 64;
-    const unsigned grid = (unsigned)g.ntn;
+    const int unit = dtype == FEA_BF16 ? 128 : 64;             // channels of a chunk
+    if (g.splits < 1) g.splits = 1;
+    g.kper = ((g.K + g.splits - 1) / g.splits + unit - 1) / unit * unit;
+    FEA_CHECK((long long)(g.splits - 1) * g.kper < g.K, FEA_E_BADARG, "lin_rows: %d parts of %d channels", g.splits, g.K);
+    const dim3 grid((unsigned)g.ntn, (unsigned)g.splits);
     if (dtype == FEA_BF16) { if (aligned) rows_launch<__bf16, true>(g, grid, s); else rows_launch<__bf16, false>(g, grid, s); }
     else                   { if (aligned) rows_launch<float, true>(g, grid, s); else rows_launch<float, false>(g, grid, s); }
     FEA_LAUNCH_CHECK();

@@ -58,6 +58,19 @@ def test_most_entries(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 4096, 5), (17, 1543, 300), (40, 2056, 1000), (64, 20600, 130), (3, 5000, 16000), (30, 3840, 3840)])
+@pytest.mark.parametrize("top", [0, 3, 256])
+def test_few_rows_and_classes_split_the_reduction(shape, dtype, top):
+    """Long reductions over few classes, in parts, with ragged last ones."""
+    c = O.case(*shape, dtype, seed=71 + top, top=top, ignored=0.1, short=0.2, bias=shape[0] % 2 == 1)
+    _compare(_run(*c), O.evaluate(*c))
+    with torch.no_grad():
+        x = [None if t is None else t.to(DEV) for t in c]
+        loss = F.linear_distillation(x[0], x[1], x[4], x[3], bias=x[2], reduction="none") if top else F.linear_cross_entropy(x[0], x[1], x[3], bias=x[2], reduction="none")
+    O.check("loss", loss, O.evaluate(*c, reduction="none")["loss"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape,top", [((100, 64, 300), 254), ((100, 64, 300), 255), ((70, 8, 170000), 5), ((300, 72, 2000), 4), ((300, 72, 2000), 40)])
 def test_where_the_entries_are(shape, top, dtype):
     """Selected logits out of the product: four entries in a column tile and more, all in one tile, in too many tiles, too many entries."""
