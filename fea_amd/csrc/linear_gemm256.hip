@@ -8,7 +8,8 @@
 //
 // 256 tile: chunks of 64 channels (whole 128-byte lines) go from memory to LDS without a register in between, a wave's 1,024 bytes per load, in
 // a ring of five operand chunks of 32 KB (all of the CU's 160 KB): 16 loads per chunk, one per 8 MFMA, 1 to 1.5 chunks ahead; one
-// barrier per chunk.  128 tile (two workgroups per CU): through registers, two chunks on the way, two LDS stages.
+// barrier per chunk.  128 tile (two workgroups per CU): through registers, three chunks on the way
+// (two: 20 % slower where few workgroups go through a long reduction, 150 x 4,096 x 8,000), two LDS stages.
 // Loads are buffer loads with every bound in the descriptor or the lane's offset: rows, classes and channels behind the end arrive as zeros
 // without a branch.
 //
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     const unsigned va = TA ? (unsigned)(tr * (int)g.lda * 2 + tc * 16) : (unsigned)(r * (int)g.lda * 2 + c * 16), va1 = DL && TA ? va + ((tc ^ 8) - tc) * 16 : va;
     const unsigned vb = TB ? (unsigned)(tr * (int)g.ldb * 2 + tc * 16) : (unsigned)(rb * (int)g.ldb * 2 + c * 16), vb1 = DL && TB ? vb + ((tc ^ 8) - tc) * 16 : vb;
     const unsigned sa = 2 * (TA ? RPP : 32) * (unsigned)g.lda, sb = 2 * (TB ? RPP : 32) * (unsigned)g.ldb;      // bytes from load i to i + 1
-    constexpr int SETS = 2;           // 128 tile: chunks on the way in registers
+    constexpr int SETS = TB && !TA ? 2 : 3;           // 128 tile: chunks on the way in registers (two where a third would not fit)
     u32x4 st[DL ? 1 : SETS][DL ? 1 : NL];
     // the XCDs start their reduction an eighth apart (it ends where it began): in step, every workgroup of the chip would ask for the
     // same columns of its rows at a time.  Within an XCD all are in step: they share operands in its L2.
@@ -315,10 +316,9 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             }
         }
     };
-    for (int ch = 0; ch < nc; ch += 2) {
-        step(ch, 0, 1);
-        if (ch + 1 < nc) step(ch + 1, 1, 0);
-    }
+    for (int ch = 0; ch < nc; ch += 2 * SETS)
+#pragma unroll
+        for (int i = 0; i < 2 * SETS; ++i) if (ch + i < nc) step(ch + i, i & 1, (i + 1) % SETS);
     }
     __syncthreads();
 
