@@ -561,7 +561,8 @@ static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
 // The form that a call's products take: the operands as they are, or fp32 as three bf16 planes where the copies pay.
 struct LinForm {
     int dt, es, mul, pad;         // dtype of the products, bytes of an element, elements of a row per channel, what a row is rounded up to
-    long long row(long long k) const { const long long r = up(k, pad) * mul; return r % 128 ? r : r + 64; }          // elements of a row of k channels
+    // elements of a row of k channels: an odd number of 64, so that rows do not lie a power of two apart (dz of 65,536 classes: 1 %)
+    long long row(long long k) const { const long long r = up(k, pad) * mul; return r % 128 ? r : r + 64; }
     int K(long long k) const { return (int)(dt == FEA_PL ? 6 * up(k, 64) : dt == FEA_BF16 ? up(k, 64) : k); }      // reduction over k channels
 };
 static LinForm lin_form(int dtype, bool planes) {
@@ -622,7 +623,7 @@ static LinBwd lin_bwd_plan(const LinDims& d, int want) {       // want: 1 dh, 2 
     };
     const double t = tiles(d.dtype, 1, tz, p.th, p.tw);
     p.planes = false;
-    if (d.dtype == FEA_F32 && 3 * up(p.vc, 64) < 1 << 21) {     // (the strides that the bf16 kernels take)
+    if (d.dtype == FEA_F32 && 3 * up(p.vc, 64) + 64 < 1 << 21) {     // (the strides that the bf16 kernels take)
         LinTile z, h, w;
         const double q = tiles(FEA_PL, 6, z, h, w);
         if (q + (((double)p.rc + p.vc) * d.D * 10 + 2.0 * p.rc * p.vc) / 4e12 + 6e-6 < t) { tz = z; p.th = h; p.tw = w; p.planes = true; }

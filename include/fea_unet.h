@@ -347,7 +347,7 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
 
 /* ---- loss heads over many classes (not in the reference: its head has 6 sigmoid classes, models.py:23) ----------------
  * A projection z = (h . w^T + bias) / T of hidden rows h[rows][ldh] onto V classes w[V][ldw] (D features, fp32 or bf16, both of
- * `dtype`; bias[V] fp32, nullable) and a loss of its softmax, without keeping z.
+ * `dtype`; bias[V] fp32, nullable) and a loss of its softmax.
  *   fea_linear_ce_fwd (T = 1): loss_n = lse_n - z_{n,target[n]}; rows with target = ignore_index do not count.
  *   fea_linear_kd_fwd: the teacher's K entries of a row are (teacher_index, teacher_logits); index < 0 = no entry;
  *     p = softmax(teacher_logits / T) over the row's entries; loss_n = T^2 sum_k p_k (log p_k - z_{n,index_k} + lse_n).
@@ -356,13 +356,16 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * teacher logit that is NaN or +inf: the row's loss and the gradients it reaches are NaN (nothing is read out of range).
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
- * psel[rows][K] (all nullable), and keep (nullable): fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned, for the logits: fp32, or with bf16
- * operands and more than 64 rows 16 bits (z below the largest of its 16 or 32 in steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0).
- * 0 bytes = none are kept (few classes with few features: recomputing them reads no more; 16 bits where grads holds a bias gradient).
- *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the
- *     logits from the forward's keep, or (NULL) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one
- *     value (gout_stride 0) or one per row (1); count: divide it by count[0] (mean) or NULL.
- * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows; other D are taken at any alignment.
+ * psel[rows][K] (all nullable), and keep (nullable): room for the logits, fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned.
+ * They are kept in fp32, or with bf16 operands and more than 64 rows in 16 bits: z below the largest of its 16 or 32 in steps of
+ * 64 / 65535, half a step off; 64 and more below counts as a share of 0.  0 bytes = none are kept (few classes with few features:
+ * recomputing them reads no more; 16 bits where grads holds a bias gradient).
+ *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the logits from the
+ *     forward's keep, or (NULL) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte
+ *     aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one value (gout_stride 0) or one per row (1);
+ *     count: divide it by count[0] (mean) or NULL.
+ * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows (bf16: less than 2^21 elements apart); other D are
+ * taken at any alignment.
  * fp32: products of a certain size run as six products of bf16 planes (24 bits in three), the others on the fp32 matrix rate.
  * ws: fea_linear_loss_ws_bytes(..., grads) bytes, 256-byte aligned; grads = 0 for the forwards, 1 dh + 2 dw + 4 db for the
  * backward, + 8 with keep

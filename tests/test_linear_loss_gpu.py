@@ -101,6 +101,19 @@ def test_pieces(shape, dtype, top, monkeypatch):
     _compare(_run(*c), O.evaluate(*c))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(300, 72, 900), (700, 40, 2000), (60, 33, 3000), (513, 643, 1999)])
+@pytest.mark.parametrize("top", [0, 4])
+@pytest.mark.parametrize("piece", [1 << 16, 1 << 27])
+def test_pieces_of_kept_logits(shape, dtype, top, piece, monkeypatch):
+    """The same from kept logits, with an upstream gradient for every row."""
+    monkeypatch.setenv("FEA_AMD_LINEAR_PIECE", str(piece))
+    c = O.case(*shape, dtype, seed=10, top=top, ignored=0.1, short=0.2)
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(2))
+    _compare(_run(*c, gout=gout, reduction="none"), O.evaluate(*c, gout=gout, reduction="none"))
+    _compare(_run(*c), O.evaluate(*c))
+
+
 @pytest.mark.parametrize("shape", [(4096, 64, 4096), (4000, 200, 4100), (2049, 1096, 2310), (4097, 72, 8185), (300, 520, 40000), (1300, 643, 2011)])
 @pytest.mark.parametrize("top", [0, 5])
 @pytest.mark.parametrize("dtype", TYPES)
