@@ -162,28 +162,22 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, B[ks][j]), __builtin_bit_cast(bf16x8, A[ks][i]), acc[i][j], 0, 0, 0);
     };
 
-    // LIN_LSE: the selected classes of the tile's row tid (asked for behind the first chunk's loads, wanted in the epilogue)
+    // LIN_LSE: the selected classes of the tile's row tid, asked for in front of the first chunk and looked at in the epilogue: where they are
+    // (lin_where_kernel), or one label
     uint2 where = make_uint2(~0u, ~0u);
-    auto look = [&]() {
-        if constexpr (EPI == LIN_LSE)
-            if (g.zsel && tid < LB_T && m0 + tid < g.M) {
-                if (g.where) where = g.where[(long long)(m0 + tid) * g.ntn + tn];
-                else {
-                    const long long t = g.index[m0 + tid];
-                    if (t >= n0 && t < min(n0 + LB_T, g.N)) where.x = 0xffff0000u | (unsigned)(t - n0);
-                }
-            }
-    };
+    if constexpr (EPI == LIN_LSE)
+        if (g.zsel && tid < LB_T && m0 + tid < g.M)
+            where = g.where ? g.where[(long long)(m0 + tid) * g.ntn + tn] : __builtin_bit_cast(uint2, g.index[m0 + tid]);
 
     if constexpr (DL) {
         // A ring of five operand chunks: A(c) in slot 2 c mod 5, B(c) in 2 c + 1 mod 5.  Half-way through chunk c its fragments are all in registers, so
         // B(c + 2) goes where A(c) was, and in the next half A(c + 3) where B(c) was.  Loads are spread evenly (one per 8 MFMA): the
         // same loads in bursts of the second half cost 3 to 5 % of the product.
-        auto landed = [&](bool all) {       // everything but A's 8 loads of the chunk after the next is there, and read by nobody any more
+        auto landed = [&](bool first) {       // everything but A's 8 loads of the chunk after the next (first: all 16 of chunk 1) is there, and read by nobody any more
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");
-            if (all) __builtin_amdgcn_s_waitcnt(0x0070);       // vmcnt(0) lgkmcnt(0)
-            else     __builtin_amdgcn_s_waitcnt(0x0078);       // vmcnt(8) lgkmcnt(0)
+            if (first) __builtin_amdgcn_s_waitcnt(0x4070);     // vmcnt(16) lgkmcnt(0)
+            else       __builtin_amdgcn_s_waitcnt(0x0078);     // vmcnt(8) lgkmcnt(0)
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
@@ -192,11 +186,10 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         advance_a(0); advance_b(0);
 #pragma unroll
         for (int i = 0; i < NL; ++i) dload(i < NT ? a0 : b0, i);
-        look();
-        landed(true);
         advance_a(1); advance_b(1);
 #pragma unroll
         for (int i = 0; i < NL; ++i) dload(i < NT ? a1 : b1, i);
+        landed(true);
         advance_a(2);
 #pragma unroll
         for (int i = 0; i < NL; ++i) fread(smem + a0 * LB_OP, smem + b0 * LB_OP, 0, i < NT ? i + NT : i - NT);
@@ -230,21 +223,17 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         // (the compiler does not know that inline asm has written the accumulators that are read from here on)
         asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");
     } else {
-    advance_a(0); advance_b(0);
+    // (in the loop's order: its waits are counted for both ways in)
+    auto ahead = [&](int ch) {
+        advance_a(ch); advance_b(ch);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) gload(0, i);
-    look();
+        for (int i = 0; i < NL; ++i) { gload(ch % SETS, i); __builtin_amdgcn_sched_barrier(0); }
+    };
+#pragma unroll
+    for (int u = 0; u < SETS; ++u) ahead(u);
 #pragma unroll
     for (int i = 0; i < NL; ++i) lput(0, 0, i);
-#pragma unroll
-    for (int u = 0; u < SETS; ++u) {
-        advance_a(1 + u); advance_b(1 + u);
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {        // (in the loop's order: its waits are counted for both ways in)
-            gload((1 + u) % SETS, i);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+    ahead(SETS);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -316,9 +305,14 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             }
         }
     };
-    for (int ch = 0; ch < nc; ch += 2 * SETS)
+    // (left in the middle, not skipped over: only so the compiler's counts of what is on the way stay exact)
+    bool more = nc > 0;
+    for (int ch = 0; more;)
 #pragma unroll
-        for (int i = 0; i < 2 * SETS; ++i) if (ch + i < nc) step(ch + i, i & 1, (i + 1) % SETS);
+        for (int i = 0; i < 2 * SETS; ++i) {
+            step(ch, i & 1, (i + 1) % SETS);
+            if (++ch >= nc) { more = false; break; }
+        }
     }
     __syncthreads();
 
@@ -399,6 +393,10 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
         float2* const red = reinterpret_cast<float2*>(smem);       // [wn, q16][labels of the tile]
         uint2* const wanted = reinterpret_cast<uint2*>(red + 8 * LB_T);
         if (g.zsel) {
+            if (!g.where) {
+                const long long t = __builtin_bit_cast(long long, where);      // (~0 where the row is none: no class)
+                where = make_uint2(t >= n0 && t < min(n0 + LB_T, g.N) ? 0xffff0000u | (unsigned)(t - n0) : ~0u, ~0u);
+            }
             if (tid < LB_T) wanted[tid] = where;
             __syncthreads();
         }
