@@ -144,7 +144,10 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
         stat, dsel, psel = _row_state(row, rows, k, tlog is not None)
         n = L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, grads)
         if 0 < n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33)):
-            keep = torch.empty(n, dtype=torch.uint8, device=dev)
+            try:
+                keep = torch.empty(n, dtype=torch.uint8, device=dev)
+            except torch.cuda.OutOfMemoryError:
+                pass                                        # the backward recomputes them
     if reduction == "none":
         loss, count = torch.empty(index.shape if tlog is None else index.shape[:-1], dtype=torch.float32, device=dev), None
         outs = (loss, None, None, 0)

@@ -141,6 +141,23 @@ def test_logits_kept_or_recomputed(shape, dtype, top, keep, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, x), want))
 
 
+def test_no_room_for_the_logits(monkeypatch):
+    """Where the logits find no room the backward recomputes them."""
+    c = O.case(300, 64, 700, torch.float32, seed=52, ignored=0.1)
+    n = L.load().fea_linear_loss_keep_bytes(300, 64, 700, L.F32, 3)
+    empty, asked = torch.empty, []
+
+    def full(*size, **how):
+        if size == (n,) and how.get("dtype") == torch.uint8:
+            asked.append(n)
+            raise torch.cuda.OutOfMemoryError("no room")
+        return empty(*size, **how)
+    monkeypatch.setattr(torch, "empty", full)
+    got = _run(*c)
+    assert asked == [n]
+    _compare(got, O.evaluate(*c))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("temperature", [1.0, 0.02])
 def test_logits_far_apart(dtype, temperature):
