@@ -90,9 +90,9 @@ SIGNATURES = {
     "fea_binarise": (I, [P, P, L, P]),
     "fea_linear_loss_ws_bytes": (Z, [L, I, I, I, I, I]),
     "fea_linear_loss_keep_bytes": (Z, [L, I, I, I, I]),
-    "fea_linear_ce_fwd": (I, [P, L, P, L, P, P, L, P, P, P, P, P, P, I, P, Z, L, I, I, I, P]),
-    "fea_linear_kd_fwd": (I, [P, L, P, L, P, P, I, P, I, F, P, P, P, P, P, P, P, I, P, Z, L, I, I, I, P]),
-    "fea_linear_loss_bwd": (I, [P, L, P, L, P, P, I, P, P, P, P, P, P, I, F, P, P, P, P, Z, L, I, I, I, P]),
+    "fea_linear_ce_fwd": (I, [P, L, P, L, P, P, L, P, P, P, I, P, P, P, I, P, Z, L, I, I, I, P]),
+    "fea_linear_kd_fwd": (I, [P, L, P, L, P, P, I, P, I, F, P, P, P, P, I, P, P, P, I, P, Z, L, I, I, I, P]),
+    "fea_linear_loss_bwd": (I, [P, L, P, L, P, P, I, P, P, P, P, I, P, P, I, F, P, P, P, P, Z, L, I, I, I, P]),
     "fea_opt_chunk": (I, []),
     "fea_sumsq_blocks": (I, [L]),
     "fea_grad_sumsq": (I, [P, L, P, P, P]),

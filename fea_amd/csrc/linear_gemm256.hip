@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             }
             const float base = mx == -INFINITY ? 0.f : mx;         // every class masked by a -inf bias: the sum is 0, not NaN
             if (g.keep && m < g.M) {
-                if constexpr (PL) {
+                if (PL || !g.top) {
                     float* const o = (float*)g.keep + m * g.ldkeep;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) if (ncol(j) < g.ldkeep) *reinterpret_cast<f32x4*>(o + ncol(j)) = z[j];

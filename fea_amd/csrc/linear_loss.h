@@ -39,9 +39,9 @@ struct LinGemm {
     const float* bias;                // [N], nullable
     float inv_t;
     float2* part;                     // LIN_LSE: [M][ntn] (max, sum of exp(z - max)) of one column tile
-    void* keep; long long ldkeep;     // LIN_LSE, nullable: the logits kept for the backward, rows of ldkeep (classes rounded up to 64): fp32 z, or (bf16) how far
+    void* keep; long long ldkeep;     // LIN_LSE, nullable: the logits kept for the backward, rows of ldkeep (classes rounded up to 64): fp32 z, or (bf16, with top) how far
                                       // z lies below the largest of its group, in steps of LIN_STEP (65535: LIN_RANGE and more, and classes behind the last)
-    float* top; long long ldtop;      // with bf16 keep: the groups' largest, [half tile][ldtop rows][4]; a group: every fourth 8 classes of half a tile's (what a lane holds of a row)
+    float* top; long long ldtop;      // the groups' largest, [half tile][ldtop rows][4]; a group: every fourth 8 classes of half a tile's (what a lane holds of a row)
     const float2* stat;               // LIN_DZ: [M] (log sum exp, gate)
     const float* gout; int gstride;   // upstream gradient, one value (stride 0) or one per row
     const int* count;                 // rows that count (mean), nullable

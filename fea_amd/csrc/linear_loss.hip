@@ -7,7 +7,7 @@
 //   dh = dz w, dw = dz^T h, db = sum_n dz
 //
 // Forward: the product with a log-sum-exp epilogue (linear_gemm256.hip, linear_gemm.hip), which also gives the few selected logits (or a
-// gathered dot product does) and, where the caller has room for them, keeps all logits in 16 bits (bf16 operands) or fp32; then one
+// gathered dot product does) and, where the caller has room for them, keeps all logits in 16 bits (bf16 operands, no bias gradient) or fp32; then one
 // pass that joins the column tiles of every row.  Backward, in pieces of the classes (and of the rows where there are very
 // many): dz from the kept logits, or by the product again with the softmax gradient as its epilogue; the selected entries from the
 // forward's fp32 values; two products.  The workspace is bounded by the piece, not by rows x classes.
@@ -681,17 +681,21 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     return c.at;
 }
 
-// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16 operands) or fp32 (fp32, and the few rows of linear_rows.hip), then, with 16 bits, the
-// groups' largest.  Not for few classes, where recomputing reads no more, and not in 16 bits for a bias gradient, which is fp32.
-static bool lin_keep_codes(const LinDims& d) { return d.dtype == FEA_BF16 && d.rows > 64; }
-static long long lin_keep_ld(const LinDims& d) { return up(d.V, 64); }
-static int lin_keep_es(const LinDims& d) { return lin_keep_codes(d) ? 2 : 4; }
-static size_t lin_keep_table(const LinDims& d) { return (size_t)up(d.rows * lin_keep_ld(d) * lin_keep_es(d), 256); }
-extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int grads) {
+// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16 operands) or fp32 (fp32 operands, the few rows of linear_rows.hip, and where the caller
+// asks for `wide` ones: a bias gradient is fp32), then, with 16 bits, the groups' largest.  Not for few classes, where recomputing
+// reads no more.
+struct LinKeep {
+    bool codes;
+    long long ld;
+    int es;
+    size_t table;                 // bytes in front of the groups' largest
+    LinKeep(const LinDims& d, int wide) : codes(d.dtype == FEA_BF16 && d.rows > 64 && !wide), ld(up(d.V, 64)), es(codes ? 2 : 4), table((size_t)up(d.rows * ld * es, 256)) {}
+};
+extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int wide) {
     if (rows <= 0 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
     const LinDims d = lin_dims(rows, D, V, 1, dtype);
-    if (lin_keep_codes(d) && grads & 4) return 0;
-    return lin_keep_table(d) + (lin_keep_codes(d) ? (size_t)rows * lin_fwd_plan(d).ntn * 8 * sizeof(float) : 0);
+    const LinKeep k(d, wide);
+    return k.table + (k.codes ? (size_t)rows * lin_fwd_plan(d).ntn * 8 * sizeof(float) : 0);
 }
 
 extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads) {
@@ -754,13 +758,13 @@ static int lin_check(const char* who, const LinDims& d, const void* h, long long
 }
 
 static int lin_forward(const char* who, LinDims d, const void* h, long long ldh, const void* w, long long ldw, const float* bias, LinJoin j,
-                       void* keep, float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
+                       void* keep, int wide, float* loss, int* count, int mean, void* ws, size_t ws_bytes, hipStream_t s) {
     LIN_TRY(lin_check(who, d, h, ldh, w, ldw, bias));
     const LinFwd p = lin_fwd_plan(d);
     LinFwdWs b;
     const size_t need = lin_fwd_carve(d, p, (char*)ws, b);
     FEA_CHECK(ws && (uintptr_t)ws % 256 == 0 && ws_bytes >= need, FEA_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, need, ws_bytes);
-    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(d.rows, d.D, d.V, (int)d.dtype, 0) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
+    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(d.rows, d.D, d.V, (int)d.dtype, wide) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
     FEA_CHECK(!loss == !count, FEA_E_BADARG, "%s: loss and count go together", who);
     FEA_CHECK(loss || j.loss_rows, FEA_E_BADARG, "%s: nothing to write", who);
 
@@ -798,8 +802,9 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         g.M = (int)n; g.N = d.V; g.K = pack ? f.K(d.D) : d.D; g.Kp = (int)up(d.D, 64);
         g.bias = bias; g.inv_t = j.inv_t; g.part = b.part;
         if (keep) {
-            g.keep = (char*)keep + r * lin_keep_ld(d) * lin_keep_es(d); g.ldkeep = lin_keep_ld(d);
-            if (lin_keep_codes(d)) { g.ldtop = d.rows; g.top = (float*)((char*)keep + lin_keep_table(d)) + r * 4; }
+            const LinKeep k(d, wide);
+            g.keep = (char*)keep + r * k.ld * k.es; g.ldkeep = k.ld;
+            if (k.codes) { g.ldtop = d.rows; g.top = (float*)((char*)keep + k.table) + r * 4; }
         }
         if (p.pick) { g.zsel = b.zsel + r * d.K; g.index = j.index + r * d.K; g.sel = d.K; }
         if (p.pick == 2) {
@@ -834,18 +839,18 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
 }
 
 extern "C" int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
-                                 long long ignore_index, float* stat, float* dsel, void* keep, float* loss_rows, float* loss, int* count,
-                                 int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream) {
+                                 long long ignore_index, float* stat, float* dsel, void* keep, int wide, float* loss_rows, float* loss,
+                                 int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream) {
     FEA_CHECK(target, FEA_E_BADARG, "fea_linear_ce_fwd: null target");
     LinJoin j{};
     j.index = target; j.ignore = ignore_index; j.t = j.inv_t = 1.f;
     j.stat = (float2*)stat; j.dsel = dsel; j.loss_rows = loss_rows;
-    return lin_forward("fea_linear_ce_fwd", lin_dims(rows, D, V, 1, dtype), h, ldh, w, ldw, bias, j, keep, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
+    return lin_forward("fea_linear_ce_fwd", lin_dims(rows, D, V, 1, dtype), h, ldh, w, ldw, bias, j, keep, wide, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const void* teacher_logits,
                                  int teacher_dtype, const long long* teacher_index, int K, float temperature, float* stat, float* dsel, float* psel,
-                                 void* keep, float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                                 void* keep, int wide, float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
                                  int dtype, void* stream) {
     FEA_CHECK(teacher_logits && teacher_index, FEA_E_BADARG, "fea_linear_kd_fwd: null teacher");
     FEA_CHECK(teacher_dtype == FEA_F32 || teacher_dtype == FEA_BF16, FEA_E_BADARG, "fea_linear_kd_fwd: teacher dtype %d", teacher_dtype);
@@ -853,12 +858,12 @@ extern "C" int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, lo
     LinJoin j{};
     j.index = teacher_index; j.tlog = teacher_logits; j.tdt = teacher_dtype; j.t = temperature; j.inv_t = 1.f / temperature;
     j.stat = (float2*)stat; j.dsel = dsel; j.psel = psel; j.loss_rows = loss_rows;
-    return lin_forward("fea_linear_kd_fwd", lin_dims(rows, D, V, K, dtype), h, ldh, w, ldw, bias, j, keep, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
+    return lin_forward("fea_linear_kd_fwd", lin_dims(rows, D, V, K, dtype), h, ldh, w, ldw, bias, j, keep, wide, loss, count, mean, ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* index, int K,
-                                   const float* stat, const float* dsel, const float* psel, const void* keep, const int* count, const float* gout,
-                                   int gout_stride, float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                                   const float* stat, const float* dsel, const float* psel, const void* keep, int wide, const int* count,
+                                   const float* gout, int gout_stride, float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
                                    int dtype, void* stream) {
     const char* who = "fea_linear_loss_bwd";
     LinDims d = lin_dims(rows, D, V, K, dtype);
@@ -870,8 +875,9 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     FEA_CHECK(((uintptr_t)dh | (uintptr_t)dw) % 16 == 0 && (uintptr_t)db % 4 == 0, FEA_E_BADARG, "%s: misaligned gradient", who);
     FEA_CHECK(K == 1 || !db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
     FEA_CHECK(temperature > 0.f && isfinite(temperature) && isfinite(1.f / temperature), FEA_E_BADARG, "%s: temperature %g", who, (double)temperature);
-    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(rows, D, V, dtype, db ? 4 : 0) > 0), FEA_E_BADARG,
-              "%s: no logits are kept of these sizes (or, in 16 bits, for a bias gradient), or misaligned", who);
+    FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(rows, D, V, dtype, wide) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
+    const LinKeep kept(d, wide);
+    FEA_CHECK(!keep || !db || !kept.codes, FEA_E_BADARG, "%s: a bias gradient needs wide kept logits", who);
     const int want = (dh ? 1 : 0) | (dw ? 2 : 0) | (db ? 4 : 0) | (keep ? 8 : 0);
     const LinBwd p = lin_bwd_plan(d, want);
     LinBwdWs b;
@@ -916,8 +922,8 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             g.colsum = db ? b.colsum : nullptr; g.ldcol = up(p.vc, 64);
             if (keep) {
                 LinDecode x{};
-                x.z = (const char*)keep + (r0 * lin_keep_ld(d) + v0) * lin_keep_es(d); x.ldz = lin_keep_ld(d);
-                x.ldtop = rows; x.top = (const float*)((const char*)keep + lin_keep_table(d)) + r0 * 4; x.shift = kp.tile == 256 ? 7 : 6;
+                x.z = (const char*)keep + (r0 * kept.ld + v0) * kept.es; x.ldz = kept.ld;
+                x.ldtop = rows; x.top = (const float*)((const char*)keep + kept.table) + r0 * 4; x.shift = kp.tile == 256 ? 7 : 6;
                 x.stat = st; x.gout = go; x.gstride = gout_stride; x.count = count; x.t = temperature;
                 x.dz = b.dz; x.lddz = g.lddz; x.Npad = g.Npad; x.colsum = g.colsum; x.ldcol = g.ldcol;
                 x.n = (int)n; x.nv = nv; x.v0 = (int)v0; x.nct = (nv + 127) / 128;
@@ -927,7 +933,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
                 FEA_CHECK(blocks < INT_MAX, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld tiles", who, blocks);
                 const dim3 grid((unsigned)blocks), bl(256);
                 auto launch = [&](auto even, auto odd) { if (d.odd()) hipLaunchKernelGGL(odd, grid, bl, 0, s, x); else hipLaunchKernelGGL(even, grid, bl, 0, s, x); };
-                if (lin_keep_codes(d))      launch(lin_decode_kernel<__bf16, true, false, true>, lin_decode_kernel<__bf16, true, false, false>);
+                if (kept.codes)             launch(lin_decode_kernel<__bf16, true, false, true>, lin_decode_kernel<__bf16, true, false, false>);
                 else if (dtype == FEA_BF16) launch(lin_decode_kernel<__bf16, false, false, true>, lin_decode_kernel<__bf16, false, false, false>);
                 else if (p.planes)          launch(lin_decode_kernel<float, false, true, true>, lin_decode_kernel<float, false, true, false>);
                 else                        launch(lin_decode_kernel<float, false, false, true>, lin_decode_kernel<float, false, false, false>);

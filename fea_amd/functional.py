@@ -142,7 +142,7 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     if grads:
         row = torch.empty(rows * (2 + k * (1 if tlog is None else 2)), dtype=torch.float32, device=dev)
         stat, dsel, psel = _row_state(row, rows, k, tlog is not None)
-        n = L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, grads)
+        n = L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, grads >> 2)
         if 0 < n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33)):
             try:
                 keep = torch.empty(n, dtype=torch.uint8, device=dev)
@@ -158,11 +158,11 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     if tlog is None:
-        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, keep, *outs, ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
+        L.call("fea_linear_ce_fwd", h, h.stride(0), w, w.stride(0), b, ix, ignore_index, stat, dsel, keep, grads >> 2, *outs, ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
     else:
         tl = tlog.detach().contiguous()
-        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, keep, *outs,
-               ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
+        L.call("fea_linear_kd_fwd", h, h.stride(0), w, w.stride(0), b, tl, L.dt_code(tl.dtype), ix, k, temperature, stat, dsel, psel, keep, grads >> 2,
+               *outs, ws, n, rows, d, v, dt, L.stream_ptr(dev.index))
     return loss, (ix, row, keep, count)
 
 
@@ -193,7 +193,7 @@ class _LinearLoss(torch.autograd.Function):
         go = gout.detach().contiguous()
         n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, grads | (8 if keep is not None else 0))
         ws = torch.empty(n, dtype=torch.uint8, device=h.device)
-        L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, keep, count, go, int(reduction == "none"),
+        L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, keep, grads >> 2, count, go, int(reduction == "none"),
                temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr(h.device.index))
         return dh, dw, db, None, None, None, None, None
 
@@ -247,8 +247,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
     Differentiable once, in hidden, weight and bias.  The logits are never there in full precision and shape: for a backward
-    the forward keeps 2 bytes of each (4 in float32 and for up to 64 rows) if that is 8 GiB or less (FEA_AMD_LINEAR_KEEP:
-    another limit in bytes, 0 for none); beyond it, and with a bias gradient in bfloat16, the backward recomputes them in pieces.
+    the forward keeps 2 bytes of each (4 in float32, with a bias gradient, and for up to 64 rows) if that is 8 GiB or less
+    (FEA_AMD_LINEAR_KEEP: another limit in bytes, 0 for none); beyond it the backward recomputes them in pieces.
     An NHWC feature map and a 1x1 convolution's weight viewed [classes, channels] are taken as they are."""
     ignore_index = int(ignore_index)
     if not -(1 << 63) <= ignore_index < 1 << 63:

@@ -357,9 +357,9 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
  * psel[rows][K] (all nullable), and keep (nullable): room for the logits, fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned.
- * They are kept in fp32, or with bf16 operands and more than 64 rows in 16 bits: z below the largest of its 16 or 32 in steps of
- * 64 / 65535, half a step off; 64 and more below counts as a share of 0.  0 bytes = none are kept (few classes with few features:
- * recomputing them reads no more; 16 bits where grads holds a bias gradient).
+ * They are kept in fp32, or with bf16 operands, more than 64 rows and wide = 0 in 16 bits: z below the largest of its 16 or 32 in
+ * steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0.  0 bytes = none are kept (few classes with few
+ * features: recomputing them reads no more).  wide is the same in all calls, and 1 where a bias gradient will be asked for.
  *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the logits from the
  *     forward's keep, or (NULL) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte
  *     aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one value (gout_stride 0) or one per row (1);
@@ -371,17 +371,17 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * backward, + 8 with keep
  * (0 bytes = sizes that are refused).  Results are the same from run to run. */
 size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);
-size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int grads);
+size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int wide);
 int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,
-                      long long ignore_index, float* stat, float* dsel, void* keep, float* loss_rows, float* loss,
-                      int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
+                      long long ignore_index, float* stat, float* dsel, void* keep, int wide, float* loss_rows,
+                      float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V, int dtype, void* stream);
 int fea_linear_kd_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const void* teacher_logits,
                       int teacher_dtype, const long long* teacher_index, int K, float temperature, float* stat, float* dsel, float* psel,
-                      void* keep, float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                      void* keep, int wide, float* loss_rows, float* loss, int* count, int mean, void* ws, size_t ws_bytes, long long rows, int D, int V,
                       int dtype, void* stream);
 int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* index, int K,
-                        const float* stat, const float* dsel, const float* psel, const void* keep, const int* count, const float* gout,
-                        int gout_stride, float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
+                        const float* stat, const float* dsel, const float* psel, const void* keep, int wide, const int* count,
+                        const float* gout, int gout_stride, float temperature, void* dh, void* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int V,
                         int dtype, void* stream);
 
 /* ---- input pipeline ------------------------------------------------

@@ -52,14 +52,16 @@ def test_workspace_sizes():
 
 def test_kept_sizes():
     keep = L.load().fea_linear_loss_keep_bytes
-    assert keep(0, 8, 8, 0, 3) == 0 and keep(1 << 20, 64, 6, 1, 3) == 0 and keep(100, 64, 1000, 5, 3) == 0
-    assert keep(100, 64, 1000, L.BF16, 7) == 0 and keep(100, 64, 1000, L.F32, 7) == 100 * 1024 * 4
-    for dt in (L.F32, L.BF16):
-        assert keep(64, 64, 1000, dt, 7) == 64 * 1024 * 4
+    assert keep(0, 8, 8, 0, 0) == 0 and keep(1 << 20, 64, 6, 1, 0) == 0 and keep(100, 64, 1000, 5, 0) == 0
+    for wide in (0, 1):
+        assert keep(100, 64, 1000, L.F32, wide) == 100 * 1024 * 4
+        for dt in (L.F32, L.BF16):
+            assert keep(64, 64, 1000, dt, wide) == 64 * 1024 * 4
+    assert keep(100, 64, 1000, L.BF16, 1) == 100 * 1024 * 4
     for rows, d, v in ((65, 8, 1), (100, 64, 1000), (8192, 4096, 131072), (1 << 20, 65, 6)):
         ld = (v + 63) // 64 * 64
-        assert rows * ld * 4 <= keep(rows, d, v, L.F32, 3) < rows * ld * 4 + 256
-        assert rows * ld * 2 < keep(rows, d, v, L.BF16, 3) <= rows * ld * 2 + 256 + rows * ((v + 127) // 128) * 32
+        assert rows * ld * 4 <= keep(rows, d, v, L.F32, 0) < rows * ld * 4 + 256
+        assert rows * ld * 2 < keep(rows, d, v, L.BF16, 0) <= rows * ld * 2 + 256 + rows * ((v + 127) // 128) * 32
 
 
 @pytest.mark.parametrize("top", [0, 4])

@@ -126,17 +126,19 @@ def test_large_tiles(shape, top, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 64, 600), (33, 515, 1000), (64, 128, 130), (65, 8, 64), (130, 33, 257), (258, 200, 333), (514, 640, 1537), (2050, 1096, 2310)])
+@pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("top", [0, 5])
 @pytest.mark.parametrize("keep", [0, 1 << 30])
-def test_logits_kept_or_recomputed(shape, dtype, top, keep, monkeypatch):
-    """A head without bias keeps its logits for the backward, within a limit; recomputed ones hold the same bounds."""
+def test_logits_kept_or_recomputed(shape, dtype, top, keep, bias, monkeypatch):
+    """A head keeps its logits for the backward, within a limit; recomputed ones hold the same bounds."""
     monkeypatch.setenv("FEA_AMD_LINEAR_KEEP", str(keep))
-    c = O.case(*shape, dtype, seed=sum(shape) + 1, top=top, ignored=0.2, short=0.3)
+    c = O.case(*shape, dtype, seed=sum(shape) + 1, top=top, ignored=0.2, short=0.3, bias=bias)
     _compare(_run(*c), O.evaluate(*c))
-    x = [_leaf(t) for t in c[:2]]
-    loss = F.linear_distillation(*x, c[4].to(DEV), c[3].to(DEV)) if top else F.linear_cross_entropy(*x, c[3].to(DEV))
+    x = [_leaf(t) for t in c[:3] if t is not None]
+    b = x[2] if bias else None
+    loss = F.linear_distillation(*x[:2], c[4].to(DEV), c[3].to(DEV), bias=b) if top else F.linear_cross_entropy(*x[:2], c[3].to(DEV), bias=b)
     held = [t.numel() for t in loss.grad_fn.saved_tensors if t is not None and t.dtype == torch.uint8]
-    assert [n >= shape[0] * shape[2] * (c[0].element_size() if shape[0] > 64 else 4) for n in held] == [True] * (keep > 0)
+    assert [n >= shape[0] * shape[2] * (c[0].element_size() if shape[0] > 64 and not bias else 4) for n in held] == [True] * (keep > 0)
     want = torch.autograd.grad(loss, x, retain_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, x), want))
 
@@ -144,7 +146,7 @@ def test_logits_kept_or_recomputed(shape, dtype, top, keep, monkeypatch):
 def test_no_room_for_the_logits(monkeypatch):
     """Where the logits find no room the backward recomputes them."""
     c = O.case(300, 64, 700, torch.float32, seed=52, ignored=0.1)
-    n = L.load().fea_linear_loss_keep_bytes(300, 64, 700, L.F32, 3)
+    n = L.load().fea_linear_loss_keep_bytes(300, 64, 700, L.F32, 0)
     empty, asked = torch.empty, []
 
     def full(*size, **how):
@@ -595,7 +597,7 @@ def test_workspace_and_operands_are_checked():
     out = torch.empty(16, device=DEV)
 
     def fwd(h=h, ldh=32, ws=ws, n=n, rows=16, d=32, v=40, dt=L.F32, keep=None):
-        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, keep, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
+        L.call("fea_linear_ce_fwd", h, ldh, w, 32, None, t, -100, None, None, keep, 0, out, None, None, 0, ws, n, rows, d, v, dt, L.stream_ptr())
     fwd()
     for bad in ({"n": n - 1}, {"ws": None}, {"ldh": 31}, {"ldh": 33}, {"h": None}, {"dt": 7}, {"rows": 0}, {"v": 0}, {"d": 0}, {"h": h.data_ptr() + 4},
                 {"ws": ws.data_ptr() + 16}, {"d": 1 << 17, "ldh": 1 << 17}, {"keep": ws.data_ptr() + 64}):
@@ -610,6 +612,6 @@ def test_workspace_and_operands_are_checked():
     f = torch.zeros(160, device=DEV)
     for kp, db in ((keep, f), (keep.data_ptr() + 64, None)):
         with pytest.raises(L.FeaError, match="kept"):
-            L.call("fea_linear_loss_bwd", x, 32, x, 32, None, t.repeat(5), 1, f, f, None, kp, None, f, 0, 1.0, x, None, db, back, back.numel(), 80, 32, 40,
+            L.call("fea_linear_loss_bwd", x, 32, x, 32, None, t.repeat(5), 1, f, f, None, kp, 0, None, f, 0, 1.0, x, None, db, back, back.numel(), 80, 32, 40,
                    L.BF16, L.stream_ptr())
     torch.cuda.synchronize()
