@@ -246,7 +246,9 @@ LinTile fea_lin_tile(int dtype, long long M, long long N, long long K, bool spli
         const long long tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
         for (int sp = 1; sp <= (split ? 32 : 1); ++sp) {
             if (sp > 1 && K / sp < (dtype == FEA_F32 ? 256 : 512)) break;
-            const double rounds = (double)((tiles * sp + (long long)slots - 1) / (long long)slots);
+            // (a workgroup of the small tile that has a CU to itself takes 0.6 of the time of two)
+            const long long n = tiles * sp, full = n / (long long)slots, rest = n % (long long)slots;
+            const double rounds = (double)full + (rest == 0 ? 0.0 : tile == 128 && rest <= 256 ? 0.6 : 1.0);
             double t = rounds * (2.0 * rows * tile * ((double)K / sp + 128) / (rate / slots));
             if (t < bytes / 4e12) t = bytes / 4e12;
             t += sp > 1 ? 2.0 * sp * M * N * 4 / 4e12 + 3e-6 : 0.0;
@@ -274,6 +276,7 @@ int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
               "lin_gemm: operands of %d x %d x %d", g.M, g.N, g.K);
     FEA_CHECK(dtype == FEA_F32 ? tile == 128 : aln && g.lda < (1 << 21) && g.ldb < (1 << 21), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
     FEA_CHECK(dtype != FEA_PL || (g.Kp > 0 && g.Kp % 64 == 0 && g.K == 6 * g.Kp && g.Kr <= g.Kp && (epi != LIN_STORE || g.slab)), FEA_E_BADARG, "lin_gemm: planes of %d, K %d", g.Kp, g.K);
+    FEA_CHECK(epi != LIN_LSE || (g.slab != nullptr) == (g.splits > 1), FEA_E_BADARG, "lin_gemm: %d parts", g.splits);
     FEA_CHECK(epi != LIN_STORE || dtype == FEA_F32 || (g.Kr > 0 && g.Kr <= (dtype == FEA_PL ? g.Kp : g.K)), FEA_E_BADARG, "lin_gemm: reduction of %d of %d", g.Kr, g.K);
     g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
     const int grp = it / (GM * g.ntn), gm = min(GM, g.ntm - grp * GM), in = it - grp * GM * g.ntn;
     const int tm = grp * GM + in % gm, tn = in / gm;
     const int m0 = tm * LB_T, n0 = tn * LB_T;
-    const int k0 = EPI == LIN_STORE ? sp * g.kper : 0, K = max((EPI == LIN_STORE ? min(k0 + g.kper, g.K) : g.K) - k0, 0);
+    const int k0 = EPI == LIN_DZ ? 0 : sp * g.kper, K = max((EPI == LIN_DZ ? g.K : min(k0 + g.kper, g.K)) - k0, 0);
     const int nc = (K + 63) >> 6;
 
     auto rsrc = [&](const __bf16* p, long long ld, int rows, int cols) {       // rows x cols of a matrix; 0 rows: nothing is read
@@ -365,6 +365,15 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
             }
         }
     }
+    if constexpr (EPI == LIN_LSE)
+        if (g.slab) {            // split: the sums as they are, joined by lin_join_split_kernel
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    if (mrow(i) < g.M && ncol(j) < g.ldo) *reinterpret_cast<f32x4*>(g.slab + ((long long)sp * g.M + mrow(i)) * g.ldo + ncol(j)) = acc[i][j];
+            return;
+        }
     // z of a lane's 4 classes of tile j, label tile i; classes behind the last are -inf (whatever 0 times the label's row gave)
     f32x4 bias[EPI == LIN_STORE ? 1 : NT];
     if constexpr (EPI != LIN_STORE) {

@@ -50,7 +50,7 @@ struct LinGemm {
     int Npad;                         // LIN_DZ: columns written (FEA_PL: of each plane), zero behind N
     float* colsum;                    // LIN_DZ: [tiles of A rows][N], nullable: sums of row scale * softmax over the tile's rows
     long long ldcol;
-    // LIN_STORE: split over K into `splits` parts of kper: direct store to out (splits == 1, slab == NULL) or fp32 slabs
+    // LIN_STORE, LIN_LSE of bf16 or FEA_PL: split over K into `splits` parts of kper: direct store to out (splits == 1, slab == NULL) or fp32 slabs (LIN_LSE: plain sums)
     void* out; long long ldo;
     float* slab;                      // [splits][M][ldo], ldo a multiple of 4 (columns behind N hold nothing)
     int scale;                        // 0: none, 1: times the row scale of C's row, 2: times the common scale (gout, count, t above)

@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256) void lin_join_rows_kernel(const LinJoin j) {
     lin_join_body(j, 64, threadIdx.x & 63, row, threadIdx.x < 64, lin_lse_of(lin_merge(lin_merge(red[0], red[1]), lin_merge(red[2], red[3]))));
 }
 
-// Few rows whose reduction is split: the parts' sums make z, one workgroup per row.
+// A split reduction: the parts' sums make z, one workgroup per row.
 struct LinParts { const float* slab; int parts; long long ld; const float* bias; float* keep; };      // keep (nullable): rows of ld
 __global__ __launch_bounds__(256) void lin_join_split_kernel(const LinJoin j, const LinParts t) {
     __shared__ float2 red[4];
@@ -289,8 +289,14 @@ __global__ __launch_bounds__(256) void lin_join_split_kernel(const LinJoin j, co
     const float* const s = t.slab + row * t.ld;
     float2 a = make_float2(-INFINITY, 0.f);
     for (int v = 4 * threadIdx.x; v < t.ld; v += 1024) {
-        f32x4 z = *reinterpret_cast<const f32x4*>(s + v);
-        for (int p = 1; p < t.parts; ++p) z += *reinterpret_cast<const f32x4*>(s + p * next + v);
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < t.parts; p += 8) {                     // (eight on the way, added in their order)
+            f32x4 x[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = p + q < t.parts ? *reinterpret_cast<const f32x4*>(s + (p + q) * next + v) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) z += x[q];
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[e] = v + e < j.V ? (z[e] + (t.bias ? t.bias[v + e] : 0.f)) * j.inv_t : -INFINITY;
         if (t.keep) *reinterpret_cast<f32x4*>(t.keep + row * t.ld + v) = z;
@@ -571,7 +577,7 @@ static LinForm lin_form(int dtype, bool planes) {
 }
 
 // Forward: rows in chunks that bound the partial table to 128 MB.
-struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; int pick, parts; };   // pick: 0 selected logits by dot products, 1 out of the product, 2 with lin_where_kernel; parts: of few rows' reduction
+struct LinFwd { long long rc; int tile, ntn, G; bool planes; long long blocks; int pick, parts; };   // pick: 0 selected logits by dot products, 1 out of the product, 2 with lin_where_kernel; parts: of a split reduction
 static LinFwd lin_fwd_plan(const LinDims& d) {
     LinFwd p;
     const long long cap = (1ll << 24) / ((d.V + 127) / 128);
@@ -579,20 +585,30 @@ static LinFwd lin_fwd_plan(const LinDims& d) {
     if (p.rc > d.rows) p.rc = d.rows;
     LinTile t = fea_lin_tile(d.dtype, p.rc, d.V, d.D, false);
     p.planes = false;
+    // few tiles: the reduction is split between workgroups where that saves more than the longer join (a training step of 387 rows x 3,264 x 2,112:
+    // fp32 307 and, split, 204 us, bf16 83 and 71)
+    const bool split = p.rc == d.rows && d.V <= 1 << 16;
+    auto product = [&](int dt, long long K) {
+        const LinTile one = fea_lin_tile(dt, p.rc, d.V, K, false);
+        const LinTile many = split ? fea_lin_tile(dt, p.rc, d.V, K, true) : one;
+        return many.splits > 1 && many.time + 6e-6 < one.time ? many : one;
+    };
+    if (d.dtype == FEA_BF16) t = product(FEA_BF16, d.D);
     if (d.dtype == FEA_F32) {     // 10 bytes per element for the copies, against a third of the matrix time
-        const LinTile q = fea_lin_tile(FEA_PL, p.rc, d.V, 6 * up(d.D, 64), false);
+        const LinTile q = product(FEA_PL, 6 * up(d.D, 64));
         if (q.time + ((double)p.rc + d.V) * d.D * 10 / 4e12 + 6e-6 < t.time) { t = q; p.planes = true; }
     }
     p.tile = t.tile;
+    p.parts = t.splits;
     if (d.rows <= 64) { p.tile = 64; p.planes = false; }
     p.ntn = (d.V + p.tile - 1) / p.tile;
     // selected logits come out of the product where it can give them
     const bool tiles = p.tile != 64 && (d.dtype == FEA_BF16 || p.planes);
-    p.parts = p.tile == 64 ? fea_lin_rows_splits((int)d.dtype, d.V, d.D) : 1;
-    p.pick = p.tile == 64 ? p.parts > 1 || d.rows * d.K <= 2048 : !tiles ? 0 : d.K == 1 ? 1 : d.K <= LIN_WHERE_K && p.ntn <= LIN_WHERE_T ? 2 : 0;
+    if (p.tile == 64) p.parts = fea_lin_rows_splits((int)d.dtype, d.V, d.D);
+    p.pick = p.parts > 1 ? 1 : p.tile == 64 ? d.rows * d.K <= 2048 : !tiles ? 0 : d.K == 1 ? 1 : d.K <= LIN_WHERE_K && p.ntn <= LIN_WHERE_T ? 2 : 0;
     p.G = 1;
     while (p.G < 64 && (p.G < (d.V + 127) / 128 || p.G < d.K)) p.G *= 2;
-    p.blocks = p.tile == 64 ? d.rows : (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
+    p.blocks = p.tile == 64 || p.parts > 1 ? d.rows : (d.rows + 256 / p.G - 1) / (256 / p.G) + (p.rc ? d.rows / p.rc + 1 : 0);     // every chunk rounds up by itself
     return p;
 }
 
@@ -681,15 +697,15 @@ static size_t lin_bwd_carve(const LinDims& d, const LinBwd& p, int want, char* b
     return c.at;
 }
 
-// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16 operands) or fp32 (fp32 operands, the few rows of linear_rows.hip, and where the caller
-// asks for `wide` ones: a bias gradient is fp32), then, with 16 bits, the groups' largest.  Not for few classes, where recomputing
+// Kept logits: [rows][V rounded up to 64] of 16 bits (bf16 operands) or fp32 (fp32 operands, the few rows of linear_rows.hip, split
+// reductions, and where the caller asks for `wide` ones: a bias gradient is fp32), then, with 16 bits, the groups' largest.  Not for few classes, where recomputing
 // reads no more.
 struct LinKeep {
     bool codes;
     long long ld;
     int es;
     size_t table;                 // bytes in front of the groups' largest
-    LinKeep(const LinDims& d, int wide) : codes(d.dtype == FEA_BF16 && d.rows > 64 && !wide), ld(up(d.V, 64)), es(codes ? 2 : 4), table((size_t)up(d.rows * ld * es, 256)) {}
+    LinKeep(const LinDims& d, int wide) : codes(d.dtype == FEA_BF16 && d.rows > 64 && !wide && lin_fwd_plan(d).parts == 1), ld(up(d.V, 64)), es(codes ? 2 : 4), table((size_t)up(d.rows * ld * es, 256)) {}
 };
 extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int wide) {
     if (rows <= 0 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
@@ -812,7 +828,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
             hipLaunchKernelGGL(lin_where_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 4 * 3 * p.ntn * sizeof(uint32_t), s, g.index, d.K, n, d.V, p.tile, p.ntn, b.where);
             FEA_LAUNCH_CHECK();
         }
-        if (p.parts > 1) { g.zsel = nullptr; g.slab = b.slab; g.ldo = up(d.V, 64); g.splits = p.parts; }
+        if (p.parts > 1) { g.zsel = nullptr; g.keep = nullptr; g.slab = b.slab; g.ldo = up(d.V, 64); g.splits = p.parts; g.kper = (int)up((g.K + p.parts - 1) / p.parts, 64); }
         if (p.tile == 64) LIN_TRY(fea_lin_rows(d.dtype, !d.odd(), g, s));
         else LIN_TRY(fea_lin_gemm(LIN_LSE, f.dt, p.tile, g, s));
         LinJoin q = j;
@@ -824,7 +840,7 @@ static int lin_forward(const char* who, LinDims d, const void* h, long long ldh,
         if (q.psel) q.psel += r * d.K;
         if (q.loss_rows) q.loss_rows += r;
         q.bsum = loss ? b.bsum + blk : nullptr; q.bcnt = b.bcnt + blk;
-        const long long grid = p.tile == 64 ? n : (n + 256 / p.G - 1) / (256 / p.G);
+        const long long grid = p.tile == 64 || p.parts > 1 ? n : (n + 256 / p.G - 1) / (256 / p.G);
         if (p.parts > 1)       hipLaunchKernelGGL(lin_join_split_kernel, dim3((unsigned)grid), dim3(256), 0, s, q, (LinParts{b.slab, p.parts, up(d.V, 64), bias, (float*)keep}));
         else if (p.tile == 64) hipLaunchKernelGGL(lin_join_rows_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);
         else              hipLaunchKernelGGL(lin_join_kernel, dim3((unsigned)grid), dim3(256), 0, s, q);

@@ -357,7 +357,7 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * Outputs: loss_rows[rows] (nullable); loss[1] and count[1] (both or neither): the sum, or with mean != 0 the mean over the rows
  * that count (0 where none does), and their number; for the backward: stat[rows][2], dsel[rows][K] (K = 1 for ce) and, for kd,
  * psel[rows][K] (all nullable), and keep (nullable): room for the logits, fea_linear_loss_keep_bytes(...) bytes, 256-byte aligned.
- * They are kept in fp32, or with bf16 operands, more than 64 rows and wide = 0 in 16 bits: z below the largest of its 16 or 32 in
+ * They are kept in fp32, or with bf16 operands, wide = 0 and more than a few rows or classes in 16 bits: z below the largest of its 16 or 32 in
  * steps of 64 / 65535, half a step off; 64 and more below counts as a share of 0.  0 bytes = none are kept (few classes with few
  * features: recomputing them reads no more).  wide is the same in all calls, and 1 where a bias gradient will be asked for.
  *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the logits from the

@@ -58,6 +58,17 @@ def test_most_entries(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(100, 2048, 500), (301, 4099, 1000), (200, 6000, 130), (387, 3264, 2112), (65, 3000, 33)])
+@pytest.mark.parametrize("top", [0, 3, 256])
+def test_few_tiles_split_the_reduction(shape, dtype, top):
+    """Long reductions over few tiles of rows and classes, in parts."""
+    c = O.case(*shape, dtype, seed=72 + top, top=top, ignored=0.1, short=0.2, bias=shape[0] % 2 == 1)
+    _compare(_run(*c), O.evaluate(*c))
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(3))
+    _compare(_run(*c, gout=gout, reduction="none"), O.evaluate(*c, gout=gout, reduction="none"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 4096, 5), (17, 1543, 300), (40, 2056, 1000), (64, 20600, 130), (3, 5000, 16000), (30, 3840, 3840)])
 @pytest.mark.parametrize("top", [0, 3, 256])
 def test_few_rows_and_classes_split_the_reduction(shape, dtype, top):
