@@ -1,5 +1,4 @@
-"""Segmentation loss, mask binarisation and IoU on the HIP kernels
-(build-defined, the reference has none), and the loss heads over many classes:
+"""Segmentation loss, mask binarisation and IoU on the HIP kernels (the reference has none), and the loss heads over many classes:
 `linear_cross_entropy`, `linear_distillation`."""
 from __future__ import annotations
 

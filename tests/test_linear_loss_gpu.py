@@ -357,6 +357,14 @@ def test_rows_of_something_very_wide(dtype):
         _compare(dict(zip(("loss", "hidden", "weight"), [loss, *torch.autograd.grad(loss, rows)])), want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(3, 65536, 50), (70, 65536, 40), (2, 1, 1 << 24), (66, 2, 1 << 20)])
+def test_longest_and_widest(shape, dtype):
+    """The most features, the most classes."""
+    c = O.case(*shape, dtype, seed=80, ignored=0.1)
+    _compare(_run(*c), O.evaluate(*c))
+
+
 def test_far_rows():
     """More than 2^31 elements of hidden states: 8,300 copies of a batch, whose rows do not depend on each other."""
     h, w, b, t = O.case(4096, 64, 6, torch.bfloat16, seed=40, ignored=0.1, bias=True)
