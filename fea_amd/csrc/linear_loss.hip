@@ -35,7 +35,7 @@ __device__ __forceinline__ void lin_split3(float v, __bf16& x0, __bf16& x1, __bf
 // holds three of Cpad.  With stat, rows whose gate is 0 count as zeros: what an ignored row holds (an infinity, a NaN) meets a zero
 // gradient in the weight's product, and 0 x NaN must not reach the weight; with gout every row is multiplied by its own
 // upstream gradient.  Up to three operands per launch, 64 x 64 elements per workgroup.
-struct LinCopy { const void* in; void* out; long long ld, ldo, R; int C, Cpad; const float2* stat; const float* gout; float t; long long tiles; };
+struct LinCopy { const void* in; void* out; long long ld, ldo, R; int C, Cpad; const float2* stat; const float* gout; const int* count; float t; long long tiles; };
 struct LinCopies { LinCopy j[3]; };
 
 template <typename T, bool PL, bool ALN>
@@ -62,7 +62,7 @@ __device__ __forceinline__ void lin_copy_tile(const LinCopies& js, long long til
 #pragma unroll
         for (int q = 0; q < NV; ++q) *reinterpret_cast<u32x4*>(x + q * EPC) = dead ? u32x4{0, 0, 0, 0} : v[i][q];
         if (j.gout) {
-            const float f = lin_row_scale(j.gout, 1, nullptr, j.t, 1.f, r);
+            const float f = lin_row_scale(j.gout, 1, j.count, j.t, 1.f, r);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = dead ? from_f32<T>(0.f) : from_f32<T>(to_f32(x[e]) * f);
         }
@@ -925,7 +925,7 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
             LinCopies js{{lin_copy_of(d, f, hr, ldh, n, pack && iv == 0 && (!keep || (dw && !gated)) ? b.hp : nullptr), lin_copy_of(d, f, wr, ldw, nv, pack && (ir == 0 || p.nvc > 1) && (!keep || dh) ? b.wp : nullptr),
                           lin_copy_of(d, f, hr, ldh, n, gated && iv == 0 ? b.hg : nullptr)}};
             js.j[0].stat = js.j[2].stat = st;
-            if (gout_stride) { js.j[2].gout = go; js.j[2].t = temperature; }
+            if (gout_stride) { js.j[2].gout = go; js.j[2].count = count; js.j[2].t = temperature; }
             if (pack && !keep) LIN_TRY(lin_copy(d, f, js, s));       // (else they go along with a kernel below)
             const void* const wk = pack ? b.wp : (const void*)wr;
             const long long ldwk = pack ? f.row(D) : ldw;

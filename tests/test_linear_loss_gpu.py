@@ -634,3 +634,49 @@ def test_workspace_and_operands_are_checked():
             L.call("fea_linear_loss_bwd", x, 32, x, 32, None, t.repeat(5), 1, f, f, None, kp, 0, None, f, 0, 1.0, x, None, db, back, back.numel(), 80, 32, 40,
                    L.BF16, L.stream_ptr())
     torch.cuda.synchronize()
+
+
+def _entry_step(h, w, b, index, tlog=None, gout=None, temperature=1.0, kept=True):
+    """A step through the C entry points: mean loss and count out of the forward, then the backward with both a count and an upstream
+    gradient for every row.  {"loss", "count", "hidden", "weight", "bias"}."""
+    (rows, d), v, k, dt = h.shape, w.shape[0], 1 if tlog is None else index.shape[1], L.dt_code(h.dtype)
+    h, w, index, gout = h.to(DEV), w.to(DEV), index.to(DEV), gout.to(DEV)
+    b = None if b is None else b.to(DEV)
+    wide = int(b is not None)
+    stat, dsel, psel = (torch.empty(rows, n, device=DEV) for n in (2, k, k))
+    n = L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, wide) if kept else 0
+    keep = torch.empty(n, dtype=torch.uint8, device=DEV) if n else None
+    loss, count = torch.empty((), device=DEV), torch.empty((), dtype=torch.int32, device=DEV)
+    n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    rest = (keep, wide, None, loss, count, 1, ws, n, rows, d, v, dt, L.stream_ptr())
+    if tlog is None:
+        L.call("fea_linear_ce_fwd", h, d, w, d, b, index, -100, stat, dsel, *rest)
+    else:
+        tlog = tlog.to(DEV)
+        L.call("fea_linear_kd_fwd", h, d, w, d, b, tlog, L.dt_code(tlog.dtype), index, k, temperature, stat, dsel, psel, *rest)
+    dh, dw, db = torch.empty_like(h), torch.empty_like(w), None if b is None else torch.empty(v, device=DEV)
+    n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 3 + 4 * wide + 8 * (keep is not None))
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    L.call("fea_linear_loss_bwd", h, d, w, d, b, index, k, stat, dsel, None if tlog is None else psel, keep, wide, count, gout, 1, temperature, dh, dw, db,
+           ws, n, rows, d, v, dt, L.stream_ptr())
+    torch.cuda.synchronize()
+    return {"loss": loss, "count": count, "hidden": dh, "weight": dw} | ({} if b is None else {"bias": db})
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(40, 64, 300), (200, 72, 500), (200, 51, 500), (1300, 643, 2011), (4100, 24, 9)])
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("kept", [True, False])
+def test_count_divides_every_gradient(shape, dtype, top, kept):
+    """A count beside an upstream gradient for every row: hidden's, weight's and bias's gradients are all divided by it."""
+    c = O.case(*shape, dtype, seed=91 + top, top=top, ignored=0.2, bias=shape[0] % 2 == 0 and not (kept and shape[0] == 200))
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(4))
+    got = _entry_step(*c, gout=gout, temperature=2.0 if top else 1.0, kept=kept)
+    on = int((c[3] != -100).sum()) if not top else int((c[3] >= 0).any(1).sum())
+    assert int(got.pop("count")) == on
+    kw = {"temperature": 2.0} if top else {}
+    mean = O.evaluate(*c, **kw)
+    want = O.evaluate(*c, gout=gout / on, reduction="none", kept=None if kept else False, **kw)        # (T is a power of two: the order of T and the division is free)
+    want["loss"] = mean["loss"]
+    _compare(got, want)
