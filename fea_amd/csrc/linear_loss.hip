@@ -889,7 +889,9 @@ extern "C" int fea_linear_loss_bwd(const void* h, long long ldh, const void* w, 
     FEA_CHECK(gout_stride == 0 || gout_stride == 1, FEA_E_BADARG, "%s: gout_stride %d", who, gout_stride);
     FEA_CHECK(dh || dw || db, FEA_E_BADARG, "%s: no gradient asked for", who);
     FEA_CHECK(((uintptr_t)dh | (uintptr_t)dw) % 16 == 0 && (uintptr_t)db % 4 == 0, FEA_E_BADARG, "%s: misaligned gradient", who);
-    FEA_CHECK(K == 1 || !db || psel, FEA_E_BADARG, "%s: the bias gradient needs psel of the forward", who);
+    // (few classes take the shares themselves, not their differences to the softmax)
+    FEA_CHECK(K == 1 || psel || !(db || fea_lin_few(rows, D, V)), FEA_E_BADARG, "%s: %d entries per row %s need psel of the forward", who, K,
+              db ? "and a bias gradient" : "over few classes");
     FEA_CHECK(temperature > 0.f && isfinite(temperature) && isfinite(1.f / temperature), FEA_E_BADARG, "%s: temperature %g", who, (double)temperature);
     FEA_CHECK(!keep || ((uintptr_t)keep % 256 == 0 && fea_linear_loss_keep_bytes(rows, D, V, dtype, wide) > 0), FEA_E_BADARG, "%s: no logits are kept of these sizes, or misaligned", who);
     const LinKeep kept(d, wide);

@@ -363,7 +363,8 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  *   fea_linear_loss_bwd (both; index = target or teacher_index, ce: K = 1, temperature 1, psel NULL): takes the logits from the
  *     forward's keep, or (NULL) recomputes them, in pieces of the classes, and writes dh[rows][D], dw[V][D] (contiguous, 16-byte
  *     aligned, `dtype`) and db[V] (fp32), each nullable.  gout: upstream gradient, one value (gout_stride 0) or one per row (1);
- *     count: divide it by count[0] (mean) or NULL.
+ *     count: divide it by count[0] (mean) or NULL.  stat and dsel are the forward's; with K > 1 so is psel where db is asked for or no
+ *     logits can be kept (fea_linear_loss_keep_bytes gives 0); else it may be NULL.
  * Where D is a multiple of 16 bytes, h and w need 16-byte aligned rows (bf16: less than 2^21 elements apart); other D are
  * taken at any alignment.
  * fp32: products of a certain size run as six products of bf16 planes (24 bits in three), the others on the fp32 matrix rate.

@@ -89,3 +89,18 @@ def test_check_finds_a_planted_error():
     for bad in ([1.002, 2.0], [float("nan"), 2.0], [float("inf"), 2.0]):
         with pytest.raises(AssertionError):
             O.check("x", torch.tensor(bad), (value, bound))
+
+
+@pytest.mark.parametrize("rows,d,v,db", [(4096, 64, 32, 0), (5000, 8, 2, 0), (100, 64, 1000, 256), (4096, 64, 32, 256)])
+def test_entries_without_their_shares_are_refused(rows, d, v, db):
+    """A backward over several teacher entries a row that needs the forward's shares and has none.  (The addresses are never used: without
+    the refusal the workspace of no bytes is refused.)"""
+    at = 1 << 20
+
+    def bwd(k, psel):
+        L.call("fea_linear_loss_bwd", at, d, at, d, None, at, k, at, at, psel, None, 1, None, at, 0, 1.0, at, at, db, at, 0, rows, d, v, L.F32, None)
+    with pytest.raises(L.FeaError, match="need psel"):
+        bwd(3, None)
+    for k, psel in ((1, None), (3, at)):
+        with pytest.raises(L.FeaError, match="workspace"):
+            bwd(k, psel)

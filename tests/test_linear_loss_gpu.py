@@ -636,7 +636,7 @@ def test_workspace_and_operands_are_checked():
     torch.cuda.synchronize()
 
 
-def _entry_step(h, w, b, index, tlog=None, gout=None, temperature=1.0, kept=True):
+def _entry_step(h, w, b, index, tlog=None, gout=None, temperature=1.0, kept=True, shares=True):
     """A step through the C entry points: mean loss and count out of the forward, then the backward with both a count and an upstream
     gradient for every row.  {"loss", "count", "hidden", "weight", "bias"}."""
     (rows, d), v, k, dt = h.shape, w.shape[0], 1 if tlog is None else index.shape[1], L.dt_code(h.dtype)
@@ -658,7 +658,7 @@ def _entry_step(h, w, b, index, tlog=None, gout=None, temperature=1.0, kept=True
     dh, dw, db = torch.empty_like(h), torch.empty_like(w), None if b is None else torch.empty(v, device=DEV)
     n = L.load().fea_linear_loss_ws_bytes(rows, d, v, k, dt, 3 + 4 * wide + 8 * (keep is not None))
     ws = torch.empty(n, dtype=torch.uint8, device=DEV)
-    L.call("fea_linear_loss_bwd", h, d, w, d, b, index, k, stat, dsel, None if tlog is None else psel, keep, wide, count, gout, 1, temperature, dh, dw, db,
+    L.call("fea_linear_loss_bwd", h, d, w, d, b, index, k, stat, dsel, psel if shares and tlog is not None else None, keep, wide, count, gout, 1, temperature, dh, dw, db,
            ws, n, rows, d, v, dt, L.stream_ptr())
     torch.cuda.synchronize()
     return {"loss": loss, "count": count, "hidden": dh, "weight": dw} | ({} if b is None else {"bias": db})
@@ -680,3 +680,14 @@ def test_count_divides_every_gradient(shape, dtype, top, kept):
     want = O.evaluate(*c, gout=gout / on, reduction="none", kept=None if kept else False, **kw)        # (T is a power of two: the order of T and the division is free)
     want["loss"] = mean["loss"]
     _compare(got, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(40, 64, 300), (200, 51, 500), (4095, 64, 32)])
+@pytest.mark.parametrize("kept", [True, False])
+def test_entries_without_their_shares(shape, dtype, kept):
+    """Without a bias gradient and with more than a few classes the backward takes the selected entries from dsel alone."""
+    c = O.case(*shape, dtype, seed=95, top=5, ignored=0.2, short=0.2)
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(5))
+    want, got = (_entry_step(*c, gout=gout, kept=kept, shares=s) for s in (True, False))
+    assert all(torch.equal(got[k], want[k]) for k in want)
