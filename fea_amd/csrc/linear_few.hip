@@ -181,17 +181,17 @@ __global__ __launch_bounds__(256) void lin_few_fwd_kernel(const LinFew g) {
             bool bad = false;
             ent.each([&](int, long long i, float a) {
                 if (i >= g.V) bad = true;
-                if (i >= 0) { a *= g.inv_t; bad |= !(a < INFINITY); tm = fmaxf(tm, a); }
+                if (i >= 0) { bad |= !(a < INFINITY); tm = fmaxf(tm, a); }
             });
             counts = in && (bad || tm != -INFINITY);
             const float tb = tm == -INFINITY ? 0.f : tm;
-            ent.each([&](int, long long i, float a) { if (i >= 0) ts += expf(a * g.inv_t - tb); });
+            ent.each([&](int, long long i, float a) { if (i >= 0) ts += expf((a - tb) * g.inv_t); });
             const float lt = logf(ts);
             float pz = 0.f, pl = 0.f;                     // sum p z over the classes of this half; sum p (log p + lse)
             ent.each([&](int k, long long i, float a) {
                 float p = 0.f;
                 if (i >= 0 && counts) {
-                    const float lp = a * g.inv_t - tb - lt;
+                    const float lp = (a - tb) * g.inv_t - lt;             // (1 / T meets the distance: the lowest value as a mask stays finite)
                     p = bad ? NAN : expf(lp);
                     if (p > 0.f) {
                         pl += p * (lp + lse);

@@ -174,7 +174,8 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
                 if (gl == 0 && j.dsel) j.dsel[row] = expm1f(-loss);
             } else if (in && gl == 0 && j.dsel) j.dsel[row] = 0.f;
         } else {
-            // teacher: softmax over its entries (those with a class and a logit above -inf); lane gl holds entries gl + G q
+            // teacher: softmax over its entries (those with a class and a logit above -inf); lane gl holds entries gl + G q.  1 / T meets the
+            // logits' distances to the largest, not the logits: a mask of the type's lowest value stays finite at T < 1
             constexpr int Q = 4;                          // K <= 256, and K <= G where G < 64
             long long ix[Q];
             float tv[Q], tm = -INFINITY, ts = 0.f;
@@ -184,7 +185,7 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
                 const int k = gl + G * q;
                 const bool there = in && k < j.K;
                 ix[q] = there ? j.index[e0 + k] : -1;
-                tv[q] = there ? lin_tlog(j, e0 + k) * j.inv_t : -INFINITY;
+                tv[q] = there ? lin_tlog(j, e0 + k) : -INFINITY;
                 if (ix[q] >= j.V) bad = true;
                 if (ix[q] >= 0) { bad |= !(tv[q] < INFINITY); tm = fmaxf(tm, tv[q]); }
             }
@@ -192,13 +193,13 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
             counts = in && (tm != -INFINITY || bad);
             const float tb = tm == -INFINITY ? 0.f : tm;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) if (ix[q] >= 0) ts += expf(tv[q] - tb);
+            for (int q = 0; q < Q; ++q) { tv[q] = (tv[q] - tb) * j.inv_t; if (ix[q] >= 0) ts += expf(tv[q]); }
             for (int d = G >> 1; d; d >>= 1) ts += __shfl_xor(ts, d);
             const float lt = logf(ts);
             if (bad) lse = NAN;
             float p[Q], all[Q];
 #pragma unroll
-            for (int q = 0; q < Q; ++q) { p[q] = counts && ix[q] >= 0 ? expf(tv[q] - tb - lt) : 0.f; all[q] = 0.f; }
+            for (int q = 0; q < Q; ++q) { p[q] = counts && ix[q] >= 0 ? expf(tv[q] - lt) : 0.f; all[q] = 0.f; }
             if (j.dsel)                                   // the same class twice in a row: each entry holds the sum over both
 #pragma unroll
                 for (int q = 0; q < Q; ++q)
@@ -217,7 +218,7 @@ __device__ __forceinline__ void lin_join_body(const LinJoin& j, int G, int gl, l
                     if (bad) { loss = ds = ps = NAN; }
                     else {
                         const float zq = j.zsel[e0 + k] - lse;
-                        if (p[q] > 0.f) loss += p[q] * (tv[q] - tb - lt - zq);
+                        if (p[q] > 0.f) loss += p[q] * (tv[q] - lt - zq);
                         ds = expf(zq) - all[q];
                         ps = p[q];
                     }

@@ -691,3 +691,27 @@ def test_entries_without_their_shares(shape, dtype, kept):
     gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(5))
     want, got = (_entry_step(*c, gout=gout, kept=kept, shares=s) for s in (True, False))
     assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(70, 64, 200), (4200, 64, 7)])
+@pytest.mark.parametrize("temperature", [0.02, 0.5, 1.0, 4.0])
+def test_teacher_logits_at_the_ends_of_the_type(shape, dtype, temperature):
+    """Entries masked by the type's lowest value have no share beside others; alone in a row they are equals and it counts, as are equal
+    ones at the largest value.  The definition does not change when a row's logits move together: the bounds are those of zeros."""
+    h, w, b, i, a = O.case(*shape, dtype, seed=17, top=4, ignored=0.1, short=0.1, bias=True)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    mask = torch.rand(a.shape, generator=torch.Generator().manual_seed(18)) < 0.3
+    mask[5], mask[6] = True, False
+    i[5:8] = torch.tensor([[1, 2, -1, 4], [0, 2, 3, -1], [3, 1, 2, 0]])
+    a[6], mask[7] = high, torch.tensor([True, True, True, False])
+    same = a.masked_fill(mask, -torch.inf)
+    alone = (mask | (i < 0)).all(1) & (i >= 0).any(1)               # only masked entries
+    assert bool(alone[5]) and not bool(alone[7])
+    same[alone], same[6] = 0.0, 0.0
+    a = a.masked_fill(mask, low).masked_fill(i < 0, torch.nan)      # (no entry, whatever the logit holds)
+    same = same.masked_fill(i < 0, 0.0)
+    want = O.evaluate(h, w, b, i, same, temperature=temperature, reduction="none")
+    gout = torch.ones(shape[0])
+    _compare(_run(h, w, b, i, a, temperature=temperature, reduction="none", gout=gout), want)
+    _compare(_run(h, w, b, i, a, temperature=temperature), O.evaluate(h, w, b, i, same, temperature=temperature))
