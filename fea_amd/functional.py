@@ -111,6 +111,8 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
         t = t.reshape(-1, t.shape[-1])
     epc = 16 // t.element_size()
     d = t.shape[1]
+    if t.shape[0] == 1 and t.stride(0) != d:           # the stride of a single row means nothing, and contiguous() would keep it
+        t = t.reshape(-1).contiguous().as_strided((1, d), (d, 1))
     if (t.stride(1) != 1 and d > 1) or t.stride(0) < d or t.stride(0) >= 1 << 21 or (d % epc == 0 and (t.data_ptr() % 16 or t.stride(0) % epc)):
         t = t.contiguous()
         if d % epc == 0 and t.data_ptr() % 16:         # contiguous already, but a view at an odd offset

@@ -103,3 +103,33 @@ def check(name, got, want):
     assert bool(same.all()), f"{name}: other infinities"
     assert far.numel() == 0 or float(far.max()) <= 0, f"{name}: {float(far.max()):.3e} beyond its bound, worst ratio " \
         f"{float(((got - value).abs() / bound)[torch.isfinite(value)].max()):.2f}"
+
+
+# Layouts of a single row [D] (the last position of a long sequence, a column, the start of wider rows, of none that is aligned, every second
+# element), as [1, D].
+ONE_ROW = ["plain", "last of many", "a column", "of rows that end off a line", "off a line", "every second"]
+
+
+def one_row(name, x):
+    """x [D] in the layout `name`, a tensor of one row."""
+    d = x.shape[0]
+    if name == "plain":
+        return x.clone()[None]
+    if name == "last of many":
+        n = (1 << 21) // d + 2
+        t = torch.zeros(1, n, d, dtype=x.dtype, device=x.device)
+        t[:, -1] = x
+        return t[:, -1]
+    if name == "a column":
+        return x.clone()[:, None].t()
+    if name == "of rows that end off a line":
+        t = torch.zeros(1, d + 3, dtype=x.dtype, device=x.device)
+        t[:, :d] = x
+        return t[:, :d]
+    if name == "off a line":
+        t = torch.zeros(3, d + 1, dtype=x.dtype, device=x.device)
+        t[1:2, 1:] = x
+        return t[1:2, 1:]
+    t = torch.zeros(1, 2 * d, dtype=x.dtype, device=x.device)
+    t[:, ::2] = x
+    return t[:, ::2]

@@ -104,3 +104,20 @@ def test_entries_without_their_shares_are_refused(rows, d, v, db):
     for k, psel in ((1, None), (3, at)):
         with pytest.raises(L.FeaError, match="workspace"):
             bwd(k, psel)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", O.ONE_ROW)
+def test_one_row_of_any_stride(name, dtype):
+    """A single row's stride means nothing (and contiguous() keeps it): the kernels get the features' number, of the same values, without a
+    copy where the row lies as they read it."""
+    for d in (64, 1024, 5, 1):
+        x = torch.randn(d, generator=torch.Generator().manual_seed(1)).to(dtype)
+        t = O.one_row(name, x)
+        assert t.shape[-1] == d and t.numel() == d
+        r = F._aligned_rows(t)
+        assert r.shape == (1, d) and r.stride() == (d, 1) and torch.equal(r[0], x)
+        if d * x.element_size() % 16 == 0:
+            assert r.data_ptr() % 16 == 0
+        if t.stride(-1) == 1 and t.data_ptr() % 16 == 0:
+            assert r.data_ptr() == t.data_ptr()

@@ -715,3 +715,23 @@ def test_teacher_logits_at_the_ends_of_the_type(shape, dtype, temperature):
     gout = torch.ones(shape[0])
     _compare(_run(h, w, b, i, a, temperature=temperature, reduction="none", gout=gout), want)
     _compare(_run(h, w, b, i, a, temperature=temperature), O.evaluate(h, w, b, i, same, temperature=temperature))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", O.ONE_ROW)
+@pytest.mark.parametrize("dim", [64, 51])
+def test_one_row_or_one_class_of_any_stride(name, dim, dtype):
+    """The score and the gradients of one hidden state, and of many over one class, whatever the single row's stride."""
+    for rows, classes in ((1, 300), (70, 1), (1, 1)):
+        h, w, b, t = O.case(rows, dim, classes, dtype, seed=24, bias=True)
+        want = O.evaluate(h, w, b, t)
+        x, y, b = h.to(DEV), w.to(DEV), b.to(DEV)
+        x = O.one_row(name, x[0]) if rows == 1 else x
+        y = O.one_row(name, y[0]) if classes == 1 else y
+        O.check("loss", F.linear_cross_entropy(x, y, t.to(DEV), bias=b), want["loss"])
+        leaves = [v.detach().requires_grad_(True) for v in (x, y, b)]
+        assert leaves[0].stride() == x.stride() and leaves[1].stride() == y.stride()
+        loss = F.linear_cross_entropy(*leaves[:2], t.to(DEV), bias=leaves[2])
+        _compare(dict(zip(("loss", "hidden", "weight", "bias"), [loss, *torch.autograd.grad(loss, leaves)])), want)
+        i, a = t[:, None].to(DEV), torch.zeros(rows, 1, device=DEV)
+        assert torch.equal(F.linear_distillation(x, y, a, i, bias=b), loss.detach())
