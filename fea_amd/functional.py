@@ -203,6 +203,8 @@ _LABELS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
+    if torch.jit.is_tracing():
+        raise L.FeaError(f"{who}: a trace (torch.jit) does not record the kernels; capture the call in a graph (torch.cuda.graph)")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"{who}: reduction {reduction!r} (use 'mean', 'sum' or 'none')")
     if not isinstance(hidden, torch.Tensor) or not isinstance(weight, torch.Tensor) or not isinstance(index, torch.Tensor):

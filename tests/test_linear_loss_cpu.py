@@ -121,3 +121,14 @@ def test_one_row_of_any_stride(name, dtype):
             assert r.data_ptr() % 16 == 0
         if t.stride(-1) == 1 and t.data_ptr() % 16 == 0:
             assert r.data_ptr() == t.data_ptr()
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_trace_is_refused(grad):
+    """torch.jit.trace would record the empty results and no kernel."""
+    with torch.set_grad_enabled(grad):
+        with pytest.raises(L.FeaError, match="linear_cross_entropy: a trace"):
+            torch.jit.trace(lambda h: F.linear_cross_entropy(h, W, T), (H,))
+        with pytest.raises(L.FeaError, match="linear_distillation: a trace"):
+            torch.jit.trace(lambda h: F.linear_distillation(h, W, A, I), (H,))
