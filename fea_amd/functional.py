@@ -106,7 +106,6 @@ def iou_from_counts(inter: torch.Tensor, union: torch.Tensor):
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """[..., D] -> [rows, D] as the kernels read it: contiguous rows, 16-byte aligned where D allows it, less than 2^21 elements apart."""
-    t = t.detach()
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     epc = 16 // t.element_size()
@@ -132,9 +131,7 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     h, w = _aligned_rows(hidden), _aligned_rows(weight)
     (rows, d), v = h.shape, w.shape[0]
     k = 1 if tlog is None else index.shape[-1]
-    ix = index.detach()
-    if ix.dtype != torch.int64:
-        ix = ix.to(torch.int64)
+    ix = index if index.dtype == torch.int64 else index.to(torch.int64)
     ix = ix.contiguous()
     b = None if bias is None else bias.detach().contiguous()
     dt = L.dt_code(h.dtype)
@@ -169,9 +166,11 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
-        grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want)
+    def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, train):
+        grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want) if train else 0
         loss, (ix, row, keep, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
+        if not grads:
+            return loss
         # the operands themselves are saved, so that autograd sees a change in place between forward and backward
         ctx.save_for_backward(hidden, weight, bias, ix, row, keep, count if reduction == "mean" else None)
         ctx.how = (temperature, reduction, 1 if tlog is None else index.shape[-1], tlog is not None, grads)
@@ -196,7 +195,7 @@ class _LinearLoss(torch.autograd.Function):
         ws = torch.empty(n, dtype=torch.uint8, device=h.device)
         L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, keep, grads >> 2, count, go, int(reduction == "none"),
                temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr(h.device.index))
-        return dh, dw, db, None, None, None, None, None
+        return dh, dw, db, None, None, None, None, None, None
 
 
 _LABELS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
@@ -236,9 +235,11 @@ def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperatu
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
-    if not train:
-        return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, 0)[0]
-    return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
+    # Where nothing wants a gradient the call need not become a node (6 of the 20 us that the host takes for a loss), unless forward-mode
+    # derivatives may be on the way, which the node refuses
+    if train or torch.autograd.forward_ad._current_level >= 0:
+        return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, train)
+    return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, 0)[0]
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor = None,

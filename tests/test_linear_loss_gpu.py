@@ -735,3 +735,21 @@ def test_one_row_or_one_class_of_any_stride(name, dim, dtype):
         _compare(dict(zip(("loss", "hidden", "weight", "bias"), [loss, *torch.autograd.grad(loss, leaves)])), want)
         i, a = t[:, None].to(DEV), torch.zeros(rows, 1, device=DEV)
         assert torch.equal(F.linear_distillation(x, y, a, i, bias=b), loss.detach())
+
+
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(top, grad):
+    """A tangent of hidden, weight or bias is refused, not dropped, whether gradients are recorded or not; a call without one is served."""
+    c = [t.to(DEV) for t in O.case(9, 16, 30, torch.float32, top=top, bias=True)]
+
+    def loss(h, w, b):
+        return F.linear_distillation(h, w, c[4], c[3], bias=b) if top else F.linear_cross_entropy(h, w, c[3], bias=b)
+    want = loss(*c[:3])
+    with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+        assert torch.equal(loss(*c[:3]), want)
+        for k in range(3):
+            x = list(c[:3])
+            x[k] = torch.autograd.forward_ad.make_dual(x[k], torch.ones_like(x[k]))
+            with pytest.raises(NotImplementedError):
+                loss(*x)
