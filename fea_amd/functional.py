@@ -125,7 +125,7 @@ def _row_state(row, rows, k, teacher):
     return at, at + rows * 8, at + rows * (8 + 4 * k) if teacher else None
 
 
-def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads):
+def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits, grads):
     """One forward call.  grads: 0, or what the backward will want (1 hidden, 2 weight, 4 bias).  Returns (loss, saved)."""
     dev = hidden.device
     h, w = _aligned_rows(hidden), _aligned_rows(weight)
@@ -140,12 +140,14 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
     if grads:
         row = torch.empty(rows * (2 + k * (1 if tlog is None else 2)), dtype=torch.float32, device=dev)
         stat, dsel, psel = _row_state(row, rows, k, tlog is not None)
-        n = L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, grads >> 2)
-        if 0 < n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33)):
+        n = 0 if keep_logits is False else L.load().fea_linear_loss_keep_bytes(rows, d, v, dt, grads >> 2)
+        if n > 0 and (keep_logits or n <= int(os.environ.get("FEA_AMD_LINEAR_KEEP", 1 << 33))):
             try:
                 keep = torch.empty(n, dtype=torch.uint8, device=dev)
             except torch.cuda.OutOfMemoryError:
-                pass                                        # the backward recomputes them
+                if keep_logits:
+                    raise
+                # (left open: the backward recomputes them)
     if reduction == "none":
         loss, count = torch.empty(index.shape if tlog is None else index.shape[:-1], dtype=torch.float32, device=dev), None
         outs = (loss, None, None, 0)
@@ -166,9 +168,9 @@ def _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperatur
 
 class _LinearLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, train):
+    def forward(ctx, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits, train):
         grads = sum(bit for bit, want in zip((1, 2, 4), ctx.needs_input_grad) if want) if train else 0
-        loss, (ix, row, keep, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, grads)
+        loss, (ix, row, keep, count) = _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits, grads)
         if not grads:
             return loss
         # the operands themselves are saved, so that autograd sees a change in place between forward and backward
@@ -195,17 +197,19 @@ class _LinearLoss(torch.autograd.Function):
         ws = torch.empty(n, dtype=torch.uint8, device=h.device)
         L.call("fea_linear_loss_bwd", h, h.stride(0), w, w.stride(0), b, ix, k, stat, dsel, psel, keep, grads >> 2, count, go, int(reduction == "none"),
                temperature, dh, dw, db, ws, n, rows, d, v, dt, L.stream_ptr(h.device.index))
-        return dh, dw, db, None, None, None, None, None, None
+        return dh, dw, db, None, None, None, None, None, None, None
 
 
 _LABELS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
-def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction):
+def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits):
     if torch.jit.is_tracing():
         raise L.FeaError(f"{who}: a trace (torch.jit) does not record the kernels; capture the call in a graph (torch.cuda.graph)")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"{who}: reduction {reduction!r} (use 'mean', 'sum' or 'none')")
+    if keep_logits is not None and not isinstance(keep_logits, bool):
+        raise ValueError(f"{who}: keep_logits {keep_logits!r} (use True, False or None)")
     if not isinstance(hidden, torch.Tensor) or not isinstance(weight, torch.Tensor) or not isinstance(index, torch.Tensor):
         raise ValueError(f"{who}: hidden, weight and the labels are tensors")
     if hidden.dtype != weight.dtype or hidden.dtype not in (torch.float32, torch.bfloat16):
@@ -234,34 +238,39 @@ def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperatu
         return zero if reduction != "none" else zero.expand(lead)
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction)
+            return _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits)
     # Where nothing wants a gradient the call need not become a node (6 of the 20 us that the host takes for a loss), unless forward-mode
     # derivatives may be on the way, which the node refuses
     if train or torch.autograd.forward_ad._current_level >= 0:
-        return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, train)
-    return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, 0)[0]
+        return _LinearLoss.apply(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits, train)
+    return _linear_loss_fwd(hidden, weight, bias, index, tlog, ignore_index, temperature, reduction, keep_logits, 0)[0]
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: torch.Tensor = None,
-                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+                         ignore_index: int = -100, reduction: str = "mean", keep_logits: bool = None) -> torch.Tensor:
     """Softmax cross entropy of `hidden @ weight.T + bias` against one label per row.
 
     hidden [..., D] and weight [classes, D]: both float32 or both bfloat16 (sums, softmax and loss in 32 bits); target [...]
     integers; bias [classes], float32 or the weight's type.  Rows whose target is `ignore_index` do not count: loss 0 and
     gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
-    Differentiable once, in hidden, weight and bias.  The logits are never there in full precision and shape: for a backward
-    the forward keeps 2 bytes of each (4 in float32, with a bias gradient, and for up to 64 rows) if that is 8 GiB or less
-    (FEA_AMD_LINEAR_KEEP: another limit in bytes, 0 for none); beyond it the backward recomputes them in pieces.
+    Differentiable once, in hidden, weight and bias.
+    keep_logits, in a call that has a backward: True, the forward keeps the logits for it, in 16 bits each (bfloat16; the gradients' shares
+    of the softmax are off by 4.9e-4 of themselves, an eighth of their rounding to bfloat16 behind that) or whole in 32 (float32, with a bias
+    gradient, up to 64 rows, a split reduction), and an allocation that fails is raised; False, none are kept and the backward computes
+    them again in pieces of up to 2^28, which takes a third more products and no memory for all of them; None, they are kept if
+    they take 8 GiB or less (FEA_AMD_LINEAR_KEEP: another limit in bytes, 0 for none) and the memory is there.  With True or False the
+    gradients are the same from run to run; with None they depend, within these roundings, on whether there was room.
+    Few classes of few features (32, 64) are always computed again, which reads no more.
     An NHWC feature map and a 1x1 convolution's weight viewed [classes, channels] are taken as they are."""
     ignore_index = int(ignore_index)
     if not -(1 << 63) <= ignore_index < 1 << 63:
         raise ValueError(f"linear_cross_entropy: ignore_index {ignore_index} is no 64-bit integer")
-    return _linear_loss("linear_cross_entropy", hidden, weight, bias, target, None, ignore_index, 1.0, reduction)
+    return _linear_loss("linear_cross_entropy", hidden, weight, bias, target, None, ignore_index, 1.0, reduction, keep_logits)
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
-                        bias: torch.Tensor = None, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+                        bias: torch.Tensor = None, temperature: float = 1.0, reduction: str = "mean", keep_logits: bool = None) -> torch.Tensor:
     """Distillation of `hidden @ weight.T + bias` from a teacher's top logits.
 
     teacher_logits [..., K] (float32 or bfloat16) and teacher_index [..., K] (integers): the teacher's K (1..256) largest logits of
@@ -269,7 +278,7 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
     q = softmax of all the student's logits / T, the loss of a row is T^2 sum_k p_k (log p_k - log q_{index_k}).  Rows without
     an entry (or with -inf logits alone) do not count.  A class named twice in a row has the sum of both shares; an index
     beyond the classes, a NaN or +inf teacher logit make the loss and the gradients NaN.  The teacher has no gradient.
-    hidden, weight, bias, reduction, the result and what is kept for the backward as in `linear_cross_entropy`."""
+    hidden, weight, bias, reduction, keep_logits and the result as in `linear_cross_entropy`."""
     who = "linear_distillation"
     if not isinstance(teacher_logits, torch.Tensor) or not isinstance(teacher_index, torch.Tensor):
         raise ValueError(f"{who}: teacher_logits and teacher_index are tensors")
@@ -281,4 +290,4 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
     temperature = float(temperature)
     if not 1e-3 <= temperature <= 1e3:
         raise ValueError(f"{who}: temperature {temperature} (0.001 to 1000)")
-    return _linear_loss(who, hidden, weight, bias, teacher_index, teacher_logits, 0, temperature, reduction)
+    return _linear_loss(who, hidden, weight, bias, teacher_index, teacher_logits, 0, temperature, reduction, keep_logits)

@@ -370,7 +370,7 @@ int fea_adamw_clip_step(const long long* seg, int nseg, const float* g_flat, flo
  * fp32: products of a certain size run as six products of bf16 planes (24 bits in three), the others on the fp32 matrix rate.
  * ws: fea_linear_loss_ws_bytes(..., grads) bytes, 256-byte aligned; grads = 0 for the forwards, 1 dh + 2 dw + 4 db for the
  * backward, + 8 with keep
- * (0 bytes = sizes that are refused).  Results are the same from run to run. */
+ * (0 bytes = sizes that are refused).  Results are the same from run to run; with and without keep they differ by the roundings above. */
 size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads);
 size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int wide);
 int fea_linear_ce_fwd(const void* h, long long ldh, const void* w, long long ldw, const float* bias, const long long* target,

@@ -132,3 +132,11 @@ def test_a_trace_is_refused(grad):
             torch.jit.trace(lambda h: F.linear_cross_entropy(h, W, T), (H,))
         with pytest.raises(L.FeaError, match="linear_distillation: a trace"):
             torch.jit.trace(lambda h: F.linear_distillation(h, W, A, I), (H,))
+
+
+@pytest.mark.parametrize("bad", [0, 1, "yes", 1 << 33])
+def test_keep_logits_is_a_choice(bad):
+    with pytest.raises(ValueError, match="linear_cross_entropy: keep_logits"):
+        F.linear_cross_entropy(H, W, T, keep_logits=bad)
+    with pytest.raises(ValueError, match="linear_distillation: keep_logits"):
+        F.linear_distillation(H, W, A, I, keep_logits=bad)

@@ -753,3 +753,71 @@ def test_forward_mode_is_refused(top, grad):
             x[k] = torch.autograd.forward_ad.make_dual(x[k], torch.ones_like(x[k]))
             with pytest.raises(NotImplementedError):
                 loss(*x)
+
+
+def _kept(loss):
+    return any(t is not None and t.dtype == torch.uint8 for t in loss.grad_fn.saved_tensors)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(33, 64, 500), (300, 72, 700), (200, 51, 500)])
+@pytest.mark.parametrize("top", [0, 3])
+def test_keep_logits_decides(shape, dtype, top, monkeypatch):
+    """keep_logits = True and False whatever the limit is, with the gradients of a limit that allows them and of none, and either within the
+    bounds."""
+    c = O.case(*shape, dtype, seed=28, top=top, ignored=0.1)
+    x = [t.to(DEV).requires_grad_(True) for t in c[:2]]
+
+    def step(**how):
+        loss = F.linear_distillation(*x, c[4].to(DEV), c[3].to(DEV), **how) if top else F.linear_cross_entropy(*x, c[3].to(DEV), **how)
+        return _kept(loss), dict(zip(("loss", "hidden", "weight"), [loss.detach(), *torch.autograd.grad(loss, x)]))
+    for choice in (True, False):
+        monkeypatch.setenv("FEA_AMD_LINEAR_KEEP", "0" if choice else str(1 << 40))
+        kept, got = step(keep_logits=choice)
+        assert kept == choice
+        _compare(got, O.evaluate(*c, kept=None if choice else False))
+        monkeypatch.setenv("FEA_AMD_LINEAR_KEEP", str(1 << 40) if choice else "0")
+        kept, same = step()
+        assert kept == choice and all(torch.equal(got[k], same[k]) for k in got)
+    monkeypatch.undo()
+    with torch.no_grad():
+        assert torch.equal(F.linear_distillation(*x, c[4].to(DEV), c[3].to(DEV), keep_logits=True) if top else
+                           F.linear_cross_entropy(*x, c[3].to(DEV), keep_logits=True), got["loss"])
+
+
+def test_keep_logits_raises_where_there_is_no_room(monkeypatch):
+    """Asked for, a failed allocation is the caller's; not wanted, none is tried."""
+    c = O.case(300, 64, 700, torch.bfloat16, seed=52, ignored=0.1)
+    n = L.load().fea_linear_loss_keep_bytes(300, 64, 700, L.BF16, 0)
+    want = _run(*c, keep_logits=False)
+    empty = torch.empty
+
+    def full(*size, **how):
+        if size == (n,) and how.get("dtype") == torch.uint8:
+            raise torch.cuda.OutOfMemoryError("no room")
+        return empty(*size, **how)
+    monkeypatch.setattr(torch, "empty", full)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        _run(*c, keep_logits=True)
+    for choice in (False, None):
+        got = _run(*c, keep_logits=choice)
+        assert all(torch.equal(got[k], want[k]) for k in want)
+
+
+def test_without_kept_logits_memory_is_bounded_by_a_piece():
+    """3.3e9 logits (6.6 GB in 16 bits): the step takes its gradients, a piece of 2^28 in 16 bits and as much again for partial sums."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    h = torch.randn(16384, 64, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    w = torch.randn(200000, 64, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    t = torch.randint(0, 200000, (16384,), generator=g, device=DEV)
+    peaks = []
+    for choice in (False, True):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        start = torch.cuda.memory_allocated()
+        loss = F.linear_cross_entropy(h, w, t, keep_logits=choice)
+        torch.autograd.grad(loss, [h, w])
+        del loss
+        torch.cuda.synchronize()
+        peaks.append(torch.cuda.max_memory_allocated() - start)
+    assert peaks[0] < 2 * (1 << 29) and peaks[1] > 16384 * 200000 * 2, peaks
