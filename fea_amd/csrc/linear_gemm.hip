@@ -19,13 +19,6 @@
 
 static constexpr int LG_T = 128, LG_CK = 32;
 
-__device__ __forceinline__ void lg_store4(float* p, const float (&v)[4], int n) {
-    if (n >= 4 && ((uintptr_t)p & 15) == 0) *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-    else
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (i < n) p[i] = v[i];
-}
-
 // TM: label rows of a tile, 128 or, for 64 rows and less in all, 64 with the four waves along the classes (64 x 32 each)
 template <int EPI, bool ALN, bool TA, int TM>
 __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
@@ -122,10 +115,8 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
-                    const int n = ncol(j, e);
-                    if (n >= g.N) continue;
-                    const float v[4] = {acc[i][j][e] * sc, acc[i][j][e + 1] * sc, acc[i][j][e + 2] * sc, acc[i][j][e + 3] * sc};
-                    lg_store4(o + n, v, (g.slab ? (int)g.ldo : g.N) - n);
+                    const int n = ncol(j, e);         // (rows of the output are whole 16 bytes)
+                    if (n < g.N) *reinterpret_cast<f32x4*>(o + n) = f32x4{acc[i][j][e] * sc, acc[i][j][e + 1] * sc, acc[i][j][e + 2] * sc, acc[i][j][e + 3] * sc};
                 }
         }
         return;
@@ -224,8 +215,7 @@ __global__ __launch_bounds__(256, 2) void lin_gemm_kernel(const LinGemm g) {
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
                     const int n = ncol(j, e);
-                    const float v[4] = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                    if (m < g.M && n < g.Npad) lg_store4((float*)g.dz + m * g.lddz + n, v, g.Npad - n);
+                    if (m < g.M && n < g.Npad) *reinterpret_cast<f32x4*>((float*)g.dz + m * g.lddz + n) = f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
                 }
         }
     }
@@ -277,6 +267,13 @@ int fea_lin_gemm(int epi, int dtype, int tile, LinGemm g, hipStream_t s) {
     FEA_CHECK(dtype == FEA_F32 ? tile == 128 : aln && g.lda < (1 << 21) && g.ldb < (1 << 21), FEA_E_UNSUPPORTED_SHAPE, "lin_gemm: tile %d, strides %lld, %lld", tile, g.lda, g.ldb);
     FEA_CHECK(dtype != FEA_PL || (g.Kp > 0 && g.Kp % 64 == 0 && g.K == 6 * g.Kp && g.Kr <= g.Kp && (epi != LIN_STORE || g.slab)), FEA_E_BADARG, "lin_gemm: planes of %d, K %d", g.Kp, g.K);
     FEA_CHECK(epi != LIN_LSE || (g.slab != nullptr) == (g.splits > 1), FEA_E_BADARG, "lin_gemm: %d parts", g.splits);
+    // what the stores take: whole 16 bytes of a row (slabs' rows are padded; gradients of other widths go through slabs)
+    const int epo = g.slab || dtype == FEA_F32 ? 4 : 8;
+    if (epi == LIN_STORE)
+        FEA_CHECK((g.slab || g.N % epo == 0) && g.ldo >= g.N && g.ldo % epo == 0 && (uintptr_t)(g.slab ? (void*)g.slab : g.out) % 16 == 0, FEA_E_BADARG,
+                  "lin_gemm: result of %d columns in rows of %lld", g.N, g.ldo);
+    if (epi == LIN_DZ)
+        FEA_CHECK(g.Npad >= g.N && g.Npad % 64 == 0 && g.lddz % 8 == 0 && (uintptr_t)g.dz % 16 == 0, FEA_E_BADARG, "lin_gemm: dz of %d columns in rows of %lld", g.Npad, g.lddz);
     FEA_CHECK(epi != LIN_STORE || dtype == FEA_F32 || (g.Kr > 0 && g.Kr <= (dtype == FEA_PL ? g.Kp : g.K)), FEA_E_BADARG, "lin_gemm: reduction of %d of %d", g.Kr, g.K);
     g.ntm = (g.M + tile - 1) / tile; g.ntn = (g.N + tile - 1) / tile;
     if (g.splits < 1) { g.splits = 1; g.kper = g.K; }

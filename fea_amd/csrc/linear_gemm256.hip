@@ -275,7 +275,7 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            // the same by group: 4 MFMA (2 where NT is 4), an LDS read, an LDS write, a load
+            // the same by group: 2 MFMA (1 before the read in every second group), an LDS read, an LDS write, a load
 #pragma unroll
             for (int q = 0; q < NL; ++q) { frd(s, 1, q); lput(u, s ^ 1, q); gload(u, q); }
 #pragma unroll
@@ -284,9 +284,8 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
                 for (int j = 0; j < NT; ++j) mma(0, i, j);
 #pragma unroll
             for (int q = 0; q < NL; ++q) {
-                if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); else if (q & 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (q & 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                if (NT == 8) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
@@ -331,7 +330,6 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
 
     if constexpr (EPI == LIN_STORE) {
         const float common = g.scale == 2 ? lin_row_scale(g.gout, 0, g.count, g.t, 1.f, 0) : 1.f;
-        const bool wide = g.slab ? g.ldo % 4 == 0 : g.N % 8 == 0 && g.ldo % 8 == 0 && (uintptr_t)g.out % 16 == 0;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int m = mrow(i);
@@ -343,24 +341,14 @@ __global__ __launch_bounds__(256, NT == 8 ? 1 : 2) void lin_gemm256_kernel(const
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const int n = ncol(j);
-                    if (wide) { if (m < g.M && n < g.N) *reinterpret_cast<f32x4*>(o + n) = acc[i][j]; }
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) if (m < g.M && n + e < g.N) o[n + e] = acc[i][j][e];
+                    if (m < g.M && n < g.N) *reinterpret_cast<f32x4*>(o + n) = acc[i][j];
                 }
             } else {
                 __bf16* const o = (__bf16*)g.out + m * g.ldo;
 #pragma unroll
                 for (int p = 0; p < NT / 2; ++p) {
-                    if (wide) {
-                        const u32x4 v = pairs(acc[i][2 * p], acc[i][2 * p + 1]);
-                        if (m < g.M && pcol + 32 * p < g.N) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
-                    } else
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int n = ncol(2 * p + (e >> 2)) + (e & 3);
-                            if (m < g.M && n < g.N) o[n] = (__bf16)acc[i][2 * p + (e >> 2)][e & 3];
-                        }
+                    const u32x4 v = pairs(acc[i][2 * p], acc[i][2 * p + 1]);
+                    if (m < g.M && pcol + 32 * p < g.N) *reinterpret_cast<u32x4*>(o + pcol + 32 * p) = v;
                 }
             }
         }

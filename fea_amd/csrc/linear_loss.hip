@@ -735,13 +735,10 @@ static int lin_copy(const LinDims& d, const LinForm& f, const LinCopies& js, hip
     if (!n) return FEA_OK;
     FEA_CHECK(n < INT_MAX, FEA_E_UNSUPPORTED_SHAPE, "lin_copy: %lld tiles", n);
     const dim3 grid((unsigned)n), bl(256);
-    const bool aln = !d.odd();
-    if (f.dt == FEA_PL && aln)       hipLaunchKernelGGL((lin_copy_kernel<float, true, true>), grid, bl, 0, s, js);
-    else if (f.dt == FEA_PL)         hipLaunchKernelGGL((lin_copy_kernel<float, true, false>), grid, bl, 0, s, js);
-    else if (f.dt == FEA_F32 && aln) hipLaunchKernelGGL((lin_copy_kernel<float, false, true>), grid, bl, 0, s, js);
-    else if (f.dt == FEA_F32)        hipLaunchKernelGGL((lin_copy_kernel<float, false, false>), grid, bl, 0, s, js);
-    else if (aln)                    hipLaunchKernelGGL((lin_copy_kernel<__bf16, false, true>), grid, bl, 0, s, js);
-    else                             hipLaunchKernelGGL((lin_copy_kernel<__bf16, false, false>), grid, bl, 0, s, js);
+    FEA_CHECK(f.dt == FEA_PL || (f.dt == FEA_BF16 && d.odd()), FEA_E_BADARG, "lin_copy: operands that are read as they lie");
+    if (f.dt == FEA_BF16) hipLaunchKernelGGL((lin_copy_kernel<__bf16, false, false>), grid, bl, 0, s, js);
+    else if (d.odd())     hipLaunchKernelGGL((lin_copy_kernel<float, true, false>), grid, bl, 0, s, js);
+    else                  hipLaunchKernelGGL((lin_copy_kernel<float, true, true>), grid, bl, 0, s, js);
     FEA_LAUNCH_CHECK();
     return FEA_OK;
 }
