@@ -1,7 +1,7 @@
 // The fp32 products of the many-class loss heads on the exact fp32 matrix rate, any alignment, and the choice of a product's kernel.
 //
 //   z[m][n] = (sum_k a[m][k] b[n][k] + bias[n]) / T
-//   LIN_LSE:   per row and column tile (max, sum exp(z - max)); no z leaves the registers
+//   LIN_LSE:   per row and column tile (max, sum exp(z - max)); z itself is stored, in fp32, where the caller keeps it for the backward
 //   LIN_DZ:    q = exp(z - lse_m), stored row-major; the label's entries are corrected behind it.  The upstream gradient is not in it: in the
 //              bf16 form a common factor would round the labels' entries, all close to it, the same way in every row (2,048 rows:
 //              3.2e-3 off in dw and dh instead of 1.8e-3)
