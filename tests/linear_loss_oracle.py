@@ -32,10 +32,15 @@ def case(rows, dim, classes, dtype, seed=0, top=0, ignored=0.0, short=0.0, bias=
     return h, w, b, i, (torch.randn(rows, top, generator=g) * 2 + 5).to(dtype)
 
 
-def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, reduction="mean", gout=None, kept=None):
+def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, reduction="mean", gout=None, kept=None, norms=False):
     """{"loss", "hidden", "weight", "bias"}: values and bounds, as (value, bound) pairs in 64 bits.  gout: upstream gradient of the losses
     (rows) for "none", else of the result.  kept: the
-    backward had the forward's logits (None: as a head whose every operand has a gradient would)."""
+    backward had the forward's logits (None: as a head whose every operand has a gradient would).
+    norms: "hidden" and "weight" as (value, bound of the Frobenius norm of all their errors together).  Element by element a bound adds up
+    the sizes of a column's errors, and from some hundred rows on one row's whole share fits in.  With E the errors of dz, |E| <= off:
+    |E w|_F <= |off|_F |w|_2 and |E^T h|_F <= |off|_F |h|_2 (the largest singular value), the products' own roundings element by element on
+    top.  With an upstream gradient for every row dw = (q - p)^T (g h), both rounded: |E^T (g h)|_F + |(q - p)^T (u |g h|)|_F, E of q - p
+    alone, the product of both errors u times the first."""
     dtype, t = h.dtype, temperature
     u = torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else E
     hd, wd = h.double().reshape(-1, h.shape[-1]), w.double()
@@ -85,6 +90,19 @@ def evaluate(h, w, b, index, tlog=None, ignore_index=-100, temperature=1.0, redu
     kept = 4.89e-4 if kept and dtype == torch.bfloat16 else 0.0
     off = g.abs()[:, None] * (q * kept * (1 + u) + (1.7e-28 if kept else 0.0) + q * 2 * dz_log[:, None] + (8 + (0 if tlog is None else index.shape[-1])) * E * (p + q) + p * arg[:, None]) + u * dz.abs() + 2 * E * dz.abs()
     dh, dw = dz @ wd, dz.T @ hd
+    if norms:
+        def largest(x):                                     # singular value, from the smaller Gram matrix; 1e-9 for its own roundings
+            return float(torch.linalg.eigvalsh(x.T @ x if x.shape[0] >= x.shape[1] else x @ x.T)[-1].clamp(min=0).sqrt()) * (1 + 1e-9)
+        sums = (v + 8) * E * (dz.abs() @ wd.abs()) + u * dh.abs()
+        out["hidden"] = (dh, float(off.norm()) * largest(wd) + float(sums.norm()))
+        sums = (rows + 8) * E * (dz.abs().T @ hd.abs()) + u * dw.abs()
+        if reduction == "none":
+            gh, size = g[:, None] * hd, g.abs()[:, None].clamp(min=1e-300)
+            first = float((off / size).norm()) * largest(gh)
+            out["weight"] = (dw, first * (1 + u) + u * float(gh.norm()) * largest(q - p) + float(sums.norm()))
+        else:
+            out["weight"] = (dw, float(off.norm()) * largest(hd) + float(sums.norm()))
+        return out
     out["hidden"] = (dh, off @ wd.abs() + (v + 8) * E * (dz.abs() @ wd.abs()) + u * dh.abs() + 1e-37)
     own = u * (1 + u) if reduction == "none" else 0.0
     out["weight"] = (dw, off.T @ hd.abs() + own * (dz.abs().T @ hd.abs()) + (rows + 8) * E * (dz.abs().T @ hd.abs()) + u * dw.abs() + 1e-37)
@@ -103,6 +121,13 @@ def check(name, got, want):
     assert bool(same.all()), f"{name}: other infinities"
     assert far.numel() == 0 or float(far.max()) <= 0, f"{name}: {float(far.max()):.3e} beyond its bound, worst ratio " \
         f"{float(((got - value).abs() / bound)[torch.isfinite(value)].max()):.2f}"
+
+
+def check_norm(name, got, want):
+    """The Frobenius norm of all errors together."""
+    value, bound = want
+    off = float((got.detach().double().cpu().reshape(value.shape) - value).norm())
+    assert off <= bound, f"{name}: errors of norm {off:.3e}, {off / bound:.2f} of their bound"
 
 
 # Layouts of a single row [D] (the last position of a long sequence, a column, the start of wider rows, of none that is aligned, every second

@@ -140,3 +140,33 @@ def test_keep_logits_is_a_choice(bad):
         F.linear_cross_entropy(H, W, T, keep_logits=bad)
     with pytest.raises(ValueError, match="linear_distillation: keep_logits"):
         F.linear_distillation(H, W, A, I, keep_logits=bad)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_norms_find_what_elements_hide(reduction):
+    """bfloat16 roundings of dz and of the results alone stay within the norms' bounds; a row lost from the weight's gradient, or dz rounded
+    to the bits of an 8-bit type, does not."""
+    h, w, _, t = O.case(513, 640, 700, torch.bfloat16, seed=33, ignored=0.1)
+    g = torch.randn(513, generator=torch.Generator().manual_seed(1))
+    how = {"reduction": reduction, "gout": g if reduction == "none" else None, "kept": False}
+    want = O.evaluate(h, w, None, t, norms=True, **how)
+    on = t != -100
+    p = torch.nn.functional.one_hot(t.clamp(min=0), 700).double()
+    g = (g.double() if reduction == "none" else torch.full((513,), 1.0 / int(on.sum()), dtype=torch.float64)) * on
+    dz = torch.softmax(h.double() @ w.double().T, 1) - p
+
+    def step(dz):
+        dh = g[:, None] * (dz @ w.double())
+        dw = dz.T @ (g[:, None] * h.double()).bfloat16().double() if reduction == "none" else (dz * g[:, None]).T @ h.double()
+        return dh.bfloat16(), dw.bfloat16()
+    dh, dw = step(dz.bfloat16().double())
+    O.check_norm("hidden", dh, want["hidden"])
+    O.check_norm("weight", dw, want["weight"])
+    lost = dz.bfloat16().double()
+    lost[int(on.nonzero()[5] if reduction == "mean" else g.abs().argmax())] = 0.0
+    with pytest.raises(AssertionError, match="weight"):
+        O.check_norm("weight", step(lost)[1], want["weight"])
+    m, e = torch.frexp(dz)
+    for k, name in enumerate(("hidden", "weight")[:2 if reduction == "mean" else 1]):      # (none: the bound allows for hidden's rounding too)
+        with pytest.raises(AssertionError, match=name):
+            O.check_norm(name, step(torch.ldexp((m * 4).round() / 4, e))[k], want[name])

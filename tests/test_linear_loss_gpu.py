@@ -821,3 +821,20 @@ def test_without_kept_logits_memory_is_bounded_by_a_piece():
         torch.cuda.synchronize()
         peaks.append(torch.cuda.max_memory_allocated() - start)
     assert peaks[0] < 2 * (1 << 29) and peaks[1] > 16384 * 200000 * 2, peaks
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(64, 128, 500), (200, 72, 500), (513, 640, 1537), (1300, 643, 2011), (2049, 1096, 2310), (300, 520, 20000), (4100, 64, 6), (4200, 33, 30)])
+@pytest.mark.parametrize("top", [0, 4])
+@pytest.mark.parametrize("keep", [True, False])
+def test_norms_of_the_errors(shape, dtype, top, keep):
+    """All errors of a gradient together, with one upstream gradient and with one for every row, logits kept and recomputed."""
+    c = O.case(*shape, dtype, seed=34 + top, top=top, ignored=0.1, short=0.2)
+    kw = {"temperature": 2.0} if top else {}
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(8))
+    for how in ({}, {"reduction": "none", "gout": gout}):
+        want = O.evaluate(*c, norms=True, kept=None if keep else False, **kw, **how)
+        got = _run(*c, keep_logits=keep, **kw, **how)
+        O.check("loss", got["loss"], want["loss"])
+        for k in ("hidden", "weight"):
+            O.check_norm(k, got[k], want[k])
