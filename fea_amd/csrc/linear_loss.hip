@@ -565,6 +565,12 @@ static LinDims lin_dims(long long rows, int D, int V, int K, int dtype) {
     return d;
 }
 
+// The sizes that are served (lin_check says which of them a call does not keep to)
+static constexpr int LIN_ROWS = INT_MAX / 2, LIN_D = 1 << 16, LIN_V = 1 << 24, LIN_K = 256;
+static bool lin_served(long long rows, int D, int V, int K, int dtype) {
+    return rows >= 1 && rows <= LIN_ROWS && D >= 1 && D <= LIN_D && V >= 1 && V <= LIN_V && K >= 1 && K <= LIN_K && (dtype == FEA_F32 || dtype == FEA_BF16);
+}
+
 // The form that a call's products take: the operands as they are, or fp32 as three bf16 planes where the copies pay.
 struct LinForm {
     int dt, es, mul, pad;         // dtype of the products, bytes of an element, elements of a row per channel, what a row is rounded up to
@@ -709,14 +715,14 @@ struct LinKeep {
     LinKeep(const LinDims& d, int wide) : codes(d.dtype == FEA_BF16 && d.rows > 64 && !wide && lin_fwd_plan(d).parts == 1), ld(up(d.V, 64)), es(codes ? 2 : 4), table((size_t)up(d.rows * ld * es, 256)) {}
 };
 extern "C" size_t fea_linear_loss_keep_bytes(long long rows, int D, int V, int dtype, int wide) {
-    if (rows <= 0 || D <= 0 || V <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16) || fea_lin_few(rows, D, V)) return 0;
+    if (!lin_served(rows, D, V, 1, dtype) || fea_lin_few(rows, D, V)) return 0;
     const LinDims d = lin_dims(rows, D, V, 1, dtype);
     const LinKeep k(d, wide);
     return k.table + (k.codes ? (size_t)rows * lin_fwd_plan(d).ntn * 8 * sizeof(float) : 0);
 }
 
 extern "C" size_t fea_linear_loss_ws_bytes(long long rows, int D, int V, int K, int dtype, int grads) {
-    if (rows <= 0 || D <= 0 || V <= 0 || K <= 0 || (dtype != FEA_F32 && dtype != FEA_BF16)) return 0;
+    if (!lin_served(rows, D, V, K, dtype)) return 0;
     const LinDims d = lin_dims(rows, D, V, K, dtype);
     if (!grads) { LinFwdWs w; return lin_fwd_carve(d, lin_fwd_plan(d), nullptr, w); }
     LinBwdWs w;
@@ -756,10 +762,10 @@ static int lin_reduce(const LinDims& d, const float* slab, int splits, long long
 
 static int lin_check(const char* who, const LinDims& d, const void* h, long long ldh, const void* w, long long ldw, const float* bias) {
     FEA_CHECK(d.dtype == FEA_F32 || d.dtype == FEA_BF16, FEA_E_BADARG, "%s: dtype %d", who, d.dtype);
-    FEA_CHECK(d.rows >= 1 && d.rows <= INT_MAX / 2, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld rows, 1..%d are served", who, d.rows, INT_MAX / 2);
-    FEA_CHECK(d.D >= 1 && d.D <= (1 << 16), FEA_E_UNSUPPORTED_SHAPE, "%s: %d features, 1..%d are served", who, d.D, 1 << 16);
-    FEA_CHECK(d.V >= 1 && d.V <= (1 << 24), FEA_E_UNSUPPORTED_SHAPE, "%s: %d classes, 1..%d are served", who, d.V, 1 << 24);
-    FEA_CHECK(d.K >= 1 && d.K <= 256, FEA_E_UNSUPPORTED_SHAPE, "%s: %d teacher entries per row, 1..256 are served", who, d.K);
+    FEA_CHECK(d.rows >= 1 && d.rows <= LIN_ROWS, FEA_E_UNSUPPORTED_SHAPE, "%s: %lld rows, 1..%d are served", who, d.rows, LIN_ROWS);
+    FEA_CHECK(d.D >= 1 && d.D <= LIN_D, FEA_E_UNSUPPORTED_SHAPE, "%s: %d features, 1..%d are served", who, d.D, LIN_D);
+    FEA_CHECK(d.V >= 1 && d.V <= LIN_V, FEA_E_UNSUPPORTED_SHAPE, "%s: %d classes, 1..%d are served", who, d.V, LIN_V);
+    FEA_CHECK(d.K >= 1 && d.K <= LIN_K, FEA_E_UNSUPPORTED_SHAPE, "%s: %d teacher entries per row, 1..%d are served", who, d.K, LIN_K);
     FEA_CHECK(h && w, FEA_E_BADARG, "%s: null operand", who);
     FEA_CHECK(ldh >= d.D && ldw >= d.D, FEA_E_BADARG, "%s: row stride below the %d features (hidden %lld, weight %lld)", who, d.D, ldh, ldw);
     FEA_CHECK(((uintptr_t)h | (uintptr_t)w) % d.es == 0 && (uintptr_t)bias % 4 == 0, FEA_E_BADARG, "%s: misaligned operand", who);

@@ -216,6 +216,8 @@ def _linear_loss(who, hidden, weight, bias, index, tlog, ignore_index, temperatu
         raise ValueError(f"{who}: hidden and weight are both float32 or both bfloat16 (got {hidden.dtype}, {weight.dtype})")
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"{who}: hidden [..., D] and weight [classes, D] do not fit (got {tuple(hidden.shape)}, {tuple(weight.shape)})")
+    if weight.shape[0] > 1 << 24 or weight.shape[1] > 1 << 16 or hidden.numel() // weight.shape[1] >= 1 << 30:
+        raise ValueError(f"{who}: up to 2^24 classes of 2^16 features and less than 2^30 rows are served (got {tuple(hidden.shape)}, {tuple(weight.shape)})")
     if index.dtype not in _LABELS:
         raise ValueError(f"{who}: labels are integers (got {index.dtype})")
     lead = index.shape if tlog is None else index.shape[:-1]
@@ -250,8 +252,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
                          ignore_index: int = -100, reduction: str = "mean", keep_logits: bool = None) -> torch.Tensor:
     """Softmax cross entropy of `hidden @ weight.T + bias` against one label per row.
 
-    hidden [..., D] and weight [classes, D]: both float32 or both bfloat16 (sums, softmax and loss in 32 bits); target [...]
-    integers; bias [classes], float32 or the weight's type.  Rows whose target is `ignore_index` do not count: loss 0 and
+    hidden [..., D] and weight [classes, D]: both float32 or both bfloat16 (sums, softmax and loss in 32 bits), up to 2^24 classes of
+    2^16 features and less than 2^30 rows; target [...] integers; bias [classes], float32 or the weight's type.  Rows whose target is `ignore_index` do not count: loss 0 and
     gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
     Differentiable once, in hidden, weight and bias.

@@ -123,7 +123,7 @@ def test_one_row_of_any_stride(name, dtype):
             assert r.data_ptr() == t.data_ptr()
 
 
-@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+@pytest.mark.filterwarnings("ignore")
 @pytest.mark.parametrize("grad", [True, False])
 def test_a_trace_is_refused(grad):
     """torch.jit.trace would record the empty results and no kernel."""
@@ -170,3 +170,23 @@ def test_norms_find_what_elements_hide(reduction):
     for k, name in enumerate(("hidden", "weight")[:2 if reduction == "mean" else 1]):      # (none: the bound allows for hidden's rounding too)
         with pytest.raises(AssertionError, match=name):
             O.check_norm(name, step(torch.ldexp((m * 4).round() / 4, e))[k], want[name])
+
+
+@pytest.mark.parametrize("h,w", [((4, 1), ((1 << 24) + 1, 1)), ((4, 1), ((1 << 32) + 5, 1)), ((4, (1 << 16) + 1), (5, (1 << 16) + 1)), ((1 << 30, 1), (5, 1)), ((2, 1 << 30, 3), (5, 3))])
+def test_more_than_is_served_is_refused(h, w):
+    """Sizes beyond the kernels' (and beyond 32 bits) are refused before anything is allocated, and never cut to 32 bits."""
+    x, y = torch.zeros(1).expand(h), torch.zeros(1).expand(w)
+    t = torch.zeros(1, dtype=torch.int64).expand(h[:-1])
+    with pytest.raises(ValueError, match="linear_cross_entropy: up to"):
+        F.linear_cross_entropy(x, y, t)
+    with pytest.raises(ValueError, match="linear_distillation: up to"):
+        F.linear_distillation(x, y, torch.zeros(1).expand(*h[:-1], 2), t[..., None].expand(*h[:-1], 2))
+
+
+def test_sizes_that_are_refused_take_no_bytes():
+    lib = L.load()
+    for rows, d, v, k in ((1 << 30, 8, 8, 1), (8, (1 << 16) + 1, 8, 1), (8, 8, (1 << 24) + 1, 1), (8, 8, (1 << 31) - 1, 1), (8, 8, 8, 257), (-1, 8, 8, 1)):
+        for dt in (L.F32, L.BF16):
+            assert [lib.fea_linear_loss_ws_bytes(rows, d, v, k, dt, g) for g in (0, 1, 7, 15)] == [0] * 4
+            assert k > 1 or lib.fea_linear_loss_keep_bytes(rows, d, v, dt, 0) == 0
+    assert lib.fea_linear_loss_ws_bytes(64, 1 << 16, 8, 256, L.F32, 0) > 0 and lib.fea_linear_loss_keep_bytes(64, 8, 1 << 24, L.F32, 0) > 0
