@@ -838,3 +838,42 @@ def test_norms_of_the_errors(shape, dtype, top, keep):
         O.check("loss", got["loss"], want["loss"])
         for k in ("hidden", "weight"):
             O.check_norm(k, got[k], want[k])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("shape", [(40, 64, 300), (130, 51, 500), (4100, 24, 9)])
+def test_saved_on_the_host_checkpointed_and_in_threads(shape, dtype, top):
+    """What the forward saves may go to the host and back, be made again in the backward, and belong to steps of several threads at once."""
+    import threading
+    from torch.utils.checkpoint import checkpoint
+    cases = [[None if t is None else t.to(DEV) for t in O.case(*shape, dtype, seed=s, top=top, ignored=0.1, bias=shape[0] == 40)] for s in (1, 2, 3, 4)]
+
+    def loss(h, w, b, i, a=None):
+        return F.linear_distillation(h, w, a, i, bias=b, temperature=2.0) if top else F.linear_cross_entropy(h, w, i, bias=b)
+
+    def step(c, call=loss):
+        x = [None if t is None else t.detach().requires_grad_(True) for t in c[:3]]
+        out = call(*x, *c[3:])
+        return [out.detach(), *torch.autograd.grad(out, [t for t in x if t is not None])]
+    wants = [step(c) for c in cases]
+    with torch.autograd.graph.save_on_cpu():
+        got = step(cases[0])
+    assert all(torch.equal(a, b) for a, b in zip(got, wants[0]))
+    got = step(cases[1], lambda *x: checkpoint(loss, *x, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(got, wants[1]))
+    torch.cuda.synchronize()
+    gots = [None] * len(cases)
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(3):
+                gots[k] = step(cases[k])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for got, want in zip(gots, wants):
+        assert got is not None and all(torch.equal(a, b) for a, b in zip(got, want))
