@@ -13,8 +13,8 @@
 // Loads are buffer loads with every bound in the descriptor or the lane's offset: rows, classes and channels behind the end arrive as zeros
 // without a branch.
 //
-// Measured on 4,096 x 4,096 x 131,072 (a third of a training step each): h w^T with softmax sums and kept logits 3.6 ms (1.21 PFLOP/s;
-// 3.36 without keeping), dz w 3.25 ms (1.35), dz^T h 3.9 ms (1.13); a library's plain products 2.98, 3.16 and 3.85 ms.  Bound by power:
+// Measured on 4,096 x 4,096 x 131,072 (a third of a training step each): h w^T with softmax sums and kept logits 3.7 ms (1.19 PFLOP/s;
+// 3.36 without keeping), dz w 3.3 ms (1.33), dz^T h 3.9 ms (1.13); a library's plain products 2.98, 3.16 and 3.85 ms.  Bound by power:
 // at 60 % of the matrix pipes' cycles the clock is down to 1.9 GHz, and a loop of nothing but these MFMA on normally distributed
 // operands reaches 2.1 PFLOP/s (32 x 32 x 16 MFMA: 1.85), so what helps is less traffic and an even one: through registers and with LDS
 // writes the step took 4 % longer, with the same direct loads in bursts 5 %.

@@ -15,7 +15,8 @@
 // Why keep: recomputing is a third of a training step's products (2,048 x 2,048 x 32,000 bf16: 281 us), taking dz from kept logits is one
 // pass over them (51 us) and 8 % on the forward's product.  Why the labels' and teacher's entries are not taken from 16 bits: there
 // softmax - share cancels.
-// 2,048 x 2,048 x 32,000, us: forward's product 248, join 6, dz 51, dh 214 + 12, dw 250; 4,096 x 4,096 x 131,072, ms: 3.6, 0.02, 0.41, 3.3, 3.9.
+// 2,048 x 2,048 x 32,000, us: forward's product 259, join 6, dz 51, dh 216 + 13, dw 248; 4,096 x 4,096 x 131,072, ms: 3.7, 0.02, 0.42, 3.3, 3.9.
+// A whole step of the first takes 729 us, and 932 where nothing is kept.
 #include "linear_loss.h"
 #include <limits.h>
 #include <type_traits>
@@ -34,7 +35,9 @@ __device__ __forceinline__ void lin_split3(float v, __bf16& x0, __bf16& x1, __bf
 // Copies of an operand's rows [R][ld]: C elements in rows of Cpad (a multiple of 64, zero behind C); with planes (fp32 in, bf16 out) a row
 // holds three of Cpad.  With stat, rows whose gate is 0 count as zeros: what an ignored row holds (an infinity, a NaN) meets a zero
 // gradient in the weight's product, and 0 x NaN must not reach the weight; with gout every row is multiplied by its own
-// upstream gradient.  Up to three operands per launch, 64 x 64 elements per workgroup.
+// upstream gradient (divided by count, where there is one) and rounded to the storage type once more, by half a step: hidden's elements differ
+// from row to row, so these errors do not add up, while the same factor on dz's entries, all labels' close to it, would round them all
+// the same way when the rows' gradients are equal (a mean taken by the caller).  Up to three operands per launch, 64 x 64 elements per workgroup.
 struct LinCopy { const void* in; void* out; long long ld, ldo, R; int C, Cpad; const float2* stat; const float* gout; const int* count; float t; long long tiles; };
 struct LinCopies { LinCopy j[3]; };
 

@@ -4,8 +4,9 @@
 // One wave owns 16 classes over the whole reduction (v_mfma 16x16: 16 classes x 16 labels per product, NR of them); a workgroup of 4
 // waves 64 classes.  The weight goes from memory to registers (a wave's 16 rows x 512 bytes in flight while the 512 bytes before
 // are multiplied); the labels' hidden states, which all waves share, through LDS in the same chunks.
-// Bound by the weight's bytes: 50,021 x 2,048 bf16 (205 MB) for 37 rows in 45.5 us (4.5 TB/s); 32,768 x 1,024 (67 MB) for one row in
-// 16.4 us (4.1 TB/s), for 64 in 18.6 us.  Copies reach 5.0 TB/s here; the rest is the start and the end of a launch of 512 workgroups.
+// Bound by the weight's bytes: 50,021 x 2,048 bf16 (205 MB) for 37 rows in 56.5 us from memory (3.6 TB/s) and 46 us (4.5 TB/s) where the
+// weight is left in the 256 MB of the Infinity Cache from the call before; 32,768 x 1,024 (67 MB, there too) for one row in
+// 16.6 us (4.0 TB/s), for 64 in 18.7 us.  Copies reach 5.0 TB/s.
 #include "linear_loss.h"
 
 __device__ __forceinline__ void mma16x16(f32x4& acc, const u32x4& a, const u32x4& b, const __bf16*) {
