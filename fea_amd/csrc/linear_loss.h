@@ -13,8 +13,8 @@ enum { LIN_LSE = 0, LIN_DZ = 1, LIN_STORE = 2 };
 // six pairs of planes whose weight is above 2^-24 (x1 y1, x2 y0, x0 y2, x1 y0, x0 y1, x0 y0, the small ones first, all into one fp32
 // sum): the bf16 matrix rate is 16 times the fp32 one, so six products still gain 2.7.  FEA_PL is the form's dtype code inside these files.
 #define FEA_PL 2
-__device__ __forceinline__ int lin_plane_a(int pair) { return (0x001021 >> (4 * pair)) & 15; }
-__device__ __forceinline__ int lin_plane_b(int pair) { return (0x010201 >> (4 * pair)) & 15; }
+__device__ __forceinline__ int lin_plane_a(int pair) { return (0x001021 >> (4 * pair & 31)) & 15; }     // (behind the last pair: any, nothing is read there)
+__device__ __forceinline__ int lin_plane_b(int pair) { return (0x010201 >> (4 * pair & 31)) & 15; }
 
 // Kept logits of a bf16 head: 16 bits each.  exp(z - lse) goes to bf16 next, which rounds it by up to 2^-8 of itself; a fixed-point z is off by
 // half a step, 4.9e-4 of exp(z - lse), whatever z is.  Entries e^-64 times the largest of their
