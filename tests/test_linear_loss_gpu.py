@@ -877,3 +877,20 @@ def test_saved_on_the_host_checkpointed_and_in_threads(shape, dtype, top):
         t.join()
     for got, want in zip(gots, wants):
         assert got is not None and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(24, 64, 300), (120, 72, 500), (4200, 24, 9)])
+def test_teacher_of_another_type_and_layout(shape, dtype):
+    """A teacher's logits in the other type, int32 classes, both cut from wider rows, in a batch of sequences."""
+    h, w, b, i, a = O.case(*shape, dtype, seed=36, top=5, ignored=0.1, short=0.2, bias=True)
+    a = a.to(torch.float32 if dtype == torch.bfloat16 else torch.bfloat16)
+    lead = (shape[0] // 12, 12)
+    wide_a, wide_i = torch.full((*lead, 9), torch.nan, dtype=a.dtype, device=DEV), torch.full((*lead, 9), 1 << 20, dtype=torch.int32, device=DEV)
+    wide_a[..., 2:7], wide_i[..., 3:8] = a.to(DEV).view(*lead, 5), i.to(DEV).view(*lead, 5).int()
+    x, y, z = _leaf(h), _leaf(w), _leaf(b)
+    loss = F.linear_distillation(x.view(*lead, -1), y, wide_a[..., 2:7], wide_i[..., 3:8], bias=z, temperature=2.0, reduction="none")
+    assert loss.shape == lead
+    gout = torch.randn(shape[0], generator=torch.Generator().manual_seed(9))
+    grads = torch.autograd.grad(loss, [x, y, z], gout.to(DEV).view(lead))
+    _compare(dict(zip(("loss", "hidden", "weight", "bias"), [loss, *grads])), O.evaluate(h, w, b, i, a, temperature=2.0, reduction="none", gout=gout))
