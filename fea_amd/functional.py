@@ -256,7 +256,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     2^16 features and less than 2^30 rows; target [...] integers; bias [classes], float32 or the weight's type.  Rows whose target is `ignore_index` do not count: loss 0 and
     gradient 0, whatever their hidden state holds.  A target outside [0, classes) makes the loss and the gradients NaN.
     reduction "mean" is over the rows that count (0 if none does), "none" gives a loss for each row.  float32 result.
-    Differentiable once, in hidden, weight and bias.
+    Differentiable once, in reverse mode, in hidden, weight and bias.
     keep_logits, in a call that has a backward: True, the forward keeps the logits for it, in 16 bits each (bfloat16; the gradients' shares
     of the softmax are off by 4.9e-4 of themselves, an eighth of their rounding to bfloat16 behind that) or whole in 32 (float32, with a bias
     gradient, up to 64 rows, a split reduction), and an allocation that fails is raised; False, none are kept and the backward computes
